@@ -1,0 +1,384 @@
+// Beam search over the paged cache: the best continuations over beams and vocabulary, and the
+// tables and part-filled pages that follow the chosen beams.  The reference draws one token for one
+// sequence (log_softmax, cv3cpu/ops.py:90-93; _sample, cv3cpu/models/llm.py:125-149).
+#include "common.hpp"
+#include "decode_common.hpp"   // DPP lane exchanges
+
+#include <algorithm>
+
+using namespace cv3;
+
+namespace {
+
+constexpr int kBeams = 16;           // beams of a request
+constexpr int kVocabMax = 1 << 19;   // at most 64 slices of 8192 logits
+constexpr int kSelThreads = 256;
+
+// Rises with f; -0 as 0, a NaN as -inf.  0 is below every number's: an absent candidate.
+__device__ __forceinline__ uint32_t rank_bits(float f) {
+  f += 0.f;
+  if (!(f == f)) f = -INFINITY;
+  const uint32_t b = __float_as_uint(f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float rank_value(uint32_t r) {
+  return __uint_as_float(r & 0x80000000u ? r & 0x7fffffffu : ~r);
+}
+__device__ __forceinline__ uint64_t rank_bits(double f) {
+  f += 0.0;
+  if (!(f == f)) f = -INFINITY;
+  const uint64_t b = (uint64_t)__double_as_longlong(f);
+  return b >> 63 ? ~b : b | (uint64_t)1 << 63;
+}
+__device__ __forceinline__ double rank_value(uint64_t r) {
+  return __longlong_as_double((int64_t)(r >> 63 ? r & ~((uint64_t)1 << 63) : ~r));
+}
+
+struct SelectArgs {
+  const float* logits;
+  const float* scores;
+  const uint8_t* done;
+  uint64_t* keys;        // [rows, slices, beams]: a slice's best logits, best first
+  double* sums;          // [rows, slices]: sum of exp(logit - the slice's largest)
+  float* tops;           // [rows, slices]
+  int64_t* tokens;
+  int32_t* parents;
+  float* scores_out;
+  uint8_t* done_out;
+  int64_t vocab, stop_lo, stop_hi, ban_lo, ban_hi, pad;
+  int beams, slices, slice;
+};
+
+// Best `beams` logits of one slice of one row, and its part of the softmax's sum.  A key is the
+// logit's rank over the complement of its token, so no two are equal.  The 64 groups of four
+// threads each have a largest key; whatever is among the slice's best W lies in a group whose
+// largest is among the best W of those, and is no less than the W-th of them: at most 4 W E keys
+// pass that bar, a few more than W as a rule, and those are ranked by counting.
+// The logits are read once, E a thread, all loads in flight together; HBM-bound.
+template <int E>
+__global__ __launch_bounds__(kSelThreads) void k_select_slices(SelectArgs a) {
+  __shared__ uint64_t s_group[64];
+  __shared__ uint64_t s_list[4 * kBeams * E];
+  __shared__ float s_max[4];
+  __shared__ double s_sum[4];
+  __shared__ int s_count;
+  const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  if (a.done[row]) return;             // its one continuation needs no logits
+  struct __attribute__((packed, aligned(4))) Four {
+    float v[4];
+  };
+  const int64_t lo = (int64_t)slice * a.slice, hi = min(lo + a.slice, a.vocab);
+  const float* x = a.logits + (int64_t)row * a.vocab;
+  float v[E];
+#pragma unroll
+  for (int e = 0; e < E; e += 4) {
+    const int64_t t = lo + (e / 4 * kSelThreads + tid) * 4;
+    if (t + 4 <= hi) {
+      const Four f = *(const Four*)(x + t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[e + i] = f.v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[e + i] = t + i < hi ? x[t + i] : -INFINITY;
+    }
+  }
+  float mx = -INFINITY;
+  uint64_t best = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int64_t t = lo + (e / 4 * kSelThreads + tid) * 4 + e % 4;
+    mx = fmaxf(mx, v[e]);
+    const bool on = t < hi && !(t >= a.ban_lo && t < a.ban_hi);
+    const uint64_t k = on ? (uint64_t)rank_bits(v[e]) << 32 | (uint32_t)~(uint32_t)t : 0;
+    best = max(best, k);
+  }
+  mx = wave_max_dpp(mx);
+  uint64_t four = max(best, dpp64<kDppXor1>(best));
+  four = max(four, dpp64<kDppXor2>(four));
+  if ((lane & 3) == 0) s_group[tid >> 2] = four;
+  if (lane == 0) s_max[wv] = mx;
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  double sum = 0.0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum += (double)expf(v[e] - ref);     // a NaN, or +inf - +inf, makes the row's sum NaN
+  sum = wave_sum_d(sum);
+  if (lane == 0) s_sum[wv] = sum;
+
+  // the W-th of the groups' largest keys, by every wave for itself
+  const uint64_t mine = s_group[lane];
+  int above = 0;
+  for (int i = 0; i < 64; ++i) above += readlane64(mine, i) > mine ? 1 : 0;
+  uint64_t bar = above >= a.beams - 1 ? mine : 0;
+  bar = max(wave_max_u64(bar), (uint64_t)1);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int64_t t = lo + (e / 4 * kSelThreads + tid) * 4 + e % 4;
+    const bool on = t < hi && !(t >= a.ban_lo && t < a.ban_hi);
+    const uint64_t k = on ? (uint64_t)rank_bits(v[e]) << 32 | (uint32_t)~(uint32_t)t : 0;
+    if (k >= bar) s_list[atomicAdd(&s_count, 1)] = k;
+  }
+  __syncthreads();
+  const int n = s_count;
+  const int64_t at = (int64_t)row * a.slices + slice;
+  uint64_t* out = a.keys + at * a.beams;
+  for (int i = tid; i < n; i += kSelThreads) {
+    const uint64_t k = s_list[i];
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += s_list[j] > k ? 1 : 0;
+    if (r < a.beams) out[r] = k;
+  }
+  if (tid >= n && tid < a.beams) out[tid] = 0;
+  if (tid == 0) {
+    a.sums[at] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+    a.tops[at] = mx;
+  }
+}
+
+struct Pick {            // larger is better: the value, then the lower beam, the larger logit, the lower token
+  uint64_t hi, lo;
+  __device__ bool operator>(const Pick& o) const { return hi != o.hi ? hi > o.hi : lo > o.lo; }
+};
+
+// One workgroup per request.  The slices' lists are sorted, so the best of a thread's lists are
+// their heads; the W-th best of the threads' bounds what can be chosen, as above, and at most
+// W lists a thread x W threads x W keys pass.
+__global__ __launch_bounds__(kSelThreads) void k_select_beams(SelectArgs a) {
+  __shared__ double s_lse[kBeams];
+  __shared__ Pick s_best[kSelThreads];
+  __shared__ Pick s_list[kBeams * 4 * kBeams];
+  __shared__ Pick s_out[kBeams];
+  __shared__ int s_count;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int64_t row0 = (int64_t)blockIdx.x * a.beams;
+  for (int b = wv; b < a.beams; b += kSelThreads / 64) {
+    if (a.done[row0 + b]) continue;
+    // at most 64 slices: a lane each
+    const int64_t at = (row0 + b) * a.slices + lane;
+    const float top = lane < a.slices ? a.tops[at] : -INFINITY;
+    const float all = wave_max_dpp(top);
+    double sum = lane < a.slices ? a.sums[at] * exp((double)top - (double)all) : 0.0;
+    if (top == -INFINITY && all > -INFINITY && lane < a.slices) sum = a.sums[at];   // 0, or NaN
+    sum = wave_sum_d(sum);
+    if (lane == 0) s_lse[b] = (double)all + log(sum);       // all -inf: NaN
+  }
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  const int lists = a.beams * a.slices;
+  auto pick = [&](int list, int rank) -> Pick {
+    const int b = list / a.slices;
+    const double score = (double)a.scores[row0 + b];
+    const uint64_t order = (uint64_t)(31 - b) << 59;
+    if (a.done[row0 + b]) {
+      if (rank || list % a.slices) return Pick{0, 0};
+      return Pick{rank_bits(score), order};
+    }
+    const uint64_t k = a.keys[((row0 + b) * a.slices + list % a.slices) * a.beams + rank];
+    if (!k) return Pick{0, 0};
+    const double value = score + ((double)rank_value((uint32_t)(k >> 32)) - s_lse[b]);
+    return Pick{rank_bits(value), order | (k >> 32) << 27 | (k & 0x7ffffff)};
+  };
+  Pick best{0, 0};
+  for (int l = tid; l < lists; l += kSelThreads) {
+    const Pick p = pick(l, 0);
+    if (p > best) best = p;
+  }
+  s_best[tid] = best;
+  __syncthreads();
+  // every thread counts for one head; the bar is the one with W - 1 above it (none: take everything)
+  const int heads = min(lists, kSelThreads);
+  int above = 0;
+  for (int i = 0; i < heads; ++i) above += s_best[i] > best ? 1 : 0;
+  if (tid < kBeams) s_out[tid] = Pick{0, 0};
+  __shared__ Pick s_bar;
+  if (tid == 0) s_bar = Pick{0, 1};
+  __syncthreads();
+  if (tid < heads && above == a.beams - 1 && best.hi) s_bar = best;
+  __syncthreads();
+  const Pick bar = s_bar;
+  for (int l = tid; l < lists; l += kSelThreads)
+    for (int r = 0; r < a.beams; ++r) {
+      const Pick p = pick(l, r);
+      if (!p.hi || bar > p) break;
+      s_list[atomicAdd(&s_count, 1)] = p;
+    }
+  __syncthreads();
+  const int n = s_count;
+  for (int i = tid; i < n; i += kSelThreads) {
+    const Pick p = s_list[i];
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += s_list[j] > p ? 1 : 0;
+    if (r < a.beams) s_out[r] = p;
+  }
+  __syncthreads();
+  // scores_out and done_out may be scores and done: read what is needed of them first
+  int parent = 0;
+  int64_t token = 0;
+  float score = 0.f;
+  bool ended = false;
+  if (tid < a.beams) {
+    const Pick p = s_out[tid];
+    parent = 31 - (int)(p.lo >> 59);
+    if (parent < 0 || parent >= a.beams) parent = 0;
+    ended = a.done[row0 + parent] != 0;
+    token = ended ? a.pad : (int64_t)(0x7ffffff - (p.lo & 0x7ffffff));
+    score = (float)rank_value(p.hi);
+    ended = ended || (token >= a.stop_lo && token < a.stop_hi);
+  }
+  __syncthreads();
+  if (tid < a.beams) {
+    a.tokens[row0 + tid] = token;
+    a.parents[row0 + tid] = parent;
+    a.scores_out[row0 + tid] = score;
+    a.done_out[row0 + tid] = ended ? 1 : 0;
+  }
+}
+
+template <int E>
+void launch_slices(const SelectArgs& a, int64_t rows, hipStream_t st) {
+  hipLaunchKernelGGL(k_select_slices<E>, dim3((unsigned)(rows * a.slices)), dim3(kSelThreads), 0, st, a);
+}
+
+// ------------------------------------------------------------------------------------------------
+
+struct ReorderArgs {
+  const int32_t* parents;
+  int32_t* tables;
+  const int32_t* own;
+  const int32_t* lengths;
+  uint4* k;
+  uint4* v;
+  int64_t pages, blocks, layers;
+  int beams, kv_heads, page, row_vecs;   // 16-byte vectors of a key row
+  int parts, table_parts;                // workgroups of a run of rows, and of a request's table
+};
+
+// Copies move a part-filled page's rows between the beams' own pages, in place and in any order: a
+// thread holds the same 16 bytes of every beam's page, reads all it needs and only then writes.
+// HBM-bound; a beam that stays itself costs nothing.  Workgroups [0, request's copies) copy, the
+// last table_parts of each request turn its table, column by column, in the same way.
+template <int W>
+__global__ __launch_bounds__(256) void k_beam_reorder(ReorderArgs a) {
+  const int64_t copies = a.layers * a.kv_heads * 2 * a.parts, per = copies + a.table_parts;
+  const int64_t r = blockIdx.x / per, in = blockIdx.x % per;
+  const int64_t cap = a.blocks * a.page;
+  const int64_t len = min((int64_t)max(a.lengths[r], 0), cap);
+  const int64_t full = len / a.page, rest = len - full * a.page;
+  const int32_t* parents = a.parents + r * a.beams;
+  if (in >= copies) {
+    int32_t* table = a.tables + r * a.beams * a.blocks;
+    const int32_t* own = a.own + r * a.beams * a.blocks;
+    const int64_t c = (in - copies) * 256 + threadIdx.x;
+    if (c >= a.blocks) return;
+    int32_t id[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      if (w < a.beams) {
+        const int p = parents[w];
+        id[w] = (unsigned)p >= (unsigned)a.beams ? table[w * a.blocks + c]
+                : c < full                       ? table[p * a.blocks + c]
+                                                 : own[w * a.blocks + c];
+      }
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      if (w < a.beams) table[w * a.blocks + c] = id[w];
+    return;
+  }
+  const int vec = (int)(in % a.parts) * 256 + (int)threadIdx.x;
+  if (vec >= rest * a.row_vecs) return;
+  const int64_t lane_of = in / a.parts;          // [layer][k or v][kv head]
+  const int kv = (int)(lane_of % a.kv_heads);
+  uint4* cache = (lane_of / a.kv_heads) % 2 ? a.v : a.k;
+  const int64_t layer = lane_of / a.kv_heads / 2;
+  const int32_t* own = a.own + r * a.beams * a.blocks + full;
+  const int64_t run = (int64_t)a.page * a.row_vecs, page_vecs = run * a.kv_heads;
+  uint4* base = cache + layer * a.pages * page_vecs + kv * run + vec;
+  uint4 x[W];
+  int64_t to[W];           // -1: this beam's rows stay
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const int p = w < a.beams ? parents[w] : w;
+    const bool other = p != w && (unsigned)p < (unsigned)a.beams;
+    const int64_t from = other ? own[p * a.blocks] : -1;
+    to[w] = other ? own[w * a.blocks] : -1;
+    if (from < 0 || from >= a.pages || to[w] >= a.pages) to[w] = -1;
+    x[w] = to[w] >= 0 ? base[from * page_vecs] : uint4{};
+  }
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+    if (to[w] >= 0) base[to[w] * page_vecs] = x[w];
+}
+
+}  // namespace
+
+extern "C" {
+
+int cv3_beam_select(const float* logits, int64_t requests, int beams, int64_t vocab, const float* scores,
+                    const uint8_t* done, int64_t stop_lo, int64_t stop_hi, int64_t ban_lo, int64_t ban_hi, int64_t pad,
+                    int64_t* tokens, int32_t* parents, float* scores_out, uint8_t* done_out, cv3_stream_t s) {
+  CV3_ALIVE();
+  CV3_REQUIRE(beams >= 1 && beams <= kBeams, CV3_EINVAL, "1 to %d beams, not %d", kBeams, beams);
+  CV3_REQUIRE(vocab >= 1 && vocab <= kVocabMax, CV3_EINVAL, "a vocabulary of 1 to %d tokens, not %lld", kVocabMax,
+              (long long)vocab);
+  CV3_REQUIRE(requests >= 0 && requests <= (1 << 20), CV3_EINVAL, "bad number of requests: %lld", (long long)requests);
+  const int64_t banned = std::max<int64_t>(0, std::min(ban_hi, vocab) - std::max<int64_t>(ban_lo, 0));
+  CV3_REQUIRE(vocab - banned >= beams, CV3_EINVAL, "%lld tokens to choose from are fewer than %d beams",
+              (long long)(vocab - banned), beams);
+  if (requests == 0) return CV3_OK;
+  CV3_REQUIRE(logits && scores && done && tokens && parents && scores_out && done_out, CV3_EINVAL, "null operand");
+  const int64_t rows = requests * beams;
+  const int e = 32;
+  SelectArgs a{logits, scores, done, nullptr, nullptr, nullptr, tokens, parents, scores_out, done_out, vocab, stop_lo,
+               stop_hi, ban_lo, ban_hi, pad, beams, 0, e * kSelThreads};
+  a.slices = (int)ceil_div(vocab, a.slice);
+  hipStream_t st = stream_of(s);
+  const int64_t lists = rows * a.slices;
+  void* work = nullptr;
+  if (int rc = scratch_alloc(&work, (size_t)lists * (beams * 8 + 16), st)) return rc;
+  a.keys = (uint64_t*)work;
+  a.sums = (double*)(a.keys + lists * beams);
+  a.tops = (float*)(a.sums + lists);
+  launch_slices<32>(a, rows, st);
+  hipLaunchKernelGGL(k_select_beams, dim3((unsigned)requests), dim3(kSelThreads), 0, st, a);
+  const hipError_t err = hipGetLastError();
+  const int rc = scratch_free(work, st);
+  CV3_REQUIRE(err == hipSuccess, CV3_EHIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return rc;
+}
+
+int cv3_beam_reorder(const int32_t* parents, int64_t requests, int beams, int32_t* tables, const int32_t* own,
+                     int64_t blocks, const int32_t* lengths, int cache_type, void* k_cache, void* v_cache,
+                     int64_t layers, int64_t pages, int kv_heads, int64_t page, int d, cv3_stream_t s) {
+  CV3_ALIVE();
+  CV3_REQUIRE(cache_type == CV3_F32 || cache_type == CV3_F16 || cache_type == CV3_BF16, CV3_EINVAL,
+              "unknown cache type %d", cache_type);
+  CV3_REQUIRE(beams >= 1 && beams <= kBeams, CV3_EINVAL, "1 to %d beams, not %d", kBeams, beams);
+  CV3_REQUIRE(page >= 1 && page <= 65536, CV3_EINVAL, "a page holds 1 to 65536 keys, not %lld", (long long)page);
+  CV3_REQUIRE(pages >= 1 && pages <= INT32_MAX && layers >= 1 && layers <= 65536 && kv_heads >= 1 && kv_heads <= 1024,
+              CV3_EINVAL, "bad cache shape");
+  CV3_REQUIRE(d >= 8 && d <= 256 && d % 8 == 0, CV3_EINVAL, "the head dim must be a multiple of 8, 8 to 256, not %d", d);
+  CV3_REQUIRE(blocks >= 1 && blocks <= (INT32_MAX - 65536) / page, CV3_EINVAL,
+              "tables of %lld blocks of %lld keys pass 2^31 keys", (long long)blocks, (long long)page);
+  CV3_REQUIRE(requests >= 0, CV3_EINVAL, "negative number of requests");
+  if (requests == 0) return CV3_OK;
+  CV3_REQUIRE(parents && tables && own && lengths && k_cache && v_cache, CV3_EINVAL, "null operand");
+  CV3_REQUIRE(((uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0, CV3_EINVAL, "the caches must be 16-byte aligned");
+  CV3_REQUIRE(tables != own, CV3_EINVAL, "the beams' own pages are a table of their own");
+  const int row_vecs = d * (cache_type == CV3_F32 ? 4 : 2) / 16;
+  ReorderArgs a{parents, tables, own, lengths, (uint4*)k_cache, (uint4*)v_cache, pages, blocks, layers, beams, kv_heads,
+                (int)page, row_vecs, (int)ceil_div(page * row_vecs, 256), (int)ceil_div(blocks, 256)};
+  const int64_t per = layers * kv_heads * 2 * a.parts + a.table_parts;
+  CV3_REQUIRE(requests <= INT32_MAX / per, CV3_EINVAL, "too many requests for one call: %lld", (long long)requests);
+  const dim3 grid((unsigned)(requests * per)), block(256);
+  hipStream_t st = stream_of(s);
+  if (beams <= 4) hipLaunchKernelGGL(k_beam_reorder<4>, grid, block, 0, st, a);
+  else if (beams <= 8) hipLaunchKernelGGL(k_beam_reorder<8>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(k_beam_reorder<16>, grid, block, 0, st, a);
+  CV3_LAUNCHED();
+  return CV3_OK;
+}
+
+}  // extern "C"

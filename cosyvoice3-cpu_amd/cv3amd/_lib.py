@@ -23,7 +23,7 @@ _ROOT = os.path.dirname(os.path.dirname(HERE))
 HEADER = os.path.join(_ROOT, "include", "cv3hip.h")
 
 OK, EINVAL, EINDEX, EASSERT, EHIP, EUNSUPPORTED, ENOMEM = 0, 1, 2, 3, 4, 5, 6
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 KIND_F32, KIND_F16, KIND_Q8, KIND_Q4 = 0, 1, 2, 3
 ACT = {"none": 0, "silu": 1, "sigmoid": 2, "gelu_tanh": 3, "gelu": 4, "mish": 5, "elu": 6,
        "leaky": 7, "tanh": 8}
