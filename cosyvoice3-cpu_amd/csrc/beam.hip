@@ -49,16 +49,23 @@ struct SelectArgs {
   int beams, slices, slice;
 };
 
-// Best `beams` logits of one slice of one row, and its part of the softmax's sum.  A key is the
-// logit's rank over the complement of its token, so no two are equal.  The 64 groups of four
-// threads each have a largest key; whatever is among the slice's best W lies in a group whose
-// largest is among the best W of those, and is no less than the W-th of them: at most 4 W E keys
-// pass that bar, a few more than W as a rule, and those are ranked by counting.
-// The logits are read once, E a thread, all loads in flight together; HBM-bound.
+constexpr int kList = 512;     // logits of a slice that may pass its bar by value alone
+
+// Best `beams` logits of one slice of one row, and its part of the softmax's sum; HBM-bound, the
+// logits read once, E a thread, all loads in flight together.
+//
+// Of the 64 groups of four threads each has a largest logit.  What is among the slice's best W is no
+// less than the W-th of those: a few more than W logits pass that bar as a rule, and are ranked by
+// counting.  A key is the logit's rank over the complement of its token, so no two are equal and
+// equal logits go by the lower token.  Where more pass than the list holds (many equal logits), or
+// the bar is -inf, the bar is set by whole keys: whatever passes it then lies in W groups, at most
+// 4 W E keys.
 template <int E>
 __global__ __launch_bounds__(kSelThreads) void k_select_slices(SelectArgs a) {
-  __shared__ uint64_t s_group[64];
-  __shared__ uint64_t s_list[4 * kBeams * E];
+  constexpr int kMost = 4 * kBeams * E;
+  __shared__ uint64_t s_list[kMost > kList ? kMost : kList];
+  __shared__ uint64_t s_key[64];
+  __shared__ float s_group[64];
   __shared__ float s_max[4];
   __shared__ double s_sum[4];
   __shared__ int s_count;
@@ -68,12 +75,13 @@ __global__ __launch_bounds__(kSelThreads) void k_select_slices(SelectArgs a) {
   struct __attribute__((packed, aligned(4))) Four {
     float v[4];
   };
-  const int64_t lo = (int64_t)slice * a.slice, hi = min(lo + a.slice, a.vocab);
+  const int lo = slice * a.slice, hi = (int)min((int64_t)lo + a.slice, a.vocab);
   const float* x = a.logits + (int64_t)row * a.vocab;
-  float v[E];
+  const int first = lo + tid * 4;      // this thread's tokens: first + 4 * kSelThreads * i + 0 .. 3
+  float v[E], four[E / 4];
 #pragma unroll
   for (int e = 0; e < E; e += 4) {
-    const int64_t t = lo + (e / 4 * kSelThreads + tid) * 4;
+    const int t = first + e * kSelThreads;
     if (t + 4 <= hi) {
       const Four f = *(const Four*)(x + t);
 #pragma unroll
@@ -83,46 +91,92 @@ __global__ __launch_bounds__(kSelThreads) void k_select_slices(SelectArgs a) {
       for (int i = 0; i < 4; ++i) v[e + i] = t + i < hi ? x[t + i] : -INFINITY;
     }
   }
-  float mx = -INFINITY;
-  uint64_t best = 0;
+  const bool bans = a.ban_lo < hi && a.ban_hi > lo;       // of this slice
+  auto banned = [&](int t) { return t >= a.ban_lo && t < a.ban_hi; };
+  float mx = -INFINITY, best = -INFINITY;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int64_t t = lo + (e / 4 * kSelThreads + tid) * 4 + e % 4;
-    mx = fmaxf(mx, v[e]);
-    const bool on = t < hi && !(t >= a.ban_lo && t < a.ban_hi);
-    const uint64_t k = on ? (uint64_t)rank_bits(v[e]) << 32 | (uint32_t)~(uint32_t)t : 0;
-    best = max(best, k);
+  for (int e = 0; e < E; e += 4) {
+    four[e / 4] = fmaxf(fmaxf(v[e], v[e + 1]), fmaxf(v[e + 2], v[e + 3]));
+    mx = fmaxf(mx, four[e / 4]);
   }
+  best = mx;
+  if (bans) {
+    best = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (!banned(first + e / 4 * 4 * kSelThreads + e % 4)) best = fmaxf(best, v[e]);
+  }
+  best = fmaxf(best, __uint_as_float(dpp32<kDppXor1>(__float_as_uint(best))));
+  best = fmaxf(best, __uint_as_float(dpp32<kDppXor2>(__float_as_uint(best))));
+  if ((lane & 3) == 0) s_group[tid >> 2] = best;
   mx = wave_max_dpp(mx);
-  uint64_t four = max(best, dpp64<kDppXor1>(best));
-  four = max(four, dpp64<kDppXor2>(four));
-  if ((lane & 3) == 0) s_group[tid >> 2] = four;
   if (lane == 0) s_max[wv] = mx;
   if (tid == 0) s_count = 0;
   __syncthreads();
   mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+
+  // the W-th largest of the groups, by every wave for itself: the least that fewer than W surpass
+  const float mine = s_group[lane];
+  int above = 0;
+#pragma unroll 16
+  for (int i = 0; i < 64; ++i)
+    above += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), i)) > mine ? 1 : 0;
+  const float bar = -wave_max_dpp(above < a.beams ? -mine : -INFINITY);
+  const bool open = bar == -INFINITY;
+  if (!open) {
+#pragma unroll
+    for (int e = 0; e < E; e += 4)
+      if (four[e / 4] >= bar) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = first + e * kSelThreads + i;
+          if (v[e + i] >= bar && !(bans && banned(t))) {
+            const int n = atomicAdd(&s_count, 1);
+            if (n < kList) s_list[n] = (uint64_t)rank_bits(v[e + i]) << 32 | (uint32_t)~(uint32_t)t;
+          }
+        }
+      }
+  }
+  // Sums of four in float32, then float64: a NaN, or +inf - +inf, makes the row's sum NaN.
   const float ref = mx == -INFINITY ? 0.f : mx;
   double sum = 0.0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) sum += (double)expf(v[e] - ref);     // a NaN, or +inf - +inf, makes the row's sum NaN
+  for (int e = 0; e < E; e += 4) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f((v[e + i] - ref) * kLog2E);
+    sum += (double)s;
+  }
   sum = wave_sum_d(sum);
   if (lane == 0) s_sum[wv] = sum;
-
-  // the W-th of the groups' largest keys, by every wave for itself
-  const uint64_t mine = s_group[lane];
-  int above = 0;
-  for (int i = 0; i < 64; ++i) above += readlane64(mine, i) > mine ? 1 : 0;
-  uint64_t bar = above >= a.beams - 1 ? mine : 0;
-  bar = max(wave_max_u64(bar), (uint64_t)1);
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int64_t t = lo + (e / 4 * kSelThreads + tid) * 4 + e % 4;
-    const bool on = t < hi && !(t >= a.ban_lo && t < a.ban_hi);
-    const uint64_t k = on ? (uint64_t)rank_bits(v[e]) << 32 | (uint32_t)~(uint32_t)t : 0;
-    if (k >= bar) s_list[atomicAdd(&s_count, 1)] = k;
-  }
   __syncthreads();
-  const int n = s_count;
+  int n = s_count;
+  if (open || n > kList) {
+    auto key_of = [&](int e) -> uint64_t {
+      const int t = first + e / 4 * 4 * kSelThreads + e % 4;
+      return t < hi && !(bans && banned(t)) ? (uint64_t)rank_bits(v[e]) << 32 | (uint32_t)~(uint32_t)t : 0;
+    };
+    uint64_t k = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) k = max(k, key_of(e));
+    k = max(k, dpp64<kDppXor1>(k));
+    k = max(k, dpp64<kDppXor2>(k));
+    if ((lane & 3) == 0) s_key[tid >> 2] = k;
+    __syncthreads();                     // every thread has read s_count, and the keys are there
+    if (tid == 0) s_count = 0;
+    const uint64_t own = s_key[lane];
+    int over = 0;
+    for (int i = 0; i < 64; ++i) over += readlane64(own, i) > own ? 1 : 0;
+    const uint64_t least = max(wave_max_u64(over >= a.beams - 1 ? own : 0), (uint64_t)1);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t u = key_of(e);
+      if (u >= least) s_list[atomicAdd(&s_count, 1)] = u;
+    }
+    __syncthreads();
+    n = s_count;
+  }
   const int64_t at = (int64_t)row * a.slices + slice;
   uint64_t* out = a.keys + at * a.beams;
   for (int i = tid; i < n; i += kSelThreads) {
@@ -143,68 +197,104 @@ struct Pick {            // larger is better: the value, then the lower beam, th
   __device__ bool operator>(const Pick& o) const { return hi != o.hi ? hi > o.hi : lo > o.lo; }
 };
 
-// One workgroup per request.  The slices' lists are sorted, so the best of a thread's lists are
-// their heads; the W-th best of the threads' bounds what can be chosen, as above, and at most
-// W lists a thread x W threads x W keys pass.
+constexpr int kLists = kBeams * 64;            // of a request: its beams' slices
+constexpr int kListsEach = kLists / kSelThreads;
+
+// One workgroup per request; bound by the chain of its few loads.  The slices' lists are sorted, so
+// the best of a thread's lists are their heads; the W-th best of the threads' bounds what can be
+// chosen, and at most W lists a thread x W threads x W keys pass.
 __global__ __launch_bounds__(kSelThreads) void k_select_beams(SelectArgs a) {
-  __shared__ double s_lse[kBeams];
+  __shared__ double s_lse[kBeams], s_score[kBeams];
+  __shared__ int s_done[kBeams];
+  __shared__ double s_sum[kLists];
+  __shared__ float s_top[kLists];
   __shared__ Pick s_best[kSelThreads];
-  __shared__ Pick s_list[kBeams * 4 * kBeams];
+  __shared__ Pick s_list[kBeams * kListsEach * kBeams];
   __shared__ Pick s_out[kBeams];
+  __shared__ Pick s_bar;
   __shared__ int s_count;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int64_t row0 = (int64_t)blockIdx.x * a.beams;
-  for (int b = wv; b < a.beams; b += kSelThreads / 64) {
-    if (a.done[row0 + b]) continue;
-    // at most 64 slices: a lane each
-    const int64_t at = (row0 + b) * a.slices + lane;
-    const float top = lane < a.slices ? a.tops[at] : -INFINITY;
-    const float all = wave_max_dpp(top);
-    double sum = lane < a.slices ? a.sums[at] * exp((double)top - (double)all) : 0.0;
-    if (top == -INFINITY && all > -INFINITY && lane < a.slices) sum = a.sums[at];   // 0, or NaN
-    sum = wave_sum_d(sum);
-    if (lane == 0) s_lse[b] = (double)all + log(sum);       // all -inf: NaN
-  }
-  if (tid == 0) s_count = 0;
-  __syncthreads();
   const int lists = a.beams * a.slices;
-  auto pick = [&](int list, int rank) -> Pick {
-    const int b = list / a.slices;
-    const double score = (double)a.scores[row0 + b];
-    const uint64_t order = (uint64_t)(31 - b) << 59;
-    if (a.done[row0 + b]) {
-      if (rank || list % a.slices) return Pick{0, 0};
-      return Pick{rank_bits(score), order};
+  // An ended beam's lists hold whatever the memory held: they are not looked at.
+  const int64_t list0 = row0 * a.slices;
+  uint64_t head[kListsEach];
+#pragma unroll
+  for (int i = 0; i < kListsEach; ++i) {
+    const int l = tid + i * kSelThreads;
+    head[i] = 0;
+    if (l < lists) {
+      head[i] = a.keys[(list0 + l) * a.beams];
+      s_sum[l] = a.sums[list0 + l];
+      s_top[l] = a.tops[list0 + l];
     }
-    const uint64_t k = a.keys[((row0 + b) * a.slices + list % a.slices) * a.beams + rank];
+  }
+  if (tid < a.beams) {
+    s_score[tid] = (double)a.scores[row0 + tid];
+    s_done[tid] = a.done[row0 + tid];
+  }
+  if (tid < kBeams) s_out[tid] = Pick{0, 0};
+  if (tid == 0) {
+    s_count = 0;
+    s_bar = Pick{0, 1};
+  }
+  __syncthreads();
+  for (int b = wv; b < a.beams; b += kSelThreads / 64) {
+    // at most 64 slices: a lane each
+    const float top = lane < a.slices ? s_top[b * a.slices + lane] : -INFINITY;
+    const float all = wave_max_dpp(top);
+    double sum = lane < a.slices ? s_sum[b * a.slices + lane] : 0.0;
+    if (top != all) sum *= exp((double)top - (double)all);     // 0 or NaN where the slice is -inf
+    sum = wave_sum_d(sum);
+    if (lane == 0) s_lse[b] = all > -INFINITY ? (double)all + log(sum) : (double)NAN;
+  }
+  __syncthreads();
+  auto pick = [&](int list, int rank, uint64_t k) -> Pick {
+    const int b = list / a.slices;
+    const uint64_t order = (uint64_t)(31 - b) << 59;
+    if (s_done[b]) return rank || list % a.slices ? Pick{0, 0} : Pick{rank_bits(s_score[b]), order};
     if (!k) return Pick{0, 0};
-    const double value = score + ((double)rank_value((uint32_t)(k >> 32)) - s_lse[b]);
+    const double value = s_score[b] + ((double)rank_value((uint32_t)(k >> 32)) - s_lse[b]);
     return Pick{rank_bits(value), order | (k >> 32) << 27 | (k & 0x7ffffff)};
   };
   Pick best{0, 0};
-  for (int l = tid; l < lists; l += kSelThreads) {
-    const Pick p = pick(l, 0);
-    if (p > best) best = p;
+#pragma unroll
+  for (int i = 0; i < kListsEach; ++i) {
+    const int l = tid + i * kSelThreads;
+    if (l < lists) {
+      const Pick p = pick(l, 0, head[i]);
+      if (p > best) best = p;
+    }
   }
   s_best[tid] = best;
   __syncthreads();
   // every thread counts for one head; the bar is the one with W - 1 above it (none: take everything)
   const int heads = min(lists, kSelThreads);
   int above = 0;
+#pragma unroll 8
   for (int i = 0; i < heads; ++i) above += s_best[i] > best ? 1 : 0;
-  if (tid < kBeams) s_out[tid] = Pick{0, 0};
-  __shared__ Pick s_bar;
-  if (tid == 0) s_bar = Pick{0, 1};
-  __syncthreads();
   if (tid < heads && above == a.beams - 1 && best.hi) s_bar = best;
   __syncthreads();
   const Pick bar = s_bar;
-  for (int l = tid; l < lists; l += kSelThreads)
-    for (int r = 0; r < a.beams; ++r) {
-      const Pick p = pick(l, r);
-      if (!p.hi || bar > p) break;
-      s_list[atomicAdd(&s_count, 1)] = p;
+  if (!(bar > best)) {
+#pragma unroll
+    for (int i = 0; i < kListsEach; ++i) {
+      const int l = tid + i * kSelThreads;
+      if (l >= lists) continue;
+      const Pick p0 = pick(l, 0, head[i]);
+      if (!p0.hi || bar > p0) continue;
+      s_list[atomicAdd(&s_count, 1)] = p0;
+      if (s_done[l / a.slices]) continue;
+      uint64_t k[kBeams];                      // the rest of the list, its loads in flight together
+#pragma unroll
+      for (int r = 1; r < kBeams; ++r) k[r] = r < a.beams ? a.keys[(list0 + l) * a.beams + r] : 0;
+#pragma unroll
+      for (int r = 1; r < kBeams; ++r) {
+        const Pick p = pick(l, r, k[r]);
+        if (p.hi && !(bar > p)) s_list[atomicAdd(&s_count, 1)] = p;
+      }
     }
+  }
   __syncthreads();
   const int n = s_count;
   for (int i = tid; i < n; i += kSelThreads) {
@@ -214,26 +304,16 @@ __global__ __launch_bounds__(kSelThreads) void k_select_beams(SelectArgs a) {
     if (r < a.beams) s_out[r] = p;
   }
   __syncthreads();
-  // scores_out and done_out may be scores and done: read what is needed of them first
-  int parent = 0;
-  int64_t token = 0;
-  float score = 0.f;
-  bool ended = false;
-  if (tid < a.beams) {
+  if (tid < a.beams) {                         // scores_out and done_out may be scores and done: those are read
     const Pick p = s_out[tid];
-    parent = 31 - (int)(p.lo >> 59);
+    int parent = 31 - (int)(p.lo >> 59);
     if (parent < 0 || parent >= a.beams) parent = 0;
-    ended = a.done[row0 + parent] != 0;
-    token = ended ? a.pad : (int64_t)(0x7ffffff - (p.lo & 0x7ffffff));
-    score = (float)rank_value(p.hi);
-    ended = ended || (token >= a.stop_lo && token < a.stop_hi);
-  }
-  __syncthreads();
-  if (tid < a.beams) {
+    const bool ended = s_done[parent] != 0;
+    const int64_t token = ended ? a.pad : (int64_t)(0x7ffffff - (p.lo & 0x7ffffff));
     a.tokens[row0 + tid] = token;
     a.parents[row0 + tid] = parent;
-    a.scores_out[row0 + tid] = score;
-    a.done_out[row0 + tid] = ended ? 1 : 0;
+    a.scores_out[row0 + tid] = (float)rank_value(p.hi);
+    a.done_out[row0 + tid] = ended || (token >= a.stop_lo && token < a.stop_hi) ? 1 : 0;
   }
 }
 
@@ -330,7 +410,8 @@ int cv3_beam_select(const float* logits, int64_t requests, int beams, int64_t vo
   if (requests == 0) return CV3_OK;
   CV3_REQUIRE(logits && scores && done && tokens && parents && scores_out && done_out, CV3_EINVAL, "null operand");
   const int64_t rows = requests * beams;
-  const int e = 32;
+  // 2048 logits a workgroup where 8192 would leave CUs idle (and a list a lane is enough)
+  const int e = rows * ceil_div(vocab, 32 * kSelThreads) < 256 && vocab <= 64 * 8 * kSelThreads ? 8 : 32;
   SelectArgs a{logits, scores, done, nullptr, nullptr, nullptr, tokens, parents, scores_out, done_out, vocab, stop_lo,
                stop_hi, ban_lo, ban_hi, pad, beams, 0, e * kSelThreads};
   a.slices = (int)ceil_div(vocab, a.slice);
@@ -341,7 +422,7 @@ int cv3_beam_select(const float* logits, int64_t requests, int beams, int64_t vo
   a.keys = (uint64_t*)work;
   a.sums = (double*)(a.keys + lists * beams);
   a.tops = (float*)(a.sums + lists);
-  launch_slices<32>(a, rows, st);
+  e == 8 ? launch_slices<8>(a, rows, st) : launch_slices<32>(a, rows, st);
   hipLaunchKernelGGL(k_select_beams, dim3((unsigned)requests), dim3(kSelThreads), 0, st, a);
   const hipError_t err = hipGetLastError();
   const int rc = scratch_free(work, st);

@@ -7,6 +7,7 @@
 // Key j of sequence b lies in page tables[b][j / page], row j % page.  Offsets are 64-bit; page
 // ids, lengths and slots come from device memory, so every one is checked against its bounds
 // where it is used, and what lies outside counts as absent.
+#include "bf16x3.hpp"
 #include "common.hpp"
 
 #include <algorithm>
@@ -242,7 +243,12 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs a, int type, unsigned
 
 constexpr int kTile = 64;       // keys of a work unit
 constexpr int kStrip = 16;      // keys that one wave multiplies at a time
-constexpr int kSplitWaves = 4, kWholeWaves = 8;
+constexpr int kWaves = 4;       // of an attention workgroup
+// Workgroups of the split form: two a CU are all resident at once, and fewer parts are left to join than
+// with more (3 x 100001 float16 keys: 39 us with 512, 37 with 768, 45 with 1024, 69 with 256; 96 ragged
+// sequences in bfloat16, 32 on 8 heads of 128: 236 us with 512, 250 with 768, 233 with 1024).
+constexpr int kGroups = 512;
+constexpr int64_t kWholeBytes = 192 << 10;
 
 struct AttnArgs {
   const float* q;
@@ -255,6 +261,7 @@ struct AttnArgs {
   float* out;
   int64_t ldo;
   float* part;                  // [2 groups][heads of a tile][d + 2]: o, m, l
+  int2* pairs;                  // [batch][kv heads][head tiles]
   int64_t pages, blocks;
   int batch, page, heads, kv_heads, group, gtiles, htile, d, groups;
   float scale;                  // times log2(e)
@@ -264,6 +271,12 @@ struct AttnArgs {
 struct Span {
   int lo, hi, tiles;
 };
+
+// A value that the whole wave holds alike, moved to the scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)(uint32_t)uniform((int)v) | (int64_t)uniform((int)(v >> 32)) << 32;
+}
 
 __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
   Span s{0, 0, 0};
@@ -275,50 +288,67 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
   return s;
 }
 
-// Units of all sequences, and the sequence that unit-of-one-head `at` (in [0, total)) falls in: *b,
-// and *before, the units of the sequences ahead of it.  Every wave finds them by itself; a lane
-// sums four sequences.  With at < 0: the units ahead of sequence *b.
-__device__ __forceinline__ int64_t find_units(const AttnArgs& a, int64_t at, int* b, int64_t* before) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  bool found = false;
-  const int want = *b;
-  for (int c = 0; c < a.batch; c += 256) {
-    int t[4];
-    int64_t mine = 0;
+__device__ __forceinline__ Span uniform_span(const AttnArgs& a, int b) {
+  const Span s = span_of(a, b);
+  return Span{uniform(s.lo), uniform(s.hi), uniform(s.tiles)};
+}
+
+// A workgroup's share of the units: [at, end) of them, the first in sequence b, `before` units of
+// one head ahead of that sequence.  n workgroups have a share.
+struct Share {
+  int64_t units, at, end, before;
+  int n, b;
+};
+
+// Every wave finds its workgroup's share by itself; a lane sums four sequences.
+__device__ __forceinline__ Share share_of(const AttnArgs& a, int w) {
+  const int lane = threadIdx.x & 63, per = a.kv_heads * a.gtiles;
+  Share s{};
+  int t[4];
+  int64_t up = 0, mine = 0, base = 0, total = 0;
+  auto scan = [&](int c) {
+    mine = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       t[i] = span_of(a, c + lane * 4 + i).tiles;
       mine += t[i];
     }
-    int64_t up = mine;
+    up = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int64_t u = __shfl_up(up, o, kWave);
       if (lane >= o) up += u;
     }
-    int64_t ahead = total + up - mine;
-    if (!found) {
-      int in = -1;
-      int64_t first = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int n = c + lane * 4 + i;
-        const bool here = at >= 0 ? at >= ahead && at < ahead + t[i] : n == want;
-        if (here) in = n, first = ahead;
-        ahead += t[i];
-      }
-      const uint64_t hit = __ballot(in >= 0);
-      if (hit) {
-        const int from = __ffsll((unsigned long long)hit) - 1;
-        *b = __builtin_amdgcn_readfirstlane(__shfl(in, from, kWave));
-        *before = __shfl(first, from, kWave);
-        found = true;
-      }
-    }
-    total += __shfl(up, 63, kWave);
+  };
+  for (int c = 0; c < a.batch; c += 256) {
+    scan(c);
+    total += uniform(__shfl(up, 63, kWave));
   }
-  return total;
+  s.units = total * per;
+  s.n = (int)min((int64_t)a.groups, s.units);
+  if (w >= s.n) return s;
+  s.at = s.units * w / s.n;
+  s.end = s.units * (w + 1) / s.n;
+  const int64_t want = s.at / per;
+  for (int c = 0; c < a.batch; c += 256) {
+    if (a.batch > 256) scan(c);
+    int64_t ahead = base + up - mine, first = 0;
+    int in = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (want >= ahead && want < ahead + t[i]) in = c + lane * 4 + i, first = ahead;
+      ahead += t[i];
+    }
+    const uint64_t hit = __ballot(in >= 0);
+    if (hit) {
+      const int from = __ffsll((unsigned long long)hit) - 1;
+      s.b = uniform(__shfl(in, from, kWave));
+      s.before = uniform(__shfl(first, from, kWave));
+      break;
+    }
+    base += uniform(__shfl(up, 63, kWave));
+  }
+  return s;
 }
 
 template <typename E>
@@ -360,126 +390,155 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // 2^(x - top), 0 where x is -inf whatever top is
 __device__ __forceinline__ float weight_of(float x, float top) { return x == -INFINITY ? 0.f : exp2_fast(x - top); }
 
-// Attention of up to 16 query heads that share kv head `kvh` over strips [s0, s1) of sequence b.
-//
-// Both products run on the float32 matrix cores, whatever the cache's type: 16x16x4 products take
-// 1024 cycles a strip of 16 keys at d = 64, room for 19 TB/s of float32 cache, so the kernel is
-// bound by HBM for one query head a kv head as for sixteen.  Scores are formed as K . q^T, so that
-// lane (g, m) = (lane / 16, lane % 16) holds those of keys 4g .. 4g + 3 and head m.  That is also
-// where V^T . P^T wants its second operand: step i takes keys {i, 4 + i, 8 + i, 12 + i}, lane (g, m)
-// its own p[i].  Nothing goes through LDS before the waves are joined.  K is loaded in the first
-// operand's layout with the sum over channels permuted so that a lane's share is 16 contiguous
-// bytes, V with the output channels permuted alike (d = 64 jj + 4 m + c in tile (jj, c)).
-//
-// The running maximum is kept for a whole wave's strips and moved only when a score passes it by
-// more than 2^8: p stays below 2^8 and the sums in float32 lose nothing.
-template <typename E, int NJ, bool FULL, int NW>
-__device__ void attend(const AttnArgs& a, int b, int kvh, int gt, const Span& sp, int s0, int s1, float* s_o,
-                       float* s_ml) {
-  constexpr int KC = 16 / sizeof(E);              // channels of a lane's 16 bytes
-  constexpr int NK = 64 * NJ / (4 * KC);          // such loads a key row
+// What one wave has of up to 16 query heads: lane (g, m) = (lane / 16, lane % 16) holds head m's
+// channels d = 64 jj + 16 g + 4 r + c in o[jj][c][r], its running maximum, and its keys' part of the sum.
+template <int NJ>
+struct Wave {
+  f32x4 o[NJ][4];
+  float top, sum;
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    top = -INFINITY;
+    sum = 0.f;
+  }
+};
+
+// The keys that one workgroup looks at for one kv head: strips [.., s1) of 16.
+template <typename E, int NJ, bool FULL>
+struct Keys {
   typedef typename Elem<E>::VRaw VRaw;
-  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-  const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int d = FULL ? 64 * NJ : a.d;
-  const int hg = min(a.htile, a.group - gt * a.htile);   // heads of this tile
-  const int head = kvh * a.group + gt * a.htile + m;
+  static constexpr int KC = 16 / sizeof(E);        // channels of a lane's 16 bytes
+  static constexpr int NK = 64 * NJ / (4 * KC);    // such loads a key row
+  const int32_t* table;
+  const E* k;
+  const E* v;
+  int64_t stride;
+  uint32_t pages, page;
+  int d, lo, hi, s1, m, g;
 
-  float qf[NK * KC];
-#pragma unroll
-  for (int j = 0; j < NK; ++j)
-#pragma unroll
-    for (int e = 0; e < KC; e += 4) {
-      const int c = 4 * KC * j + KC * g + e;
-      f32x4u x{};
-      if (m < hg && (FULL || c < d)) x = *(const f32x4u*)(a.q + (int64_t)b * a.ldq + (int64_t)head * d + c);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) qf[j * KC + e + i] = x.v[i] * a.scale;
-    }
-
-  const int32_t* table = a.tables + (int64_t)b * a.blocks;
-  const E* kb = (const E*)a.k + (int64_t)kvh * a.page * d;
-  const E* vb = (const E*)a.v + (int64_t)kvh * a.page * d;
-  const int64_t stride = (int64_t)a.kv_heads * a.page;
-
+  __device__ __forceinline__ Keys(const AttnArgs& a, int b, int kvh, const Span& sp, int end) {
+    const int lane = threadIdx.x & 63;
+    m = lane & 15, g = lane >> 4;
+    d = FULL ? 64 * NJ : a.d;
+    table = a.tables + (int64_t)b * a.blocks;
+    k = (const E*)a.k + (int64_t)kvh * a.page * d;
+    v = (const E*)a.v + (int64_t)kvh * a.page * d;
+    stride = (int64_t)a.kv_heads * a.page;
+    pages = (uint32_t)a.pages, page = (uint32_t)a.page;
+    lo = sp.lo, hi = sp.hi, s1 = end;
+  }
   // Offset of key 16 s + m in the cache, -1 where there is none to see.
-  auto locate = [&](int s) -> int64_t {
+  __device__ __forceinline__ int64_t locate(int s) const {
     const int key = s * kStrip + m;
-    if (s >= s1 || key < sp.lo || key >= sp.hi) return -1;
-    const int blk = (uint32_t)key / (uint32_t)a.page;
+    if (s >= s1 || key < lo || key >= hi) return -1;
+    const uint32_t blk = (uint32_t)key / page;
     const int32_t id = table[blk];
-    if ((uint32_t)id >= (uint64_t)a.pages) return -1;
-    return ((int64_t)id * stride + (key - blk * a.page)) * d;
-  };
-  uint4 kr[NK];
-  VRaw vr[4][NJ];
-  auto load_k = [&](int64_t off) {
-    const E* p = kb + max(off, (int64_t)0) + KC * g;      // a key that is not there reads the first page's
+    if ((uint32_t)id >= pages) return -1;
+    return ((int64_t)id * stride + ((uint32_t)key - blk * page)) * d;
+  }
+  // Key row m, the lane's 16 bytes of each 64 (a key that is not there reads the first page's row).
+  __device__ __forceinline__ void load_k(int64_t off, uint4 (&r)[NK]) const {
+    const E* p = k + max(off, (int64_t)0) + KC * g;
 #pragma unroll
-    for (int j = 0; j < NK; ++j)
-      kr[j] = FULL || 4 * KC * j + KC * g < d ? *(const uint4*)(p + 4 * KC * j) : uint4{};
-  };
-  int64_t ov[4];
-  auto load_v = [&](int64_t off) {
+    for (int j = 0; j < NK; ++j) r[j] = FULL || 4 * KC * j + KC * g < d ? *(const uint4*)(p + 4 * KC * j) : uint4{};
+  }
+  // Rows of keys 4g .. 4g + 3, channels 64 jj + 4 m ..; ov: their offsets.
+  __device__ __forceinline__ void load_v(int64_t off, VRaw (&r)[4][NJ], int64_t (&ov)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       ov[i] = __shfl(off, 4 * g + i, kWave);
-      const E* p = vb + max(ov[i], (int64_t)0) + 4 * m;
+      const E* p = v + max(ov[i], (int64_t)0) + 4 * m;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) vr[i][j] = FULL || 64 * j + 4 * m < d ? *(const VRaw*)(p + 64 * j) : VRaw{};
+      for (int j = 0; j < NJ; ++j) r[i][j] = FULL || 64 * j + 4 * m < d ? *(const VRaw*)(p + 64 * j) : VRaw{};
     }
-  };
+  }
+};
 
-  f32x4 o[NJ][4];
+// The query's channels from c on, times scale * log2(e); zeros past the head's and for heads that are not there.
+template <int N, bool FULL>
+__device__ __forceinline__ void load_q(const AttnArgs& a, const float* q, bool on, int c, int d, float* f) {
 #pragma unroll
-  for (int j = 0; j < NJ; ++j)
+  for (int e = 0; e < N; e += 4) {
+    f32x4u x{};
+    if (on && (FULL || c + e < d)) x = *(const f32x4u*)(q + c + e);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float top = -INFINITY, sum = 0.f;
+    for (int i = 0; i < 4; ++i) f[e + i] = x.v[i] * a.scale;
+  }
+}
 
-  int s = s0 + wv;
-  int64_t off = locate(s), next = locate(s + NW);
-  load_k(off);
-  load_v(off);
-  for (; s < s1; s += NW) {
+// The running maximum moves only when a score passes it by more than 2^8: weights stay below 2^8 and
+// float32 sums lose nothing by it.  Returns the factor for what has been summed (1: nothing moved).
+__device__ __forceinline__ float raise(float mx, float& top) {
+  if (!__any(!(mx <= top + 8.f) && mx != -INFINITY)) return 1.f;     // NaN scores too: they reach the output
+  float t = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+  t = fmaxf(fmaxf(t, __shfl_xor(t, 32, kWave)), top);
+  const float f = weight_of(top, t);
+  top = t;
+  return f;
+}
+
+// Strips s, s + NW, .. on the float32 matrix cores, whatever the cache's type: 16x16x4 products take
+// 1024 cycles a strip at d = 64, room for 19 TB/s of float32 cache, so HBM bounds it for one query
+// head a kv head as for sixteen.  Scores are formed as K . q^T, so that lane (g, m) holds those of keys
+// 4g .. 4g + 3 and head m.  That is also where V^T . P^T wants its second operand: step i takes keys
+// {i, 4 + i, 8 + i, 12 + i}, lane (g, m) its own p[i].  Nothing goes through LDS or across lanes.  K is
+// loaded in the first operand's layout with the sum over channels permuted so that a lane's share
+// is 16 contiguous bytes, V with the output channels permuted alike (64 jj + 4 m + c in tile (jj, c)).
+template <typename E, int NJ, bool FULL, int NW>
+__device__ __forceinline__ void strips_f32(const AttnArgs& a, const Keys<E, NJ, FULL>& keys, const float* q, bool on,
+                                           int s, Wave<NJ>& w) {
+  typedef Keys<E, NJ, FULL> K;
+  float qf[K::NK * K::KC];
+#pragma unroll
+  for (int j = 0; j < K::NK; ++j)
+    load_q<K::KC, FULL>(a, q, on, 4 * K::KC * j + K::KC * keys.g, keys.d, qf + j * K::KC);
+  uint4 kr[K::NK];
+  typename K::VRaw vr[4][NJ];
+  int64_t ov[4];
+  w.clear();
+  int64_t off = keys.locate(s), next = keys.locate(s + NW);
+  keys.load_k(off, kr);
+  keys.load_v(off, vr, ov);
+  for (; s < keys.s1; s += NW) {
     // scores of this strip; then its K registers take the next one's rows
-    f32x4 sc{0.f, 0.f, 0.f, 0.f};
+    f32x4 sc{0.f, 0.f, 0.f, 0.f}, sc1{0.f, 0.f, 0.f, 0.f};     // two chains: shorter, and the rounding less
 #pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      float kf[KC];
+    for (int j = 0; j < K::NK; ++j) {
+      float kf[K::KC];
       Elem<E>::wide(kr[j], kf);
 #pragma unroll
-      for (int e = 0; e < KC; ++e) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[j * KC + e], sc, 0, 0, 0);
+      for (int e = 0; e < K::KC; e += 2) {
+        sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[j * K::KC + e], sc, 0, 0, 0);
+        sc1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e + 1], qf[j * K::KC + e + 1], sc1, 0, 0, 0);
+      }
     }
-    load_k(next);
-    const int64_t after = locate(s + 2 * NW);
-
+    sc += sc1;
+    keys.load_k(next, kr);
+    const int64_t after = keys.locate(s + 2 * NW);
     // masked keys: score -inf, and V zeroed (a NaN there would survive a zero weight)
     const bool all = __all(off >= 0);
     if (!all) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) sc[i] = ov[i] >= 0 ? sc[i] : -INFINITY;
     }
-    const float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-    if (__any(!(mx <= top + 8.f) && mx != -INFINITY)) {     // NaN scores too: they reach the output
-      float t = mx;
-      t = fmaxf(t, __shfl_xor(t, 16, kWave));
-      t = fmaxf(t, __shfl_xor(t, 32, kWave));
-      t = fmaxf(t, top);
-      const float f = weight_of(top, t);
-      sum *= f;
-      top = t;
+    const float f = raise(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), w.top);
+    if (__any(f != 1.f)) {
+      w.sum *= f;
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[j][c] *= f;
+        for (int c = 0; c < 4; ++c) w.o[j][c] *= f;
     }
-    const float ref = top == -INFINITY ? 0.f : top;
+    const float ref = w.top == -INFINITY ? 0.f : w.top;
     float p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       p[i] = exp2_fast(sc[i] - ref);
-      sum += p[i];
+      w.sum += p[i];
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -490,27 +549,241 @@ __device__ void attend(const AttnArgs& a, int b, int kvh, int gt, const Span& sp
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const float x = all || ov[i] >= 0 ? vf[c] : 0.f;
-          o[j][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, p[i], o[j][c], 0, 0, 0);
+          w.o[j][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, p[i], w.o[j][c], 0, 0, 0);
         }
       }
-    load_v(next);
+    keys.load_v(next, vr, ov);
     off = next;
     next = after;
   }
+}
+
+// Two-byte keys and values are whole operands of the two-byte matrix products, which run at sixteen
+// times the float32 rate; only the queries and the weights, float32, are split into planes.
+template <typename E>
+struct Planes;
+template <>
+struct Planes<__bf16> {      // three planes carry all 24 bits
+  static constexpr int N = 3;
+  static __device__ __forceinline__ void split(const float* x, uint4* p) {
+    split_x3(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), p[0], p[1], p[2]);
+  }
+  static __device__ __forceinline__ f32x4 mul(const uint4& a, const uint4& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  }
+};
+template <>
+struct Planes<_Float16> {    // two planes of 11 bits, the second 2^11 times what the first leaves: within 2^-22
+  static constexpr int N = 2;
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ void split(const float* x, uint4* p) {
+    h8 a, b;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = (_Float16)x[i];
+      b[i] = (_Float16)((x[i] - (float)a[i]) * 2048.f);
+    }
+    p[0] = __builtin_bit_cast(uint4, a);
+    p[1] = __builtin_bit_cast(uint4, b);
+  }
+  static __device__ __forceinline__ f32x4 mul(const uint4& a, const uint4& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  }
+};
+
+// The same strips two at a time (s and s + NW) on the two-byte matrix cores.  Scores: 16 keys by 32
+// channels by 16 heads a product, K straight from memory.  V^T . P^T sums over both strips' 32 keys in
+// one product, keys 4g .. 4g + 3 of each in lane group g: the weights' planes again stay in their
+// lanes, and V's four rows a lane are turned into channels by eight byte permutations a 4 x 4 block.
+// float16 weights are held 2^7 up and queries scaled to one by their head's largest, so that both
+// planes stay in float16's range.  False where the outputs are not finite (an infinity or a NaN
+// among what is seen, whose planes are not its own): the caller forms them in float32.
+template <typename E, int NJ, bool FULL, int NW>
+__device__ __forceinline__ bool strips_16(const AttnArgs& a, const Keys<E, NJ, FULL>& keys, const float* q, bool on,
+                                          int s, Wave<NJ>& w) {
+  typedef Keys<E, NJ, FULL> K;
+  typedef Planes<E> P;
+  constexpr bool kHalf = P::N == 2;
+  constexpr float kUp = kHalf ? 7.f : 0.f;
+  uint4 qp[P::N][K::NK];
+  float unit = 1.f;            // float16: 2^E of this head's largest |q|
+  {
+    float qf[K::NK][8];
+    float big = 0.f;
+#pragma unroll
+    for (int j = 0; j < K::NK; ++j) {
+      load_q<8, FULL>(a, q, on, 32 * j + 8 * keys.g, keys.d, qf[j]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(qf[j][e]));
+    }
+    if constexpr (kHalf) {
+      big = fmaxf(big, __shfl_xor(big, 16, kWave));
+      big = fmaxf(big, __shfl_xor(big, 32, kWave));
+      const int e2 = big > 0.f && big < INFINITY ? max(min(__builtin_amdgcn_frexp_expf(big), 126), -126) : 0;
+      unit = ldexpf(1.f, e2);
+      const float down = ldexpf(1.f, -e2);
+#pragma unroll
+      for (int j = 0; j < K::NK; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qf[j][e] *= down;
+    }
+#pragma unroll
+    for (int j = 0; j < K::NK; ++j) {
+      uint4 t[P::N];
+      P::split(qf[j], t);
+#pragma unroll
+      for (int n = 0; n < P::N; ++n) qp[n][j] = t[n];
+    }
+  }
+  uint4 kr[2][K::NK];
+  typename K::VRaw vr[2][4][NJ];
+  int64_t ov[2][4], off[2], next[2], after[2];
+  f32x4 low[NJ][4];            // float16: the second plane's sums, 2^11 up
+  w.clear();
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) low[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    off[t] = keys.locate(s + t * NW);
+    next[t] = keys.locate(s + (2 + t) * NW);
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    keys.load_k(off[t], kr[t]);
+    keys.load_v(off[t], vr[t], ov[t]);
+  }
+  for (; s < keys.s1; s += 2 * NW) {
+    f32x4 sc[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x4 big{0.f, 0.f, 0.f, 0.f}, small{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < K::NK; ++j) {
+        big = P::mul(kr[t][j], qp[0][j], big);
+        small = P::mul(kr[t][j], qp[1][j], small);
+        if constexpr (P::N == 3) small = P::mul(kr[t][j], qp[2][j], small);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sc[t][i] = kHalf ? fmaf(small[i], 0x1p-11f, big[i]) * unit : big[i] + small[i];
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      keys.load_k(next[t], kr[t]);
+      after[t] = keys.locate(s + (4 + t) * NW);
+    }
+    const bool all = __all(off[0] >= 0 && off[1] >= 0);
+    if (!all) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool there = ov[t][i] >= 0;
+          sc[t][i] = there ? sc[t][i] : -INFINITY;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) vr[t][i][j] = there ? vr[t][i][j] : typename K::VRaw{};
+        }
+    }
+    float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+    mx = fmaxf(mx, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    const float f = raise(mx, w.top);
+    if (__any(f != 1.f)) {
+      w.sum *= f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          w.o[j][c] *= f;
+          if constexpr (kHalf) low[j][c] *= f;
+        }
+    }
+    const float ref = (w.top == -INFINITY ? 0.f : w.top) - kUp;
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = exp2_fast(sc[i / 4][i % 4] - ref);
+      w.sum += p[i];
+    }
+    uint4 pp[P::N];
+    P::split(p, pp);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t x[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[t][i] = c < 2 ? vr[t][i][j].x : vr[t][i][j].y;
+        const uint32_t sel = c % 2 ? 0x07060302u : 0x05040100u;
+        const uint4 av = {__builtin_amdgcn_perm(x[0][1], x[0][0], sel), __builtin_amdgcn_perm(x[0][3], x[0][2], sel),
+                          __builtin_amdgcn_perm(x[1][1], x[1][0], sel), __builtin_amdgcn_perm(x[1][3], x[1][2], sel)};
+        w.o[j][c] = P::mul(av, pp[0], w.o[j][c]);
+        if constexpr (kHalf) {
+          low[j][c] = P::mul(av, pp[1], low[j][c]);
+        } else {
+          w.o[j][c] = P::mul(av, pp[1], w.o[j][c]);
+          w.o[j][c] = P::mul(av, pp[2], w.o[j][c]);
+        }
+      }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      keys.load_v(next[t], vr[t], ov[t]);
+      off[t] = next[t];
+      next[t] = after[t];
+    }
+  }
+  float none = w.sum * 0.f;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if constexpr (kHalf) w.o[j][c] = (low[j][c] * 0x1p-11f + w.o[j][c]) * 0x1p-7f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) none += w.o[j][c][r] * 0.f;
+    }
+  if constexpr (kHalf) w.sum *= 0x1p-7f;
+  return !__any(on && none != 0.f);
+}
+
+// Attention of up to 16 query heads that share kv head `kvh` over strips [s0, s1) of sequence b, by
+// the NW waves of a workgroup, which are then joined through LDS.
+template <typename E, int NJ, bool FULL, int NW>
+__device__ __forceinline__ void attend(const AttnArgs& a, int b, int kvh, int gt, const Span& sp, int s0, int s1,
+                                       float* s_o, float* s_ml) {
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wv = uniform((int)threadIdx.x >> 6);
+  const int d = FULL ? 64 * NJ : a.d;
+  const int hg = min(a.htile, a.group - gt * a.htile);   // heads of this tile
+  const int head = kvh * a.group + gt * a.htile + m;
+  const bool on = m < hg;
+  const float* q = a.q + (int64_t)b * a.ldq + (int64_t)(on ? head : 0) * d;
+  const Keys<E, NJ, FULL> keys(a, b, kvh, sp, s1);
+  Wave<NJ> w;
+  if constexpr (sizeof(E) == 2) {
+    if (!strips_16<E, NJ, FULL, NW>(a, keys, q, on, s0 + wv, w))
+      strips_f32<E, NJ, FULL, NW>(a, keys, q, on, s0 + wv, w);
+  } else {
+    strips_f32<E, NJ, FULL, NW>(a, keys, q, on, s0 + wv, w);
+  }
+  float sum = w.sum;
   sum += __shfl_xor(sum, 16, kWave);
   sum += __shfl_xor(sum, 32, kWave);
 
   // The waves' maxima and sums, then their outputs 64 channels at a time: s_o[wave][head][64 + 4].
   if (g == 0) {
-    s_ml[(wv * 16 + m) * 2] = top;
+    s_ml[(wv * 16 + m) * 2] = w.top;
     s_ml[(wv * 16 + m) * 2 + 1] = sum;
   }
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
-    if (m < hg) {
+    if (on) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float4 x = make_float4(o[j][0][r], o[j][1][r], o[j][2][r], o[j][3][r]);
+        float4 x = make_float4(w.o[j][0][r], w.o[j][1][r], w.o[j][2][r], w.o[j][3][r]);
         *(float4*)(s_o + (wv * 16 + m) * 68 + 16 * g + 4 * r) = x;
       }
     }
@@ -518,13 +791,13 @@ __device__ void attend(const AttnArgs& a, int b, int kvh, int gt, const Span& sp
     for (int h = wv; h < hg; h += NW) {
       float t = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) t = fmaxf(t, s_ml[(w * 16 + h) * 2]);
+      for (int u = 0; u < NW; ++u) t = fmaxf(t, s_ml[(u * 16 + h) * 2]);
       float l = 0.f, x = 0.f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float f = weight_of(s_ml[(w * 16 + h) * 2], t);
-        l += f * s_ml[(w * 16 + h) * 2 + 1];
-        x += f * s_o[(w * 16 + h) * 68 + lane];
+      for (int u = 0; u < NW; ++u) {
+        const float f = weight_of(s_ml[(u * 16 + h) * 2], t);
+        l += f * s_ml[(u * 16 + h) * 2 + 1];
+        x += f * s_o[(u * 16 + h) * 68 + lane];
       }
       const int c = 64 * j + lane;
       const bool whole = s_ml[NW * 32] != 0.f;    // the pair's every key was here: this is the output
@@ -545,105 +818,128 @@ __device__ void attend(const AttnArgs& a, int b, int kvh, int gt, const Span& sp
   }
 }
 
+// Waves a SIMD that the registers are held to: what they need is 16 NJ floats each of output, keys
+// and values, and the query (half as much again as planes).
+template <typename E, int NJ>
+constexpr int waves_per_simd() {
+  return NJ == 1 ? (sizeof(E) == 2 ? 3 : 4) : NJ == 2 ? 2 : 1;
+}
+
 // One workgroup per (sequence, kv head, tile of query heads): one launch, for caches short enough.
+// Eight waves where a key row is short: 6.9 us against 7.6 with four at one sequence of 256 float32 keys
+// (14 on 2 heads of 64); at d = 128 they only crowd the CU (256 bfloat16 keys of 128 sequences, 32 on 8
+// heads: 37 us against 27).
+template <int NJ>
+constexpr int kWholeWaves = NJ == 1 ? 8 : 4;
+
 template <typename E, int NJ, bool FULL>
-__global__ __launch_bounds__(kWholeWaves * 64) void k_paged_whole(AttnArgs a) {
-  __shared__ float s_o[kWholeWaves * 16 * 68];
-  __shared__ float s_ml[kWholeWaves * 32 + 2];
+__global__ __launch_bounds__(kWholeWaves<NJ> * 64, (waves_per_simd<E, NJ>())) void k_paged_whole(AttnArgs a) {
+  constexpr int NW = kWholeWaves<NJ>;
+  __shared__ float s_o[NW * 16 * 68];
+  __shared__ float s_ml[NW * 32 + 2];
   const int per = a.kv_heads * a.gtiles, b = blockIdx.x / per, p = blockIdx.x % per;
-  const Span sp = span_of(a, b);
-  if (threadIdx.x == 0) s_ml[kWholeWaves * 32] = 1.f;
+  const Span sp = uniform_span(a, b);
+  if (threadIdx.x == 0) s_ml[NW * 32] = 1.f;
   __syncthreads();
-  attend<E, NJ, FULL, kWholeWaves>(a, b, p / a.gtiles, p % a.gtiles, sp, sp.lo / kStrip,
-                                   (sp.hi + kStrip - 1) / kStrip, s_o, s_ml);
+  attend<E, NJ, FULL, NW>(a, b, p / a.gtiles, p % a.gtiles, sp, sp.lo / kStrip, (sp.hi + kStrip - 1) / kStrip, s_o,
+                          s_ml);
 }
 
 // The units of all sequences and heads, in order, shared out evenly over `groups` workgroups by the
 // lengths on the device: a ragged batch fills the machine as an even one does, and a captured
-// launch serves every length.  A pair that one workgroup holds whole is written by it; of a pair
-// that crosses workgroups each leaves its maximum, sum and output in `part` (slot 2 w, or 2 w + 1
-// where the pair begins inside w's share), and k_paged_join adds them up.
-__device__ __forceinline__ int groups_for(const AttnArgs& a, int64_t units) {
-  return (int)min((int64_t)a.groups, units);
-}
-
+// launch serves every length.  A pair (sequence, tile of heads) that one workgroup holds whole is
+// written by it; of a pair that crosses workgroups each leaves its maximum, sum and output in `part`
+// (slot 2 w, or 2 w + 1 where the pair begins inside w's share), and k_paged_join adds them up.
+// The workgroup that begins a pair enters it into `pairs`: its first slot and last workgroup, or -1.
 template <typename E, int NJ, bool FULL>
-__global__ __launch_bounds__(kSplitWaves * 64) void k_paged_split(AttnArgs a) {
-  __shared__ float s_o[kSplitWaves * 16 * 68];
-  __shared__ float s_ml[kSplitWaves * 32 + 2];
-  const int per = a.kv_heads * a.gtiles;
-  // total first, then the sequence of this workgroup's first unit
-  int b = 0;
-  int64_t before = 0;
-  const int64_t units = find_units(a, 0, &b, &before) * per;
-  const int n = groups_for(a, units), w = blockIdx.x;
-  if (w >= n) return;
-  int64_t at = units * w / n;
-  const int64_t end = units * (w + 1) / n;
-  find_units(a, at / per, &b, &before);
-  Span sp = span_of(a, b);
-  int64_t in = at - before * per;                 // unit within the sequence: [pair][tile]
-  const int64_t first = at;
-  while (at < end) {
+__global__ __launch_bounds__(kWaves * 64, (waves_per_simd<E, NJ>())) void k_paged_split(AttnArgs a) {
+  __shared__ float s_o[kWaves * 16 * 68];
+  __shared__ float s_ml[kWaves * 32 + 2];
+  const int per = a.kv_heads * a.gtiles, w = blockIdx.x;
+  const Share sh = share_of(a, w);
+  if (w >= sh.n) return;
+  int64_t at = sh.at, in = at - sh.before * per;  // the unit, and the unit within the sequence: [pair][tile]
+  int b = sh.b;
+  Span sp = uniform_span(a, b);
+  while (at < sh.end) {
     while (in >= (int64_t)sp.tiles * per) {
       in -= (int64_t)sp.tiles * per;
       if (++b >= a.batch) return;                 // lengths that changed under the call
-      sp = span_of(a, b);
+      sp = uniform_span(a, b);
     }
-    const int p = (int)(in / sp.tiles), t = (int)(in % sp.tiles);
-    const int take = (int)min((int64_t)(sp.tiles - t), end - at);
+    const int p = (int)(in / sp.tiles), t = (int)(in - (int64_t)p * sp.tiles);
+    const int take = (int)min((int64_t)(sp.tiles - t), sh.end - at), slot = 2 * w + (at == sh.at ? 0 : 1);
+    const bool whole = take == sp.tiles;
     if (threadIdx.x == 0) {
-      s_ml[kSplitWaves * 32] = take == sp.tiles ? 1.f : 0.f;
-      s_ml[kSplitWaves * 32 + 1] = __int_as_float(2 * w + (at == first ? 0 : 1));
+      s_ml[kWaves * 32] = whole ? 1.f : 0.f;
+      s_ml[kWaves * 32 + 1] = __int_as_float(slot);
+      if (t == 0)
+        a.pairs[(int64_t)b * per + p] =
+            make_int2(whole ? -1 : slot, whole ? 0 : (int)(((at + sp.tiles) * sh.n - 1) / sh.units));
     }
     __syncthreads();
     const int t0 = sp.lo / kTile + t, per_tile = kTile / kStrip;
-    attend<E, NJ, FULL, kSplitWaves>(a, b, p / a.gtiles, p % a.gtiles, sp, max(t0 * per_tile, sp.lo / kStrip),
+    attend<E, NJ, FULL, kWaves>(a, b, p / a.gtiles, p % a.gtiles, sp, max(t0 * per_tile, sp.lo / kStrip),
                                      min((t0 + take) * per_tile, (sp.hi + kStrip - 1) / kStrip), s_o, s_ml);
     at += take;
     in += take;
   }
 }
 
-constexpr int kJoinWaves = 8;
+constexpr int kJoinWaves = 4, kJoinAhead = 8;
 
 // One workgroup per (sequence, query head): the parts of a pair that crossed workgroups, and zeros
-// for a sequence with no key to see.  The waves take the parts in turn, then meet in LDS.
+// for a sequence with no key to see.  The waves take the parts in turn, eight at a time so that
+// their loads are in flight together, then meet in LDS.
+template <int NJ>
 __global__ __launch_bounds__(kJoinWaves * 64) void k_paged_join(AttnArgs a) {
-  __shared__ float s_o[kJoinWaves * 256];
+  __shared__ float s_o[kJoinWaves * 64 * NJ];
   __shared__ float s_ml[kJoinWaves * 2];
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int want = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
-  const int per = a.kv_heads * a.gtiles, kvh = head / a.group, gh = head % a.group;
-  const int p = kvh * a.gtiles + gh / a.htile, h = gh % a.htile;
-  int b = want;
-  int64_t before = 0;
-  const int64_t units = find_units(a, -1, &b, &before) * per;
-  const Span sp = span_of(a, b);
+  const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
+  const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kvh = head / a.group, gh = head % a.group;
+  const int h = gh % a.htile;
+  const int2 pair = a.pairs[((int64_t)b * a.kv_heads + kvh) * a.gtiles + gh / a.htile];
   float* out = a.out + (int64_t)b * a.ldo + (int64_t)head * a.d;
-  if (sp.tiles == 0) {
+  if (span_of(a, b).tiles == 0) {
     for (int c = threadIdx.x; c < a.d; c += kJoinWaves * 64) out[c] = 0.f;
     return;
   }
-  const int n = groups_for(a, units);
-  const int64_t t0 = before * per + (int64_t)p * sp.tiles, t1 = t0 + sp.tiles - 1;
-  const int w0 = (int)(((t0 + 1) * n - 1) / units), w1 = (int)(((t1 + 1) * n - 1) / units);
-  if (w0 == w1) return;                         // written by the one workgroup that held it
-  const int first = 2 * w0 + (units * w0 / n == t0 ? 0 : 1);
-  float x[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
-  for (int w = w0 + wv; w <= w1; w += kJoinWaves) {
-    const float* src = a.part + ((int64_t)(w == w0 ? first : 2 * w) * a.htile + h) * (a.d + 2);
-    const float t = fmaxf(top, src[a.d]), f = weight_of(top, t), u = weight_of(src[a.d], t);
-    sum = sum * f + u * src[a.d + 1];
+  if (pair.x < 0) return;                       // written by the one workgroup that held it
+  const int w0 = min(pair.x >> 1, a.groups - 1), count = min(pair.y, a.groups - 1) - w0 + 1;
+  float x[NJ], top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = 64 * j + lane;
-      x[j] = x[j] * f + (c < a.d ? u * src[c] : 0.f);
+  for (int j = 0; j < NJ; ++j) x[j] = 0.f;
+  for (int i = wv; i < count; i += kJoinWaves * kJoinAhead) {
+    float y[kJoinAhead][NJ], t[kJoinAhead], l[kJoinAhead];
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) {
+      const int n = i + u * kJoinWaves;
+      const float* src = a.part + ((int64_t)(n ? 2 * (w0 + min(n, count - 1)) : 2 * w0 + (pair.x & 1)) * a.htile + h) * (a.d + 2);
+      t[u] = n < count ? src[a.d] : -INFINITY;
+      l[u] = src[a.d + 1];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) y[u][j] = 64 * j + lane < a.d ? src[64 * j + lane] : 0.f;
     }
-    top = t;
+    float now = top;
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) now = fmaxf(now, t[u]);
+    const float f = weight_of(top, now);
+    sum *= f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) x[j] *= f;
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) {
+      if (i + u * kJoinWaves < count) {
+        const float g = weight_of(t[u], now);
+        sum += g * l[u];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) x[j] += g * y[u][j];
+      }
+    }
+    top = now;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) s_o[wv * 256 + 64 * j + lane] = x[j];
+  for (int j = 0; j < NJ; ++j) s_o[(wv * NJ + j) * 64 + lane] = x[j];
   if (lane == 0) {
     s_ml[2 * wv] = top;
     s_ml[2 * wv + 1] = sum;
@@ -651,11 +947,13 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_paged_join(AttnArgs a) {
   __syncthreads();
   for (int c = threadIdx.x; c < a.d; c += kJoinWaves * 64) {
     float t = -INFINITY, l = 0.f, y = 0.f;
+#pragma unroll
     for (int w = 0; w < kJoinWaves; ++w) t = fmaxf(t, s_ml[2 * w]);
+#pragma unroll
     for (int w = 0; w < kJoinWaves; ++w) {
       const float f = weight_of(s_ml[2 * w], t);
       l += f * s_ml[2 * w + 1];
-      y += f * s_o[w * 256 + c];
+      y += f * s_o[w * NJ * 64 + c];
     }
     out[c] = l != 0.f ? y / l : 0.f;
   }
@@ -664,11 +962,11 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_paged_join(AttnArgs a) {
 template <typename E, int NJ, bool FULL>
 void launch_attention(const AttnArgs& a, bool whole, hipStream_t st) {
   if (whole) {
-    hipLaunchKernelGGL((k_paged_whole<E, NJ, FULL>), dim3(a.batch * a.kv_heads * a.gtiles), dim3(kWholeWaves * 64), 0,
+    hipLaunchKernelGGL((k_paged_whole<E, NJ, FULL>), dim3(a.batch * a.kv_heads * a.gtiles), dim3(kWholeWaves<NJ> * 64), 0,
                        st, a);
   } else {
-    hipLaunchKernelGGL((k_paged_split<E, NJ, FULL>), dim3(a.groups), dim3(kSplitWaves * 64), 0, st, a);
-    hipLaunchKernelGGL(k_paged_join, dim3(a.batch * a.heads), dim3(kJoinWaves * 64), 0, st, a);
+    hipLaunchKernelGGL((k_paged_split<E, NJ, FULL>), dim3(a.groups), dim3(kWaves * 64), 0, st, a);
+    hipLaunchKernelGGL(k_paged_join<NJ>, dim3(a.batch * a.heads), dim3(kJoinWaves * 64), 0, st, a);
   }
 }
 
@@ -773,17 +1071,22 @@ int cv3_paged_attention(const float* q, int64_t ldq, int64_t batch, int heads, i
   if (batch == 0) return CV3_OK;
   CV3_REQUIRE(q && tables && lengths && out, CV3_EINVAL, "null operand");
   const int group = heads / kv_heads, htile = std::min(group, 16), gtiles = (group + htile - 1) / htile;
-  AttnArgs a{q, ldq, k_cache, v_cache, tables, lengths, starts, out, ldo, nullptr, pages, blocks, (int)batch, (int)page,
+  AttnArgs a{q, ldq, k_cache, v_cache, tables, lengths, starts, out, ldo, nullptr, nullptr, pages, blocks, (int)batch, (int)page,
              heads, kv_heads, group, gtiles, htile, d, 0, scale * 1.4426950408889634f};
   hipStream_t st = stream_of(s);
-  bool whole = blocks * page <= 1024;
+  // One workgroup a pair where a full table's keys and values are few: it takes 5.5 us and 1.3 more each
+  // 64 KB, the split form 9.7 and hardly more (one sequence, 14 on 2 heads of 64: 256 float32 keys 6.9
+  // against 9.6 us, 512 keys 10.7 against 9.6; 512 bfloat16 keys 7.2 against 9.7, 1024 10.6 against 9.7).
+  bool whole = blocks * page * 2 * d * elem_size(cache_type) <= kWholeBytes;
   if (!whole) {
-    a.groups = 1024;
-    void* part = nullptr;
-    const int rc = scratch_alloc(&part, (size_t)2 * a.groups * htile * (d + 2) * sizeof(float), st);
+    a.groups = kGroups;
+    const size_t parts = (size_t)2 * a.groups * htile * (d + 2) * sizeof(float);   // a multiple of 8
+    void* work = nullptr;
+    const int rc = scratch_alloc(&work, parts + (size_t)batch * kv_heads * gtiles * sizeof(int2), st);
     if (rc == CV3_ENOMEM) whole = true;      // one workgroup a pair needs no memory of its own
     else if (rc) return rc;
-    a.part = (float*)part;
+    a.part = (float*)work;
+    a.pairs = (int2*)((char*)work + parts);
   }
   if (cache_type == CV3_F32) attention_for<float>(a, whole, st);
   else if (cache_type == CV3_F16) attention_for<_Float16>(a, whole, st);
