@@ -34,6 +34,19 @@ __device__ __forceinline__ double rank_value(uint64_t r) {
   return __longlong_as_double((int64_t)(r >> 63 ? r & ~((uint64_t)1 << 63) : ~r));
 }
 
+// Sum over the wave by DPP row permutations and four lane reads.
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  return __longlong_as_double((int64_t)dpp64<CTRL>((uint64_t)__double_as_longlong(v)));
+}
+__device__ __forceinline__ double wave_sum_dpp(double v) {
+  v += dpp_d<kDppXor1>(v);
+  v += dpp_d<kDppXor2>(v);
+  v += dpp_d<kDppHalfMirror>(v);
+  v += dpp_d<kDppMirror>(v);
+  return (readlane_d(v, 0) + readlane_d(v, 16)) + (readlane_d(v, 32) + readlane_d(v, 48));
+}
+
 struct SelectArgs {
   const float* logits;
   const float* scores;
@@ -57,11 +70,11 @@ constexpr int kList = 512;     // logits of a slice that may pass its bar by val
 // Of the 64 groups of four threads each has a largest logit.  What is among the slice's best W is no
 // less than the W-th of those: a few more than W logits pass that bar as a rule, and are ranked by
 // counting.  A key is the logit's rank over the complement of its token, so no two are equal and
-// equal logits go by the lower token.  Where more pass than the list holds (many equal logits), or
-// the bar is -inf, the bar is set by whole keys: whatever passes it then lies in W groups, at most
-// 4 W E keys.
+// equal logits go by the lower token.  Where more pass than the list holds (many equal logits), the
+// bar is -inf or some of the slice's tokens are banned, the bar is set by whole keys: whatever passes
+// it then lies in W groups, at most 4 W E keys.
 template <int E>
-__global__ __launch_bounds__(kSelThreads) void k_select_slices(SelectArgs a) {
+__global__ __launch_bounds__(kSelThreads, 6) void k_select_slices(SelectArgs a) {
   constexpr int kMost = 4 * kBeams * E;
   __shared__ uint64_t s_list[kMost > kList ? kMost : kList];
   __shared__ uint64_t s_key[64];
@@ -91,21 +104,13 @@ __global__ __launch_bounds__(kSelThreads) void k_select_slices(SelectArgs a) {
       for (int i = 0; i < 4; ++i) v[e + i] = t + i < hi ? x[t + i] : -INFINITY;
     }
   }
-  const bool bans = a.ban_lo < hi && a.ban_hi > lo;       // of this slice
-  auto banned = [&](int t) { return t >= a.ban_lo && t < a.ban_hi; };
-  float mx = -INFINITY, best = -INFINITY;
+  float mx = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; e += 4) {
     four[e / 4] = fmaxf(fmaxf(v[e], v[e + 1]), fmaxf(v[e + 2], v[e + 3]));
     mx = fmaxf(mx, four[e / 4]);
   }
-  best = mx;
-  if (bans) {
-    best = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (!banned(first + e / 4 * 4 * kSelThreads + e % 4)) best = fmaxf(best, v[e]);
-  }
+  float best = mx;
   best = fmaxf(best, __uint_as_float(dpp32<kDppXor1>(__float_as_uint(best))));
   best = fmaxf(best, __uint_as_float(dpp32<kDppXor2>(__float_as_uint(best))));
   if ((lane & 3) == 0) s_group[tid >> 2] = best;
@@ -122,19 +127,18 @@ __global__ __launch_bounds__(kSelThreads) void k_select_slices(SelectArgs a) {
   for (int i = 0; i < 64; ++i)
     above += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), i)) > mine ? 1 : 0;
   const float bar = -wave_max_dpp(above < a.beams ? -mine : -INFINITY);
-  const bool open = bar == -INFINITY;
-  if (!open) {
+  const bool whole_keys = bar == -INFINITY || (a.ban_lo < hi && a.ban_hi > lo);
+  if (!whole_keys) {
 #pragma unroll
     for (int e = 0; e < E; e += 4)
       if (four[e / 4] >= bar) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = first + e * kSelThreads + i;
-          if (v[e + i] >= bar && !(bans && banned(t))) {
+        for (int i = 0; i < 4; ++i)
+          if (v[e + i] >= bar) {
             const int n = atomicAdd(&s_count, 1);
-            if (n < kList) s_list[n] = (uint64_t)rank_bits(v[e + i]) << 32 | (uint32_t)~(uint32_t)t;
+            const uint32_t t = (uint32_t)(first + e * kSelThreads + i);
+            if (n < kList) s_list[n] = (uint64_t)rank_bits(v[e + i]) << 32 | ~t;
           }
-        }
       }
   }
   // Sums of four in float32, then float64: a NaN, or +inf - +inf, makes the row's sum NaN.
@@ -147,18 +151,19 @@ __global__ __launch_bounds__(kSelThreads) void k_select_slices(SelectArgs a) {
     for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f((v[e + i] - ref) * kLog2E);
     sum += (double)s;
   }
-  sum = wave_sum_d(sum);
+  sum = wave_sum_dpp(sum);
   if (lane == 0) s_sum[wv] = sum;
   __syncthreads();
   int n = s_count;
-  if (open || n > kList) {
-    auto key_of = [&](int e) -> uint64_t {
-      const int t = first + e / 4 * 4 * kSelThreads + e % 4;
-      return t < hi && !(bans && banned(t)) ? (uint64_t)rank_bits(v[e]) << 32 | (uint32_t)~(uint32_t)t : 0;
+  if (whole_keys || n > kList) {
+    // rolled loops over the logits again, from L2: this is rare, and the code small
+    auto key_at = [&](int e) -> uint64_t {
+      const int t = first + (e >> 2) * 4 * kSelThreads + (e & 3);
+      return t < hi && !(t >= a.ban_lo && t < a.ban_hi) ? (uint64_t)rank_bits(x[t]) << 32 | ~(uint32_t)t : 0;
     };
     uint64_t k = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) k = max(k, key_of(e));
+#pragma unroll 1
+    for (int e = 0; e < E; ++e) k = max(k, key_at(e));
     k = max(k, dpp64<kDppXor1>(k));
     k = max(k, dpp64<kDppXor2>(k));
     if ((lane & 3) == 0) s_key[tid >> 2] = k;
@@ -166,12 +171,13 @@ __global__ __launch_bounds__(kSelThreads) void k_select_slices(SelectArgs a) {
     if (tid == 0) s_count = 0;
     const uint64_t own = s_key[lane];
     int over = 0;
+#pragma unroll 1
     for (int i = 0; i < 64; ++i) over += readlane64(own, i) > own ? 1 : 0;
     const uint64_t least = max(wave_max_u64(over >= a.beams - 1 ? own : 0), (uint64_t)1);
     __syncthreads();
-#pragma unroll
+#pragma unroll 1
     for (int e = 0; e < E; ++e) {
-      const uint64_t u = key_of(e);
+      const uint64_t u = key_at(e);
       if (u >= least) s_list[atomicAdd(&s_count, 1)] = u;
     }
     __syncthreads();
@@ -182,6 +188,7 @@ __global__ __launch_bounds__(kSelThreads) void k_select_slices(SelectArgs a) {
   for (int i = tid; i < n; i += kSelThreads) {
     const uint64_t k = s_list[i];
     int r = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) r += s_list[j] > k ? 1 : 0;
     if (r < a.beams) out[r] = k;
   }
@@ -197,37 +204,39 @@ struct Pick {            // larger is better: the value, then the lower beam, th
   __device__ bool operator>(const Pick& o) const { return hi != o.hi ? hi > o.hi : lo > o.lo; }
 };
 
+constexpr int kPickThreads = 512;
 constexpr int kLists = kBeams * 64;            // of a request: its beams' slices
-constexpr int kListsEach = kLists / kSelThreads;
+constexpr int kListsEach = kLists / kPickThreads;
+constexpr int kPicks = kBeams * kListsEach * kBeams;
+constexpr int kAhead = 4;                     // keys of a list that are loaded together
 
 // One workgroup per request; bound by the chain of its few loads.  The slices' lists are sorted, so
-// the best of a thread's lists are their heads; the W-th best of the threads' bounds what can be
-// chosen, and at most W lists a thread x W threads x W keys pass.
-__global__ __launch_bounds__(kSelThreads) void k_select_beams(SelectArgs a) {
+// the best of a thread's lists are their heads.  As above, the W-th largest value of 64 groups of
+// threads is a bar that a few more than W pass; where equal values bring more than the list holds, the
+// W-th best head of the threads, whole, bounds them by W lists a thread x W threads x W keys.
+__global__ __launch_bounds__(kPickThreads) void k_select_beams(SelectArgs a) {
   __shared__ double s_lse[kBeams], s_score[kBeams];
   __shared__ int s_done[kBeams];
   __shared__ double s_sum[kLists];
   __shared__ float s_top[kLists];
-  __shared__ Pick s_best[kSelThreads];
-  __shared__ Pick s_list[kBeams * kListsEach * kBeams];
+  __shared__ Pick s_best[kPickThreads];
+  __shared__ Pick s_list[kPicks];
   __shared__ Pick s_out[kBeams];
   __shared__ Pick s_bar;
+  __shared__ uint32_t s_high[kPickThreads];
   __shared__ int s_count;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int64_t row0 = (int64_t)blockIdx.x * a.beams;
   const int lists = a.beams * a.slices;
   // An ended beam's lists hold whatever the memory held: they are not looked at.
   const int64_t list0 = row0 * a.slices;
-  uint64_t head[kListsEach];
+  uint64_t mine[kAhead];                       // the first keys of this thread's first list
 #pragma unroll
-  for (int i = 0; i < kListsEach; ++i) {
-    const int l = tid + i * kSelThreads;
-    head[i] = 0;
-    if (l < lists) {
-      head[i] = a.keys[(list0 + l) * a.beams];
-      s_sum[l] = a.sums[list0 + l];
-      s_top[l] = a.tops[list0 + l];
-    }
+  for (int i = 0; i < kAhead; ++i) mine[i] = tid < lists && i < a.beams ? a.keys[(list0 + tid) * a.beams + i] : 0;
+#pragma unroll 1
+  for (int l = tid; l < lists; l += kPickThreads) {
+    s_sum[l] = a.sums[list0 + l];
+    s_top[l] = a.tops[list0 + l];
   }
   if (tid < a.beams) {
     s_score[tid] = (double)a.scores[row0 + tid];
@@ -239,67 +248,93 @@ __global__ __launch_bounds__(kSelThreads) void k_select_beams(SelectArgs a) {
     s_bar = Pick{0, 1};
   }
   __syncthreads();
-  for (int b = wv; b < a.beams; b += kSelThreads / 64) {
+  for (int b = wv; b < a.beams; b += kPickThreads / 64) {
     // at most 64 slices: a lane each
     const float top = lane < a.slices ? s_top[b * a.slices + lane] : -INFINITY;
     const float all = wave_max_dpp(top);
     double sum = lane < a.slices ? s_sum[b * a.slices + lane] : 0.0;
     if (top != all) sum *= exp((double)top - (double)all);     // 0 or NaN where the slice is -inf
-    sum = wave_sum_d(sum);
+    sum = wave_sum_dpp(sum);
     if (lane == 0) s_lse[b] = all > -INFINITY ? (double)all + log(sum) : (double)NAN;
   }
   __syncthreads();
-  auto pick = [&](int list, int rank, uint64_t k) -> Pick {
-    const int b = list / a.slices;
+  // The candidate of beam b that key k, of that rank in one of its lists, stands for.
+  auto pick = [&](int b, bool leads, uint64_t k) -> Pick {
     const uint64_t order = (uint64_t)(31 - b) << 59;
-    if (s_done[b]) return rank || list % a.slices ? Pick{0, 0} : Pick{rank_bits(s_score[b]), order};
+    if (s_done[b]) return leads ? Pick{rank_bits(s_score[b]), order} : Pick{0, 0};
     if (!k) return Pick{0, 0};
     const double value = s_score[b] + ((double)rank_value((uint32_t)(k >> 32)) - s_lse[b]);
     return Pick{rank_bits(value), order | (k >> 32) << 27 | (k & 0x7ffffff)};
   };
   Pick best{0, 0};
-#pragma unroll
-  for (int i = 0; i < kListsEach; ++i) {
-    const int l = tid + i * kSelThreads;
-    if (l < lists) {
-      const Pick p = pick(l, 0, head[i]);
-      if (p > best) best = p;
-    }
+#pragma unroll 1
+  for (int l = tid; l < lists; l += kPickThreads) {
+    const int b = l / a.slices;
+    const Pick p = pick(b, l == b * a.slices, l == tid ? mine[0] : a.keys[(list0 + l) * a.beams]);
+    if (p > best) best = p;
   }
   s_best[tid] = best;
+  s_high[tid] = (uint32_t)(best.hi >> 32);     // the upper half of a value's rank is enough for the bar
   __syncthreads();
-  // every thread counts for one head; the bar is the one with W - 1 above it (none: take everything)
-  const int heads = min(lists, kSelThreads);
+  uint32_t group = 0;                          // of threads 64 apart: one beam's lists are neighbours
+#pragma unroll
+  for (int i = 0; i < kPickThreads; i += 64) group = max(group, s_high[i + lane]);
   int above = 0;
-#pragma unroll 8
-  for (int i = 0; i < heads; ++i) above += s_best[i] > best ? 1 : 0;
-  if (tid < heads && above == a.beams - 1 && best.hi) s_bar = best;
-  __syncthreads();
-  const Pick bar = s_bar;
-  if (!(bar > best)) {
 #pragma unroll
-    for (int i = 0; i < kListsEach; ++i) {
-      const int l = tid + i * kSelThreads;
-      if (l >= lists) continue;
-      const Pick p0 = pick(l, 0, head[i]);
-      if (!p0.hi || bar > p0) continue;
-      s_list[atomicAdd(&s_count, 1)] = p0;
-      if (s_done[l / a.slices]) continue;
-      uint64_t k[kBeams];                      // the rest of the list, its loads in flight together
+  for (int i = 0; i < 64; ++i) above += (uint32_t)__builtin_amdgcn_readlane((int)group, i) > group ? 1 : 0;
+  // the least that fewer than W surpass; 0 (there are fewer heads): everything
+  uint32_t least = above < a.beams ? ~group : 0;
+  least = max(least, dpp32<kDppXor1>(least));
+  least = max(least, dpp32<kDppXor2>(least));
+  least = max(least, dpp32<kDppHalfMirror>(least));
+  least = max(least, dpp32<kDppMirror>(least));
+  least = ~max(max((uint32_t)__builtin_amdgcn_readlane((int)least, 0), (uint32_t)__builtin_amdgcn_readlane((int)least, 16)),
+               max((uint32_t)__builtin_amdgcn_readlane((int)least, 32), (uint32_t)__builtin_amdgcn_readlane((int)least, 48)));
+  Pick bar{(uint64_t)least << 32, 0};
+#pragma unroll 1
+  for (bool whole = false;; whole = true) {
+    // Lists whose head passes the bar enter what of them does.
+#pragma unroll 1
+    for (int l = tid; l < lists && !(bar > best); l += kPickThreads) {
+      const int b = l / a.slices;
+      uint64_t k[kAhead];
+      bool more = true;
+#pragma unroll 1
+      for (int r0 = 0; more && r0 < a.beams; r0 += kAhead) {
 #pragma unroll
-      for (int r = 1; r < kBeams; ++r) k[r] = r < a.beams ? a.keys[(list0 + l) * a.beams + r] : 0;
+        for (int i = 0; i < kAhead; ++i) {
+          if (l == tid && r0 == 0) k[i] = mine[i];
+          else k[i] = r0 + i < a.beams ? a.keys[(list0 + l) * a.beams + r0 + i] : 0;
+        }
 #pragma unroll
-      for (int r = 1; r < kBeams; ++r) {
-        const Pick p = pick(l, r, k[r]);
-        if (p.hi && !(bar > p)) s_list[atomicAdd(&s_count, 1)] = p;
+        for (int i = 0; i < kAhead; ++i) {
+          const Pick p = r0 + i < a.beams ? pick(b, r0 + i == 0 && l == b * a.slices, k[i]) : Pick{0, 0};
+          more = more && p.hi && !(bar > p);          // sorted: what follows does not pass either
+          if (more) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kPicks) s_list[at] = p;
+          }
+        }
       }
     }
+    __syncthreads();
+    if (whole || s_count <= kPicks) break;
+    // more equal values than the list holds: a bar of one whole head
+    const int heads = min(lists, kPickThreads);
+    above = 0;
+#pragma unroll 1
+    for (int i = 0; i < heads; ++i) above += s_best[i] > best ? 1 : 0;
+    if (tid < heads && above == a.beams - 1 && best.hi) s_bar = best;
+    __syncthreads();                           // every thread has read s_count
+    if (tid == 0) s_count = 0;
+    bar = s_bar;
+    __syncthreads();
   }
-  __syncthreads();
   const int n = s_count;
-  for (int i = tid; i < n; i += kSelThreads) {
+  for (int i = tid; i < n; i += kPickThreads) {
     const Pick p = s_list[i];
     int r = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) r += s_list[j] > p ? 1 : 0;
     if (r < a.beams) s_out[r] = p;
   }
@@ -423,7 +458,7 @@ int cv3_beam_select(const float* logits, int64_t requests, int beams, int64_t vo
   a.sums = (double*)(a.keys + lists * beams);
   a.tops = (float*)(a.sums + lists);
   e == 8 ? launch_slices<8>(a, rows, st) : launch_slices<32>(a, rows, st);
-  hipLaunchKernelGGL(k_select_beams, dim3((unsigned)requests), dim3(kSelThreads), 0, st, a);
+  hipLaunchKernelGGL(k_select_beams, dim3((unsigned)requests), dim3(kPickThreads), 0, st, a);
   const hipError_t err = hipGetLastError();
   const int rc = scratch_free(work, st);
   CV3_REQUIRE(err == hipSuccess, CV3_EHIP, "kernel launch failed: %s", hipGetErrorString(err));
