@@ -44,7 +44,7 @@ def _in(x, dtype, name, shape=None) -> DeviceArray:
     """An input on the device, of the type and shape that the call takes."""
     if not isinstance(x, DeviceArray):
         x = to_device(np.ascontiguousarray(x, dtype=dtype))
-    elif x.dtype != dtype:
+    elif x.dtype is not dtype and x.dtype != dtype:
         raise TypeError(f"{name} holds {x.dtype}, not {dtype}")
     if shape is not None and x.shape != shape:
         raise ValueError(f"{name} has the shape {x.shape}, not {shape}")
