@@ -373,12 +373,11 @@ struct ReorderArgs {
 
 // Copies move a part-filled page's rows between the beams' own pages, in place and in any order: a
 // thread holds the same 16 bytes of every beam's page, reads all it needs and only then writes.
-// HBM-bound; a beam that stays itself costs nothing.  Workgroups [0, request's copies) copy, the
-// last table_parts of each request turn its table, column by column, in the same way.
+// HBM-bound; a beam that stays itself costs nothing.  Of a request's workgroups
+// the last table_parts turn its table, column by column, in the same way.
 template <int W>
 __global__ __launch_bounds__(256) void k_beam_reorder(ReorderArgs a) {
-  const int64_t copies = a.layers * a.kv_heads * 2 * a.parts, per = copies + a.table_parts;
-  const int64_t r = blockIdx.x / per, in = blockIdx.x % per;
+  const int64_t copies = a.layers * a.kv_heads * 2 * a.parts, r = blockIdx.y, in = blockIdx.x;
   const int64_t cap = a.blocks * a.page;
   const int64_t len = min((int64_t)max(a.lengths[r], 0), cap);
   const int64_t full = len / a.page, rest = len - full * a.page;
@@ -438,7 +437,8 @@ int cv3_beam_select(const float* logits, int64_t requests, int beams, int64_t vo
   CV3_REQUIRE(beams >= 1 && beams <= kBeams, CV3_EINVAL, "1 to %d beams, not %d", kBeams, beams);
   CV3_REQUIRE(vocab >= 1 && vocab <= kVocabMax, CV3_EINVAL, "a vocabulary of 1 to %d tokens, not %lld", kVocabMax,
               (long long)vocab);
-  CV3_REQUIRE(requests >= 0 && requests <= (1 << 20), CV3_EINVAL, "bad number of requests: %lld", (long long)requests);
+  CV3_REQUIRE(requests >= 0 && requests <= (1 << 23) && requests * beams <= (1 << 23) / ceil_div(vocab, 8 * kSelThreads), CV3_EINVAL,
+              "%lld requests of %d beams are too many for one call", (long long)requests, beams);
   const int64_t banned = std::max<int64_t>(0, std::min(ban_hi, vocab) - std::max<int64_t>(ban_lo, 0));
   CV3_REQUIRE(vocab - banned >= beams, CV3_EINVAL, "%lld tokens to choose from are fewer than %d beams",
               (long long)(vocab - banned), beams);
@@ -487,8 +487,9 @@ int cv3_beam_reorder(const int32_t* parents, int64_t requests, int beams, int32_
   ReorderArgs a{parents, tables, own, lengths, (uint4*)k_cache, (uint4*)v_cache, pages, blocks, layers, beams, kv_heads,
                 (int)page, row_vecs, (int)ceil_div(page * row_vecs, 256), (int)ceil_div(blocks, 256)};
   const int64_t per = layers * kv_heads * 2 * a.parts + a.table_parts;
-  CV3_REQUIRE(requests <= INT32_MAX / per, CV3_EINVAL, "too many requests for one call: %lld", (long long)requests);
-  const dim3 grid((unsigned)(requests * per)), block(256);
+  CV3_REQUIRE(requests <= 65535 && per < (1 << 24), CV3_EINVAL, "%lld requests, or pages of %lld copies, are too many for one call",
+              (long long)requests, (long long)per);
+  const dim3 grid((unsigned)per, (unsigned)requests), block(256);
   hipStream_t st = stream_of(s);
   if (beams <= 4) hipLaunchKernelGGL(k_beam_reorder<4>, grid, block, 0, st, a);
   else if (beams <= 8) hipLaunchKernelGGL(k_beam_reorder<8>, grid, block, 0, st, a);

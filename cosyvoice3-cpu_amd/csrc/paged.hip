@@ -80,7 +80,8 @@ __global__ __launch_bounds__(kTabThreads) void k_block_tables(TabArgs a) {
   __shared__ int32_t s_first[kTabRequests];   // index of the request's first new page among the free ones
   __shared__ uint32_t s_red[kTabThreads / 64];
   const uint32_t page = (uint32_t)a.page, cap = (uint32_t)a.blocks * page, most = (uint32_t)a.tokens;
-  const int64_t taken = a.taken[0];
+  const bool reserved = !a.free_pages;        // the tables hold every page already
+  const int64_t taken = reserved ? 0 : a.taken[0];
   uint32_t tok = 0, pages = 0;                // of the requests so far; tok at most `most`
   for (int r0 = 0; r0 < a.requests; r0 += kTabThreads * kTabEach) {
     const int r = r0 + (int)threadIdx.x * kTabEach;
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(kTabThreads) void k_block_tables(TabArgs a) {
       start[i] = min(at, most);
       at = __builtin_elementwise_add_sat(at, want[i]);
       now[i] = held[i] + (min(at, most) - start[i]);
-      need[i] = (now[i] + page - 1) / page - (held[i] + page - 1) / page;
+      need[i] = reserved ? 0 : (now[i] + page - 1) / page - (held[i] + page - 1) / page;
       more += need[i];
     }
     uint32_t upto = pages + block_scan(more, s_red, &all);
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(kTabThreads) void k_block_tables(TabArgs a) {
   if (threadIdx.x == 0) s_start[a.requests] = (int32_t)tok;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.starts[a.requests] = (int32_t)tok;
-    a.taken_out[0] = (int32_t)min(taken + pages, (int64_t)INT32_MAX);
+    if (!reserved) a.taken_out[0] = (int32_t)min(taken + pages, (int64_t)INT32_MAX);
   }
   __syncthreads();
   for (int64_t t0 = ((int64_t)blockIdx.x * kTabThreads + threadIdx.x) * kTabEach; t0 < a.tokens;
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(kTabThreads) void k_block_tables(TabArgs a) {
       const uint32_t block = pos / page, row = pos - block * page, have = (held + page - 1) / page;
       int32_t* entry = a.tables + (int64_t)r * a.blocks + block;
       int32_t id;
-      if (block < have) {
+      if (block < have || reserved) {
         id = *entry;
       } else {
         const int64_t n = (int64_t)s_first[r] + (block - have);
@@ -1015,6 +1016,8 @@ void attention_for(const AttnArgs& a, bool whole, hipStream_t st) {
   }
 }
 
+constexpr int64_t kLaunchBlocks = 1 << 23;       // of at most 512 threads: a launch has fewer than 2^32 of them
+
 int elem_size(int type) { return type == CV3_F32 ? 4 : 2; }
 
 // What every call on a cache checks.
@@ -1046,10 +1049,10 @@ int cv3_paged_tables(const int32_t* lengths, const int32_t* new_tokens, int64_t 
               "tables of %lld blocks of %lld keys pass 2^31 keys", (long long)blocks, (long long)page);
   CV3_REQUIRE(tokens >= 0 && tokens <= INT32_MAX - 65536, CV3_EINVAL, "too many tokens: %lld", (long long)tokens);
   CV3_REQUIRE(free_count >= 0 && free_count <= INT32_MAX, CV3_EINVAL, "bad number of free pages");
-  CV3_REQUIRE(taken && taken_out && starts && (requests == 0 || (lengths && new_tokens && tables && total)) &&
-                  (tokens == 0 || (slots && positions)) && (free_count == 0 || free_pages),
+  CV3_REQUIRE(starts && (requests == 0 || (lengths && new_tokens && tables && total)) &&
+                  (tokens == 0 || (slots && positions)) && (free_pages ? taken && taken_out : free_count == 0),
               CV3_EINVAL, "null operand");
-  CV3_REQUIRE((requests == 0 || (const void*)total != (const void*)lengths) && taken_out != taken, CV3_EINVAL,
+  CV3_REQUIRE((requests == 0 || (const void*)total != (const void*)lengths) && (!taken || taken_out != taken), CV3_EINVAL,
               "total and taken_out are arrays of their own: every workgroup reads lengths and taken");
   TabArgs a{lengths, new_tokens, free_pages, taken, tables, total, taken_out, starts, slots, positions,
             free_count, (int)requests, (int)page, (int)blocks, (int)tokens};
@@ -1080,7 +1083,7 @@ int cv3_paged_append(const float* rows, int64_t n, int64_t ld, int heads, int kv
   const bool wide = (uintptr_t)rows % 16 == 0 && ld % 4 == 0 && (!q || ((uintptr_t)q % 16 == 0 && ldq % 4 == 0));
   const unsigned per_row = (unsigned)(heads + 2 * kv_heads) * (d / 2) / (wide ? 4 : 1);
   const unsigned threads = std::min(256u, (per_row + 63) / 64 * 64), per = (per_row + threads - 1) / threads;
-  CV3_REQUIRE(n <= (int64_t)INT32_MAX / per, CV3_EINVAL, "too many rows: %lld", (long long)n);
+  CV3_REQUIRE(n <= (int64_t)kLaunchBlocks / per, CV3_EINVAL, "too many rows for one call: %lld", (long long)n);
   if (wide)
     hipLaunchKernelGGL(k_append<4>, dim3((unsigned)n * per), dim3(threads), 0, stream_of(s), a, cache_type, per_row, per);
   else
@@ -1100,7 +1103,8 @@ int cv3_paged_attention(const float* q, int64_t ldq, int64_t batch, int heads, i
   CV3_REQUIRE(heads <= 65536, CV3_EINVAL, "at most 65536 query heads, not %d", heads);
   CV3_REQUIRE(blocks >= 1 && blocks <= (INT32_MAX - 65536) / page, CV3_EINVAL,
               "tables of %lld blocks of %lld keys pass 2^31 keys", (long long)blocks, (long long)page);
-  CV3_REQUIRE(batch >= 0 && batch <= INT32_MAX / heads, CV3_EINVAL, "bad batch of %lld", (long long)batch);
+  CV3_REQUIRE(batch >= 0 && batch <= kLaunchBlocks / heads, CV3_EINVAL, "%lld sequences of %d heads are too many for one call",
+              (long long)batch, heads);
   CV3_REQUIRE(ldq >= (int64_t)heads * d && ldo >= (int64_t)heads * d, CV3_EINVAL, "rows are too short for %d heads of %d",
               heads, d);
   if (batch == 0) return CV3_OK;

@@ -43,7 +43,12 @@ def new_cache(pages: int, kv_heads: int, page: int, dim: int, dtype="float32", l
 def _in(x, dtype, name, shape=None) -> DeviceArray:
     """An input on the device, of the type and shape that the call takes."""
     if not isinstance(x, DeviceArray):
-        x = to_device(np.ascontiguousarray(x, dtype=dtype))
+        a = np.asarray(x)
+        if dtype.kind != "f" and a.size:
+            lim = np.iinfo(dtype)
+            if a.dtype.kind not in "iub" or int(a.min()) < lim.min or int(a.max()) > lim.max:
+                raise ValueError(f"{name} does not hold whole numbers of {dtype}")
+        x = to_device(np.ascontiguousarray(a, dtype=dtype))
     elif x.dtype is not dtype and x.dtype != dtype:
         raise TypeError(f"{name} holds {x.dtype}, not {dtype}")
     if shape is not None and x.shape != shape:
@@ -93,23 +98,33 @@ def block_tables(lengths, new, page: int, free, taken, tables: DeviceArray, toke
     ran out (their entries and slots are -1); each request's first token in the list (requests + 1); and the
     list of ``tokens`` slots (int64, page id * page + row) and positions, -1 behind the last token.
     ``tokens`` may be left out for a NumPy ``new``, whose sum it then is, or with ``out``.  Tokens past a
-    request's table, or past ``tokens``, are not given.  ``out``: those five arrays, none of them ``lengths``
-    or ``taken`` themselves."""
+    request's table, or past ``tokens``, are not given.  ``free`` None: the tables hold every page already (a
+    search's reserved pages), none is taken, and the result's ``taken`` is None.  ``out``: those five arrays,
+    none of them ``lengths`` or ``taken`` themselves."""
     if not isinstance(tables, DeviceArray) or tables.ndim != 2:
         raise TypeError("tables is a DeviceArray (requests, blocks)")
     r, blocks = tables.shape
     if tokens is None:
-        if out is not None:
+        if out is not None and len(out) == 5:
             tokens = out[3].size
         elif isinstance(new, DeviceArray):
             raise ValueError("tokens, the length of the list, is needed with counts on the device")
         else:
             tokens = int(np.maximum(np.asarray(new, dtype=np.int64), 0).sum())
+    if out is not None and len(out) != 5:
+        raise ValueError(f"out takes 5 arrays, got {len(out)}")
     first = lengths
     _held(tables, _I32, "tables")
     lengths, new = _in(lengths, _I32, "lengths", (r,)), _in(new, _I32, "new", (r,))
+    shapes = (((r,), _I32), ((1,), _I32), ((r + 1,), _I32), ((tokens,), _I64), ((tokens,), _I32))
+    if free is None:
+        outs = None if out is None else (out[0], *out[2:])
+        total, starts, slots, positions = _outs(outs, (shapes[0], *shapes[2:]), ("total", "starts", "slots", "positions"))
+        _lib.call("paged_tables", lengths.ptr, new.ptr, r, page, None, 0, None, tables.ptr, blocks, tokens, total.ptr,
+                  None, starts.ptr, slots.ptr, positions.ptr, None)
+        return _given(total, first), None, _given(starts, first), _given(slots, first), _given(positions, first)
     free, taken = _in(free, _I32, "free"), _in(taken, _I32, "taken", (1,))
-    got = _outs(out, (((r,), _I32), ((1,), _I32), ((r + 1,), _I32), ((tokens,), _I64), ((tokens,), _I32)), _TABLE_OUTS)
+    got = _outs(out, shapes, _TABLE_OUTS)
     total, took, starts, slots, positions = got
     _lib.call("paged_tables", lengths.ptr, new.ptr, r, page, free.ptr, free.size, taken.ptr, tables.ptr, blocks,
               tokens, total.ptr, took.ptr, starts.ptr, slots.ptr, positions.ptr, None)

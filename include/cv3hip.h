@@ -565,7 +565,8 @@ int cv3_qwen2_embed_token(const cv3_qwen2_model* m, const cv3_qwen2_state* s, cv
 /* Pages and slots for new_tokens[r] more tokens after lengths[r].  Requests take pages in order from
  * free_pages[taken ..], one for each block past those that their length has begun, entered into tables [requests,
  * blocks]; taken_out counts what was asked for (at most 2^31 - 1), and where free_pages ends first (taken_out > free_count) the entry and
- * the slots are -1.  Tokens that pass a request's table, or `tokens` in all, are not given: total[r] = the length
+ * the slots are -1.  free_pages NULL: the tables hold every page already, none is taken (taken, taken_out: NULL too,
+ * or not looked at).  Tokens that pass a request's table, or `tokens` in all, are not given: total[r] = the length
  * after those given.  starts [requests + 1]: each request's first token in the list; slots and positions [tokens], -1
  * behind the last.  At most 4096 requests; total and taken_out must not alias lengths and taken. */
 int cv3_paged_tables(const int32_t* lengths, const int32_t* new_tokens, int64_t requests, int64_t page,

@@ -110,6 +110,27 @@ def test_block_tables(paged, requests, page, blocks):
     check_tables(paged, lengths, new, page, free[:max(1, requests // 3)], 0, blocks)        # pages run out
 
 
+def test_block_tables_of_reserved_pages(paged):
+    """Without free pages the tables are as they are, and give every slot."""
+    rng = np.random.default_rng(3)
+    for requests, page, blocks in ((1, 1, 5), (70, 16, 6), (1100, 5, 9)):
+        tables = rng.integers(-1, 500, (requests, blocks)).astype(I32)
+        lengths, new = (rng.integers(0, page * blocks // 2 + 3, requests).astype(I32) for _ in range(2))
+        tokens = int(new.sum()) + 3
+        td = dev(tables)
+        total, taken, starts, slots, positions = paged.block_tables(lengths, new, page, None, None, td, tokens=tokens)
+        pos = [p for n, g in zip(lengths, new) for p in range(n, min(n + g, page * blocks))]
+        row = [i for i, (n, g) in enumerate(zip(lengths, new)) for _ in range(n, min(n + g, page * blocks))]
+        pos, row = np.array(pos, int), np.array(row, int)
+        of = tables[row, pos // page].astype(I64)
+        assert taken is None and np.array_equal(td.numpy(), tables)
+        assert np.array_equal(total, np.maximum(lengths, np.minimum(lengths + new, page * blocks)))
+        assert np.array_equal(starts, np.concatenate([[0], np.cumsum(total - lengths)]))
+        assert np.array_equal(positions, np.concatenate([pos, -np.ones(tokens - len(pos), int)]))
+        assert np.array_equal(slots[:len(pos)], np.where(of >= 0, of * page + pos % page, -1))
+        assert np.all(slots[len(pos):] == -1)
+
+
 def test_block_tables_at_the_edges(paged):
     free = np.arange(100, 140)
     check_tables(paged, [0, 0, 0], [0, 0, 0], 16, free, 0, 4)                  # no token at all
@@ -629,3 +650,238 @@ def test_reorder_pages_outside_the_cache_are_not_copied(paged):
     paged.beam_reorder(parents, td, own, np.array([21], I32), k, v)
     assert np.array_equal(td.numpy(), want)
     assert np.array_equal(k.numpy(), new[0][0]) and np.array_equal(v.numpy(), new[1][0])
+
+
+# ------------------------------------------------------------------------------------------------
+# infinities among what is seen; streams, threads and graphs; the operators as one step
+# ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("blocks", [13, 150])
+@pytest.mark.parametrize("h,kv,d", [(14, 2, 64), (4, 2, 128)])
+def test_attention_seen_infinities(paged, h, kv, d, blocks, kind):
+    """An infinite key channel makes a score +inf (NaN outputs, inf - inf) or -inf (weight zero) by the query's sign;
+    an infinite value is its channel's output.  Two-byte caches form such outputs in float32."""
+    rng = np.random.default_rng([d, blocks])
+    lengths = np.array([200, 200, 200, 200, 200], I32)
+    tables, pages = batch(rng, lengths, blocks, 16)
+    q = rng.normal(size=(5, h, d)).astype(np.float32)
+    ks, vs = (rng.normal(size=(pages, kv, 16, d)).astype(np.float32) for _ in range(2))
+    ks[tables[1, 2], 0, 5, 7] = np.inf
+    ks[tables[2, 12], 1, 3, d - 1] = -np.inf
+    vs[tables[3, 0], 0, 0, 1] = -np.inf
+    vs[tables[3, 6], 1, 15, 9], vs[tables[3, 9], 1, 2, 9] = np.inf, -np.inf
+    q[4, 1, 3] = np.inf
+    (ks, k64), (vs, v64) = stored(ks, kind), stored(vs, kind)
+    with np.errstate(invalid="ignore"):
+        want = attention_ref(q, k64, v64, tables, lengths, None, 1 / np.sqrt(d))
+    got = paged.attention(q, dev(ks), dev(vs), tables, lengths)
+    assert np.isnan(want).any() and np.isinf(want).any()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    fine = np.isfinite(want)
+    assert rel_err(got[fine], want[fine]) <= TOL
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_attention_sizes_of_queries(paged, kind):
+    """Queries from 2^-120 to 2^40 beside each other: each head has its own scale."""
+    rng = np.random.default_rng(11)
+    for blocks in (4, 90):
+        lengths = np.array([50, 17], I32)
+        tables, pages = batch(rng, lengths, blocks, 16)
+        q = rng.normal(size=(2, 14, 64)) * 2.0 ** np.linspace(-120, 0, 14)[None, :, None]
+        q[1, 3] = 0.0
+        q[1, 5] *= 2.0 ** 85         # scores of 2^40 and more: one key takes all
+        (ks, k64), (vs, v64) = (stored(rng.normal(size=(pages, 2, 16, 64)), kind) for _ in range(2))
+        q = q.astype(np.float32)
+        want = attention_ref(q, k64, v64, tables, lengths, None, 0.125)
+        assert rel_err(paged.attention(q, dev(ks), dev(vs), tables, lengths), want) <= TOL
+
+
+@pytest.mark.parametrize("vocab", [500, 6761, 30000])
+def test_select_bans_whole_slices(paged, vocab):
+    rng = np.random.default_rng(vocab)
+    x = rng.normal(size=(2, 4, vocab))
+    s, none = rng.normal(size=(2, 4)), np.zeros((2, 4))
+    for ban in ((0, vocab - 4), (4, vocab), (2, vocab - 2), (-5, 10), (vocab - 10, vocab + 50), (7, 7), (9, 3),
+                (0, vocab // 2)):
+        check_select(paged, x, s, none, (vocab - 3, vocab), ban=ban)
+
+
+def attention_inputs(rng, b, n, blocks, kind="bfloat16", h=14, kv=2, d=64, page=16):
+    lengths = rng.integers(1, n + 1, b).astype(I32)
+    tables, pages = batch(rng, lengths, blocks, page)
+    q = rng.normal(size=(b, h, d)).astype(np.float32)
+    (ks, k64), (vs, v64) = (stored(rng.normal(size=(pages, kv, page, d)), kind) for _ in range(2))
+    want = attention_ref(q, k64, v64, tables, lengths, None, 1 / np.sqrt(d))
+    return [dev(a) for a in (q, ks, vs, tables, lengths)], want
+
+
+def test_calls_on_an_explicit_stream(gpu, paged):
+    """The C entries on a stream of the caller's own, beside the thread's: scratch and results are that stream's."""
+    from cv3amd import _lib, device
+    rng = np.random.default_rng(12)
+    (q, k, v, t, n), want = attention_inputs(rng, 9, 900, 120)
+    out, st = dev(np.zeros((9, 14, 64), np.float32)), device.Stream()
+    x, s = rng.normal(size=(2, 4, 9000)).astype(np.float32), rng.normal(size=(2, 4)).astype(np.float32)
+    ref = select_ref(x, s, np.zeros((2, 4)), (0, 1), (0, 0), 0)
+    xd, sd, dd = dev(x), dev(s), dev(np.zeros((2, 4), U8))
+    tok, par, so, do = (dev(np.zeros((2, 4), t_)) for t_ in (I64, I32, np.float32, U8))
+    for _ in range(3):
+        _lib.call("paged_attention", q.ptr, 14 * 64, 9, 14, 2, 64, _lib.BF16, k.ptr, v.ptr, k.shape[0], 16, t.ptr, 120,
+                  n.ptr, None, ctypes.c_float(0.125), out.ptr, 14 * 64, st.handle)
+        _lib.call("beam_select", xd.ptr, 2, 4, 9000, sd.ptr, dd.ptr, 0, 1, 0, 0, 0, tok.ptr, par.ptr, so.ptr, do.ptr,
+                  st.handle)
+    _lib.call("stream_sync", st.handle)
+    assert rel_err(out.numpy(), want) <= TOL
+    assert np.array_equal(tok.numpy(), ref[0]) and np.array_equal(par.numpy(), ref[1])
+
+
+def test_calls_from_four_threads(gpu, paged):
+    import threading
+    from cv3amd import device
+    wrong = []
+
+    def work(i):
+        try:
+            rng = np.random.default_rng([13, i])
+            ins, want = attention_inputs(rng, 5 + i, 700 + 100 * i, 150)
+            x = rng.normal(size=(3, 4, 7000 + i)).astype(np.float32)
+            s, d = rng.normal(size=(3, 4)).astype(np.float32), np.zeros((3, 4), U8)
+            ref = select_ref(x, s, d, (0, 1), (0, 0), 0)
+            xd, sd, dd = dev(x), dev(s), dev(d)
+            outs = [(paged.attention(*ins), paged.beam_select(xd, sd, dd, (0, 1))) for _ in range(20)]
+            device.synchronize()
+            for o, sel in outs:
+                if rel_err(o.numpy(), want) > TOL or not np.array_equal(sel[0].numpy(), ref[0]):
+                    wrong.append(i)
+        except Exception as e:      # noqa: BLE001
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+class Step:
+    """One beam-search step over a one-layer model that is nothing but the operators: rows and logits are drawn from
+    tables by token, so that every step's inputs follow from the choices before it."""
+
+    R, W, V, H, KV, D, PAGE, BLOCKS, LAYERS = 3, 4, 300, 6, 2, 32, 4, 8, 2
+
+    def __init__(self, paged, kind):
+        self.paged, self.kind = paged, kind
+        rng = np.random.default_rng(14)
+        rows = self.R * self.W
+        pages = rows * self.BLOCKS
+        self.own = rng.permutation(pages).reshape(self.R, self.W, self.BLOCKS).astype(I32)
+        self.qkv = rng.normal(size=(rows, (self.H + 2 * self.KV) * self.D)).astype(np.float32)
+        self.logits = rng.normal(size=(self.R, self.W, self.V)).astype(np.float32)
+        self.k0 = rng.normal(size=(2, self.LAYERS, pages, self.KV, self.PAGE, self.D)).astype(np.float32)
+        self.cos, self.sin = rotary(self.D, 64)
+
+    def state(self):
+        rows = self.R * self.W
+        s = dict(tables=dev(self.own), own=dev(self.own), k=dev(stored(self.k0[0], self.kind)[0]),
+                 v=dev(stored(self.k0[1], self.kind)[0]), len_r=dev(np.array([0, 3, 9], I32)),
+                 len_w=dev(np.repeat(np.array([0, 3, 9], I32), self.W)), one_r=dev(np.ones(self.R, I32)),
+                 one_w=dev(np.ones(rows, I32)), qkv=dev(self.qkv), logits=dev(self.logits),
+                 scores=dev(np.zeros((self.R, self.W), np.float32)), done=dev(np.zeros((self.R, self.W), U8)),
+                 cos=dev(self.cos), sin=dev(self.sin), total_r=dev(np.zeros(self.R, I32)), total_w=dev(np.zeros(rows, I32)),
+                 starts=dev(np.zeros(rows + 1, I32)), slots=dev(np.zeros(rows, I64)), pos=dev(np.zeros(rows, I32)),
+                 r_starts=dev(np.zeros(self.R + 1, I32)), r_slots=dev(np.zeros(self.R, I64)),
+                 r_pos=dev(np.zeros(self.R, I32)), r_tables=dev(np.zeros((self.R, self.BLOCKS), I32)),
+                 q=dev(np.zeros((rows, self.H, self.D), np.float32)), out=dev(np.zeros((rows, self.H, self.D), np.float32)),
+                 tokens=dev(np.zeros((self.R, self.W), I64)), parents=dev(np.zeros((self.R, self.W), I32)))
+        return s
+
+    def run(self, s):
+        """Enqueues one step: the new token's slots, the cache write of both layers, attention, the choice, the
+        reordering.  Every beam's pages are reserved from the start: slots come from `own`, none is taken."""
+        from cv3amd import _lib
+        p, rows = self.paged, self.R * self.W
+        flat = s["tables"].reshape(rows, self.BLOCKS)
+        p.block_tables(s["len_w"], s["one_w"], self.PAGE, None, None, s["own"].reshape(rows, self.BLOCKS),
+                       out=(s["total_w"], None, s["starts"], s["slots"], s["pos"]))
+        for i in range(self.LAYERS):
+            k, v = (s[c].rows(i, i + 1).reshape(s[c].shape[1:]) for c in "kv")
+            p.append(s["qkv"], self.H, s["pos"], s["slots"], s["cos"], s["sin"], k, v, out=s["q"])
+            p.attention(s["q"], k, v, flat, s["total_w"], out=s["out"])
+        p.beam_select(s["logits"], s["scores"], s["done"], (290, 300), out=(s["tokens"], s["parents"], s["scores"], s["done"]))
+        _lib.call("copy_d2d", s["len_w"].ptr, s["total_w"].ptr, 4 * rows, None)
+        p.block_tables(s["len_r"], s["one_r"], self.PAGE, None, None, s["r_tables"],
+                       out=(s["total_r"], None, s["r_starts"], s["r_slots"], s["r_pos"]))
+        _lib.call("copy_d2d", s["len_r"].ptr, s["total_r"].ptr, 4 * self.R, None)
+        p.beam_reorder(s["parents"], s["tables"], s["own"], s["len_r"], s["k"], s["v"])
+
+
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+def test_steps_captured_and_replayed(gpu, paged, kind):
+    """A captured step, replayed with eager work in between, leaves what the same steps leave eagerly; two graphs of
+    two states replay in turn (each has its own scratch)."""
+    from cv3amd import device
+    step = Step(paged, kind)
+
+    names = ("tables", "k", "v", "len_w", "len_r", "scores", "done", "out", "tokens", "parents")
+    eager = step.state()
+    want = []
+    for _ in range(6):
+        step.run(eager)
+        want.append({n: eager[n].numpy() for n in names})
+    states, graphs = [step.state(), step.state()], []
+    for s in states:
+        g = device.Graph()
+        with g:
+            step.run(s)
+        graphs.append(g)
+    other = step.state()
+    for i in range(6):
+        for s, g in zip(states, graphs):
+            g.launch()
+            step.run(other)             # eager calls between the replays
+            if i == 3:
+                device.synchronize()
+            for n in names:
+                got = s[n].numpy()
+                assert np.array_equal(got.view(np.uint8), want[i][n].view(np.uint8)), (i, n)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_steps_against_the_reference(gpu, paged, kind):
+    """The same steps followed in NumPy: slots, cache, attention outputs, choices and tables after every step."""
+    step = Step(paged, kind)
+    s = step.state()
+    R, W, H, KV, D, PAGE = step.R, step.W, step.H, step.KV, step.D, step.PAGE
+    tables, n = step.own.copy(), np.array([0, 3, 9])
+    k, v = (values(stored(c, kind)[0], kind) for c in step.k0)
+    scores, done = np.zeros((R, W), np.float32), np.zeros((R, W), U8)
+    x = step.qkv.astype(np.float64).reshape(R * W, H + 2 * KV, D)
+    for _ in range(6):
+        step.run(s)
+        at = np.repeat(n, W)
+        turned, _ = turn(x, step.cos.astype(np.float64)[at], step.sin.astype(np.float64)[at])
+        for i in range(R * W):
+            p = step.own.reshape(R * W, -1)[i, at[i] // PAGE]
+            k[:, p, :, at[i] % PAGE], v[:, p, :, at[i] % PAGE] = turned[i, H:H + KV], x[i, H + KV:]
+        n = n + 1
+        # the last layer's attention, over the tables before the reordering
+        want = attention_ref(turned[:, :H], k[-1], v[-1], tables.reshape(R * W, -1), np.repeat(n, W), None, 1 / np.sqrt(D))
+        # a stored key is off by half a step of its type: the scores by that share of sum |q k|, the values by theirs
+        eps = {"float32": 2.0 ** -23, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}[kind]
+        most = np.abs(turned[:, :H]).sum(-1).max() * np.abs(k).max() / np.sqrt(D)
+        assert np.abs(s["out"].numpy() - want).max() <= (2 * eps * most + eps + TOL) * np.abs(v).max()
+        tok, par, sc, done = select_ref(step.logits, scores, done, (290, 300), (0, 0), 290)
+        scores = sc.astype(np.float32)
+        assert np.array_equal(s["tokens"].numpy(), tok) and np.array_equal(s["parents"].numpy(), par)
+        assert np.array_equal(s["done"].numpy(), done)
+        assert np.abs(s["scores"].numpy() - scores).max() <= 1e-5
+        scores = s["scores"].numpy()
+        tables, (k, v) = reorder_ref(par, tables, step.own, n, [k, v], PAGE)
+        assert np.array_equal(s["tables"].numpy(), tables)
+        assert np.array_equal(s["len_r"].numpy(), n) and np.array_equal(s["len_w"].numpy(), np.repeat(n, W))
+    for c, w in ((s["k"], k), (s["v"], v)):
+        assert np.abs(values(c.numpy(), kind) - w).max() <= 2 * eps * np.abs(w).max()

@@ -43,7 +43,7 @@ def reorder(**k):
 
 REFUSED = [
     tables(requests=-1), tables(requests=4097), tables(page=0), tables(page=70000), tables(blocks=0),
-    tables(blocks=1 << 40), tables(tokens=-1), tables(tokens=1 << 31), tables(free_count=-1), tables(free=None),
+    tables(blocks=1 << 40), tables(tokens=-1), tables(tokens=1 << 31), tables(free_count=-1), tables(free=None), tables(taken=None, taken_out=None),
     tables(lengths=None), tables(new=None), tables(taken=None), tables(tables=None), tables(total=None),
     tables(taken_out=None), tables(starts=None), tables(slots=None), tables(positions=None), tables(total=P),
     tables(taken_out=P),
@@ -51,18 +51,18 @@ REFUSED = [
     append(heads=-1), append(ld=18 * 64 - 1), append(ldq=14 * 64 - 1), append(cos=None), append(sin=None),
     append(positions=None), append(rope_rows=0), append(rows=None), append(slots=None), append(type=3),
     append(k=None), append(v=None), append(k=P + 8), append(pages=0), append(pages=1 << 31), append(page=0),
-    append(n=1 << 40),
+    append(n=1 << 40), append(n=1 << 23 | 1),
     attention(heads=15), attention(heads=0), attention(kv_heads=0), attention(d=12), attention(type=-1),
     attention(k=None), attention(v=P + 4), attention(pages=0), attention(page=0), attention(blocks=0),
-    attention(blocks=1 << 30), attention(batch=-1), attention(batch=1 << 31), attention(ldq=14 * 64 - 1),
+    attention(blocks=1 << 30), attention(batch=-1), attention(batch=1 << 31), attention(batch=600000), attention(ldq=14 * 64 - 1),
     attention(ldo=0), attention(q=None), attention(tables=None), attention(lengths=None), attention(out=None),
-    select(beams=0), select(beams=17), select(vocab=0), select(vocab=(1 << 19) + 1), select(requests=-1),
+    select(beams=0), select(beams=17), select(vocab=0), select(vocab=(1 << 19) + 1), select(requests=-1), select(requests=1 << 40), select(requests=1 << 22),
     select(ban_lo=2, ban_hi=99), select(vocab=3), select(logits=None), select(scores=None), select(done=None),
     select(tokens=None), select(parents=None), select(scores_out=None), select(done_out=None),
     reorder(beams=0), reorder(beams=17), reorder(type=7), reorder(page=0), reorder(pages=0), reorder(layers=0),
     reorder(kv_heads=0), reorder(d=20), reorder(blocks=0), reorder(requests=-1), reorder(parents=None),
     reorder(tables=None), reorder(own=None), reorder(own=P), reorder(lengths=None), reorder(k=None),
-    reorder(v=P + 8), reorder(requests=1 << 31),
+    reorder(v=P + 8), reorder(requests=1 << 31), reorder(requests=65536), reorder(layers=65536, kv_heads=1024),
 ]
 
 
@@ -145,5 +145,8 @@ def test_python_checks_types_and_shapes():
         paged.beam_reorder(par, bt, bt, dev((2,), i32), k, v)
     with pytest.raises(ValueError):
         paged.beam_reorder(dev((2, 3), i32), bt, dev((2, 4, 4), i32), dev((2,), i32), k, v)
+    for bad in ([1 << 31, 0, 0], [0.5, 0, 0], ["a", "b", "c"]):     # host numbers that the device's type does not hold
+        with pytest.raises(ValueError):
+            paged.block_tables(bad, n, 16, n, dev((1,), i32), t, tokens=5)
     with pytest.raises(ValueError):
         paged.new_cache(1, 1, 1, 8, dtype="float64")
