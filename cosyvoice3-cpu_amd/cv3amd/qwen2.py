@@ -20,11 +20,11 @@ Layout in HBM (L layers, D = hidden, dh = head_dim, I = intermediate):
 from __future__ import annotations
 
 import ctypes
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import numpy as np
 
-from . import _lib
+from . import _lib, paged
 from .device import DeviceArray, Graph, to_device
 
 c_i64, c_vp = ctypes.c_int64, ctypes.c_void_p
@@ -338,6 +338,15 @@ class DeviceQwen2:
         _lib.call("linear_q", kind, x, m, w.k, w.k, q, sc, sdt, kp, block, n, bias, y, ldy,
                   ctypes.byref(epi) if epi is not None else None, None)
 
+    def _after_attention(self, l: int, t: int, att, h, n, u, a, res, swiglu):
+        """o_proj + residual, RMSNorm, SwiGLU, down + residual of layer l on t rows (qwen2.py:171-177)."""
+        D, I = self.hidden, self.inter
+        self._linear(att.ptr, t, self.o, l, h.ptr, D, epi=res)
+        _lib.call("rms_norm", h.ptr, self.ln2.ptr + l * D * 4, n.ptr, t, D, self.eps, None)
+        self._linear(n.ptr, t, self.gate_up, l, u.ptr, I, row0=I, rows=I)        # up
+        self._linear(n.ptr, t, self.gate_up, l, a.ptr, I, row0=0, rows=I, epi=swiglu)  # u * silu(gate)
+        self._linear(a.ptr, t, self.down, l, h.ptr, D, epi=res)
+
     def prefill(self, x, pos0: int = 0):
         """Qwen2Model.forward over T input embeddings at positions pos0 .. pos0 + T - 1
         (qwen2.py:139-179) on the device: RMSNorm, [q; k; v] projection with bias, half-split
@@ -391,11 +400,7 @@ class DeviceQwen2:
             _lib.call("attention", qkv.ptr, self.k_cache.ptr + kv, self.v_cache.ptr + kv, att.ptr, 1, H, Hk, t,
                       pos0 + t, dh, c64(0, dh, R), c64(0, cap * dh, dh), c64(0, cap * dh, dh), c64(0, dh, D),
                       1.0 / np.sqrt(dh), 1 if t > 1 else 0, pos0, 0, None)
-            self._linear(att.ptr, t, self.o, l, h.ptr, D, epi=res)
-            _lib.call("rms_norm", h.ptr, self.ln2.ptr + l * D * 4, n.ptr, t, D, self.eps, None)
-            self._linear(n.ptr, t, self.gate_up, l, u.ptr, I, row0=I, rows=I)        # up
-            self._linear(n.ptr, t, self.gate_up, l, a.ptr, I, row0=0, rows=I, epi=swiglu)  # u * silu(gate)
-            self._linear(a.ptr, t, self.down, l, h.ptr, D, epi=res)
+            self._after_attention(l, t, att, h, n, u, a, res, swiglu)
         _lib.call("rms_norm", h.ptr + (t - 1) * D * 4, self.norm.ptr, n.ptr, 1, D, self.eps, None)
         self._linear(n.ptr, 1, self.head, 0, self.logits.ptr, self.vocab,
                      bias=self.head_bias.ptr if self.head_bias is not None else None)
@@ -553,3 +558,100 @@ class DeviceQwen2:
             self.step(graph)
         ints = self.ints.numpy()
         return [int(t) for t in ints[2 + pos + 1: 2 + pos + 1 + steps]]
+
+    # -- several sequences, greedy or by beam search, over a paged cache ----
+    def _paged_layers(self, x: DeviceArray, pos, slots, tables, lengths, cos, sin, k: DeviceArray, v: DeviceArray):
+        """The body over rows of any sequences (qwen2.py:139-179): each row's k and v go to its slot, and it sees the
+        ``lengths`` keys of its own table row.  Returns the residual stream."""
+        t = x.shape[0]
+        D, H, R, I = self.hidden, self.heads, self.qkv.rows, self.inter
+        h, n, qkv = x.copy(), DeviceArray((t, D)), DeviceArray((t, R))
+        q, att = DeviceArray((t, H, self.head_dim)), DeviceArray((t, H, self.head_dim))
+        u, a = DeviceArray((t, I)), DeviceArray((t, I))
+        res = _lib.epilogue(residual=h.ptr, ld_res=D)
+        swiglu = _lib.epilogue(act="silu", gate=u.ptr, gate_stride=I, rows_per_gate=1)
+        for l in range(self.layers):
+            kl, vl = (c.rows(l, l + 1).reshape(c.shape[1:]) for c in (k, v))
+            _lib.call("rms_norm", h.ptr, self.ln1.ptr + l * D * 4, n.ptr, t, D, self.eps, None)
+            self._linear(n.ptr, t, self.qkv, l, qkv.ptr, R, bias=self.qkv_bias.ptr + l * R * 4)
+            paged.append(qkv, H, pos, slots, cos, sin, kl, vl, out=q)
+            paged.attention(q, kl, vl, tables, lengths, out=att)
+            self._after_attention(l, t, att, h, n, u, a, res, swiglu)
+        return h
+
+    def _head(self, h: DeviceArray) -> DeviceArray:
+        """Head logits of every row (llm.py:74-77)."""
+        n, logits = DeviceArray(h.shape), DeviceArray((h.shape[0], self.vocab))
+        _lib.call("rms_norm", h.ptr, self.norm.ptr, n.ptr, h.shape[0], self.hidden, self.eps, None)
+        self._linear(n.ptr, h.shape[0], self.head, 0, logits.ptr, self.vocab,
+                     bias=self.head_bias.ptr if self.head_bias is not None else None)
+        return logits
+
+    def generate_batch(self, prompts, max_len: int, min_len: int = 0, speech_token_size: int = 6561, beams: int = 1,
+                       page: int = 16, cache: str = "float32") -> List[Tuple[List[int], float]]:
+        """Speech tokens for several prompts at once ((T, hidden) embeddings, of any lengths), from one pass of the
+        weights a step: greedy, or by beam search with up to 16 ``beams`` a prompt.  Every prompt ends before its
+        first stop id (speech_token_size .. + 199; none is chosen below ``min_len``) or after ``max_len`` tokens.
+        Returns each prompt's best tokens and the sum of their log probabilities, the stop id's included.
+
+        The sequences share nothing with this object's own cache: theirs is paged (``cache`` "float32", "float16" or
+        "bfloat16"), a prompt's whole pages held once for its beams, and is not bound to 1024 positions."""
+        xs = [x.numpy() if isinstance(x, DeviceArray) else np.asarray(x, np.float32) for x in prompts]
+        if any(x.ndim != 2 or x.shape[1] != self.hidden or x.shape[0] < 1 for x in xs):
+            raise ValueError(f"prompts are (T, {self.hidden}) embeddings")
+        stop = (int(speech_token_size), min(int(speech_token_size) + 200, self.vocab))
+        if max_len < 1 or page < 1 or not 1 <= beams <= 16 or not 0 < stop[0] < stop[1]:
+            raise ValueError("generation takes at least one token, a page of one key, 1 to 16 beams, and stop ids inside "
+                             "the vocabulary")
+        if not xs:
+            return []
+        r, w, dh = len(xs), int(beams), self.head_dim
+        held = np.array([x.shape[0] for x in xs], np.int32)
+        most = int(held.max()) + max_len
+        blocks = -(-most // page)
+        cos, sin = (to_device(a) for a in rope_tables(dh, self.theta, most))
+        k, v = paged.new_cache(r * w * blocks, self.kv_heads, page, dh, cache, layers=self.layers)
+        own_h = np.arange(r * w * blocks, dtype=np.int32).reshape(r, w, blocks)
+        shared = np.arange(blocks) < (held // page)[:, None, None]         # a prompt's whole pages lie with beam 0
+        own, tables = to_device(own_h), to_device(np.where(shared, own_h[:, :1], own_h))
+        # the prompts: every token a row that sees its own sequence up to itself
+        rows = np.repeat(np.arange(r), held)
+        _, _, _, slots, pos = paged.block_tables(to_device(np.zeros(r, np.int32)), held, page, None, None,
+                                                      to_device(own_h[:, 0]), tokens=len(rows))
+        upto = np.concatenate([np.arange(1, n + 1) for n in held]).astype(np.int32)
+        h = self._paged_layers(to_device(np.concatenate(xs).astype(np.float32)), pos, slots, to_device(own_h[rows, 0]),
+                               to_device(upto), cos, sin, k, v)
+        last = DeviceArray((r * w, self.hidden))
+        for i, at in enumerate(np.repeat(np.cumsum(held) - 1, w)):
+            _lib.call("copy_d2d", last.ptr + i * self.hidden * 4, h.ptr + int(at) * self.hidden * 4, self.hidden * 4, None)
+        logits = self._head(last)
+        scores_h = np.full((r, w), -np.inf, np.float32)                    # at first one beam a prompt lives
+        scores_h[:, 0] = 0.0
+        scores, done = to_device(scores_h), to_device(np.zeros((r, w), np.uint8))
+        chosen, parents = DeviceArray((r, w), np.int64), DeviceArray((r, w), np.int32)
+        lengths, ones, x = to_device(np.repeat(held, w)), to_device(np.ones(r * w, np.int32)), DeviceArray((r * w, self.hidden))
+        trail = []
+        for i in range(max_len):
+            paged.beam_select(logits.reshape(r, w, self.vocab), scores, done, stop, stop if i < min_len else (0, 0),
+                              out=(chosen, parents, scores, done))
+            trail.append((chosen.numpy(), parents.numpy()))
+            if i + 1 == max_len or done.numpy().all():
+                break
+            if w > 1:
+                paged.beam_reorder(parents, tables, own, held + i, k, v)
+            kind, q, sc, sdt, kp, block, n = self.emb.layer(0)
+            _lib.call("embedding", kind, q, sc, sdt, n, self.hidden, kp, block, chosen.ptr, r * w, x.ptr, None)
+            lengths, _, _, slots, pos = paged.block_tables(lengths, ones, page, None, None, own.reshape(r * w, blocks),
+                                                           tokens=r * w)
+            h = self._paged_layers(x, pos, slots, tables.reshape(r * w, blocks), lengths, cos, sin, k, v)
+            logits = self._head(h)
+        best, out = scores.numpy(), []
+        for i in range(r):
+            tokens, b = [], 0
+            for ids, up in reversed(trail):
+                tokens.append(int(ids[i, b]))
+                b = int(up[i, b])
+            tokens.reverse()
+            ends = [j for j, t in enumerate(tokens) if stop[0] <= t < stop[1]]
+            out.append((tokens[:ends[0]] if ends else tokens, float(best[i, 0])))
+        return out

@@ -1,0 +1,127 @@
+"""DeviceQwen2.generate_batch: several prompts from one set of weights, greedy and by beam search, over the paged cache,
+against the oracle's LM run one sequence at a time (Qwen2-0.5B's geometry, two layers, synthetic weights)."""
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+SIZE = 6561     # ids from here on stop
+
+
+def setup(profile):
+    import oracle.quant
+    import cv3amd.quant
+    from cv3amd import synth
+    from cv3amd.weights import WeightStore
+    from oracle.llm import CosyVoice3LM
+    t = synth.quantize_store(synth.qwen2_tensors(layers=2), profile, oracle.quant.quantize_q8, oracle.quant.quantize_q4)
+    meta = synth.qwen2_meta(layers=2)
+    return (CosyVoice3LM(WeightStore(t, meta, oracle.quant.QTensor), "llm."),
+            WeightStore(t, meta, cv3amd.quant.QTensor))
+
+
+def prompts(rng, lengths):
+    return [(rng.standard_normal((n, 896)) * 0.02).astype(np.float32) for n in lengths]
+
+
+def logp(lm, prompt, tokens):
+    """Log probabilities (float64) of the next token after a prompt and its tokens."""
+    x = prompt if not tokens else np.concatenate([prompt, lm.speech_emb(tokens)])
+    z = lm.head(lm.body.forward(x, lm.body.new_cache())[-1:])[0].astype(np.float64)
+    return z - z.max() - np.log(np.exp(z - z.max()).sum())
+
+
+def search(lm, prompt, beams, max_len, min_len, size):
+    """Plain beam search: (score, tokens, ended) hypotheses, best first; ties are not met."""
+    live = [(0.0, [], False)]
+    for i in range(max_len):
+        every = []
+        for score, tokens, ended in live:
+            if ended:
+                every.append((score, tokens, True))
+                continue
+            p = logp(lm, prompt, tokens)
+            if i < min_len:
+                p[size:size + 200] = -np.inf
+            for t in np.argsort(-p, kind="stable")[:beams]:
+                every.append((score + p[t], tokens + [int(t)], size <= t < size + 200))
+        live = sorted(every, key=lambda c: -c[0])[:beams]
+        if all(e for _, _, e in live):
+            break
+    score, tokens, _ = live[0]
+    return [t for t in tokens if not size <= t < size + 200], score
+
+
+@pytest.mark.parametrize("profile,page", [("per_channel", 16), ("balanced", 5), ("tiny", 64)])
+def test_greedy_batch_is_the_oracles_sequences(gpu, profile, page):
+    from cv3amd.qwen2 import DeviceQwen2
+    lm, store = setup(profile)
+    d = DeviceQwen2(store, cap=64)
+    xs = prompts(np.random.default_rng(1), (37, 1, 16, 50, 5, 64))
+    got = d.generate_batch(xs, 8, min_len=8, page=page)
+    for x, (tokens, score) in zip(xs, got):
+        seen, total = [], 0.0
+        for _ in range(8):
+            p = logp(lm, x, seen)
+            total += p[:SIZE].max()
+            seen.append(int(p[:SIZE].argmax()))
+        assert tokens == seen
+        assert abs(score - total) <= 1e-4     # eight log probabilities from logits within 1e-5 of about 1
+    # the same object's own cache and the single-sequence path are as before
+    d.prefill(xs[0], 0)
+    assert d.generate_after_prefill(1, graph=False)[0] == int(logp(lm, xs[0], []).argmax())
+
+
+def test_beam_search_is_the_plain_one(gpu):
+    from cv3amd.qwen2 import DeviceQwen2
+    lm, store = setup("per_channel")
+    d = DeviceQwen2(store, cap=64)
+    xs = prompts(np.random.default_rng(2), (19, 33, 4))
+    for beams, page in ((3, 16), (5, 4)):
+        for x, (tokens, score) in zip(xs, d.generate_batch(xs, 6, min_len=2, beams=beams, page=page)):
+            want, total = search(lm, x, beams, 6, 2, SIZE)
+            assert tokens == want
+            assert abs(score - total) <= 1e-4
+
+
+def test_beams_end_at_their_stop(gpu):
+    """A wide range of stop ids, so that hypotheses end at different lengths while others go on."""
+    from cv3amd.qwen2 import DeviceQwen2
+    lm, store = setup("per_channel")
+    d = DeviceQwen2(store, cap=64)
+    xs = prompts(np.random.default_rng(3), (12, 7))
+    first = [int(logp(lm, x, []).argmax()) for x in xs]
+    size = max(1, min(first) - 100)           # the likeliest first token of one prompt lies among the stop ids
+    for min_len in (0, 1, 3):
+        for x, (tokens, score) in zip(xs, d.generate_batch(xs, 5, min_len=min_len, speech_token_size=size, beams=4)):
+            want, total = search(lm, x, 4, 5, min_len, size)
+            assert tokens == want
+            assert abs(score - total) <= 1e-4
+
+
+@pytest.mark.parametrize("cache", ["float16", "bfloat16"])
+def test_two_byte_caches(gpu, cache):
+    """Scores of the tokens that were chosen: keys and values off by half a step of their type (2^-11, 2^-8) move a
+    score q.k by that share of sum |q k|, and through two layers the log probabilities by less than ten such shares."""
+    from cv3amd.qwen2 import DeviceQwen2
+    lm, store = setup("per_channel")
+    d = DeviceQwen2(store, cap=64)
+    xs = prompts(np.random.default_rng(4), (40, 9))
+    for x, (tokens, score) in zip(xs, d.generate_batch(xs, 5, min_len=5, beams=2, cache=cache)):
+        total = sum(logp(lm, x, tokens[:i])[t] for i, t in enumerate(tokens))
+        assert len(tokens) == 5 and abs(score - total) <= 5 * 10 * (2.0 ** -11 if cache == "float16" else 2.0 ** -8)
+
+
+def test_refusals(gpu):
+    from cv3amd.qwen2 import DeviceQwen2
+    _, store = setup("per_channel")
+    d = DeviceQwen2(store, cap=64)
+    x = prompts(np.random.default_rng(5), (3,))
+    assert d.generate_batch([], 5) == []
+    for bad in (dict(prompts=[np.zeros((3, 10))], max_len=2), dict(prompts=[np.zeros((0, 896))], max_len=2),
+                dict(prompts=x, max_len=0), dict(prompts=x, max_len=2, beams=17), dict(prompts=x, max_len=2, beams=0),
+                dict(prompts=x, max_len=2, cache="int8"), dict(prompts=x, max_len=2, page=0),
+                dict(prompts=x, max_len=2, speech_token_size=7000)):
+        with pytest.raises(ValueError):
+            d.generate_batch(**bad)
