@@ -336,53 +336,44 @@ struct Share {
   int n, b;
 };
 
-// Every wave finds its workgroup's share by itself; a lane sums four sequences.
-__device__ __forceinline__ Share share_of(const AttnArgs& a, int w) {
-  const int lane = threadIdx.x & 63, per = a.kv_heads * a.gtiles;
-  Share s{};
-  int t[4];
-  int64_t up = 0, mine = 0, base = 0, total = 0;
-  auto scan = [&](int c) {
-    mine = 0;
+__device__ __forceinline__ int64_t wave_scan(int64_t v) {      // inclusive
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      t[i] = span_of(a, c + lane * 4 + i).tiles;
-      mine += t[i];
-    }
-    up = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t u = __shfl_up(up, o, kWave);
-      if (lane >= o) up += u;
-    }
-  };
-  for (int c = 0; c < a.batch; c += 256) {
-    scan(c);
-    total += uniform(__shfl(up, 63, kWave));
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t u = __shfl_up(v, o, kWave);
+    if (lane >= o) v += u;
   }
-  s.units = total * per;
+  return v;
+}
+
+// Every wave finds its workgroup's share by itself: a lane sums a 64th of the sequences, the lane
+// that holds the share's first unit is found, then the sequence among that lane's.
+__device__ __forceinline__ Share share_of(const AttnArgs& a, int w) {
+  const int lane = threadIdx.x & 63, per = a.kv_heads * a.gtiles, each = (a.batch + 63) / 64;
+  Share s{};
+  int64_t mine = 0;
+#pragma unroll 4
+  for (int i = 0; i < each; ++i) mine += span_of(a, lane * each + i).tiles;
+  int64_t up = wave_scan(mine);
+  s.units = uniform(__shfl(up, 63, kWave)) * per;
   s.n = (int)min((int64_t)a.groups, s.units);
   if (w >= s.n) return s;
   s.at = s.units * w / s.n;
   s.end = s.units * (w + 1) / s.n;
   const int64_t want = s.at / per;
-  for (int c = 0; c < a.batch; c += 256) {
-    if (a.batch > 256) scan(c);
-    int64_t ahead = base + up - mine, first = 0;
-    int in = -1;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (want >= ahead && want < ahead + t[i]) in = c + lane * 4 + i, first = ahead;
-      ahead += t[i];
-    }
-    const uint64_t hit = __ballot(in >= 0);
+  int from = __ffsll((unsigned long long)__ballot(want < up)) - 1;     // the first lane that passes it
+  s.before = uniform(__shfl(up - mine, from, kWave));
+  s.b = uniform(from) * each;
+  for (int i = 0; each > 1 && i < each; i += 64) {
+    const int64_t t = i + lane < each ? span_of(a, s.b + i + lane).tiles : 0;
+    up = s.before + wave_scan(t);
+    const uint64_t hit = __ballot(want < up);
+    from = hit ? __ffsll((unsigned long long)hit) - 1 : 63;
+    s.before = uniform(__shfl(hit ? up - t : up, from, kWave));
     if (hit) {
-      const int from = __ffsll((unsigned long long)hit) - 1;
-      s.b = uniform(__shfl(in, from, kWave));
-      s.before = uniform(__shfl(first, from, kWave));
+      s.b += i + uniform(from);
       break;
     }
-    base += uniform(__shfl(up, 63, kWave));
   }
   return s;
 }

@@ -15,6 +15,11 @@ everything else may be a NumPy array, uploaded for the call, and results come ba
 as NumPy arrays where the first argument was one.  ``out`` takes the results' arrays from the caller.
 Calls are enqueued on the calling thread's stream and do not synchronise; lengths, page ids and slots are
 read on the device and checked there.
+
+``attention`` over long caches and ``beam_select`` take scratch from the allocator.  Captured into a graph they
+take it from the allocator's cache, and the graph keeps it: run them once eagerly before each capture.  Where the
+cache has none, ``beam_select`` raises ``ScratchError`` and ``attention`` runs one workgroup a (sequence, kv head),
+which is slow for few long sequences.
 """
 
 from __future__ import annotations

@@ -585,7 +585,8 @@ int cv3_paged_append(const float* rows, int64_t n, int64_t ld, int heads, int kv
 /* out[b] = softmax(scale q[b] . k_j) v_j over keys starts[b] <= j < lengths[b] (starts NULL: 0), one query a
  * sequence, heads a multiple of kv_heads.  Everything is float32 but the cache.  No key to see (an empty sequence, a
  * padding row, absent pages alone): zeros.  What lies in rows that are not seen, NaN too, reaches nothing.  Long
- * caches take scratch of the caching allocator, ordered on s. */
+ * caches take scratch of the caching allocator, ordered on s (a capture: from its cache, where it must be; without
+ * it one workgroup a pair walks the whole cache). */
 int cv3_paged_attention(const float* q, int64_t ldq, int64_t batch, int heads, int kv_heads, int d, int cache_type,
                         const void* k_cache, const void* v_cache, int64_t pages, int64_t page, const int32_t* tables,
                         int64_t blocks, const int32_t* lengths, const int32_t* starts, float scale, float* out,
@@ -596,7 +597,8 @@ int cv3_paged_attention(const float* q, int64_t ldq, int64_t batch, int heads, i
  * lower beam, in one beam the larger logit, then the lower token.  A value that is no number (a row with a NaN or
  * +inf, or all -inf; such a score) counts as -inf.  tokens, parents, scores_out and done_out are [requests, beams]
  * (scores_out may be scores, done_out may be done); done_out: the parent's, or a token of [stop_lo, stop_hi).
- * 1 to 16 beams, vocab up to 524288 with at least `beams` tokens to choose.  Takes scratch of the allocator. */
+ * 1 to 16 beams, vocab up to 524288 with at least `beams` tokens to choose.  Takes scratch of the allocator, as above
+ * (CV3_ENOMEM where a capture finds none). */
 int cv3_beam_select(const float* logits, int64_t requests, int beams, int64_t vocab, const float* scores,
                     const uint8_t* done, int64_t stop_lo, int64_t stop_hi, int64_t ban_lo, int64_t ban_hi, int64_t pad,
                     int64_t* tokens, int32_t* parents, float* scores_out, uint8_t* done_out, cv3_stream_t s);

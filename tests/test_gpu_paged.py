@@ -767,6 +767,34 @@ def test_calls_from_four_threads(gpu, paged):
     assert not wrong
 
 
+def test_attention_captured_without_scratch(gpu, paged):
+    """A capture takes scratch from the allocator's cache alone; where there is none, long caches run one workgroup a
+    pair.  The graph replays with eager calls in between."""
+    from cv3amd import _lib, device
+    rng = np.random.default_rng(15)
+    ins, want = attention_inputs(rng, 4, 1500, 200)
+    out = dev(np.zeros((4, 14, 64), np.float32))
+    device.synchronize()
+    _lib.call("empty_cache")
+    g = device.Graph()
+    with g:
+        paged.attention(*ins, out=out)
+    for _ in range(3):
+        out.zero_()
+        g.launch()
+        assert rel_err(out.numpy(), want) <= TOL
+        assert rel_err(paged.attention(*ins).numpy(), want) <= TOL
+
+
+@pytest.mark.parametrize("b", [63, 64, 65, 257, 1000, 4097, 9000])
+def test_attention_large_batches(paged, b):
+    """More sequences than lanes, and than lanes can hold one each: shares are found in a batch of any size."""
+    rng = np.random.default_rng(b)
+    lengths = np.where(rng.random(b) < 0.4, 0, rng.integers(1, 60, b))
+    lengths[rng.integers(0, b, 3)] = 700
+    check_attention(paged, lengths, 2, 1, 16, 16, 1700, "float16")
+
+
 class Step:
     """One beam-search step over a one-layer model that is nothing but the operators: rows and logits are drawn from
     tables by token, so that every step's inputs follow from the choices before it."""
@@ -833,12 +861,13 @@ def test_steps_captured_and_replayed(gpu, paged, kind):
         step.run(eager)
         want.append({n: eager[n].numpy() for n in names})
     states, graphs = [step.state(), step.state()], []
+    other = step.state()
     for s in states:
+        step.run(other)                 # leaves scratch in the allocator's cache, which the capture then owns
         g = device.Graph()
         with g:
             step.run(s)
         graphs.append(g)
-    other = step.state()
     for i in range(6):
         for s, g in zip(states, graphs):
             g.launch()
