@@ -497,15 +497,30 @@ __device__ __forceinline__ void load_q(const AttnArgs& a, const float* q, bool o
   }
 }
 
-// The running maximum moves only when a score passes it by more than 2^8: weights stay below 2^8 and
-// float32 sums lose nothing by it.  Returns the factor for what has been summed (1: nothing moved).
-__device__ __forceinline__ float raise(float mx, float& top) {
-  if (!__any(!(mx <= top + 8.f) && mx != -INFINITY)) return 1.f;     // NaN scores too: they reach the output
+// The running maximum moves only when a score passes it by more than 2^slack: with 8, weights stay below
+// 2^8, and float32 sums lose nothing by it but their top eight powers of two.  Returns the factor for
+// what has been summed (1: nothing moved).
+__device__ __forceinline__ float raise(float mx, float& top, float slack) {
+  if (!__any(!(mx <= top + slack) && mx != -INFINITY)) return 1.f;   // NaN scores too: they reach the output
   float t = fmaxf(mx, __shfl_xor(mx, 16, kWave));
   t = fmaxf(fmaxf(t, __shfl_xor(t, 32, kWave)), top);
   const float f = weight_of(top, t);
   top = t;
   return f;
+}
+
+// Whether what a wave has summed, for the heads that there are, is finite and small enough for the sums of
+// hundreds of waves.
+template <int NJ>
+__device__ __forceinline__ bool in_bounds(const Wave<NJ>& w, bool on) {
+  bool bad = !(w.sum < 0x1p110f);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bad = bad || !(fabsf(w.o[j][c][r]) < 0x1p110f);
+  return !__any(on && bad);
 }
 
 // Strips s, s + NW, .. on the float32 matrix cores, whatever the cache's type: 16x16x4 products take
@@ -517,7 +532,7 @@ __device__ __forceinline__ float raise(float mx, float& top) {
 // is 16 contiguous bytes, V with the output channels permuted alike (64 jj + 4 m + c in tile (jj, c)).
 template <typename E, int NJ, bool FULL, int NW>
 __device__ __forceinline__ void strips_f32(const AttnArgs& a, const Keys<E, NJ, FULL>& keys, const float* q, bool on,
-                                           int s, Wave<NJ>& w) {
+                                           int s, float slack, Wave<NJ>& w) {
   typedef Keys<E, NJ, FULL> K;
   float qf[K::NK * K::KC];
 #pragma unroll
@@ -552,7 +567,7 @@ __device__ __forceinline__ void strips_f32(const AttnArgs& a, const Keys<E, NJ, 
 #pragma unroll
       for (int i = 0; i < 4; ++i) sc[i] = ov[i] >= 0 ? sc[i] : -INFINITY;
     }
-    const float f = raise(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), w.top);
+    const float f = raise(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), w.top, slack);
     if (__any(f != 1.f)) {
       w.sum *= f;
 #pragma unroll
@@ -624,10 +639,10 @@ struct Planes<_Float16> {    // two planes of 11 bits, the second 2^11 times wha
 // one product, keys 4g .. 4g + 3 of each in lane group g: the weights' planes again stay in their
 // lanes, and V's four rows a lane are turned into channels by eight byte permutations a 4 x 4 block.
 // float16 weights are held 2^7 up and queries scaled to one by their head's largest, so that both
-// planes stay in float16's range.  False where the outputs are not finite (an infinity or a NaN
-// among what is seen, whose planes are not its own): the caller forms them in float32.
+// planes stay in float16's range.  An infinity among what is seen has no planes of its own: the caller
+// forms outputs that are not finite again in float32.
 template <typename E, int NJ, bool FULL, int NW>
-__device__ __forceinline__ bool strips_16(const AttnArgs& a, const Keys<E, NJ, FULL>& keys, const float* q, bool on,
+__device__ __forceinline__ void strips_16(const AttnArgs& a, const Keys<E, NJ, FULL>& keys, const float* q, bool on,
                                           int s, Wave<NJ>& w) {
   typedef Keys<E, NJ, FULL> K;
   typedef Planes<E> P;
@@ -716,7 +731,7 @@ __device__ __forceinline__ bool strips_16(const AttnArgs& a, const Keys<E, NJ, F
     }
     float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
     mx = fmaxf(mx, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-    const float f = raise(mx, w.top);
+    const float f = raise(mx, w.top, 8.f);
     if (__any(f != 1.f)) {
       w.sum *= f;
 #pragma unroll
@@ -763,17 +778,13 @@ __device__ __forceinline__ bool strips_16(const AttnArgs& a, const Keys<E, NJ, F
       next[t] = after[t];
     }
   }
-  float none = w.sum * 0.f;
+  if constexpr (kHalf) {
 #pragma unroll
-  for (int j = 0; j < NJ; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if constexpr (kHalf) w.o[j][c] = (low[j][c] * 0x1p-11f + w.o[j][c]) * 0x1p-7f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) none += w.o[j][c][r] * 0.f;
-    }
-  if constexpr (kHalf) w.sum *= 0x1p-7f;
-  return !__any(on && none != 0.f);
+      for (int c = 0; c < 4; ++c) w.o[j][c] = (low[j][c] * 0x1p-11f + w.o[j][c]) * 0x1p-7f;
+    w.sum *= 0x1p-7f;
+  }
 }
 
 // Attention of up to 16 query heads that share kv head `kvh` over strips [s0, s1) of sequence b, by
@@ -790,11 +801,19 @@ __device__ __forceinline__ void attend(const AttnArgs& a, int b, int kvh, int gt
   const float* q = a.q + (int64_t)b * a.ldq + (int64_t)(on ? head : 0) * d;
   const Keys<E, NJ, FULL> keys(a, b, kvh, sp, s1);
   Wave<NJ> w;
+  // What is not finite, or near the largest float, is formed again in float32 with weights of at most one:
+  // the slack alone may have brought it there.
+  float slack = 8.f;
+  bool fine = false;
   if constexpr (sizeof(E) == 2) {
-    if (!strips_16<E, NJ, FULL, NW>(a, keys, q, on, s0 + wv, w))
-      strips_f32<E, NJ, FULL, NW>(a, keys, q, on, s0 + wv, w);
-  } else {
-    strips_f32<E, NJ, FULL, NW>(a, keys, q, on, s0 + wv, w);
+    strips_16<E, NJ, FULL, NW>(a, keys, q, on, s0 + wv, w);
+    fine = in_bounds(w, on);
+    slack = 0.f;
+  }
+#pragma unroll 1
+  for (; !fine; slack = 0.f) {
+    strips_f32<E, NJ, FULL, NW>(a, keys, q, on, s0 + wv, slack, w);
+    fine = slack == 0.f || in_bounds(w, on);
   }
   float sum = w.sum;
   sum += __shfl_xor(sum, 16, kWave);

@@ -47,6 +47,8 @@ def new_cache(pages: int, kv_heads: int, page: int, dim: int, dtype="float32", l
 
 def _in(x, dtype, name, shape=None) -> DeviceArray:
     """An input on the device, of the type and shape that the call takes."""
+    if x.__class__ is DeviceArray and x.dtype is dtype and (shape is None or x.shape == shape):
+        return x        # on every call's path
     if not isinstance(x, DeviceArray):
         a = np.asarray(x)
         if dtype.kind != "f" and a.size:
@@ -54,7 +56,7 @@ def _in(x, dtype, name, shape=None) -> DeviceArray:
             if a.dtype.kind not in "iub" or int(a.min()) < lim.min or int(a.max()) > lim.max:
                 raise ValueError(f"{name} does not hold whole numbers of {dtype}")
         x = to_device(np.ascontiguousarray(a, dtype=dtype))
-    elif x.dtype is not dtype and x.dtype != dtype:
+    elif x.dtype != dtype:
         raise TypeError(f"{name} holds {x.dtype}, not {dtype}")
     if shape is not None and x.shape != shape:
         raise ValueError(f"{name} has the shape {x.shape}, not {shape}")
@@ -68,13 +70,19 @@ def _held(x, dtype, name, shape=None) -> DeviceArray:
     return _in(x, dtype, name, shape)
 
 
-def _outs(out, shapes, names):
-    """The results' arrays: new ones, or the caller's."""
+def _out(x, shape, dtype, name) -> DeviceArray:
+    """A result's array: a new one, or the caller's."""
+    if x.__class__ is DeviceArray and x.dtype is dtype and x.shape == shape:
+        return x
+    return DeviceArray(shape, dtype) if x is None else _held(x, dtype, name, shape)
+
+
+def _outs(out, n):
     if out is None:
-        return [DeviceArray(s, t) for s, t in shapes]
-    if len(out) != len(shapes):
-        raise ValueError(f"out takes {len(shapes)} arrays, got {len(out)}")
-    return [_held(o, t, n, s) for o, (s, t), n in zip(out, shapes, names)]
+        return (None,) * n
+    if len(out) != n or any(x is None for x in out):
+        raise ValueError(f"out takes {n} arrays")
+    return out
 
 
 def _cache(k, v, ndim=4):
@@ -89,9 +97,6 @@ def _cache(k, v, ndim=4):
 
 def _given(x, like):
     return x if isinstance(like, DeviceArray) else x.numpy()
-
-
-_TABLE_OUTS = ("total", "taken", "starts", "slots", "positions")
 
 
 def block_tables(lengths, new, page: int, free, taken, tables: DeviceArray, tokens: Optional[int] = None, out=None):
@@ -109,31 +114,33 @@ def block_tables(lengths, new, page: int, free, taken, tables: DeviceArray, toke
     if not isinstance(tables, DeviceArray) or tables.ndim != 2:
         raise TypeError("tables is a DeviceArray (requests, blocks)")
     r, blocks = tables.shape
+    given, out = out is not None, (None,) * 5 if out is None else out
+    if len(out) != 5 or given and any(x is None for i, x in enumerate(out) if i != 1 or free is not None):
+        raise ValueError("out takes five arrays: total, taken, starts, slots, positions")
     if tokens is None:
-        if out is not None and len(out) == 5:
+        if given:
             tokens = out[3].size
         elif isinstance(new, DeviceArray):
             raise ValueError("tokens, the length of the list, is needed with counts on the device")
         else:
             tokens = int(np.maximum(np.asarray(new, dtype=np.int64), 0).sum())
-    if out is not None and len(out) != 5:
-        raise ValueError(f"out takes 5 arrays, got {len(out)}")
     first = lengths
-    _held(tables, _I32, "tables")
+    tables = _in(tables, _I32, "tables")
     lengths, new = _in(lengths, _I32, "lengths", (r,)), _in(new, _I32, "new", (r,))
-    shapes = (((r,), _I32), ((1,), _I32), ((r + 1,), _I32), ((tokens,), _I64), ((tokens,), _I32))
-    if free is None:
-        outs = None if out is None else (out[0], *out[2:])
-        total, starts, slots, positions = _outs(outs, (shapes[0], *shapes[2:]), ("total", "starts", "slots", "positions"))
-        _lib.call("paged_tables", lengths.ptr, new.ptr, r, page, None, 0, None, tables.ptr, blocks, tokens, total.ptr,
-                  None, starts.ptr, slots.ptr, positions.ptr, None)
-        return _given(total, first), None, _given(starts, first), _given(slots, first), _given(positions, first)
-    free, taken = _in(free, _I32, "free"), _in(taken, _I32, "taken", (1,))
-    got = _outs(out, shapes, _TABLE_OUTS)
-    total, took, starts, slots, positions = got
-    _lib.call("paged_tables", lengths.ptr, new.ptr, r, page, free.ptr, free.size, taken.ptr, tables.ptr, blocks,
-              tokens, total.ptr, took.ptr, starts.ptr, slots.ptr, positions.ptr, None)
-    return tuple(_given(x, first) for x in got)
+    reserved = free is None
+    if reserved:
+        free_ptr, free_size, taken_ptr, took, took_ptr = None, 0, None, None, None
+    else:
+        free, taken = _in(free, _I32, "free"), _in(taken, _I32, "taken", (1,))
+        took = _out(out[1], (1,), _I32, "taken")
+        free_ptr, free_size, taken_ptr, took_ptr = free.ptr, free.size, taken.ptr, took.ptr
+    total, starts = _out(out[0], (r,), _I32, "total"), _out(out[2], (r + 1,), _I32, "starts")
+    slots, positions = _out(out[3], (tokens,), _I64, "slots"), _out(out[4], (tokens,), _I32, "positions")
+    _lib.call("paged_tables", lengths.ptr, new.ptr, r, page, free_ptr, free_size, taken_ptr, tables.ptr, blocks, tokens,
+              total.ptr, took_ptr, starts.ptr, slots.ptr, positions.ptr, None)
+    if isinstance(first, DeviceArray):
+        return total, took, starts, slots, positions
+    return total.numpy(), None if reserved else took.numpy(), starts.numpy(), slots.numpy(), positions.numpy()
 
 
 def append(rows, heads: int, positions, slots, cos, sin, k_cache: DeviceArray, v_cache: DeviceArray, out=None):
@@ -159,7 +166,7 @@ def append(rows, heads: int, positions, slots, cos, sin, k_cache: DeviceArray, v
         if cos.ndim != 2 or cos.shape[1] != d:
             raise ValueError(f"rotary tables are (rows, {d}), got {cos.shape}")
         sin = _in(sin, _F32, "sin", cos.shape)
-    q = DeviceArray((n, heads, d)) if out is None else _held(out, _F32, "out", (n, heads, d))
+    q = _out(out, (n, heads, d), _F32, "out")
     _lib.call("paged_append", rows.ptr, n, rows.shape[1], heads, kv_heads, d, positions.ptr if turn else None,
               slots.ptr, cos.ptr if turn else None, sin.ptr if turn else None, cos.shape[0] if turn else 0, kind,
               k_cache.ptr, v_cache.ptr, pages, page, q.ptr, heads * d, None)
@@ -187,14 +194,11 @@ def attention(q, k_cache: DeviceArray, v_cache: DeviceArray, tables, lengths, st
         starts = _in(starts, _I32, "starts", (b,))
     if scale is None:
         scale = 1.0 / math.sqrt(d)
-    o = DeviceArray(q.shape) if out is None else _held(out, _F32, "out", q.shape)
+    o = _out(out, q.shape, _F32, "out")
     _lib.call("paged_attention", q.ptr, h * d, b, h, kv_heads, d, kind, k_cache.ptr, v_cache.ptr, pages, page,
               tables.ptr, tables.shape[1], lengths.ptr, starts.ptr if starts is not None else None, float(scale),
               o.ptr, h * d, None)
     return _given(o, first)
-
-
-_SELECT_OUTS = ("tokens", "parents", "scores", "done")
 
 
 def beam_select(logits, scores, done, stop: Tuple[int, int], ban: Tuple[int, int] = (0, 0),
@@ -212,11 +216,12 @@ def beam_select(logits, scores, done, stop: Tuple[int, int], ban: Tuple[int, int
         raise ValueError(f"logits are (requests, beams, vocab), got {logits.shape}")
     r, w, v = logits.shape
     scores, done = _in(scores, _F32, "scores", (r, w)), _in(done, _U8, "done", (r, w))
-    shape = (r, w)
-    got = _outs(out, ((shape, _I64), (shape, _I32), (shape, _F32), (shape, _U8)), _SELECT_OUTS)
+    shape, out = (r, w), _outs(out, 4)
+    tokens, parents = _out(out[0], shape, _I64, "tokens"), _out(out[1], shape, _I32, "parents")
+    scored, ended = _out(out[2], shape, _F32, "scores"), _out(out[3], shape, _U8, "done")
     _lib.call("beam_select", logits.ptr, r, w, v, scores.ptr, done.ptr, stop[0], stop[1], ban[0], ban[1],
-              stop[0] if pad is None else pad, got[0].ptr, got[1].ptr, got[2].ptr, got[3].ptr, None)
-    return tuple(_given(x, first) for x in got)
+              stop[0] if pad is None else pad, tokens.ptr, parents.ptr, scored.ptr, ended.ptr, None)
+    return tuple(_given(x, first) for x in (tokens, parents, scored, ended))
 
 
 def beam_reorder(parents, tables: DeviceArray, own, lengths, k_cache: DeviceArray, v_cache: DeviceArray):

@@ -699,6 +699,29 @@ def test_attention_sizes_of_queries(paged, kind):
         assert rel_err(paged.attention(q, dev(ks), dev(vs), tables, lengths), want) <= TOL
 
 
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("blocks", [6, 300])
+@pytest.mark.parametrize("gap", [1.0, 5.0, 7.9, 30.0])
+def test_attention_values_near_the_largest_float(paged, kind, blocks, gap):
+    """A key whose weight is 2^gap times those before it, with values near the largest float: weights past one would
+    pass it."""
+    rng = np.random.default_rng(16)
+    lengths = np.array([90], I32)
+    tables, pages = batch(rng, lengths, blocks, 16)
+    q = np.zeros((1, 2, 64), np.float32)
+    q[:, :, 0] = 1.0
+    ks, vs = np.zeros((2, pages, 2, 16, 64), np.float32)
+    ks[tables[0, 5], :, 3, 0] = gap * np.log(2) * 8             # scale 1/8
+    vs[tables[0, 5], :, 3, ::2], vs[tables[0, 5], :, 3, 1::2] = 3e38, -3e38
+    for i in range(5):      # one such key more in each strip and wave, their values' sum within the float's range
+        ks[tables[0, i], :, 9, 0] = gap * np.log(2) * 8
+        vs[tables[0, i], :, 9] = 5e36
+    (ks, k64), (vs, v64) = stored(ks, kind), stored(vs, kind)
+    want = attention_ref(q, k64, v64, tables, lengths, None, 0.125)
+    got = paged.attention(q, dev(ks), dev(vs), tables, lengths)
+    assert np.isfinite(want).all() and rel_err(got, want) <= TOL
+
+
 @pytest.mark.parametrize("vocab", [500, 6761, 30000])
 def test_select_bans_whole_slices(paged, vocab):
     rng = np.random.default_rng(vocab)
