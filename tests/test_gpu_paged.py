@@ -210,6 +210,27 @@ def test_append(paged, n, heads, kv, d, page, kind):
     assert np.all(np.abs(values(v.numpy(), kind) - held_v) <= tol_v)
 
 
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+def test_append_of_many_rows(paged, kind):
+    """A call that moves more than 256 MB: the same values at both ends and in between."""
+    rng = np.random.default_rng(4)
+    n, heads, kv, d, page = 32001, 14, 2, 64, 16
+    pages = -(-n // page)
+    rows = rng.normal(size=(n, 18 * d)).astype(np.float32)
+    slots, positions = rng.permutation(pages * page)[:n].astype(I64), rng.integers(0, 500, n).astype(I32)
+    cos, sin = rotary(d, 500)
+    k, v = paged.new_cache(pages, kv, page, d, kind)
+    q = paged.append(rows, heads, positions, slots, cos, sin, k, v)
+    at = np.concatenate([np.arange(500), rng.integers(0, n, 2000), np.arange(n - 500, n)])
+    x = rows[at].astype(np.float64).reshape(len(at), 18, d)
+    want, bound = turn(x, cos.astype(np.float64)[positions[at]], sin.astype(np.float64)[positions[at]])
+    assert np.all(np.abs(q[at] - want[:, :heads]) <= bound[:, :heads])
+    got_k, got_v = (values(c.numpy(), kind).transpose(0, 2, 1, 3).reshape(-1, kv, d)[slots[at]] for c in (k, v))
+    k_want = want[:, heads:heads + kv]
+    assert np.all(np.abs(got_k - k_want) <= rounding(k_want, kind) * (1 + 2.0 ** -10) + bound[:, heads:heads + kv])
+    assert np.all(np.abs(got_v - x[:, heads + kv:]) <= rounding(x[:, heads + kv:], kind))
+
+
 def test_append_without_rotary_and_unaligned(paged):
     """No tables: q and k as they are, bit for bit.  Rows that start on any float, longer than the heads need; q in
     place of the rows'."""
