@@ -73,6 +73,17 @@ def test_greedy_batch_is_the_oracles_sequences(gpu, profile, page):
     assert d.generate_after_prefill(1, graph=False)[0] == int(logp(lm, xs[0], []).argmax())
 
 
+def test_prompts_longer_than_the_single_sequences_cache(gpu):
+    from cv3amd.device import to_device
+    from cv3amd.qwen2 import DeviceQwen2
+    lm, store = setup("per_channel")
+    d = DeviceQwen2(store, cap=64, prompt_planes=False)
+    xs = prompts(np.random.default_rng(6), (1100, 3))
+    for x, (tokens, _) in zip(xs, d.generate_batch([to_device(xs[0]), xs[1].astype(np.float64)], 2, min_len=2, page=64)):
+        first = int(logp(lm, x, [])[:SIZE].argmax())
+        assert tokens == [first, int(logp(lm, x, [first])[:SIZE].argmax())]
+
+
 def test_beam_search_is_the_plain_one(gpu):
     from cv3amd.qwen2 import DeviceQwen2
     lm, store = setup("per_channel")

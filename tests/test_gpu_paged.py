@@ -830,6 +830,22 @@ def test_attention_captured_without_scratch(gpu, paged):
         assert rel_err(paged.attention(*ins).numpy(), want) <= TOL
 
 
+def test_attention_of_empty_batches(paged):
+    """Nothing to see at all, with tables long enough for the split form."""
+    for lengths in ([0], [0, 0, 0], [0] * 300):
+        check_attention(paged, lengths, 14, 2, 64, 16, 300, "float32")
+    check_attention(paged, [500, 40, 7], 4, 2, 128, 16, 300, "bfloat16", starts=[500, 41, 2**31 - 1])
+    check_attention(paged, [0, 4000, 0], 14, 2, 64, 16, 300, "float16")
+
+
+def test_attention_in_place_of_its_queries(paged):
+    rng = np.random.default_rng(17)
+    for blocks in (60, 400):
+        (q, k, v, t, n), want = attention_inputs(rng, 7, 900, blocks)
+        assert paged.attention(q, k, v, t, n, out=q) is q
+        assert rel_err(q.numpy(), want) <= TOL
+
+
 @pytest.mark.parametrize("b", [63, 64, 65, 257, 1000, 4097, 9000])
 def test_attention_large_batches(paged, b):
     """More sequences than lanes, and than lanes can hold one each: shares are found in a batch of any size."""
