@@ -153,15 +153,16 @@ class _Stacked:
         return QWeight(self.q.ptr, self.scales.ptr, self.rows, self.k, self.kp, self.block,
                        _lib.F16 if self.sf16 else _lib.F32, _lib.KIND_Q4 if self.kind == "q4" else _lib.KIND_Q8)
 
-    def planes(self, span: int = 0, limit: int = 0):
-        """(fragments, scales) of every layer's rows for cv3_linear_code_planes, each layer packed on its
-        own; ``span`` / ``limit`` interleave rows as cv3_pack_code_planes does."""
+    def planes(self, span: int = 0, limit: int = 0, row0: int = 0, rows: Optional[int] = None):
+        """(fragments, scales) of every layer's rows (or rows [row0, row0 + rows)) for cv3_linear_code_planes, each
+        layer packed on its own; ``span`` / ``limit`` interleave rows as cv3_pack_code_planes does."""
         layers = self.q.shape[0] // self.rows
+        rows = self.rows - row0 if rows is None else rows
         nc, ns = ctypes.c_int64(), ctypes.c_int64()
-        _lib.call("code_planes_elems", self.rows, self.k, self.block, ctypes.byref(nc), ctypes.byref(ns))
+        _lib.call("code_planes_elems", rows, self.k, self.block, ctypes.byref(nc), ctypes.byref(ns))
         frag, scales = DeviceArray((layers, nc.value), np.uint16), DeviceArray((layers, ns.value))
         for l in range(layers):
-            kind, q, sc, sdt, kp, block, n = self.layer(l)
+            kind, q, sc, sdt, kp, block, n = self.layer(l, row0, rows)
             _lib.call("pack_code_planes", kind, q, n, self.k, sc, sdt, kp, block, span, limit,
                       frag.ptr + 2 * l * nc.value, scales.ptr + 4 * l * ns.value, None)
         return frag, scales
@@ -236,6 +237,7 @@ class DeviceQwen2:
         self.state = State(self.k_cache.ptr, self.v_cache.ptr, self.cap, p0, p0 + 8, p0 + 16, self.x.ptr,
                            self.logits.ptr, self.workspace.ptr, nws)
         self._prompt, self._prompt_arrays = None, []
+        self._batch = None    # the body's projections for generate_batch, packed on its first call
         if prompt_planes:
             try:
                 self._prompt = self._prompt_planes()
@@ -560,6 +562,27 @@ class DeviceQwen2:
         return [int(t) for t in ints[2 + pos + 1: 2 + pos + 1 + steps]]
 
     # -- several sequences, greedy or by beam search, over a paged cache ----
+    def _batch_planes(self) -> dict:
+        """The body's projections as code planes for rows of several sequences (cv3_linear_rows_planes), each in its own
+        row order: two bytes a code beside the decode's rows, o and down shared with the prompt's.  Empty for geometries
+        that the planes do not take, or without the memory: the decode's rows serve then (twice to four times the time
+        of a step)."""
+        if self._batch is None:
+            parts = {"qkv": (self.qkv, 0, None), "o": (self.o, 0, None), "gate": (self.gate_up, 0, self.inter),
+                     "up": (self.gate_up, self.inter, self.inter), "down": (self.down, 0, None)}
+            ok = all(w.k % 64 == 0 and w.k >= 256 and w.rows % 4 == 0 and (w.block in (32, 64) or w.block >= w.k)
+                     and w.kp % 16 == 0 for w, _, _ in parts.values()) and self.inter % 4 == 0
+            self._batch = {}
+            try:
+                shared = {"o": 2, "down": 6} if self._prompt is not None else {}
+                made = {n: tuple(self._prompt_arrays[shared[n]:shared[n] + 2]) if n in shared
+                        else w.planes(0, 0, row0, rows) for n, (w, row0, rows) in parts.items()} if ok else {}
+                self._batch = {n: (w, w.rows if rows is None else rows, *made[n])
+                               for n, (w, _, rows) in parts.items() if made}
+            except _lib.HIPError:    # out of memory
+                pass
+        return self._batch
+
     def _paged_layers(self, x: DeviceArray, pos, slots, tables, lengths, cos, sin, k: DeviceArray, v: DeviceArray):
         """The body over rows of any sequences (qwen2.py:139-179): each row's k and v go to its slot, and it sees the
         ``lengths`` keys of its own table row.  Returns the residual stream."""
@@ -570,13 +593,33 @@ class DeviceQwen2:
         u, a = DeviceArray((t, I)), DeviceArray((t, I))
         res = _lib.epilogue(residual=h.ptr, ld_res=D)
         swiglu = _lib.epilogue(act="silu", gate=u.ptr, gate_stride=I, rows_per_gate=1)
+        planes = self._batch_planes() if t > 1 else {}
+
+        def linear(name, x, y, ldy, bias=None, epi=None):
+            w, rows, frag, scales = planes[name]
+            _lib.call("linear_rows_planes", _lib.KIND_Q4 if w.kind == "q4" else _lib.KIND_Q8, x, t, w.k, w.k,
+                      frag.ptr + 2 * l * frag.shape[1], scales.ptr + 4 * l * scales.shape[1], w.block, rows, bias, y, ldy,
+                      ctypes.byref(epi) if epi is not None else None, None)
+
         for l in range(self.layers):
             kl, vl = (c.rows(l, l + 1).reshape(c.shape[1:]) for c in (k, v))
             _lib.call("rms_norm", h.ptr, self.ln1.ptr + l * D * 4, n.ptr, t, D, self.eps, None)
-            self._linear(n.ptr, t, self.qkv, l, qkv.ptr, R, bias=self.qkv_bias.ptr + l * R * 4)
+            bias = self.qkv_bias.ptr + l * R * 4
+            if planes:
+                linear("qkv", n.ptr, qkv.ptr, R, bias)
+            else:
+                self._linear(n.ptr, t, self.qkv, l, qkv.ptr, R, bias=bias)
             paged.append(qkv, H, pos, slots, cos, sin, kl, vl, out=q)
             paged.attention(q, kl, vl, tables, lengths, out=att)
-            self._after_attention(l, t, att, h, n, u, a, res, swiglu)
+            if not planes:
+                self._after_attention(l, t, att, h, n, u, a, res, swiglu)
+                continue
+            linear("o", att.ptr, h.ptr, D, None, res)
+            _lib.call("rms_norm", h.ptr, self.ln2.ptr + l * D * 4, n.ptr, t, D, self.eps, None)
+            linear("gate", n.ptr, a.ptr, I)
+            linear("up", n.ptr, u.ptr, I)
+            _lib.call("binary", 2, a.ptr, u.ptr, a.ptr, t * I, 0.0, 0.0, None)       # silu(gate) * up
+            linear("down", a.ptr, h.ptr, D, None, res)
         return h
 
     def _head(self, h: DeviceArray) -> DeviceArray:
