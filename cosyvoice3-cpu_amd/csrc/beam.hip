@@ -208,7 +208,7 @@ constexpr int kPickThreads = 512;
 constexpr int kLists = kBeams * 64;            // of a request: its beams' slices
 constexpr int kListsEach = kLists / kPickThreads;
 constexpr int kPicks = kBeams * kListsEach * kBeams;
-constexpr int kAhead = 4;                     // keys of a list that are loaded together
+constexpr int kEarly = 2;                     // candidates of a thread that are loaded with the heads
 
 // One workgroup per request; bound by the chain of its few loads.  The slices' lists are sorted, so
 // the best of a thread's lists are their heads.  As above, the W-th largest value of 64 groups of
@@ -230,9 +230,12 @@ __global__ __launch_bounds__(kPickThreads) void k_select_beams(SelectArgs a) {
   const int lists = a.beams * a.slices;
   // An ended beam's lists hold whatever the memory held: they are not looked at.
   const int64_t list0 = row0 * a.slices;
-  uint64_t mine[kAhead];                       // the first keys of this thread's first list
+  const uint64_t* keys = a.keys + list0 * a.beams;
+  const unsigned beams = (unsigned)a.beams, slices = (unsigned)a.slices, candidates = (unsigned)lists * beams;
+  const uint64_t head = tid < lists ? keys[tid * a.beams] : 0;
+  uint64_t early[kEarly];                      // this thread's first candidates, loaded with the heads
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) mine[i] = tid < lists && i < a.beams ? a.keys[(list0 + tid) * a.beams + i] : 0;
+  for (int i = 0; i < kEarly; ++i) early[i] = tid + i * kPickThreads < candidates ? keys[tid + i * kPickThreads] : 0;
 #pragma unroll 1
   for (int l = tid; l < lists; l += kPickThreads) {
     s_sum[l] = a.sums[list0 + l];
@@ -269,8 +272,8 @@ __global__ __launch_bounds__(kPickThreads) void k_select_beams(SelectArgs a) {
   Pick best{0, 0};
 #pragma unroll 1
   for (int l = tid; l < lists; l += kPickThreads) {
-    const int b = l / a.slices;
-    const Pick p = pick(b, l == b * a.slices, l == tid ? mine[0] : a.keys[(list0 + l) * a.beams]);
+    const unsigned b = (unsigned)l / slices;
+    const Pick p = pick(b, l == b * slices, l == tid ? head : keys[l * a.beams]);
     if (p > best) best = p;
   }
   s_best[tid] = best;
@@ -293,28 +296,17 @@ __global__ __launch_bounds__(kPickThreads) void k_select_beams(SelectArgs a) {
   Pick bar{(uint64_t)least << 32, 0};
 #pragma unroll 1
   for (bool whole = false;; whole = true) {
-    // Lists whose head passes the bar enter what of them does.
+    // Every candidate against the bar, a thread each.
 #pragma unroll 1
-    for (int l = tid; l < lists && !(bar > best); l += kPickThreads) {
-      const int b = l / a.slices;
-      uint64_t k[kAhead];
-      bool more = true;
-#pragma unroll 1
-      for (int r0 = 0; more && r0 < a.beams; r0 += kAhead) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          if (l == tid && r0 == 0) k[i] = mine[i];
-          else k[i] = r0 + i < a.beams ? a.keys[(list0 + l) * a.beams + r0 + i] : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const Pick p = r0 + i < a.beams ? pick(b, r0 + i == 0 && l == b * a.slices, k[i]) : Pick{0, 0};
-          more = more && p.hi && !(bar > p);          // sorted: what follows does not pass either
-          if (more) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kPicks) s_list[at] = p;
-          }
-        }
+    for (unsigned c = tid, i = 0; c < candidates; c += kPickThreads, ++i) {
+      const unsigned list = c / beams, b = list / slices;
+      if (s_high[list % kPickThreads] < (uint32_t)(bar.hi >> 32)) continue;      // the list's head does not pass
+      uint64_t k = early[0];
+      if (i > 0) k = i == 1 ? early[1] : keys[c];
+      const Pick p = pick(b, list * beams == c && list == b * slices, k);
+      if (p.hi && !(bar > p)) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kPicks) s_list[at] = p;
       }
     }
     __syncthreads();
