@@ -74,7 +74,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* red, uint32
 // workgroups), then lists a share of the tokens, four neighbours a thread.  A token finds its request
 // among the starts in LDS; the token that opens a page also enters it into the table.  Pages before
 // `have` are the request's own already; page have + i is free_pages[first + i].  Bound by the chain of
-// its loads: 4 us for a decode step of eight requests, 6 us for 384 prompts of up to 1200 tokens.
+// its loads: 4.9 us for a decode step of eight requests, 7.8 us for 384 prompts of up to 1200 tokens.
 __global__ __launch_bounds__(kTabThreads) void k_block_tables(TabArgs a) {
   __shared__ int32_t s_start[kTabRequests + 1];
   __shared__ int32_t s_first[kTabRequests];   // index of the request's first new page among the free ones
@@ -296,7 +296,7 @@ constexpr int kTile = 64;       // keys of a work unit
 constexpr int kStrip = 16;      // keys that one wave multiplies at a time
 constexpr int kWaves = 4;       // of an attention workgroup
 // Workgroups of the split form: two a CU are all resident at once, and fewer parts are left to join than
-// with more (3 x 100001 float16 keys: 39 us with 512, 37 with 768, 45 with 1024, 69 with 256; 96 ragged
+// with more (3 x 100001 float16 keys: 39 us with 512, 37 with 768, 45 with 1024; 96 ragged
 // sequences in bfloat16, 32 on 8 heads of 128: 236 us with 512, 250 with 768, 233 with 1024).
 constexpr int kGroups = 512;
 constexpr int64_t kWholeBytes = 192 << 10;
@@ -906,6 +906,10 @@ __global__ __launch_bounds__(kWholeWaves<NJ> * 64, (waves_per_simd<E, NJ>())) vo
                           s_ml);
 }
 
+// HBM-bound for large batches: 96 ragged sequences of up to 6000 bfloat16 keys, 32 on 8 heads of 128, 1.2 GB in
+// 231 us, 5.2 TB/s; 3 x 100001 float16 keys, 14 on 2 heads of 64, 36 us, 4.2 TB/s with its start; 24 x 1000 and
+// fewer keys by five dependent latencies, 6 - 9 us.
+//
 // The units of all sequences and heads, in order, shared out evenly over `groups` workgroups by the
 // lengths on the device: a ragged batch fills the machine as an even one does, and a captured
 // launch serves every length.  A pair (sequence, tile of heads) that one workgroup holds whole is
@@ -949,7 +953,8 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<E, NJ>())) void k_page
 
 constexpr int kJoinWaves = 4, kJoinAhead = 8;
 
-// One workgroup per (sequence, query head): the parts of a pair that crossed workgroups, and zeros
+// One workgroup per (sequence, query head), 2 us for one sequence, 5.4 for 42 heads of 85 parts each, 8 for
+// 3.1 thousand heads of one or two: the parts of a pair that crossed workgroups, and zeros
 // for a sequence with no key to see.  The waves take the parts in turn, eight at a time so that
 // their loads are in flight together, then meet in LDS.
 template <int NJ>

@@ -356,6 +356,25 @@ def test_attention_pages(paged, h, kv, d, page):
     check_attention(paged, [1, 77, 2000, 129], h, kv, d, page, -(-4000 // page), "float32")
 
 
+def test_the_largest_page(paged):
+    """65536 keys a page, through all that address one: slots, the write, the attention, the move."""
+    page, kv, d = 65536, 1, 16
+    check_attention(paged, [70000, 5, 65536, 65537], 2, kv, d, page, 2, "float16")
+    k, v = paged.new_cache(2, kv, page, d)
+    own = np.array([[[0], [1]]], I32)
+    total, _, _, slots, pos = paged.block_tables(np.array([60000, 65535], I32), np.array([3, 4], I32), page, None, None,
+                                                 dev(own.reshape(2, 1)))
+    assert list(slots) == [60000, 60001, 60002, 2 * 65536 - 1, -1, -1, -1] and list(total) == [60003, 65536]
+    assert list(pos) == [60000, 60001, 60002, 65535, -1, -1, -1]
+    rows = np.random.default_rng(18).normal(size=(7, 4 * d)).astype(np.float32)
+    paged.append(rows, 2, None, slots, None, None, k, v)
+    assert np.array_equal(k.numpy()[0, 0, 60000:60003], rows[:3, 2 * d:3 * d])
+    assert np.array_equal(v.numpy()[1, 0, 65535], rows[3, 3 * d:])
+    paged.beam_reorder(np.array([[0, 0]], I32), dev(own), own, np.array([65535], I32), k, v)
+    assert np.array_equal(k.numpy()[1, 0, :65535], k.numpy()[0, 0, :65535]) and np.array_equal(
+        v.numpy()[1, 0, 65535], rows[3, 3 * d:])
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("lengths", [[1], [64], [500], [1024], [1025], [4096], [4097], [30011], [131072],
                                      [0, 0, 0], [1] * 130, [70000, 3, 0, 900], list(range(0, 1500, 7))])
