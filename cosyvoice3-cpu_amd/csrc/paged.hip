@@ -945,7 +945,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<E, NJ>())) void k_page
     __syncthreads();
     const int t0 = sp.lo / kTile + t, per_tile = kTile / kStrip;
     attend<E, NJ, FULL, kWaves>(a, b, p / a.gtiles, p % a.gtiles, sp, max(t0 * per_tile, sp.lo / kStrip),
-                                     min((t0 + take) * per_tile, (sp.hi + kStrip - 1) / kStrip), s_o, s_ml);
+                                min((t0 + take) * per_tile, (sp.hi + kStrip - 1) / kStrip), s_o, s_ml);
     at += take;
     in += take;
   }

@@ -20,12 +20,13 @@ Layout in HBM (L layers, D = hidden, dh = head_dim, I = intermediate):
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import List, Optional, Tuple
 
 import numpy as np
 
 from . import _lib, paged
-from .device import DeviceArray, Graph, to_device
+from .device import DeviceArray, Graph, synchronize, to_device
 
 c_i64, c_vp = ctypes.c_int64, ctypes.c_void_p
 
@@ -237,7 +238,8 @@ class DeviceQwen2:
         self.state = State(self.k_cache.ptr, self.v_cache.ptr, self.cap, p0, p0 + 8, p0 + 16, self.x.ptr,
                            self.logits.ptr, self.workspace.ptr, nws)
         self._prompt, self._prompt_arrays = None, []
-        self._batch = None    # the body's projections for generate_batch, packed on its first call
+        # the body's projections for generate_batch, packed on its first call
+        self._batch, self._batch_lock = None, threading.Lock()
         if prompt_planes:
             try:
                 self._prompt = self._prompt_planes()
@@ -567,20 +569,22 @@ class DeviceQwen2:
         row order: two bytes a code beside the decode's rows, o and down shared with the prompt's.  Empty for geometries
         that the planes do not take, or without the memory: the decode's rows serve then (twice to four times the time
         of a step)."""
-        if self._batch is None:
+        with self._batch_lock:
+            if self._batch is not None:
+                return self._batch
             parts = {"qkv": (self.qkv, 0, None), "o": (self.o, 0, None), "gate": (self.gate_up, 0, self.inter),
                      "up": (self.gate_up, self.inter, self.inter), "down": (self.down, 0, None)}
             ok = all(w.k % 64 == 0 and w.k >= 256 and w.rows % 4 == 0 and (w.block in (32, 64) or w.block >= w.k)
                      and w.kp % 16 == 0 for w, _, _ in parts.values()) and self.inter % 4 == 0
-            self._batch = {}
+            made = {}
             try:
                 shared = {"o": 2, "down": 6} if self._prompt is not None else {}
                 made = {n: tuple(self._prompt_arrays[shared[n]:shared[n] + 2]) if n in shared
                         else w.planes(0, 0, row0, rows) for n, (w, row0, rows) in parts.items()} if ok else {}
-                self._batch = {n: (w, w.rows if rows is None else rows, *made[n])
-                               for n, (w, _, rows) in parts.items() if made}
             except _lib.HIPError:    # out of memory
                 pass
+            synchronize()            # whole before a call on another thread's stream can read them
+            self._batch = {n: (w, w.rows if rows is None else rows, *made[n]) for n, (w, _, rows) in parts.items() if made}
         return self._batch
 
     def _paged_layers(self, x: DeviceArray, pos, slots, tables, lengths, cos, sin, k: DeviceArray, v: DeviceArray):

@@ -124,6 +124,41 @@ def test_two_byte_caches(gpu, cache):
         assert len(tokens) == 5 and abs(score - total) <= 5 * 10 * (2.0 ** -11 if cache == "float16" else 2.0 ** -8)
 
 
+def test_two_calls_at_once(gpu, monkeypatch):
+    """Two threads, each with its own stream: the weights' layout that the first call makes is whole before the other
+    reads it, and both answer as a call alone."""
+    import threading
+    from cv3amd import qwen2
+    _, store = setup("per_channel")
+    d = qwen2.DeviceQwen2(store, cap=64)
+    xs = prompts(np.random.default_rng(7), (21, 8, 30))
+    order, wait, pack = [], qwen2.synchronize, qwen2._Stacked.planes
+
+    def packing(self, *args):
+        order.append(("pack", d._batch is None))
+        return pack(self, *args)
+
+    def waiting():
+        order.append(("wait", d._batch is None))
+        wait()
+
+    monkeypatch.setattr(qwen2._Stacked, "planes", packing)
+    monkeypatch.setattr(qwen2, "synchronize", waiting)
+    got = [None, None]
+
+    def one(i):
+        got[i] = d.generate_batch(xs, 6, min_len=6, beams=2)
+
+    threads = [threading.Thread(target=one, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    # packed once, waited for, and seen by nobody before
+    assert [n for n, _ in order] == ["pack"] * (len(order) - 1) + ["wait"] and all(unseen for _, unseen in order)
+    assert got[0] == got[1] == d.generate_batch(xs, 6, min_len=6, beams=2)
+
+
 def test_refusals(gpu):
     from cv3amd.qwen2 import DeviceQwen2
     _, store = setup("per_channel")
