@@ -432,6 +432,10 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // 2^(x - top), 0 where x is -inf whatever top is
 __device__ __forceinline__ float weight_of(float x, float top) { return x == -INFINITY ? 0.f : exp2_fast(x - top); }
 
+// A maximum for keys that are there and score -inf every one, with a sum of 0: their softmax is 0 / 0 = NaN, unless
+// another part has a score that is a number, beside which it weighs nothing.  -inf says that no key is there.
+constexpr float kNoScore = -3.402823466e38f;
+
 // What one wave has of up to 16 query heads: lane (g, m) = (lane / 16, lane % 16) holds head m's
 // channels d = 64 jj + 16 g + 4 r + c in o[jj][c][r], its running maximum, and its keys' part of the sum.
 template <int NJ>
@@ -833,6 +837,12 @@ __device__ __forceinline__ void attend(const AttnArgs& a, int b, int kvh, int gt
   float sum = w.sum;
   sum += __shfl_xor(sum, 16, kWave);
   sum += __shfl_xor(sum, 32, kWave);
+  if (__any(on && w.top == -INFINITY)) {         // rare: no score that is a number.  Is there a key at all?
+    bool there = false;
+#pragma unroll 1
+    for (int s = s0 + wv; s < s1 && !there; s += NW) there = __any(keys.locate(s) >= 0);
+    if (there) w.top = fmaxf(w.top, kNoScore);
+  }
 
   // The waves' maxima and sums, then their outputs 64 channels at a time: s_o[wave][head][64 + 4].
   if (g == 0) {
@@ -864,7 +874,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, int b, int kvh, int gt
       const bool whole = s_ml[NW * 32] != 0.f;    // the pair's every key was here: this is the output
       if (c < d) {
         if (whole) {
-          a.out[(int64_t)b * a.ldo + (int64_t)(kvh * a.group + gt * a.htile + h) * d + c] = l != 0.f ? x / l : 0.f;
+          a.out[(int64_t)b * a.ldo + (int64_t)(kvh * a.group + gt * a.htile + h) * d + c] =
+              t != -INFINITY ? x / l : 0.f;
         } else {
           float* dst = a.part + ((int64_t)__float_as_int(s_ml[NW * 32 + 1]) * a.htile + h) * (d + 2);
           dst[c] = x;
@@ -1021,7 +1032,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_paged_join(AttnArgs a) {
       l += f * s_ml[2 * w + 1];
       y += f * s_o[w * NJ * 64 + c];
     }
-    out[c] = l != 0.f ? y / l : 0.f;
+    out[c] = t != -INFINITY ? y / l : 0.f;
   }
 }
 

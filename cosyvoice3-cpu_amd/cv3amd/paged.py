@@ -177,8 +177,8 @@ def attention(q, k_cache: DeviceArray, v_cache: DeviceArray, tables, lengths, st
               scale: Optional[float] = None, out=None):
     """One new token per sequence: softmax(scale q . k) v of ``q`` (batch, heads, dim) over the ``lengths[b]`` keys
     that ``tables[b]`` (batch, blocks) lists, from key ``starts[b]`` on (a window; default 0).  Query heads
-    share kv heads in groups.  A sequence with no key to see, such as a padding row, gives zeros; what lies in
-    rows that are not seen reaches nothing."""
+    share kv heads in groups.  A sequence with no key to see, such as a padding row, gives zeros, one whose
+    scores are all -inf NaN (0 / 0); what lies in rows that are not seen reaches nothing."""
     kind = _cache(k_cache, v_cache)
     pages, kv_heads, page, d = k_cache.shape
     first = q

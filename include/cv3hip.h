@@ -584,7 +584,7 @@ int cv3_paged_append(const float* rows, int64_t n, int64_t ld, int heads, int kv
                      float* q, int64_t ldq, cv3_stream_t s);
 /* out[b] = softmax(scale q[b] . k_j) v_j over keys starts[b] <= j < lengths[b] (starts NULL: 0), one query a
  * sequence, heads a multiple of kv_heads.  Everything is float32 but the cache.  No key to see (an empty sequence, a
- * padding row, absent pages alone): zeros.  What lies in rows that are not seen, NaN too, reaches nothing.  Long
+ * padding row, absent pages alone): zeros; keys whose scores are all -inf: NaN, as the softmax is 0 / 0.  What lies in rows that are not seen, NaN too, reaches nothing.  Long
  * caches take scratch of the caching allocator, ordered on s (a capture: from its cache, where it must be; without
  * it one workgroup a pair walks the whole cache). */
 int cv3_paged_attention(const float* q, int64_t ldq, int64_t batch, int heads, int kv_heads, int d, int cache_type,

@@ -993,3 +993,41 @@ def test_steps_against_the_reference(gpu, paged, kind):
         assert np.array_equal(s["len_r"].numpy(), n) and np.array_equal(s["len_w"].numpy(), np.repeat(n, W))
     for c, w in ((s["k"], k), (s["v"], v)):
         assert np.abs(values(c.numpy(), kind) - w).max() <= 2 * eps * np.abs(w).max()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("blocks", [4, 13, 400])
+@pytest.mark.parametrize("h,kv,d", [(14, 2, 64), (4, 2, 128)])
+def test_attention_of_scores_that_are_all_minus_infinity(paged, h, kv, d, blocks, kind):
+    """Keys that are there and whose scores are -inf every one: the softmax is 0 / 0, NaN, and not the zeros of a
+    sequence with no key to see.  One score that is a number takes it all, wherever it lies."""
+    rng = np.random.default_rng([d, blocks, 2])
+    n = min(16 * blocks, 3000) - 3
+    lengths = np.array([n, n, n, 1, n, n, 0, n], I32)
+    starts = np.array([0, 0, n - 9, 0, 0, 20, 0, 0], I32)
+    tables, pages = batch(rng, lengths, blocks, 16)
+    q = rng.normal(size=(8, h, d)).astype(np.float32)
+    q[..., 0] = 1.0
+    ks, vs = (rng.normal(size=(pages, kv, 16, d)).astype(np.float32) for _ in range(2))
+
+    def away(i, lo, hi, heads=slice(None)):
+        for j in range(lo, hi):
+            ks[tables[i, j // 16], heads, j % 16, 0] = -np.inf
+
+    away(0, 0, n)                       # every key
+    away(1, 0, n, 1)                    # of one kv head
+    away(2, n - 9, n)                   # every key of a window
+    away(3, 0, 1)                       # the only one
+    away(4, 0, n - 1)                   # all but the last, and all but the first
+    away(5, 21, n)
+    away(7, 0, n)                       # every key that is there: pages of the others are not
+    tables[7, ::2] = -1
+    (ks, k64), (vs, v64) = stored(ks, kind), stored(vs, kind)
+    with np.errstate(invalid="ignore"):
+        want = attention_ref(q, k64, v64, tables, lengths, starts, 1 / np.sqrt(d))
+    assert list(np.isnan(want).all(axis=(1, 2))) == [True, False, True, True, False, False, False, blocks > 1]
+    assert np.isnan(want[1, h // 2:]).all() and not want[6].any()
+    got = paged.attention(q, dev(ks), dev(vs), tables, lengths, starts=starts)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    fine = ~np.isnan(want)
+    assert rel_err(got[fine], want[fine]) <= TOL
