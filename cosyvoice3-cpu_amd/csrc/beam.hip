@@ -440,6 +440,10 @@ int cv3_beam_select(const float* logits, int64_t requests, int beams, int64_t vo
   if (requests == 0) return CV3_OK;
   CV3_REQUIRE(logits && scores && done && tokens && parents && scores_out && done_out, CV3_EINVAL, "null operand");
   const int64_t rows = requests * beams;
+  const double n = (double)rows;
+  const Run in[] = {{logits, 4 * n * vocab}, {scores, scores == scores_out ? 0 : 4 * n}, {done, done == done_out ? 0 : n}};
+  const Run out[] = {{tokens, 8 * n}, {parents, 4 * n}, {scores_out, 4 * n}, {done_out, n}};
+  CV3_REQUIRE(apart(out, in), CV3_EINVAL, "results that overlap: only scores_out may be scores, and done_out done");
   // 2048 logits a workgroup where 8192 would leave half the CUs idle (16 x 4 rows of 6761: 10.0 us a call
   // against 11.1; 64 x 4: 11.9 against 11.2; 2 x 8 of 128000: 13.8 against 12.3), and a list a lane is enough
   const int e = rows * ceil_div(vocab, 32 * kSelThreads) < 128 && vocab <= 64 * 8 * kSelThreads ? 8 : 32;
@@ -478,7 +482,11 @@ int cv3_beam_reorder(const int32_t* parents, int64_t requests, int beams, int32_
   if (requests == 0) return CV3_OK;
   CV3_REQUIRE(parents && tables && own && lengths && k_cache && v_cache, CV3_EINVAL, "null operand");
   CV3_REQUIRE(((uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0, CV3_EINVAL, "the caches must be 16-byte aligned");
-  CV3_REQUIRE(tables != own, CV3_EINVAL, "the beams' own pages are a table of their own");
+  const double n = (double)requests * beams,
+               cache = (double)layers * pages * kv_heads * page * d * (cache_type == CV3_F32 ? 4 : 2);
+  const Run in[] = {{parents, 4 * n}, {own, 4 * n * blocks}, {lengths, 4.0 * requests}};
+  const Run out[] = {{tables, 4 * n * blocks}, {k_cache, cache}, {v_cache, cache}};
+  CV3_REQUIRE(apart(out, in), CV3_EINVAL, "tables, caches, parents, lengths and the beams' own pages overlap");
   const int row_vecs = d * (cache_type == CV3_F32 ? 4 : 2) / 16;
   ReorderArgs a{parents, tables, own, lengths, (uint4*)k_cache, (uint4*)v_cache, pages, blocks, layers, beams, kv_heads,
                 (int)page, row_vecs, (int)ceil_div(page * row_vecs, 256), (int)ceil_div(blocks, 256)};

@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <string>
@@ -27,6 +28,39 @@ bool shut_down();
 // cached and the thread or st is capturing.
 int scratch_alloc(void** ptr, size_t bytes, hipStream_t st);
 int scratch_free(void* ptr, hipStream_t st);
+
+// Memory that a call reads or writes.  Doubles hold the sizes: those of a mistaken call may pass 2^63 bytes.
+struct Run {
+  const void* p;
+  double bytes;
+};
+inline bool overlap(const Run& a, const Run& b) {
+  const double x = (double)(uintptr_t)a.p, y = (double)(uintptr_t)b.p;
+  return a.p && b.p && a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
+}
+// Whether a call's results share nothing with its inputs or each other.
+template <int N, int M>
+bool apart(const Run (&out)[N], const Run (&in)[M]) {
+  for (int i = 0; i < N; ++i) {
+    for (int j = 0; j < M; ++j)
+      if (overlap(out[i], in[j])) return false;
+    for (int j = 0; j < i; ++j)
+      if (overlap(out[i], out[j])) return false;
+  }
+  return true;
+}
+// n rows of wa floats, la apart, against n of wb, lb apart: whether they are the same rows, or share nothing (rows of
+// one pitch may lie between each other).  A row that is rewritten by who reads it may be the same; what lies across
+// two rows may be written before it is read.
+inline bool rows_alike_or_apart(const float* a, int64_t la, int64_t wa, const float* b, int64_t lb, int64_t wb, int64_t n) {
+  const double pa = 4.0 * la, pb = 4.0 * lb, sa = 4.0 * wa, sb = 4.0 * wb;
+  if (a == b && (la == lb || n == 1)) return true;
+  if (!overlap({a, (n - 1) * pa + sa}, {b, (n - 1) * pb + sb})) return true;
+  if (n == 1 || la != lb) return false;
+  double at = fmod((double)(uintptr_t)b - (double)(uintptr_t)a, pa);
+  if (at < 0) at += pa;
+  return at >= sa && at + sb <= pa;
+}
 
 constexpr int kWave = 64;
 

@@ -1093,8 +1093,12 @@ int cv3_paged_tables(const int32_t* lengths, const int32_t* new_tokens, int64_t 
   CV3_REQUIRE(starts && (requests == 0 || (lengths && new_tokens && tables && total)) &&
                   (tokens == 0 || (slots && positions)) && (free_pages ? taken && taken_out : free_count == 0),
               CV3_EINVAL, "null operand");
-  CV3_REQUIRE((requests == 0 || (const void*)total != (const void*)lengths) && (!taken || taken_out != taken), CV3_EINVAL,
-              "total and taken_out are arrays of their own: every workgroup reads lengths and taken");
+  const double r = (double)requests, t = (double)tokens, one = free_pages ? 4 : 0;
+  const Run in[] = {{lengths, 4 * r}, {new_tokens, 4 * r}, {free_pages, 4.0 * free_count}, {taken, one}};
+  const Run out[] = {{tables, 4 * r * blocks}, {total, 4 * r}, {taken_out, one}, {starts, 4 * (r + 1)}, {slots, 8 * t},
+                     {positions, 4 * t}};
+  CV3_REQUIRE(apart(out, in), CV3_EINVAL,
+              "results that overlap: every workgroup reads the lengths, the counts and the free pages while others write");
   TabArgs a{lengths, new_tokens, free_pages, taken, tables, total, taken_out, starts, slots, positions,
             free_count, (int)requests, (int)page, (int)blocks, (int)tokens};
   const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(tokens, kTabThreads * kTabEach), 1024));
@@ -1118,6 +1122,10 @@ int cv3_paged_append(const float* rows, int64_t n, int64_t ld, int heads, int kv
   CV3_REQUIRE(!cos_tab || (positions && rope_rows >= 1), CV3_EINVAL, "the rotary needs positions and table rows");
   if (n == 0) return CV3_OK;
   CV3_REQUIRE(rows && slots, CV3_EINVAL, "null operand");
+  const double cache = (double)pages * page * kv_heads * d * elem_size(cache_type);
+  CV3_REQUIRE(!overlap({k_cache, cache}, {v_cache, cache}), CV3_EINVAL, "the caches of keys and values overlap");
+  CV3_REQUIRE(!q || rows_alike_or_apart(rows, ld, (int64_t)(heads + 2 * kv_heads) * d, q, ldq, (int64_t)heads * d, n),
+              CV3_EINVAL, "q and the rows overlap: q may be the rows themselves, at their pitch");
   AppendArgs a{rows, n, ld, positions, slots, cos_tab, sin_tab, rope_rows, k_cache, v_cache, pages * page, q, ldq,
                (int)page, heads, kv_heads, d};
   // four channels a thread where rows start on 16 bytes (the tables are read by single floats)
@@ -1149,6 +1157,8 @@ int cv3_paged_attention(const float* q, int64_t ldq, int64_t batch, int heads, i
               heads, d);
   if (batch == 0) return CV3_OK;
   CV3_REQUIRE(q && tables && lengths && out, CV3_EINVAL, "null operand");
+  CV3_REQUIRE(rows_alike_or_apart(q, ldq, (int64_t)heads * d, out, ldo, (int64_t)heads * d, batch), CV3_EINVAL,
+              "out and q overlap: out may be q itself, at its pitch");
   const int group = heads / kv_heads, htile = std::min(group, 16), gtiles = (group + htile - 1) / htile;
   AttnArgs a{q, ldq, k_cache, v_cache, tables, lengths, starts, out, ldo, nullptr, nullptr, pages, blocks, (int)batch, (int)page,
              heads, kv_heads, group, gtiles, htile, d, 0, scale * 1.4426950408889634f};

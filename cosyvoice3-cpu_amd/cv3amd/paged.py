@@ -110,7 +110,7 @@ def block_tables(lengths, new, page: int, free, taken, tables: DeviceArray, toke
     ``tokens`` may be left out for a NumPy ``new``, whose sum it then is, or with ``out``.  Tokens past a
     request's table, or past ``tokens``, are not given.  ``free`` None: the tables hold every page already (a
     search's reserved pages), none is taken, and the result's ``taken`` is None.  ``out``: those five arrays,
-    none of them ``lengths`` or ``taken`` themselves."""
+    which share no memory with each other, ``tables`` or the inputs."""
     if not isinstance(tables, DeviceArray) or tables.ndim != 2:
         raise TypeError("tables is a DeviceArray (requests, blocks)")
     r, blocks = tables.shape

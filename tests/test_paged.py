@@ -150,3 +150,79 @@ def test_python_checks_types_and_shapes():
             paged.block_tables(bad, n, 16, n, dev((1,), i32), t, tokens=5)
     with pytest.raises(ValueError):
         paged.new_cache(1, 1, 1, 8, dtype="float64")
+
+
+M = 1 << 28     # apart: further than any of these calls' arrays are long
+
+
+def tables_apart(**k):
+    return tables(**{**dict(lengths=M, new=2 * M, free=3 * M, taken=4 * M, tables=5 * M, total=6 * M, taken_out=7 * M,
+                            starts=8 * M, slots=9 * M, positions=10 * M), **k})
+
+
+def append_apart(**k):
+    return append(**{**dict(rows=M, positions=2 * M, slots=3 * M, cos=4 * M, sin=5 * M, k=6 * M, v=7 * M, q=8 * M), **k})
+
+
+def attention_apart(**k):
+    return attention(**{**dict(q=M, k=2 * M, v=3 * M, tables=4 * M, lengths=5 * M, out=6 * M), **k})
+
+
+def select_apart(**k):
+    return select(**{**dict(logits=M, scores=2 * M, done=3 * M, tokens=4 * M, parents=5 * M, scores_out=6 * M,
+                            done_out=7 * M), **k})
+
+
+def reorder_apart(**k):
+    return reorder(**{**dict(parents=M, tables=2 * M, own=3 * M, lengths=4 * M, k=5 * M, v=6 * M), **k})
+
+
+LD, QD, CACHE = 18 * 64 * 4, 14 * 64 * 4, 9 * 2 * 16 * 64 * 4      # bytes of a row, of its queries, of a layer's keys
+OVERLAPPING = [
+    # what every workgroup of the tables reads, while the first writes its results (3 requests, 4 blocks, 5 tokens)
+    *(tables_apart(**{out: at * M + off}) for at, size in ((1, 12), (2, 12), (3, 32), (4, 4)) for off in (0, size - 4)
+      for out in ("total", "starts", "taken_out", "positions", "tables")),
+    *(tables_apart(slots=at * M - off) for at in (1, 2, 3, 4) for off in (0, 36)),
+    tables_apart(total=5 * M + 44), tables_apart(starts=6 * M + 8), tables_apart(positions=9 * M + 36),
+    tables_apart(taken_out=8 * M + 12),
+    tables_apart(free=None, free_count=0, taken=None, taken_out=None, total=2 * M),
+    append_apart(v=6 * M), append_apart(v=6 * M + CACHE - 16), append_apart(k=7 * M + CACHE - 16),
+    append_apart(q=M, ldq=14 * 64), append_apart(q=M + 16), append_apart(q=M + QD, ldq=18 * 64),
+    append_apart(q=M + LD - 4, ldq=18 * 64, n=2), append_apart(q=M - QD + 4, ldq=14 * 64, n=1),
+    append_apart(q=M + 8 * LD, ldq=20 * 64, n=9),
+    attention_apart(out=M, ldo=15 * 64), attention_apart(out=M + 4), attention_apart(out=M + QD),
+    attention_apart(out=M + QD - 4, ldq=28 * 64, ldo=28 * 64), attention_apart(out=M + QD + 4, ldq=28 * 64, ldo=28 * 64),
+    attention_apart(out=M - 4, batch=1),
+    select_apart(scores_out=2 * M + 4), select_apart(done_out=3 * M + 7), select_apart(done_out=2 * M),
+    select_apart(tokens=2 * M), select_apart(parents=3 * M - 28), select_apart(tokens=M + 8 * 100 * 4 - 8),
+    select_apart(parents=4 * M + 60), select_apart(done_out=6 * M + 31),
+    select_apart(scores_out=2 * M, parents=2 * M),
+    reorder_apart(v=5 * M), reorder_apart(v=5 * M + 2 * CACHE - 16), reorder_apart(own=2 * M + 124),
+    reorder_apart(parents=2 * M), reorder_apart(lengths=2 * M + 64), reorder_apart(own=6 * M), reorder_apart(parents=5 * M + 64),
+]
+
+
+@pytest.mark.parametrize("args", OVERLAPPING, ids=lambda a: a[0])
+def test_results_that_overlap_are_refused(args):
+    """Workgroups run in any order: a result in the place of an input that another one reads would be a race."""
+    from cv3amd import _lib
+    with pytest.raises(ValueError, match="overlap"):
+        _lib.call(*args)
+
+
+def test_results_in_place_and_beside_are_not_refused():
+    """Queries in their own rows' place, results between rows of one pitch, neighbours: past the checks, to the launch
+    that fails here for want of a GPU."""
+    import torch
+    from cv3amd import _lib
+    if torch.cuda.device_count():
+        pytest.skip("addresses that stand for memory")
+    for args in (tables_apart(total=M + 12), tables_apart(starts=2 * M - 16), tables_apart(slots=10 * M - 40),
+                 append_apart(q=M, ldq=18 * 64), append_apart(q=M + LD, n=1), append_apart(v=6 * M + CACHE),
+                 append_apart(ld=32 * 64, ldq=32 * 64, q=M + LD), append_apart(ld=32 * 64, ldq=32 * 64, q=M - QD),
+                 attention_apart(out=M), attention_apart(out=M, ldo=15 * 64, batch=1), attention_apart(out=M + 2 * QD),
+                 attention_apart(out=M + QD, ldq=28 * 64, ldo=28 * 64), attention_apart(out=M - QD, ldq=30 * 64, ldo=30 * 64),
+                 select_apart(scores_out=2 * M, done_out=3 * M), select_apart(parents=2 * M + 32),
+                 reorder_apart(own=2 * M + 128), reorder_apart(v=5 * M + 2 * CACHE)):
+        with pytest.raises(RuntimeError):
+            _lib.call(*args)
