@@ -432,7 +432,8 @@ int cv3_beam_select(const float* logits, int64_t requests, int beams, int64_t vo
   CV3_REQUIRE(beams >= 1 && beams <= kBeams, CV3_EINVAL, "1 to %d beams, not %d", kBeams, beams);
   CV3_REQUIRE(vocab >= 1 && vocab <= kVocabMax, CV3_EINVAL, "a vocabulary of 1 to %d tokens, not %lld", kVocabMax,
               (long long)vocab);
-  CV3_REQUIRE(requests >= 0 && requests <= (1 << 23) && requests * beams <= (1 << 23) / ceil_div(vocab, 8 * kSelThreads), CV3_EINVAL,
+  // a launch has fewer than 2^32 threads: 512 a request, 256 a slice
+  CV3_REQUIRE(requests >= 0 && requests < (1 << 23) && requests * beams <= (1 << 23) / ceil_div(vocab, 8 * kSelThreads), CV3_EINVAL,
               "%lld requests of %d beams are too many for one call", (long long)requests, beams);
   const int64_t banned = std::max<int64_t>(0, std::min(ban_hi, vocab) - std::max<int64_t>(ban_lo, 0));
   CV3_REQUIRE(vocab - banned >= beams, CV3_EINVAL, "%lld tokens to choose from are fewer than %d beams",

@@ -1057,7 +1057,8 @@ void attention_for(const AttnArgs& a, bool whole, hipStream_t st) {
   }
 }
 
-constexpr int64_t kLaunchBlocks = 1 << 23;       // of at most 512 threads: a launch has fewer than 2^32 of them
+// Workgroups of a launch, which has fewer than 2^32 threads: one less where they have 512.
+constexpr int64_t kLaunchBlocks = 1 << 23;
 
 int elem_size(int type) { return type == CV3_F32 ? 4 : 2; }
 
@@ -1151,7 +1152,7 @@ int cv3_paged_attention(const float* q, int64_t ldq, int64_t batch, int heads, i
   CV3_REQUIRE(heads <= 65536, CV3_EINVAL, "at most 65536 query heads, not %d", heads);
   CV3_REQUIRE(blocks >= 1 && blocks <= (INT32_MAX - 65536) / page, CV3_EINVAL,
               "tables of %lld blocks of %lld keys pass 2^31 keys", (long long)blocks, (long long)page);
-  CV3_REQUIRE(batch >= 0 && batch <= kLaunchBlocks / heads, CV3_EINVAL, "%lld sequences of %d heads are too many for one call",
+  CV3_REQUIRE(batch >= 0 && batch <= (kLaunchBlocks - 1) / heads, CV3_EINVAL, "%lld sequences of %d heads are too many for one call",
               (long long)batch, heads);
   CV3_REQUIRE(ldq >= (int64_t)heads * d && ldo >= (int64_t)heads * d, CV3_EINVAL, "rows are too short for %d heads of %d",
               heads, d);

@@ -226,3 +226,16 @@ def test_results_in_place_and_beside_are_not_refused():
                  reorder_apart(own=2 * M + 128), reorder_apart(v=5 * M + 2 * CACHE)):
         with pytest.raises(RuntimeError):
             _lib.call(*args)
+
+
+@pytest.mark.parametrize("args", [
+    attention_apart(batch=1 << 23, heads=1, kv_heads=1, ldq=64, ldo=64, out=1 << 40, k=1 << 41, v=1 << 42),
+    attention_apart(batch=1 << 19, heads=16, kv_heads=16, ldq=1024, ldo=1024, out=1 << 40, k=1 << 41, v=1 << 42),
+    select_apart(requests=1 << 23, beams=1, logits=1 << 40, **{x: i << 41 for i, x in enumerate(
+        ("scores", "done", "tokens", "parents", "scores_out", "done_out"), 1)}),
+], ids=lambda a: a[0])
+def test_a_launch_of_all_its_threads_is_refused(args):
+    """2^23 workgroups of 512 threads are 2^32, one more than a launch has."""
+    from cv3amd import _lib
+    with pytest.raises(ValueError, match="too many"):
+        _lib.call(*args)
