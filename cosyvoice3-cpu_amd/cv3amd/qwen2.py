@@ -30,6 +30,10 @@ from .device import DeviceArray, Graph, synchronize, to_device
 
 c_i64, c_vp = ctypes.c_int64, ctypes.c_void_p
 
+# generate_batch: requests of one call of the block tables or the reordering, prompt tokens of one pass of the body
+# (3.6 GB of rows at Qwen2-0.5B's sizes)
+_TABLE_ROWS, _PROMPT_ROWS = 4096, 65536
+
 
 class QWeight(ctypes.Structure):
     _fields_ = [("q", c_vp), ("scales", c_vp), ("rows", c_i64), ("k", c_i64), ("kp", c_i64), ("block", c_i64),
@@ -626,6 +630,23 @@ class DeviceQwen2:
             linear("down", a.ptr, h.ptr, D, None, res)
         return h
 
+    @staticmethod
+    def _slots(lengths: DeviceArray, new: DeviceArray, counts, page: int, tables: DeviceArray):
+        """block_tables of reserved pages for any number of requests, ``counts`` the host's copy of ``new``: (total, slots,
+        positions).  Pages are taken from nobody, so requests can be listed in parts."""
+        n = lengths.shape[0]
+        if n <= _TABLE_ROWS:
+            total, _, _, slots, pos = paged.block_tables(lengths, new, page, None, None, tables, tokens=int(counts.sum()))
+            return total, slots, pos
+        ends = np.concatenate([[0], np.cumsum(counts, dtype=np.int64)])
+        total, slots, pos = DeviceArray((n,), np.int32), DeviceArray((ends[-1],), np.int64), DeviceArray((ends[-1],), np.int32)
+        for r0 in range(0, n, _TABLE_ROWS):
+            r1 = min(r0 + _TABLE_ROWS, n)
+            paged.block_tables(lengths.rows(r0, r1), new.rows(r0, r1), page, None, None, tables.rows(r0, r1),
+                               out=(total.rows(r0, r1), None, DeviceArray((r1 - r0 + 1,), np.int32),
+                                    slots.rows(ends[r0], ends[r1]), pos.rows(ends[r0], ends[r1])))
+        return total, slots, pos
+
     def _head(self, h: DeviceArray) -> DeviceArray:
         """Head logits of every row (llm.py:74-77)."""
         n, logits = DeviceArray(h.shape), DeviceArray((h.shape[0], self.vocab))
@@ -642,14 +663,18 @@ class DeviceQwen2:
         Returns each prompt's best tokens and the sum of their log probabilities, the stop id's included.
 
         The sequences share nothing with this object's own cache: theirs is paged (``cache`` "float32", "float16" or
-        "bfloat16"), a prompt's whole pages held once for its beams, and is not bound to 1024 positions."""
+        "bfloat16"), a prompt's whole pages held once for its beams, and is not bound to 1024 positions.  There may be
+        as many (prompts times beams) as one launch serves: 2^23 over the query heads, or over the head's slices of 2048
+        logits (599 thousand for Qwen2-0.5B); memory ends before, at 27 KB of logits a sequence."""
         xs = [x.numpy() if isinstance(x, DeviceArray) else np.asarray(x, np.float32) for x in prompts]
         if any(x.ndim != 2 or x.shape[1] != self.hidden or x.shape[0] < 1 for x in xs):
             raise ValueError(f"prompts are (T, {self.hidden}) embeddings")
         stop = (int(speech_token_size), min(int(speech_token_size) + 200, self.vocab))
-        if max_len < 1 or page < 1 or not 1 <= beams <= 16 or not 0 < stop[0] < stop[1]:
-            raise ValueError("generation takes at least one token, a page of one key, 1 to 16 beams, and stop ids inside "
-                             "the vocabulary")
+        if max_len < 1 or not 1 <= page <= 65536 or not 1 <= beams <= 16 or not 0 < stop[0] < stop[1]:
+            raise ValueError("generation takes at least one token, pages of 1 to 65536 keys, 1 to 16 beams, and stop ids "
+                             "inside the vocabulary")
+        if len(xs) * beams > (2**23 - 1) // max(self.heads, -(-self.vocab // 2048)):
+            raise ValueError(f"{len(xs)} prompts of {beams} beams are too many for one call")
         if not xs:
             return []
         r, w, dh = len(xs), int(beams), self.head_dim
@@ -663,20 +688,26 @@ class DeviceQwen2:
         own, tables = to_device(own_h), to_device(np.where(shared, own_h[:, :1], own_h))
         # the prompts: every token a row that sees its own sequence up to itself
         rows = np.repeat(np.arange(r), held)
-        _, _, _, slots, pos = paged.block_tables(to_device(np.zeros(r, np.int32)), held, page, None, None,
-                                                      to_device(own_h[:, 0]), tokens=len(rows))
+        _, slots, pos = self._slots(to_device(np.zeros(r, np.int32)), to_device(held), held, page, to_device(own_h[:, 0]))
         upto = np.concatenate([np.arange(1, n + 1) for n in held]).astype(np.int32)
-        h = self._paged_layers(to_device(np.concatenate(xs).astype(np.float32)), pos, slots, to_device(own_h[rows, 0]),
-                               to_device(upto), cos, sin, k, v)
+        ends, every = np.cumsum(held, dtype=np.int64), np.concatenate(xs).astype(np.float32)
         last = DeviceArray((r * w, self.hidden))
-        for i, at in enumerate(np.repeat(np.cumsum(held) - 1, w)):
-            _lib.call("copy_d2d", last.ptr + i * self.hidden * 4, h.ptr + int(at) * self.hidden * 4, self.hidden * 4, None)
+        part = min(_PROMPT_ROWS, (2**23 - 1) // self.heads)
+        for t0 in range(0, len(rows), part):       # a row's earlier keys are in the cache, wherever the cut is
+            t1 = min(t0 + part, len(rows))
+            h = self._paged_layers(to_device(every[t0:t1]), pos.rows(t0, t1), slots.rows(t0, t1),
+                                   to_device(own_h[rows[t0:t1], 0]), to_device(upto[t0:t1]), cos, sin, k, v)
+            for i in np.flatnonzero((ends > t0) & (ends <= t1)):
+                for j in range(w):
+                    _lib.call("copy_d2d", last.ptr + (int(i) * w + j) * self.hidden * 4,
+                              h.ptr + int(ends[i] - 1 - t0) * self.hidden * 4, self.hidden * 4, None)
         logits = self._head(last)
         scores_h = np.full((r, w), -np.inf, np.float32)                    # at first one beam a prompt lives
         scores_h[:, 0] = 0.0
         scores, done = to_device(scores_h), to_device(np.zeros((r, w), np.uint8))
         chosen, parents = DeviceArray((r, w), np.int64), DeviceArray((r, w), np.int32)
-        lengths, ones, x = to_device(np.repeat(held, w)), to_device(np.ones(r * w, np.int32)), DeviceArray((r * w, self.hidden))
+        each = np.ones(r * w, np.int32)
+        lengths, ones, x = to_device(np.repeat(held, w)), to_device(each), DeviceArray((r * w, self.hidden))
         trail = []
         for i in range(max_len):
             paged.beam_select(logits.reshape(r, w, self.vocab), scores, done, stop, stop if i < min_len else (0, 0),
@@ -684,12 +715,12 @@ class DeviceQwen2:
             trail.append((chosen.numpy(), parents.numpy()))
             if i + 1 == max_len or done.numpy().all():
                 break
-            if w > 1:
-                paged.beam_reorder(parents, tables, own, held + i, k, v)
+            for r0 in range(0, r if w > 1 else 0, _TABLE_ROWS):
+                r1 = min(r0 + _TABLE_ROWS, r)
+                paged.beam_reorder(parents.rows(r0, r1), tables.rows(r0, r1), own.rows(r0, r1), (held + i)[r0:r1], k, v)
             kind, q, sc, sdt, kp, block, n = self.emb.layer(0)
             _lib.call("embedding", kind, q, sc, sdt, n, self.hidden, kp, block, chosen.ptr, r * w, x.ptr, None)
-            lengths, _, _, slots, pos = paged.block_tables(lengths, ones, page, None, None, own.reshape(r * w, blocks),
-                                                           tokens=r * w)
+            lengths, slots, pos = self._slots(lengths, ones, each, page, own.reshape(r * w, blocks))
             h = self._paged_layers(x, pos, slots, tables.reshape(r * w, blocks), lengths, cos, sin, k, v)
             logits = self._head(h)
         best, out = scores.numpy(), []

@@ -171,3 +171,55 @@ def test_refusals(gpu):
                 dict(prompts=x, max_len=2, speech_token_size=7000)):
         with pytest.raises(ValueError):
             d.generate_batch(**bad)
+
+
+def greedy(lm, x, steps):
+    seen = []
+    for _ in range(steps):
+        seen.append(int(logp(lm, x, seen)[:SIZE].argmax()))
+    return seen
+
+
+def test_more_prompts_than_one_call_of_the_tables(gpu):
+    """4100 sequences: each step's slots are listed 4096 requests at a time."""
+    from cv3amd.qwen2 import DeviceQwen2
+    lm, store = setup("per_channel")
+    d = DeviceQwen2(store, cap=64)
+    few = prompts(np.random.default_rng(10), (1, 3, 2, 1))
+    xs = [few[0]] * 4095 + few + [few[0]]
+    got = d.generate_batch(xs, 3, min_len=3, page=2)
+    for at in (0, 4094, 4095, 4096, 4097, 4098, 4099):
+        assert got[at][0] == greedy(lm, xs[at], 3)
+    got = d.generate_batch([few[1]] * 300, 3, min_len=3, beams=14)      # 4200 sequences of 300 prompts
+    want, total = search(lm, few[1], 14, 3, 3, SIZE)
+    for tokens, score in (got[0], got[292], got[293], got[299]):
+        assert tokens == want and abs(score - total) <= 1e-4
+
+
+def test_batches_in_parts(gpu, monkeypatch):
+    """The limits of a call made small: slots of four requests and prompts of twenty tokens at a time, cuts inside a
+    prompt and between two."""
+    from cv3amd import qwen2
+    _, store = setup("per_channel")
+    d = qwen2.DeviceQwen2(store, cap=64)
+    xs = prompts(np.random.default_rng(11), (30, 1, 9, 20, 45, 2))
+    want = [d.generate_batch(xs, 5, min_len=5, beams=b, page=7) for b in (1, 3)]
+    monkeypatch.setattr(qwen2, "_TABLE_ROWS", 4)
+    monkeypatch.setattr(qwen2, "_PROMPT_ROWS", 20)
+    for b, w in zip((1, 3), want):
+        for (tokens, score), (expected, total) in zip(d.generate_batch(xs, 5, min_len=5, beams=b, page=7), w):
+            assert tokens == expected and abs(score - total) <= 1e-4
+
+
+def test_refused_before_any_work(gpu, monkeypatch):
+    """What a step would refuse is refused before memory is taken and a prompt is run."""
+    from cv3amd import paged
+    from cv3amd.qwen2 import DeviceQwen2
+    _, store = setup("per_channel")
+    d = DeviceQwen2(store, cap=64)
+    monkeypatch.setattr(paged, "new_cache", None)       # reached: TypeError
+    x, = prompts(np.random.default_rng(14), (2,))
+    for bad in (dict(prompts=[x], max_len=2, page=65537), dict(prompts=[x] * 600000, max_len=2),
+                dict(prompts=[x] * 40000, max_len=2, beams=16)):
+        with pytest.raises(ValueError):
+            d.generate_batch(**bad)
