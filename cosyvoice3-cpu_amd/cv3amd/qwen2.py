@@ -631,6 +631,18 @@ class DeviceQwen2:
         return h
 
     @staticmethod
+    def _reserve(held, beams: int, new: int, page: int):
+        """Pages for ``held`` keys a prompt and ``new`` more a beam: ids (prompts, beams, blocks), -1 behind a prompt's
+        last, and their number.  A prompt's whole pages are its beams' together, all others each beam's own."""
+        held = held.astype(np.int64)
+        shared, last = held // page, -(-(held + new) // page)
+        used = shared + beams * (last - shared)
+        base, j = (np.cumsum(used) - used)[:, None, None], np.arange(last.max())
+        shared, last = shared[:, None, None], last[:, None, None]
+        own = np.where(j < shared, base + j, base + shared + np.arange(beams)[None, :, None] * (last - shared) + j - shared)
+        return np.where(j < last, own, -1).astype(np.int32), int(used.sum())
+
+    @staticmethod
     def _slots(lengths: DeviceArray, new: DeviceArray, counts, page: int, tables: DeviceArray):
         """block_tables of reserved pages for any number of requests, ``counts`` the host's copy of ``new``: (total, slots,
         positions).  Pages are taken from nobody, so requests can be listed in parts."""
@@ -663,9 +675,10 @@ class DeviceQwen2:
         Returns each prompt's best tokens and the sum of their log probabilities, the stop id's included.
 
         The sequences share nothing with this object's own cache: theirs is paged (``cache`` "float32", "float16" or
-        "bfloat16"), a prompt's whole pages held once for its beams, and is not bound to 1024 positions.  There may be
-        as many (prompts times beams) as one launch serves: 2^23 over the query heads, or over the head's slices of 2048
-        logits (599 thousand for Qwen2-0.5B); memory ends before, at 27 KB of logits a sequence."""
+        "bfloat16") and not bound to 1024 positions.  A prompt's whole pages are held once for its beams; from there each
+        beam has its own for ``max_len`` tokens.  There may be as many sequences (prompts times beams) as one launch
+        serves: 2^23 over the query heads, or over the head's slices of 2048 logits (599 thousand for Qwen2-0.5B);
+        memory ends before, at 27 KB of logits a sequence."""
         xs = [x.numpy() if isinstance(x, DeviceArray) else np.asarray(x, np.float32) for x in prompts]
         if any(x.ndim != 2 or x.shape[1] != self.hidden or x.shape[0] < 1 for x in xs):
             raise ValueError(f"prompts are (T, {self.hidden}) embeddings")
@@ -680,12 +693,11 @@ class DeviceQwen2:
         r, w, dh = len(xs), int(beams), self.head_dim
         held = np.array([x.shape[0] for x in xs], np.int32)
         most = int(held.max()) + max_len
-        blocks = -(-most // page)
         cos, sin = (to_device(a) for a in rope_tables(dh, self.theta, most))
-        k, v = paged.new_cache(r * w * blocks, self.kv_heads, page, dh, cache, layers=self.layers)
-        own_h = np.arange(r * w * blocks, dtype=np.int32).reshape(r, w, blocks)
-        shared = np.arange(blocks) < (held // page)[:, None, None]         # a prompt's whole pages lie with beam 0
-        own, tables = to_device(own_h), to_device(np.where(shared, own_h[:, :1], own_h))
+        own_h, pages = self._reserve(held, w, max_len - 1, page)           # the last token's key is not asked for
+        blocks = own_h.shape[2]
+        k, v = paged.new_cache(pages, self.kv_heads, page, dh, cache, layers=self.layers)
+        own, tables = to_device(own_h), to_device(own_h)
         # the prompts: every token a row that sees its own sequence up to itself
         rows = np.repeat(np.arange(r), held)
         _, slots, pos = self._slots(to_device(np.zeros(r, np.int32)), to_device(held), held, page, to_device(own_h[:, 0]))

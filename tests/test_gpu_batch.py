@@ -223,3 +223,17 @@ def test_refused_before_any_work(gpu, monkeypatch):
                 dict(prompts=[x] * 40000, max_len=2, beams=16)):
         with pytest.raises(ValueError):
             d.generate_batch(**bad)
+
+
+def test_pages_that_are_reserved(gpu, monkeypatch):
+    """A prompt's whole pages once for its beams, and each beam's own from there to its last token: no more."""
+    from cv3amd import paged
+    from cv3amd.qwen2 import DeviceQwen2
+    _, store = setup("per_channel")
+    d = DeviceQwen2(store, cap=64)
+    made, new_cache = [], paged.new_cache
+    monkeypatch.setattr(paged, "new_cache", lambda pages, *a, **k: made.append(pages) or new_cache(pages, *a, **k))
+    lengths = (160, 3, 32, 47)
+    for beams, max_len in ((1, 6), (4, 6), (4, 1)):
+        d.generate_batch(prompts(np.random.default_rng(12), lengths), max_len, min_len=max_len, beams=beams, page=16)
+        assert made.pop() == sum(n // 16 + beams * (-(-(n + max_len - 1) // 16) - n // 16) for n in lengths)

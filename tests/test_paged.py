@@ -239,3 +239,20 @@ def test_a_launch_of_all_its_threads_is_refused(args):
     from cv3amd import _lib
     with pytest.raises(ValueError, match="too many"):
         _lib.call(*args)
+
+
+@pytest.mark.parametrize("held,beams,new,page", [([1], 1, 0, 1), ([160, 3, 32, 47], 4, 5, 16), ([16, 17, 15], 16, 0, 16),
+                                                 ([5, 70000], 3, 40, 65536), ([7, 1, 900], 2, 33, 5)])
+def test_reserved_pages(held, beams, new, page):
+    """Every key of a prompt and of what follows has a page; a prompt's whole pages are its beams' together, and no
+    other page is anybody else's."""
+    import numpy as np
+    from cv3amd.qwen2 import DeviceQwen2
+    own, pages = DeviceQwen2._reserve(np.array(held, np.int32), beams, new, page)
+    seen = []
+    for n, tables in zip(held, own):
+        whole, last = n // page, -(-(n + new) // page)
+        assert (tables[:, :last] >= 0).all() and (tables[:, last:] == -1).all()
+        assert (tables[:, :whole] == tables[0, :whole]).all()
+        seen += [*tables[0, :whole], *tables[:, whole:last].reshape(-1)]
+    assert sorted(seen) == list(range(pages)) and own.dtype == np.int32
