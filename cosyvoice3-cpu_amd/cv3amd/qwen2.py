@@ -158,18 +158,21 @@ class _Stacked:
         return QWeight(self.q.ptr, self.scales.ptr, self.rows, self.k, self.kp, self.block,
                        _lib.F16 if self.sf16 else _lib.F32, _lib.KIND_Q4 if self.kind == "q4" else _lib.KIND_Q8)
 
-    def planes(self, span: int = 0, limit: int = 0, row0: int = 0, rows: Optional[int] = None):
+    def plane_arrays(self, rows: int):
+        """(fragments, scales), empty, for ``rows`` rows of every layer: all the memory that ``planes`` takes."""
+        layers, nc, ns = self.q.shape[0] // self.rows, ctypes.c_int64(), ctypes.c_int64()
+        _lib.call("code_planes_elems", rows, self.k, self.block, ctypes.byref(nc), ctypes.byref(ns))
+        return DeviceArray((layers, nc.value), np.uint16), DeviceArray((layers, ns.value))
+
+    def planes(self, span: int = 0, limit: int = 0, row0: int = 0, rows: Optional[int] = None, arrays=None):
         """(fragments, scales) of every layer's rows (or rows [row0, row0 + rows)) for cv3_linear_code_planes, each
         layer packed on its own; ``span`` / ``limit`` interleave rows as cv3_pack_code_planes does."""
-        layers = self.q.shape[0] // self.rows
         rows = self.rows - row0 if rows is None else rows
-        nc, ns = ctypes.c_int64(), ctypes.c_int64()
-        _lib.call("code_planes_elems", rows, self.k, self.block, ctypes.byref(nc), ctypes.byref(ns))
-        frag, scales = DeviceArray((layers, nc.value), np.uint16), DeviceArray((layers, ns.value))
-        for l in range(layers):
+        frag, scales = self.plane_arrays(rows) if arrays is None else arrays
+        for l in range(frag.shape[0]):
             kind, q, sc, sdt, kp, block, n = self.layer(l, row0, rows)
             _lib.call("pack_code_planes", kind, q, n, self.k, sc, sdt, kp, block, span, limit,
-                      frag.ptr + 2 * l * nc.value, scales.ptr + 4 * l * ns.value, None)
+                      frag.ptr + 2 * l * frag.shape[1], scales.ptr + 4 * l * scales.shape[1], None)
         return frag, scales
 
     @property
@@ -286,8 +289,15 @@ class DeviceQwen2:
 
     @property
     def prompt_nbytes(self) -> int:
-        """Bytes held in HBM for ``prefill`` alone."""
+        """Bytes held in HBM for ``prefill``; o and down of them serve ``generate_batch`` too."""
         return sum(a.nbytes for a in self._prompt_arrays)
+
+    @property
+    def batch_nbytes(self) -> int:
+        """Bytes held in HBM for ``generate_batch`` besides: none before its first call on several rows, or where there
+        was no memory for them."""
+        prompt = {a.ptr for a in self._prompt_arrays}
+        return sum(a.nbytes for _, _, *arrays in (self._batch or {}).values() for a in arrays if a.ptr not in prompt)
 
     # -- weights streamed per token (the HBM roofline numerator) -----------
     def bytes_per_token(self, length: int) -> dict:
@@ -570,9 +580,9 @@ class DeviceQwen2:
     # -- several sequences, greedy or by beam search, over a paged cache ----
     def _batch_planes(self) -> dict:
         """The body's projections as code planes for rows of several sequences (cv3_linear_rows_planes), each in its own
-        row order: two bytes a code beside the decode's rows, o and down shared with the prompt's.  Empty for geometries
-        that the planes do not take, or without the memory: the decode's rows serve then (twice to four times the time
-        of a step)."""
+        row order: two bytes a code beside the decode's rows (``batch_nbytes``), o and down shared with the prompt's.
+        Empty for geometries that the planes do not take, or without the memory, which is asked for once: the decode's
+        rows serve then (twice to four times the time of a step)."""
         with self._batch_lock:
             if self._batch is not None:
                 return self._batch
@@ -580,13 +590,16 @@ class DeviceQwen2:
                      "up": (self.gate_up, self.inter, self.inter), "down": (self.down, 0, None)}
             ok = all(w.k % 64 == 0 and w.k >= 256 and w.rows % 4 == 0 and (w.block in (32, 64) or w.block >= w.k)
                      and w.kp % 16 == 0 for w, _, _ in parts.values()) and self.inter % 4 == 0
-            made = {}
+            shared = {"o": 2, "down": 6} if self._prompt is not None else {}
+            made = {n: tuple(self._prompt_arrays[at:at + 2]) for n, at in shared.items()} if ok else {}
+            new = [n for n in parts if n not in made] if ok else []
             try:
-                shared = {"o": 2, "down": 6} if self._prompt is not None else {}
-                made = {n: tuple(self._prompt_arrays[shared[n]:shared[n] + 2]) if n in shared
-                        else w.planes(0, 0, row0, rows) for n, (w, row0, rows) in parts.items()} if ok else {}
+                made.update({n: parts[n][0].plane_arrays(parts[n][2] or parts[n][0].rows) for n in new})
             except _lib.HIPError:    # out of memory
-                pass
+                made, new = {}, []
+            for n in new:
+                w, row0, rows = parts[n]
+                w.planes(0, 0, row0, rows, made[n])
             synchronize()            # whole before a call on another thread's stream can read them
             self._batch = {n: (w, w.rows if rows is None else rows, *made[n]) for n, (w, _, rows) in parts.items() if made}
         return self._batch

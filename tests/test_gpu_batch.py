@@ -237,3 +237,45 @@ def test_pages_that_are_reserved(gpu, monkeypatch):
     for beams, max_len in ((1, 6), (4, 6), (4, 1)):
         d.generate_batch(prompts(np.random.default_rng(12), lengths), max_len, min_len=max_len, beams=beams, page=16)
         assert made.pop() == sum(n // 16 + beams * (-(-(n + max_len - 1) // 16) - n // 16) for n in lengths)
+
+
+def test_weights_that_fail_to_be_packed(gpu, monkeypatch):
+    """Without memory the decode's weights serve; any other failure is the caller's to see, and the next call packs."""
+    from cv3amd import _lib, qwen2
+    from cv3amd.device import DeviceArray
+    _, store = setup("per_channel")
+    d = qwen2.DeviceQwen2(store, cap=64, prompt_planes=False)
+    xs = prompts(np.random.default_rng(13), (5, 8))
+    real = _lib.call
+
+    def call(name, *args):
+        if name == "pack_code_planes":
+            raise _lib.HIPError("kernel launch failed")
+        return real(name, *args)
+
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "call", call)
+        with pytest.raises(_lib.HIPError, match="launch failed"):
+            d.generate_batch(xs, 4, min_len=4)
+    want = d.generate_batch(xs, 4, min_len=4)
+    codes = 1152 * 896 + 896 * 896 + 9728 * 896 + 896 * 4864
+    assert d._batch and d.batch_nbytes == 2 * (2 * codes + 4 * (1152 + 896 + 9728 + 896))     # two layers
+    full = qwen2.DeviceQwen2(store, cap=64)
+    held = full.prompt_nbytes
+    assert full.batch_nbytes == 0
+    full.generate_batch(xs, 2)
+    assert full.prompt_nbytes == held        # o and down are the prompt's
+    assert full.batch_nbytes == 2 * (2 * (1152 + 9728) * 896 + 4 * (1152 + 9728))
+
+    class NoMemory(DeviceArray):
+        def __init__(self, shape, dtype=np.float32, *a, **k):
+            if np.dtype(dtype) == np.uint16:
+                raise _lib.HIPError("hipMalloc failed")
+            super().__init__(shape, dtype, *a, **k)
+
+    bare = qwen2.DeviceQwen2(store, cap=64, prompt_planes=False)
+    with monkeypatch.context() as m:
+        m.setattr(qwen2, "DeviceArray", NoMemory)
+        got = bare.generate_batch(xs, 4, min_len=4)
+    assert bare._batch == {} and bare.batch_nbytes == 0
+    assert [t for t, _ in got] == [t for t, _ in want] == [t for t, _ in bare.generate_batch(xs, 4, min_len=4)]
