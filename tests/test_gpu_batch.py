@@ -279,3 +279,32 @@ def test_weights_that_fail_to_be_packed(gpu, monkeypatch):
         got = bare.generate_batch(xs, 4, min_len=4)
     assert bare._batch == {} and bare.batch_nbytes == 0
     assert [t for t, _ in got] == [t for t, _ in want] == [t for t, _ in bare.generate_batch(xs, 4, min_len=4)]
+
+
+@pytest.mark.parametrize("profile", ["per_channel", "balanced", "tiny"])
+def test_one_prompt_alone(gpu, profile):
+    """One greedy prompt: a row a step, on the decode's own weights; also one of a single token."""
+    from cv3amd.qwen2 import DeviceQwen2
+    lm, store = setup(profile)
+    d = DeviceQwen2(store, cap=64)
+    for x in prompts(np.random.default_rng(8), (23, 1)):
+        (tokens, _), = d.generate_batch([x], 6, min_len=6)
+        assert tokens == greedy(lm, x, 6)
+    assert d.generate_batch([x], 1, min_len=1)[0][0] == greedy(lm, x, 1)
+
+
+@pytest.mark.parametrize("profile", ["per_channel", "balanced", "tiny"])
+def test_without_the_code_planes(gpu, profile):
+    """Several prompts on the decode's own weights, as where the planes find no memory: the planes' tokens."""
+    from cv3amd.qwen2 import DeviceQwen2
+    lm, store = setup(profile)
+    d = DeviceQwen2(store, cap=64)
+    xs = prompts(np.random.default_rng(9), (30, 1, 9))
+    want = [d.generate_batch(xs, 6, min_len=6, beams=b) for b in (1, 3)]
+    assert d._batch
+    bare = DeviceQwen2(store, cap=64, prompt_planes=False)
+    bare._batch = {}
+    for b, w in zip((1, 3), want):
+        for (tokens, score), (expected, total) in zip(bare.generate_batch(xs, 6, min_len=6, beams=b), w):
+            assert tokens == expected and abs(score - total) <= 1e-4
+    assert [t for t, _ in want[0]] == [greedy(lm, x, 6) for x in xs]
