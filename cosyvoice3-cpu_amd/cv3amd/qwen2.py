@@ -699,6 +699,8 @@ class DeviceQwen2:
         if max_len < 1 or not 1 <= page <= 65536 or not 1 <= beams <= 16 or not 0 < stop[0] < stop[1]:
             raise ValueError("generation takes at least one token, pages of 1 to 65536 keys, 1 to 16 beams, and stop ids "
                              "inside the vocabulary")
+        if self.vocab - (stop[1] - stop[0] if min_len > 0 else 0) < beams:
+            raise ValueError(f"the vocabulary has fewer tokens to choose from than {beams} beams")
         if len(xs) * beams > (2**23 - 1) // max(self.heads, -(-self.vocab // 2048)):
             raise ValueError(f"{len(xs)} prompts of {beams} beams are too many for one call")
         if not xs:

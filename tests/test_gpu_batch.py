@@ -223,6 +223,12 @@ def test_refused_before_any_work(gpu, monkeypatch):
                 dict(prompts=[x] * 40000, max_len=2, beams=16)):
         with pytest.raises(ValueError):
             d.generate_batch(**bad)
+    monkeypatch.setattr(d, "vocab", 205)                # ids 10 .. 204 stop: ten to choose from while they are banned
+    with pytest.raises(ValueError, match="fewer tokens"):
+        d.generate_batch([x], 2, min_len=1, beams=11, speech_token_size=10)
+    monkeypatch.setattr(d, "vocab", 10)
+    with pytest.raises(ValueError, match="fewer tokens"):
+        d.generate_batch([x], 2, beams=11, speech_token_size=9)
 
 
 def test_pages_that_are_reserved(gpu, monkeypatch):
