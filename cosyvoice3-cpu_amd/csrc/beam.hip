@@ -72,7 +72,7 @@ constexpr int kList = 512;     // logits of a slice that may pass its bar by val
 // counting.  A key is the logit's rank over the complement of its token, so no two are equal and
 // equal logits go by the lower token.  Where more pass than the list holds (many equal logits), the
 // bar is -inf or some of the slice's tokens are banned, the bar is set by whole keys: whatever passes
-// it then lies in W groups, at most 4 W E keys.  24 x 8 rows of 128000: 21.3 us, 4.6 TB/s; 4 rows of 6761:
+// it then lies in W groups, at most 4 W E keys.  24 x 8 rows of 128000: 21.6 us, 4.6 TB/s; 4 rows of 6761:
 // 4.8 us, the chain of load, two joins of the waves and a ranking.
 template <int E>
 __global__ __launch_bounds__(kSelThreads, 6) void k_select_slices(SelectArgs a) {
@@ -211,8 +211,8 @@ constexpr int kListsEach = kLists / kPickThreads;
 constexpr int kPicks = kBeams * kListsEach * kBeams;
 constexpr int kEarly = 2;                     // candidates of a thread that are loaded with the heads
 
-// One workgroup per request; bound by the chain of its few loads (24 requests of 8 x 16 lists 6.6 us, one of
-// 4 x 4 lists 4.6).  The slices' lists are sorted, so
+// One workgroup per request; bound by the chain of its few loads (24 requests of 8 x 16 lists 6.4 us, one of
+// 4 x 4 lists 4.7).  The slices' lists are sorted, so
 // the best of a thread's lists are their heads.  As above, the W-th largest value of 64 groups of
 // threads is a bar that a few more than W pass; where equal values bring more than the list holds, the
 // W-th best head of the threads, whole, bounds them by W lists a thread x W threads x W keys.
@@ -367,7 +367,7 @@ struct ReorderArgs {
 
 // Copies move a part-filled page's rows between the beams' own pages, in place and in any order: a
 // thread holds the same 16 bytes of every beam's page, reads all it needs and only then writes.
-// HBM-bound (16 requests of 8 beams, 24 layers of bfloat16, pages of 64: 16.5 - 18.5 us, 4.7 - 5.2 TB/s); a beam
+// HBM-bound (16 requests of 8 beams, 24 layers of bfloat16, pages of 64: 19.6 us, 16.7 at best, 4.4 - 5.2 TB/s); a beam
 // that stays itself costs nothing.  Of a request's workgroups
 // the last table_parts turn its table, column by column, in the same way.
 template <int W>

@@ -74,7 +74,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* red, uint32
 // workgroups), then lists a share of the tokens, four neighbours a thread.  A token finds its request
 // among the starts in LDS; the token that opens a page also enters it into the table.  Pages before
 // `have` are the request's own already; page have + i is free_pages[first + i].  Bound by the chain of
-// its loads: 4.9 us for a decode step of eight requests, 7.8 us for 384 prompts of up to 1200 tokens.
+// its loads: 5.0 us for a decode step of eight requests, 7.9 us for 384 prompts of up to 1200 tokens.
 __global__ __launch_bounds__(kTabThreads) void k_block_tables(TabArgs a) {
   __shared__ int32_t s_start[kTabRequests + 1];
   __shared__ int32_t s_first[kTabRequests];   // index of the request's first new page among the free ones
@@ -221,7 +221,7 @@ __device__ __forceinline__ void store_elems(void* base, int type, int64_t at, co
 // out[j] = x[j] cos[j] - x[j + d/2] sin[j], out[j + d/2] = x[j + d/2] cos[j + d/2] + x[j] sin[j + d/2].
 // HBM-bound: each row is read once, q written in float32, k and v rounded (to nearest even) to the
 // cache's type as they are written.  PAST: rows and q go past the caches, for calls that move more
-// than the 256 MB of the last one (6001 tokens of 32 + 2 x 8 heads of 128, bfloat16, 272 MB: 46.5 us,
+// than the 256 MB of the last one (6001 tokens of 32 + 2 x 8 heads of 128, bfloat16, 272 MB: 46.7 us,
 // 5.8 TB/s, against 50.2).
 template <int V, bool PAST>
 __global__ __launch_bounds__(256) void k_append(AppendArgs a, int type, unsigned per_row, unsigned blocks_per_row) {
@@ -918,8 +918,8 @@ __global__ __launch_bounds__(kWholeWaves<NJ> * 64, (waves_per_simd<E, NJ>())) vo
 }
 
 // HBM-bound for large batches: 96 ragged sequences of up to 6000 bfloat16 keys, 32 on 8 heads of 128, 1.2 GB in
-// 231 us, 5.2 TB/s; 3 x 100001 float16 keys, 14 on 2 heads of 64, 36 us, 4.2 TB/s with its start; 24 x 1000 and
-// fewer keys by five dependent latencies, 6 - 9 us.
+// 248 us, 4.7 TB/s (232 at best); 3 x 100001 float16 keys, 14 on 2 heads of 64, 36.3 us, 4.2 TB/s with its start;
+// 24 x 1000 and fewer keys by five dependent latencies, 7 - 10 us.
 //
 // The units of all sequences and heads, in order, shared out evenly over `groups` workgroups by the
 // lengths on the device: a ragged batch fills the machine as an even one does, and a captured
@@ -964,7 +964,7 @@ __global__ __launch_bounds__(kWaves * 64, (waves_per_simd<E, NJ>())) void k_page
 
 constexpr int kJoinWaves = 4, kJoinAhead = 8;
 
-// One workgroup per (sequence, query head), 2 us for one sequence, 5.4 for 42 heads of 85 parts each, 8 for
+// One workgroup per (sequence, query head), 3.4 us for one sequence, 5.4 for 42 heads of 85 parts each, 8 for
 // 3.1 thousand heads of one or two: the parts of a pair that crossed workgroups, and zeros
 // for a sequence with no key to see.  The waves take the parts in turn, eight at a time so that
 // their loads are in flight together, then meet in LDS.

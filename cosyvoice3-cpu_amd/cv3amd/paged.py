@@ -178,7 +178,8 @@ def attention(q, k_cache: DeviceArray, v_cache: DeviceArray, tables, lengths, st
     """One new token per sequence: softmax(scale q . k) v of ``q`` (batch, heads, dim) over the ``lengths[b]`` keys
     that ``tables[b]`` (batch, blocks) lists, from key ``starts[b]`` on (a window; default 0).  Query heads
     share kv heads in groups.  A sequence with no key to see, such as a padding row, gives zeros, one whose
-    scores are all -inf NaN (0 / 0); what lies in rows that are not seen reaches nothing."""
+    scores are all -inf NaN (0 / 0); what lies in rows that are not seen reaches nothing.  Weights (at most one)
+    times values are summed in float32 and then divided: a sum past the largest float is infinite."""
     kind = _cache(k_cache, v_cache)
     pages, kv_heads, page, d = k_cache.shape
     first = q
@@ -203,13 +204,15 @@ def attention(q, k_cache: DeviceArray, v_cache: DeviceArray, tables, lengths, st
 
 def beam_select(logits, scores, done, stop: Tuple[int, int], ban: Tuple[int, int] = (0, 0),
                 pad: Optional[int] = None, out=None):
-    """The best continuations of each request's beams: ``logits`` (requests, beams, vocab), ``scores`` and ``done``
-    (requests, beams) float32 and uint8.  Beam b with token t is worth scores[b] + log_softmax(logits[b])[t],
-    formed in float64; an ended beam goes on with ``pad`` (default the first stop id) at its own score.
-    Tokens of [ban[0], ban[1]) are not chosen (below a minimal length, the stop ids).  Returns (tokens int64,
-    parents int32, scores, done), best first; equal values: the lower beam, in one beam the larger logit,
-    then the lower token.  ``done`` of the result: the parent's, or a token of [stop[0], stop[1]).  ``out``:
-    those four arrays; scores and done may be the call's own."""
+    """The best continuations of each request's beams: ``logits`` (requests, beams, vocab), ``scores`` and
+    ``done`` (requests, beams) float32 and uint8. Beam b with token t is worth scores[b] +
+    log_softmax(logits[b])[t], formed in float64 but for the exponentials of the softmax's sum, which are float32
+    (its log within 1e-6: candidates of two beams that lie closer may change places, those of one beam never); an
+    ended beam goes on with ``pad`` (default the first stop id) at its own score. Tokens of [ban[0], ban[1]) are
+    not chosen (below a minimal length, the stop ids). Returns (tokens int64, parents int32, scores, done), best
+    first; equal values: the lower beam, in one beam the larger logit, then the lower token. ``done`` of the
+    result: the parent's, or a token of [stop[0], stop[1]). ``out``: those four arrays; scores and done may be the
+    call's own."""
     first = logits
     logits = _in(logits, _F32, "logits")
     if logits.ndim != 3:

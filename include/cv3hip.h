@@ -564,52 +564,55 @@ int cv3_qwen2_embed_token(const cv3_qwen2_model* m, const cv3_qwen2_state* s, cv
  * page ids and slots outside the cache count as absent, negative lengths as 0, lengths past the table as its end. */
 /* Pages and slots for new_tokens[r] more tokens after lengths[r].  Requests take pages in order from
  * free_pages[taken ..], one for each block past those that their length has begun, entered into tables [requests,
- * blocks]; taken_out counts what was asked for (at most 2^31 - 1), and where free_pages ends first (taken_out > free_count) the entry and
- * the slots are -1.  free_pages NULL: the tables hold every page already, none is taken (taken, taken_out: NULL too,
- * or not looked at).  Tokens that pass a request's table, or `tokens` in all, are not given: total[r] = the length
- * after those given.  starts [requests + 1]: each request's first token in the list; slots and positions [tokens], -1
- * behind the last.  At most 4096 requests; tables and results share no memory with
+ * blocks]; taken_out counts what was asked for (at most 2^31 - 1), and where free_pages ends first (taken_out >
+ * free_count) the entry and the slots are -1.  free_pages NULL: the tables hold every page already, none is taken
+ * (taken, taken_out: NULL too, or not looked at).  Tokens that pass a request's table, or `tokens` in all, are not
+ * given: total[r] = the length after those given.  starts [requests + 1]: each request's first token in the list;
+ * slots and positions [tokens], -1 behind the last.  At most 4096 requests; tables and results share no memory with
  * each other or the inputs. */
 int cv3_paged_tables(const int32_t* lengths, const int32_t* new_tokens, int64_t requests, int64_t page,
                      const int32_t* free_pages, int64_t free_count, const int32_t* taken, int32_t* tables,
                      int64_t blocks, int64_t tokens, int32_t* total, int32_t* taken_out, int32_t* starts,
                      int64_t* slots, int32_t* positions, cv3_stream_t s);
 /* n rows [q heads; k heads; v heads] of d floats, `ld` apart: q and k turned by the half-split rotary of
- * positions[i] (tables [rope_rows, d]; both NULL: not turned), q into its rows (`ldq` apart; NULL: not wanted; may be
- * `rows` itself with ldq = ld, no other part of them), k and v rounded to the cache's type into slots[i].  A slot outside the cache (-1) writes nothing; a
- * position outside the tables writes nothing and gives zeros for q.  Slots are distinct: of rows with the same one,
- * either may remain. */
+ * positions[i] (tables [rope_rows, d]; both NULL: not turned), q into its rows (`ldq` apart; NULL: not wanted; may
+ * be `rows` itself with ldq = ld, no other part of them), k and v rounded to the cache's type into slots[i].  A
+ * slot outside the cache (-1) writes nothing; a position outside the tables writes nothing and gives zeros for q.
+ * Slots are distinct: of rows with the same one, either may remain. */
 int cv3_paged_append(const float* rows, int64_t n, int64_t ld, int heads, int kv_heads, int d,
                      const int32_t* positions, const int64_t* slots, const float* cos_tab, const float* sin_tab,
                      int64_t rope_rows, int cache_type, void* k_cache, void* v_cache, int64_t pages, int64_t page,
                      float* q, int64_t ldq, cv3_stream_t s);
 /* out[b] = softmax(scale q[b] . k_j) v_j over keys starts[b] <= j < lengths[b] (starts NULL: 0), one query a
- * sequence, heads a multiple of kv_heads.  Everything is float32 but the cache.  No key to see (an empty sequence, a
- * padding row, absent pages alone): zeros; keys whose scores are all -inf: NaN, as the softmax is 0 / 0.  out may be q with
- * ldo = ldq, no other part of it.  What lies in rows that are not seen, NaN too, reaches nothing.  Long
- * caches take scratch of the caching allocator, ordered on s (a capture: from its cache, where it must be; without
- * it one workgroup a pair walks the whole cache). */
+ * sequence, heads a multiple of kv_heads.  Everything is float32 but the cache: weights of at most one times values
+ * are summed first and divided after, so an output is infinite where that sum passes the largest float, be its
+ * quotient smaller.  No key to see (an empty sequence, a padding row, absent pages alone): zeros; keys whose scores
+ * are all -inf: NaN, as the softmax is 0 / 0.  out may be q with ldo = ldq, no other part of it.  What lies in rows
+ * that are not seen, NaN too, reaches nothing.  Long caches take scratch of the caching allocator, ordered on s (a
+ * capture: from its cache, where it must be; without it one workgroup a pair walks the whole cache). */
 int cv3_paged_attention(const float* q, int64_t ldq, int64_t batch, int heads, int kv_heads, int d, int cache_type,
                         const void* k_cache, const void* v_cache, int64_t pages, int64_t page, const int32_t* tables,
                         int64_t blocks, const int32_t* lengths, const int32_t* starts, float scale, float* out,
                         int64_t ldo, cv3_stream_t s);
-/* The `beams` best continuations of each request.  Beam b with token t is worth scores[b] + log_softmax(logits[b])[t],
- * formed in float64 from the float32 logits; an ended beam (done != 0) goes on with `pad` at its own score and nothing
- * else.  Tokens of [ban_lo, ban_hi) are not chosen (they count in the softmax).  The best first; of equal values the
- * lower beam, in one beam the larger logit, then the lower token.  A value that is no number (a row with a NaN or
- * +inf, or all -inf; such a score) counts as -inf.  tokens, parents, scores_out and done_out are [requests, beams]
- * (scores_out may be scores, done_out may be done; nothing else is shared); done_out: the parent's, or a token of [stop_lo, stop_hi).
- * 1 to 16 beams, vocab up to 524288 with at least `beams` tokens to choose.  Takes scratch of the allocator, as above
- * (CV3_ENOMEM where a capture finds none). */
+/* The `beams` best continuations of each request.  Beam b with token t is worth scores[b] +
+ * log_softmax(logits[b])[t], formed in float64 from the float32 logits but for the exponentials of the softmax's
+ * sum, which are float32 (its log within 1e-6: candidates of two beams that lie closer may change places, those of
+ * one beam never); an ended beam (done != 0) goes on with `pad` at its own score and nothing else.  Tokens of
+ * [ban_lo, ban_hi) are not chosen (they count in the softmax).  The best first; of equal values the lower beam, in
+ * one beam the larger logit, then the lower token.  A value that is no number (a row with a NaN or +inf, or all
+ * -inf; such a score) counts as -inf.  tokens, parents, scores_out and done_out are [requests, beams] (scores_out
+ * may be scores, done_out may be done; nothing else is shared); done_out: the parent's, or a token of [stop_lo,
+ * stop_hi).  1 to 16 beams, vocab up to 524288 with at least `beams` tokens to choose.  Takes scratch of the
+ * allocator, as above (CV3_ENOMEM where a capture finds none). */
 int cv3_beam_select(const float* logits, int64_t requests, int beams, int64_t vocab, const float* scores,
                     const uint8_t* done, int64_t stop_lo, int64_t stop_hi, int64_t ban_lo, int64_t ban_hi, int64_t pad,
                     int64_t* tokens, int32_t* parents, float* scores_out, uint8_t* done_out, cv3_stream_t s);
 /* Beams follow their parents in a paged cache [layers, pages, kv_heads, page, d].  Beam w of request r writes the
- * pages own[r][w][block]; of its lengths[r] keys, whole pages may lie with any beam (tables[r][w][block]), the last,
- * part-filled one is its own.  tables[r][w] becomes tables[r][parents[r][w]] for the whole pages and own[r][w] from
- * there on; the part-filled page's rows are copied from the parent's page to the beam's, in every layer.  A parent
- * outside [0, beams) leaves its beam as it is; pages outside the cache are not copied.  No
- * array is part of another.  1 to 16 beams. */
+ * pages own[r][w][block]; of its lengths[r] keys, whole pages may lie with any beam (tables[r][w][block]), the
+ * last, part-filled one is its own.  tables[r][w] becomes tables[r][parents[r][w]] for the whole pages and
+ * own[r][w] from there on; the part-filled page's rows are copied from the parent's page to the beam's, in every
+ * layer.  A parent outside [0, beams) leaves its beam as it is; pages outside the cache are not copied.  No array
+ * is part of another.  1 to 16 beams. */
 int cv3_beam_reorder(const int32_t* parents, int64_t requests, int beams, int32_t* tables, const int32_t* own,
                      int64_t blocks, const int32_t* lengths, int cache_type, void* k_cache, void* v_cache,
                      int64_t layers, int64_t pages, int kv_heads, int64_t page, int d, cv3_stream_t s);
