@@ -9,6 +9,14 @@ and draws one token (``_sample``, cv3cpu/models/llm.py:125-149).  These operator
 * ``beam_select``   the best continuations over beams and vocabulary (``log_softmax``, ops.py:90-93);
 * ``beam_reorder``  tables and part-filled pages follow the chosen beams.
 
+For sets of sequences that change, and texts that are scored:
+
+* ``extend``          several new tokens per sequence over the cache, each seeing its own sequence up to itself;
+* ``token_logprobs``  log probabilities of given tokens, entropy, the best alternatives;
+* ``fork``            sequences that go on from others, whole pages shared;
+* ``free_pages``      the pages that no sequence holds: what ``block_tables`` and ``fork`` take from;
+* ``compact``         the pages that are held, into another cache.
+
 A cache is a pair of device arrays (pages, kv heads, page, head dim): float32, float16, or bfloat16 as
 uint16 bit patterns (``new_cache``).  Caches and tables live on the device and are updated in place;
 everything else may be a NumPy array, uploaded for the call, and results come back as device arrays, or
@@ -16,10 +24,11 @@ as NumPy arrays where the first argument was one.  ``out`` takes the results' ar
 Calls are enqueued on the calling thread's stream and do not synchronise; lengths, page ids and slots are
 read on the device and checked there.
 
-``attention`` over long caches and ``beam_select`` take scratch from the allocator.  Captured into a graph they
-take it from the allocator's cache, and the graph keeps it: run them once eagerly before each capture.  Where the
-cache has none, ``beam_select`` raises ``ScratchError`` and ``attention`` runs one workgroup a (sequence, kv head),
-which is slow for few long sequences.
+``attention`` and ``extend`` over long caches, ``beam_select``, ``compact``, and ``token_logprobs`` and ``free_pages``
+of large inputs take scratch from the allocator.  Captured into a graph they take it from the allocator's cache, and
+the graph keeps it: run them once eagerly before each capture.  Where the cache has none, ``attention`` and ``extend``
+run without splitting a sequence's keys over workgroups, which is slow for few long sequences; the others raise
+``ScratchError``.
 """
 
 from __future__ import annotations
@@ -32,6 +41,7 @@ import numpy as np
 from . import _lib
 from .device import DeviceArray, to_device
 
+_ALL = 2**63 - 1             # a window of all keys
 _F32, _I32, _I64, _U8 = (np.dtype(t) for t in (np.float32, np.int32, np.int64, np.uint8))
 _CACHE_TYPES = {_F32: _lib.F32, np.dtype(np.float16): _lib.F16, np.dtype(np.uint16): _lib.BF16}
 
@@ -245,3 +255,129 @@ def beam_reorder(parents, tables: DeviceArray, own, lengths, k_cache: DeviceArra
     lengths = _in(lengths, _I32, "lengths", (r,))
     _lib.call("beam_reorder", parents.ptr, r, w, tables.ptr, own.ptr, blocks, lengths.ptr, kind, k_cache.ptr,
               v_cache.ptr, layers, pages, kv_heads, page, d, None)
+
+
+def extend(q, k_cache: DeviceArray, v_cache: DeviceArray, tables, lengths, starts, window: Optional[int] = None,
+           scale: Optional[float] = None, out=None):
+    """New tokens of several sequences over the cache: softmax(scale q . k) v of the ragged list ``q`` (rows, heads,
+    dim).  Rows ``starts[b]`` to ``starts[b + 1]`` (batch + 1, rising, as ``block_tables`` gives them) are sequence b's
+    last tokens, whose keys are in the cache already (``append``): the last of them is at position ``lengths[b]`` - 1.
+    A query at position p sees the keys up to p that ``tables[b]`` (batch, blocks) lists, the last ``window`` of them
+    alone if that is given.  Query heads share kv heads in groups.  Rows outside [starts[0], starts[-1]) are left as
+    they are (zeros in an array that the call makes).  A query with no key to see gives zeros, one whose scores are
+    all -inf NaN (0 / 0); what lies in rows that are not seen reaches nothing.  Queries and weights enter the products
+    with 22 bits of the largest in their row or tile, float32 keys and values too, and sums are float32: the error is
+    that of float32 arithmetic but for values 2^17 times smaller than others of the same sequence and head, whose last
+    bits are lost beside those.  Outputs that are not finite are formed again in float32."""
+    kind = _cache(k_cache, v_cache)
+    pages, kv_heads, page, d = k_cache.shape
+    first = q
+    q = _in(q, _F32, "q")
+    if q.ndim != 3 or q.shape[2] != d:
+        raise ValueError(f"queries are (rows, heads, {d}), got {q.shape}")
+    n, h, _ = q.shape
+    tables = _in(tables, _I32, "tables")
+    if tables.ndim != 2:
+        raise ValueError(f"tables are (batch, blocks), got {tables.shape}")
+    b, blocks = tables.shape
+    lengths, starts = _in(lengths, _I32, "lengths", (b,)), _in(starts, _I32, "starts", (b + 1,))
+    if window is not None and window < 1:
+        raise ValueError(f"a window of {window} keys")
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    o = DeviceArray(q.shape, _F32).zero_() if out is None else _out(out, q.shape, _F32, "out")
+    _lib.call("paged_extend", q.ptr, h * d, n, h, kv_heads, d, kind, k_cache.ptr, v_cache.ptr, pages, page, tables.ptr,
+              blocks, lengths.ptr, starts.ptr, b, _ALL if window is None else window, float(scale), o.ptr, h * d, None)
+    return _given(o, first)
+
+
+def token_logprobs(logits, tokens, top: int = 0, out=None):
+    """What given tokens are worth: of each row of ``logits`` (rows, vocab) the log probability of ``tokens`` (rows,)
+    int64 (0 for a token outside the vocabulary, such as a padding row's -1), the entropy of the distribution in nats,
+    and its ``top`` (0 to 32) best tokens with their log probabilities, best first, equal logits by the lower token.
+    Returns (logprobs, entropy, ids (rows, top) int64, values (rows, top)).  Formed in float64 but for the exponentials
+    of the sums, which are float32.  A row with a NaN or +inf, or of -inf alone, gives NaN (and ids, for which NaN counts
+    as -inf).  ``out``: those four arrays."""
+    first = logits
+    logits = _in(logits, _F32, "logits")
+    if logits.ndim != 2:
+        raise ValueError(f"logits are (rows, vocab), got {logits.shape}")
+    n, v = logits.shape
+    tokens = _in(tokens, _I64, "tokens", (n,))
+    out = _outs(out, 4)
+    if not 0 <= top <= min(32, v):
+        raise ValueError(f"0 to 32 alternatives out of {v} tokens, not {top}")
+    lp, entropy = _out(out[0], (n,), _F32, "logprobs"), _out(out[1], (n,), _F32, "entropy")
+    ids, values = _out(out[2], (n, top), _I64, "ids"), _out(out[3], (n, top), _F32, "values")
+    _lib.call("token_logprobs", logits.ptr, n, v, tokens.ptr, top, lp.ptr, entropy.ptr, ids.ptr, values.ptr, None)
+    return tuple(_given(x, first) for x in (lp, entropy, ids, values))
+
+
+def _layered(k, v):
+    """(type, layers, pages, kv heads, page, dim) of caches with or without an axis of layers."""
+    kind = _cache(k, v, k.ndim if getattr(k, "ndim", 0) == 5 else 4)
+    return (kind, k.shape[0] if k.ndim == 5 else 1, *k.shape[-4:])
+
+
+def fork(parents, children, tables: DeviceArray, lengths: DeviceArray, free, taken, k_cache: DeviceArray,
+         v_cache: DeviceArray, out=None):
+    """Sequences that go on from others, in place: row ``children[i]`` of ``tables`` (sequences, blocks) and ``lengths``
+    becomes row ``parents[i]``.  Whole pages are shared; the rows of a part-filled last page are copied into a page of
+    the child's own, the next of the page ids ``free`` from index ``taken[0]`` on, forks in order, in every layer of the
+    caches (layers, pages, kv heads, page, dim), or (pages, kv heads, page, dim).  Returns the pages taken so far, more
+    than ``len(free)`` where they ran out (the child's entry is then -1).  Children are distinct and no parents of the
+    call; a fork whose child is, or whose rows do not exist, is not made."""
+    kind, layers, pages, kv_heads, page, d = _layered(k_cache, v_cache)
+    if not isinstance(tables, DeviceArray) or tables.ndim != 2:
+        raise TypeError("tables is a DeviceArray (sequences, blocks)")
+    rows, blocks = tables.shape
+    _held(tables, _I32, "tables")
+    _held(lengths, _I32, "lengths", (rows,))
+    first = taken
+    parents = _in(parents, _I32, "parents")
+    children = _in(children, _I32, "children", parents.shape)
+    if parents.ndim != 1:
+        raise ValueError(f"parents are a list, got {parents.shape}")
+    free, taken = _in(free, _I32, "free"), _in(taken, _I32, "taken", (1,))
+    took = _out(out, (1,), _I32, "out")
+    _lib.call("paged_fork", parents.ptr, children.ptr, parents.size, tables.ptr, rows, blocks, lengths.ptr, free.ptr,
+              free.size, taken.ptr, took.ptr, kind, k_cache.ptr, v_cache.ptr, layers, pages, kv_heads, page, d, None)
+    return _given(took, first)
+
+
+def free_pages(tables, lengths, page: int, pages: int, out=None):
+    """The page ids of [0, ``pages``) that no sequence holds, ascending: (ids (pages,) int32 with -1 behind the last,
+    their number (1,) int32).  Sequence b holds the first ceil(``lengths[b]`` / ``page``) entries of its row of ``tables``
+    (sequences, blocks), so one that has ended is given up by setting its length to 0.  The ids are ``free`` for
+    ``block_tables`` and ``fork``, with ``taken`` set to 0."""
+    first = tables
+    tables = _in(tables, _I32, "tables")
+    if tables.ndim != 2:
+        raise ValueError(f"tables are (sequences, blocks), got {tables.shape}")
+    rows, blocks = tables.shape
+    lengths, out = _in(lengths, _I32, "lengths", (rows,)), _outs(out, 2)
+    free, count = _out(out[0], (pages,), _I32, "free"), _out(out[1], (1,), _I32, "count")
+    _lib.call("paged_free", tables.ptr, rows, blocks, lengths.ptr, page, pages, free.ptr, count.ptr, None)
+    return _given(free, first), _given(count, first)
+
+
+def compact(tables, lengths, k_cache: DeviceArray, v_cache: DeviceArray, k_new: DeviceArray, v_new: DeviceArray,
+            out=None):
+    """What is held of a cache, moved into another one of any number of pages (a smaller one for what is left, a larger
+    one to go on): every page that a sequence holds (as in ``free_pages``) is copied once, in the order of their ids, to
+    the pages 0, 1, .. of ``k_new`` and ``v_new``, in every layer.  Returns (tables (sequences, blocks) for the new cache,
+    -1 behind a sequence's last block, and the number of pages held (1,), more than the new cache has where it was
+    too small: what did not fit is -1).  Pages that sequences share stay shared."""
+    kind, layers, pages, kv_heads, page, d = _layered(k_cache, v_cache)
+    if _layered(k_new, v_new) != (kind, layers, k_new.shape[-4], kv_heads, page, d) or k_new.ndim != k_cache.ndim:
+        raise ValueError(f"the new caches are {k_new.shape}, those in use {k_cache.shape}")
+    first = tables
+    tables = _in(tables, _I32, "tables")
+    if tables.ndim != 2:
+        raise ValueError(f"tables are (sequences, blocks), got {tables.shape}")
+    rows, blocks = tables.shape
+    lengths, out = _in(lengths, _I32, "lengths", (rows,)), _outs(out, 2)
+    turned, used = _out(out[0], tables.shape, _I32, "tables"), _out(out[1], (1,), _I32, "used")
+    _lib.call("paged_compact", tables.ptr, rows, blocks, lengths.ptr, kind, k_cache.ptr, v_cache.ptr, layers, pages,
+              kv_heads, page, d, k_new.ptr, v_new.ptr, k_new.shape[-4], turned.ptr, used.ptr, None)
+    return _given(turned, first), _given(used, first)

@@ -616,6 +616,52 @@ int cv3_beam_select(const float* logits, int64_t requests, int beams, int64_t vo
 int cv3_beam_reorder(const int32_t* parents, int64_t requests, int beams, int32_t* tables, const int32_t* own,
                      int64_t blocks, const int32_t* lengths, int cache_type, void* k_cache, void* v_cache,
                      int64_t layers, int64_t pages, int kv_heads, int64_t page, int d, cv3_stream_t s);
+/* out[i] = softmax(scale q[i] . k_j) v_j for n queries of several sequences, each over its own sequence's keys up to
+ * itself.  The list holds sequence b's queries in rows starts[b] .. starts[b + 1] (starts [batch + 1], rising): they are
+ * its last tokens, so that the last of them is at position lengths[b] - 1, and a query at position p sees the keys
+ * max(0, p - window + 1) .. p (window INT64_MAX: all).  Rows before starts[0] and from starts[batch] on are left as they
+ * are.  A query with no key to see (absent pages alone, a position before 0) gives zeros, one whose scores are all -inf
+ * NaN.  float32 queries and results; products and sums carry float32 accuracy whatever the cache's type: |error| is a
+ * few 2^-22 of the largest |v| that the call's workgroup has met, and outputs that are not finite are formed in
+ * float32.  out may be q with ldo = ldq, no other part of it.  What lies in rows that are not seen, NaN too, reaches
+ * nothing.  Takes scratch of the allocator as cv3_paged_attention does. */
+int cv3_paged_extend(const float* q, int64_t ldq, int64_t n, int heads, int kv_heads, int d, int cache_type,
+                     const void* k_cache, const void* v_cache, int64_t pages, int64_t page, const int32_t* tables,
+                     int64_t blocks, const int32_t* lengths, const int32_t* starts, int64_t batch, int64_t window,
+                     float scale, float* out, int64_t ldo, cv3_stream_t s);
+/* Of each row of logits: logprobs[i] = log_softmax(logits[i])[tokens[i]] (0 for a token outside the vocabulary, such as
+ * a padding row's -1), the distribution's entropy in nats, and its `top` (0 to 32) largest logits, best first, equal ones
+ * by the lower token: top_ids and top_logprobs [rows, top].  Formed in float64 but for the exponentials, which are
+ * float32 (the log of their sum within 1e-6).  A row with a NaN or +inf, or of -inf alone, has NaN for numbers (its
+ * top_ids: NaN counts as -inf).  vocab up to 524288.  Takes scratch of the allocator for more than 8192 logits a row
+ * (CV3_ENOMEM where a capture finds none). */
+int cv3_token_logprobs(const float* logits, int64_t rows, int64_t vocab, const int64_t* tokens, int top,
+                       float* logprobs, float* entropy, int64_t* top_ids, float* top_logprobs, cv3_stream_t s);
+/* Sequences that go on from others: of tables [rows, blocks] and lengths [rows], row children[i] becomes row parents[i].
+ * Whole pages are shared; a part-filled last page's rows are copied, in every layer of the cache [layers, pages,
+ * kv_heads, page, d], into a page of its own, the next of free_pages from index *taken on, forks in order (where they
+ * run out its entry is -1); entries behind are -1.  taken_out: the pages taken so far, more than free_count where they
+ * ran out.  A fork is not made, and takes no page, if parent or child is no row, if the child is a parent of the
+ * call, or if another fork names the same child.  At most 4096 forks and 65536 rows. */
+int cv3_paged_fork(const int32_t* parents, const int32_t* children, int64_t forks, int32_t* tables, int64_t rows,
+                   int64_t blocks, int32_t* lengths, const int32_t* free_pages, int64_t free_count,
+                   const int32_t* taken, int32_t* taken_out, int cache_type, void* k_cache, void* v_cache,
+                   int64_t layers, int64_t pages, int kv_heads, int64_t page, int d, cv3_stream_t s);
+/* The ids of [0, pages) that none of the first ceil(lengths[b] / page) entries of a table names, ascending, into
+ * free_pages [pages], -1 behind the last; *count of them.  That is what a sequence held that has ended (length 0), and
+ * what cv3_paged_tables and cv3_paged_fork take from.  At most 2^24 pages.  More than 131072 pages or 262144 table
+ * entries take scratch of the allocator (CV3_ENOMEM where a capture finds none). */
+int cv3_paged_free(const int32_t* tables, int64_t rows, int64_t blocks, const int32_t* lengths, int64_t page,
+                   int64_t pages, int32_t* free_pages, int32_t* count, cv3_stream_t s);
+/* The pages that the tables' first ceil(lengths[b] / page) entries name, each once and in the order of their ids, copied
+ * to the pages 0, 1, .. of another cache [layers, pages_new, kv_heads, page, d] of the same type; tables_new [rows,
+ * blocks] names them there, -1 behind a sequence's last block.  *used: how many there are, more than pages_new where the
+ * new cache was too small (what did not fit is absent: -1).  The new cache's other pages are left as they are.  At most
+ * 2^24 pages.  Takes scratch of the allocator (CV3_ENOMEM where a capture finds none). */
+int cv3_paged_compact(const int32_t* tables, int64_t rows, int64_t blocks, const int32_t* lengths, int cache_type,
+                      const void* k_cache, const void* v_cache, int64_t layers, int64_t pages, int kv_heads,
+                      int64_t page, int d, void* k_new, void* v_new, int64_t pages_new, int32_t* tables_new,
+                      int32_t* used, cv3_stream_t s);
 
 #ifdef __cplusplus
 }
