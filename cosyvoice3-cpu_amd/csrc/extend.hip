@@ -4,6 +4,7 @@
 //
 // The queries are a ragged list: rows starts[b] .. starts[b + 1] are sequence b's last tokens, the last of them at
 // position lengths[b] - 1.  Page ids, lengths and starts come from device memory and are checked where they are used.
+#include "decode_common.hpp"   // DPP lane exchanges
 #include "paged_common.hpp"
 
 #include <algorithm>
@@ -28,7 +29,7 @@ struct ExtArgs {
   int64_t ldo;
   int64_t pages, blocks, n;
   int window;                  // keys that a query sees at most
-  int batch, page, heads, kv_heads, group, d;
+  int batch, page, heads, kv_heads, group, d, slots;
   float scale;                 // times log2(e)
 };
 
@@ -109,31 +110,520 @@ struct RowSum {
   }
 };
 
-// One wave a query.
+// ------------------------------------------------------------------------------------------------
+// tiles on the matrix cores
+// ------------------------------------------------------------------------------------------------
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kRows = 128;          // (token, head) rows of a workgroup: 32 a wave
+constexpr int kThreads = 256;
+constexpr int kSplitSlots = 2048;   // tiles of rows whose keys may be shared out
+constexpr float kUp = 12.f, kSlack = 3.f;   // weights are held 2^12 up, and pass that by at most 2^3: below the largest float16
+
+// How a cache's numbers become float16 operands.  float32: two planes, x 2^s = hi + lo within 2^-23 of x or 2^-25.
+// bfloat16: one plane that holds x 2^s whole, down to 2^-17 of the largest's.  float16: as it is.
 template <typename E>
-__global__ __launch_bounds__(256) void k_extend_rows(ExtArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + uniform((int)threadIdx.x >> 6);
-  const int64_t row = item / a.heads;
-  const int head = (int)(item % a.heads);
-  if (row >= a.n) return;
-  int b = -1;
-  Seq s{};
-  for (int i = 0; i < a.batch; ++i) {
-    s = seq_of(a, i);
-    if (row >= s.first && row < s.first + s.count) {
-      b = i;
-      break;
+struct Cell;
+template <>
+struct Cell<float> {
+  typedef uint4 Raw;                // four channels
+  static constexpr int N = 2;
+  static constexpr bool SCALED = true;
+  static __device__ __forceinline__ void four(const uint4& r, float* f) {
+    f[0] = __uint_as_float(r.x), f[1] = __uint_as_float(r.y), f[2] = __uint_as_float(r.z), f[3] = __uint_as_float(r.w);
+  }
+};
+template <>
+struct Cell<__bf16> {
+  typedef uint2 Raw;
+  static constexpr int N = 1;
+  static constexpr bool SCALED = true;
+  static __device__ __forceinline__ void four(const uint2& r, float* f) {
+    f[0] = __uint_as_float(r.x << 16), f[1] = __uint_as_float(r.x & 0xffff0000u);
+    f[2] = __uint_as_float(r.y << 16), f[3] = __uint_as_float(r.y & 0xffff0000u);
+  }
+};
+template <>
+struct Cell<_Float16> {
+  typedef uint2 Raw;
+  static constexpr int N = 1;
+  static constexpr bool SCALED = false;
+  static __device__ __forceinline__ void four(const uint2&, float*) {}
+};
+
+__device__ __forceinline__ h2 half2_of(float a, float b) { return __builtin_convertvector((f32x2{a, b}), h2); }
+// x = hi + lo
+__device__ __forceinline__ void split2(float a, float b, h2& hi, h2& lo) {
+  hi = half2_of(a, b);
+  lo = half2_of(a - (float)hi[0], b - (float)hi[1]);
+}
+__device__ __forceinline__ h4 join4(h2 a, h2 b) { return h4{a[0], a[1], b[0], b[1]}; }
+
+// 2^15 over the power of two above x: what brings numbers of at most x below the largest float16.
+__device__ __forceinline__ int up_of(float x) {
+  return x > 0.f && x < INFINITY ? min(15 - __builtin_amdgcn_frexp_expf(x), 126) : 15;
+}
+
+// A tile of rows: rows row0 .. row0 + rows of sequence b's count * group (token, head of the group) rows, for one kv head.
+struct Item {
+  int b, kvh, first, base, len, row0, rows;
+  __device__ __forceinline__ int hi_of(const ExtArgs& a, int r) const {     // keys seen: [lo, hi)
+    return max(0, base + (row0 + r) / a.group + 1);
+  }
+  static __device__ __forceinline__ int lo_of(const ExtArgs& a, int hi) { return max(0, hi - a.window); }
+};
+
+// Slots: sequence b's tiles are those from floor(starts[b] group / 128) + b on, so that no two sequences share one.
+__device__ __forceinline__ int slot_of(const ExtArgs& a, int first, int b) {
+  return (int)((int64_t)first * a.group / kRows) + b;
+}
+__device__ __forceinline__ bool item_of(const ExtArgs& a, int b, int tile, Item& it) {
+  const Seq s = seq_of(a, b);
+  it.b = b;
+  it.first = uniform(s.first), it.base = uniform(s.base), it.len = uniform(s.len);
+  const int64_t left = (int64_t)uniform(s.count) * a.group - (int64_t)tile * kRows;
+  if (tile < 0 || left <= 0) return false;
+  it.row0 = tile * kRows;
+  it.rows = (int)min(left, (int64_t)kRows);
+  return true;
+}
+// Its tiles of KT keys: [t0, t1).
+template <int KT>
+__device__ __forceinline__ void tiles_of(const ExtArgs& a, const Item& it, int& t0, int& t1) {
+  const int hi = it.hi_of(a, it.rows - 1);
+  t0 = Item::lo_of(a, it.hi_of(a, 0)) / KT;
+  t1 = max(t0, (hi + KT - 1) / KT);
+  if (hi == 0) t1 = t0;
+}
+// The sequence of a slot, by every thread of the workgroup alike: how many begin at or before it.
+__device__ __forceinline__ bool find_item(const ExtArgs& a, int slot, Item& it) {
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+    const int b = b0 + (int)threadIdx.x;
+    const bool at = b < a.batch && slot_of(a, (int)min((int64_t)max(a.starts[b], 0), a.n), b) <= slot;
+    before += __syncthreads_count(at);
+  }
+  if (before == 0) return false;
+  const int b = uniform(before - 1);
+  return item_of(a, b, slot - uniform(slot_of(a, (int)min((int64_t)max(a.starts[b], 0), a.n), b)), it);
+}
+
+template <typename E, int ND>
+struct Shape {
+  static constexpr int DP = 32 * ND;                   // channels, padded
+  static constexpr int KT = ND <= 4 ? 64 : 32;         // keys of a tile
+  static constexpr int N = Cell<E>::N;
+  static constexpr int KS = DP + 8, VS = KT + 8;       // strides: 16 rows 16 bytes apart lie in distinct banks
+  static constexpr int BLOCKS = KT / 4 * (DP / 4), NB = (BLOCKS + kThreads - 1) / kThreads;
+  struct Mem {
+    _Float16 k[N][KT * KS];                            // [key][channel]
+    _Float16 v[N][DP * VS];                            // [channel][key], keys in the order that the product takes them
+    int64_t off[KT];
+    uint64_t mask;
+    float mx[kThreads / 64][2];
+  };
+};
+
+// Rows of one item over key tiles [t0, t1).
+//
+// S^T = K Q^T on 32 keys x 32 rows x 16 channels: a lane has one row (two lanes share it) and half the keys of each 8,
+// which is what O^T = V^T P^T wants as its second operand once V's keys lie in that order, so the weights stay in their
+// lanes and the softmax needs one exchange between two lanes a tile.  Everything enters the float16 matrix cores as
+// planes: queries and weights as two (float32 in 22 bits), keys and values by their type (Cell); lo x lo is left out
+// (2^-24).  That is 3 products a product for float32 caches, 2 for the two-byte ones, where bfloat16 planes would take 6
+// and 3.  Keys are scaled by a power of two a tile, values by one that only grows over the tiles.  What that loses, small
+// numbers beside large ones, is looked for: a row whose scores could be off (their factor is large), whose outputs are
+// below 2^-15 of the largest value, or whose results are not finite is formed again in float32 (RowSum).
+template <typename E, int ND, bool FULL>
+__device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0, int t1, int whole_t0, int whole_t1,
+                                       float* part, typename Shape<E, ND>::Mem& mem) {
+  typedef Shape<E, ND> S;
+  typedef Cell<E> C;
+  typedef typename C::Raw Raw;
+  constexpr int KT = S::KT, DP = S::DP, N = S::N, KS = S::KS, VS = S::VS, NB = S::NB, CG = DP / 4;
+  const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), n = lane & 31, g = lane >> 5;
+  const int d = FULL ? DP : a.d;
+  const int row = wv * 32 + n;
+  const bool valid = row < it.rows;
+  const int flat = it.row0 + (valid ? row : 0);
+  const int tok = it.first + flat / a.group, head = it.kvh * a.group + flat % a.group;
+  const int hi = valid ? it.hi_of(a, row) : 0, lo = Item::lo_of(a, hi);
+  // of the wave: keys that any of its rows sees [w_lo, w_hi), and that all of them see [s_lo, s_hi)
+  const bool active = wv * 32 < it.rows;
+  const int w_hi = active ? it.hi_of(a, min(it.rows, wv * 32 + 32) - 1) : 0, s_hi = active ? it.hi_of(a, wv * 32) : 0;
+  const int w_lo = Item::lo_of(a, s_hi), s_lo = Item::lo_of(a, w_hi);
+  const float* q = a.q + (int64_t)tok * a.ldq + (int64_t)head * d;
+
+  // the row's channels 16 s + 8 g .. + 8, in two planes
+  h8 qh[DP / 16], ql[DP / 16];
+  float factor;                        // of the row's scores: |scale| log2(e) over its power of two
+  {
+    float x[DP / 16][8], big = 0.f;
+    const float sign = a.scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const int c = 16 * s + 8 * g + e;
+        f32x4u y{};
+        if (valid && (FULL || c < d)) y = *(const f32x4u*)(q + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[s][e + i] = sign * y.v[i];
+          big = fmaxf(big, fabsf(y.v[i]));
+        }
+      }
+    big = fmaxf(big, __shfl_xor(big, 32, kWave));
+    const int up = up_of(big);
+    factor = ldexpf(fabsf(a.scale), -up);
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        h2 h, l;
+        split2(ldexpf(x[s][e], up), ldexpf(x[s][e + 1], up), h, l);
+        qh[s][e] = h[0], qh[s][e + 1] = h[1];
+        ql[s][e] = l[0], ql[s][e + 1] = l[1];
+      }
+  }
+
+  const int32_t* table = a.tables + (int64_t)it.b * a.blocks;
+  const E* kc = (const E*)a.k + (int64_t)it.kvh * a.page * d;
+  const E* vc = (const E*)a.v + (int64_t)it.kvh * a.page * d;
+  // page id and row of this thread's key of tile t; -1: not there
+  auto lookup = [&](int t, int32_t& id, uint32_t& in) {
+    id = -1;
+    in = 0;
+    const int key = t * KT + tid;
+    if (tid < KT && t < t1 && key < it.len) {
+      const uint32_t blk = (uint32_t)key / (uint32_t)a.page;
+      in = (uint32_t)key - blk * (uint32_t)a.page;
+      id = table[blk];
+    }
+  };
+  auto place = [&](int32_t id, uint32_t in) {
+    if (tid < 64) {
+      const bool there = (uint32_t)id < (uint64_t)a.pages;
+      if (tid < KT) mem.off[tid] = there ? ((int64_t)id * a.kv_heads * a.page + in) * d : -1;
+      const uint64_t mask = __ballot(there);
+      if (tid == 0) mem.mask = mask;
+    }
+  };
+  // this thread's blocks of 4 keys x 4 channels
+  Raw kr[NB][4], vr[NB][4];
+  uint64_t mask = 0;
+  auto fetch = [&]() {
+    mask = mem.mask;
+    mask = (uint64_t)uniform((int64_t)mask);
+    const bool all = mask == (KT == 64 ? ~(uint64_t)0 : ((uint64_t)1 << (KT & 63)) - 1);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int at = tid + j * kThreads, cg = at % CG, kg = at / CG;
+      const bool on = (S::BLOCKS % kThreads == 0 || at < S::BLOCKS) && (FULL || 4 * cg < d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t off = on ? mem.off[4 * kg + i] : -1;
+        kr[j][i] = vr[j][i] = Raw{};
+        if (FULL && S::BLOCKS % kThreads == 0 && all) {
+          kr[j][i] = *(const Raw*)(kc + off + 4 * cg);
+          vr[j][i] = *(const Raw*)(vc + off + 4 * cg);
+        } else if (off >= 0) {
+          kr[j][i] = *(const Raw*)(kc + off + 4 * cg);
+          vr[j][i] = *(const Raw*)(vc + off + 4 * cg);
+        }
+      }
+    }
+  };
+
+  f32x16 o[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+  float top = -INFINITY, sum = 0.f;
+  bool there = false, coarse = false;
+  float v_big = 0.f;                   // largest |v| so far
+  int v_up = 126, o_up = 126;          // powers of two of the values now, and of o
+
+  if (t0 < t1) {
+    int32_t id;
+    uint32_t in;
+    lookup(t0, id, in);
+    place(id, in);
+    __syncthreads();
+    fetch();
+    lookup(t0 + 1, id, in);
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+      const uint64_t now = mask;
+      float kx[NB][4][4], vx[NB][4][4];
+      if constexpr (C::SCALED) {
+        float km = 0.f, vm = 0.f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            C::four(kr[j][i], kx[j][i]);
+            C::four(vr[j][i], vx[j][i]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              km = fmaxf(km, fabsf(kx[j][i][c]));
+              vm = fmaxf(vm, fabsf(vx[j][i][c]));
+            }
+          }
+        km = wave_max_dpp(km);
+        vm = wave_max_dpp(vm);
+        if (lane == 0) mem.mx[wv][0] = km, mem.mx[wv][1] = vm;
+      }
+      __syncthreads();                 // the last tile is done with, and the maxima are there
+      float down = 1.f;                // of the keys
+      if constexpr (C::SCALED) {
+        float km = 0.f;
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) {
+          km = fmaxf(km, mem.mx[w][0]);
+          v_big = fmaxf(v_big, mem.mx[w][1]);
+        }
+        const int up = uniform(up_of(km));
+        down = ldexpf(1.f, -up);
+        if (!(km < INFINITY)) coarse = true;
+        v_up = uniform(min(v_up, v_big > 0.f ? up_of(v_big) : 126));
+        const float ku = ldexpf(1.f, up), vu = ldexpf(1.f, v_up);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const int at = tid + j * kThreads, cg = at % CG, kg = at / CG;
+          if (S::BLOCKS % kThreads != 0 && at >= S::BLOCKS) continue;
+          const int slot = 16 * (kg >> 2) + 8 * (kg & 1) + 4 * (kg >> 1 & 1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            h2 h0, l0, h1, l1;
+            split2(kx[j][i][0] * ku, kx[j][i][1] * ku, h0, l0);
+            split2(kx[j][i][2] * ku, kx[j][i][3] * ku, h1, l1);
+            *(h4*)&mem.k[0][(4 * kg + i) * KS + 4 * cg] = join4(h0, h1);
+            if constexpr (N == 2) *(h4*)&mem.k[1][(4 * kg + i) * KS + 4 * cg] = join4(l0, l1);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            h2 h0, l0, h1, l1;
+            split2(vx[j][0][c] * vu, vx[j][1][c] * vu, h0, l0);
+            split2(vx[j][2][c] * vu, vx[j][3][c] * vu, h1, l1);
+            *(h4*)&mem.v[0][(4 * cg + c) * VS + slot] = join4(h0, h1);
+            if constexpr (N == 2) *(h4*)&mem.v[1][(4 * cg + c) * VS + slot] = join4(l0, l1);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const int at = tid + j * kThreads, cg = at % CG, kg = at / CG;
+          if (S::BLOCKS % kThreads != 0 && at >= S::BLOCKS) continue;
+          const int slot = 16 * (kg >> 2) + 8 * (kg & 1) + 4 * (kg >> 1 & 1);
+          uint32_t x[4][2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint2 kw = __builtin_bit_cast(uint2, kr[j][i]), vw = __builtin_bit_cast(uint2, vr[j][i]);
+            *(uint2*)&mem.k[0][(4 * kg + i) * KS + 4 * cg] = kw;
+            x[i][0] = vw.x, x[i][1] = vw.y;
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {      // 4 x 4 two-byte values turned by byte permutations
+            const uint32_t sel = c % 2 ? 0x07060302u : 0x05040100u;
+            *(uint2*)&mem.v[0][(4 * cg + c) * VS + slot] = make_uint2(__builtin_amdgcn_perm(x[1][c / 2], x[0][c / 2], sel),
+                                                                     __builtin_amdgcn_perm(x[3][c / 2], x[2][c / 2], sel));
+          }
+        }
+      }
+      place(id, in);
+      __syncthreads();                 // the tile is there
+      if (t + 1 < t1) {
+        fetch();
+        lookup(t + 2, id, in);
+      }
+      const int k0 = t * KT;
+      if (k0 >= w_hi || k0 + KT <= w_lo) continue;
+
+      f32x16 sc[KT / 32];
+#pragma unroll
+      for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[u][r] = 0.f;
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) {
+          const h8 kh = *(const h8*)&mem.k[0][(32 * u + n) * KS + 16 * s + 8 * g];
+          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[s], sc[u], 0, 0, 0);
+          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[s], sc[u], 0, 0, 0);
+          if constexpr (N == 2) {
+            const h8 kl = *(const h8*)&mem.k[1][(32 * u + n) * KS + 16 * s + 8 * g];
+            sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[s], sc[u], 0, 0, 0);
+          }
+        }
+      // register r of sc[u]: key 32 u + 8 (r / 4) + 4 g + r % 4
+      const bool every = now == (KT == 64 ? ~(uint64_t)0 : ((uint64_t)1 << (KT & 63)) - 1) && k0 + KT <= s_hi && k0 >= s_lo;
+      if (every) {
+        there = true;
+      } else {
+        const int b0 = max(lo - k0, 0), b1 = min(hi - k0, KT);
+        uint64_t m = b1 > b0 ? now & (~(uint64_t)0 >> (64 - b1)) & (~(uint64_t)0 << b0) : 0;
+        there = there || m != 0;
+        m >>= 4 * g;
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const uint32_t bits = (uint32_t)(m >> 32 * u);
+            sc[u][r] = bits >> (8 * (r / 4) + r % 4) & 1 ? sc[u][r] : -INFINITY;
+          }
+      }
+      const float c = factor * down;
+      // a score's terms are up to 2^30 c, and off by 2^-10 c where the small planes end: 2^-23 with 16 of them
+      coarse = coarse || !(c <= (C::SCALED ? 0x1p-17f : 0x1p-8f));
+      float mx = sc[0][0];
+#pragma unroll
+      for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[u][r]);
+      {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
+      }
+      // the running maximum moves only when a score passes it by more than 2^kSlack
+      float f = 1.f;
+      if (__any(!(mx <= top + kSlack) && mx != -INFINITY)) {
+        const float up = fmaxf(mx, top);
+        f = weight_of(top, up);
+        top = up;
+        sum *= f;
+      }
+      if (C::SCALED && o_up != v_up) {
+        f *= ldexpf(1.f, v_up - o_up);
+        o_up = v_up;
+      }
+      if (__any(f != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[i][r] *= f;
+      }
+      const float ref = (top == -INFINITY ? 0.f : top) - kUp;
+#pragma unroll
+      for (int u = 0; u < KT / 16; ++u) {
+        h8 ph, pl;
+        float part_sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float p0 = exp2_fast(fmaf(sc[u / 2][8 * (u % 2) + e], c, -ref));
+          const float p1 = exp2_fast(fmaf(sc[u / 2][8 * (u % 2) + e + 1], c, -ref));
+          part_sum += p0 + p1;
+          h2 h, l;
+          split2(p0, p1, h, l);
+          ph[e] = h[0], ph[e + 1] = h[1];
+          pl[e] = l[0], pl[e + 1] = l[1];
+        }
+        sum += part_sum;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          const h8 vh = *(const h8*)&mem.v[0][(32 * i + n) * VS + 16 * u + 8 * g];
+          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph, o[i], 0, 0, 0);
+          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl, o[i], 0, 0, 0);
+          if constexpr (N == 2) {
+            const h8 vl = *(const h8*)&mem.v[1][(32 * i + n) * VS + 16 * u + 8 * g];
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, o[i], 0, 0, 0);
+          }
+        }
+      }
     }
   }
-  if (b < 0) return;
-  const int hi = max(0, s.base + (int)(row - s.first) + 1), lo = max(0, hi - a.window);
-  RowSum<E> r;
-  r.run(a, b, head / a.group, a.q + row * a.ldq + (int64_t)head * a.d, lo, hi);
-  float* out = a.out + row * a.ldo + (int64_t)head * a.d;
+
+  // register r of o[i]: channel 32 i + 8 (r / 4) + 4 g + r % 4
+  sum += __shfl_xor(sum, 32, kWave);
+  const float inv = 1.f / sum;
+  float big = 0.f;
+  bool odd = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (64 * i + lane < a.d) out[64 * i + lane] = r.there ? r.o[i] / r.sum : 0.f;
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      o[i][r] *= inv;
+      odd = odd || !(fabsf(o[i][r]) < INFINITY);
+      big = fmaxf(big, fabsf(o[i][r]));
+    }
+  big = fmaxf(big, __shfl_xor(big, 32, kWave));
+  odd = odd || coarse || !(sum > 0.f && sum < INFINITY) || (C::SCALED && big < 1.f && v_big > 0.f);
+  odd = __shfl_xor((int)odd, 32, kWave) || odd;
+  const bool again = valid && there && odd, whole = t0 == whole_t0 && t1 == whole_t1;
+  const float unit = C::SCALED ? ldexpf(1.f, -o_up) : 1.f;
+  float* dst = whole ? a.out + (int64_t)tok * a.ldo + (int64_t)head * d : part + (int64_t)row * (d + 2);
+  if (valid && !again) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int c = 32 * i + 8 * (r / 4) + 4 * g;
+        f32x4u x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.v[e] = there ? o[i][r + e] * unit : 0.f;
+        if (FULL || c < d) *(f32x4u*)(dst + c) = x;
+      }
+    if (!whole && g == 0) {
+      dst[d] = there ? top : -INFINITY;
+      dst[d + 1] = there ? sum : 0.f;
+    }
+  }
+  uint64_t rest = __ballot(again && g == 0);
+  while (rest) {
+    const int r = uniform(__ffsll((unsigned long long)rest) - 1);
+    rest &= rest - 1;
+    const int r_tok = uniform(__shfl(tok, r, kWave)), r_head = uniform(__shfl(head, r, kWave));
+    const int r_hi = min(uniform(__shfl(hi, r, kWave)), t1 * KT), r_lo = max(uniform(__shfl(lo, r, kWave)), t0 * KT);
+    RowSum<E> x;
+    x.run(a, it.b, it.kvh, a.q + (int64_t)r_tok * a.ldq + (int64_t)r_head * d, r_lo, r_hi);
+    const bool none = x.there && x.top == -INFINITY;       // scores of -inf alone
+    float* to = whole ? a.out + (int64_t)r_tok * a.ldo + (int64_t)r_head * d : part + (int64_t)(wv * 32 + r) * (d + 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (64 * i + lane < d) to[64 * i + lane] = !x.there || (none && !whole) ? 0.f : x.o[i] / x.sum;
+    if (!whole && lane == 0) {
+      to[d] = none ? kNoScore : x.top;
+      to[d + 1] = x.sum * 0x1p12f;
+    }
+  }
+}
+
+// One workgroup a (tile of rows, kv head).
+template <typename E, int ND, bool FULL>
+__global__ __launch_bounds__(kThreads, ND <= 4 ? 2 : 1) void k_extend_whole(ExtArgs a) {
+  __shared__ typename Shape<E, ND>::Mem mem;
+  Item it;
+  // the last tiles of a sequence see the most keys: they go first
+  if (!find_item(a, a.slots - 1 - (int)(blockIdx.x / (unsigned)a.kv_heads), it)) return;
+  it.kvh = (int)(blockIdx.x % (unsigned)a.kv_heads);
+  int t0, t1;
+  tiles_of<Shape<E, ND>::KT>(a, it, t0, t1);
+  attend<E, ND, FULL>(a, it, t0, t1, t0, t1, nullptr, mem);
+}
+
+template <typename E, int ND, bool FULL>
+void launch_tiles(const ExtArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((k_extend_whole<E, ND, FULL>), dim3((unsigned)a.slots * a.kv_heads), dim3(kThreads), 0, st, a);
+}
+
+template <typename E>
+void extend_for(const ExtArgs& a, hipStream_t st) {
+  switch ((a.d + 31) / 32) {
+    case 1:
+    case 2: a.d == 64 ? launch_tiles<E, 2, true>(a, st) : launch_tiles<E, 2, false>(a, st); break;
+    case 3: launch_tiles<E, 3, false>(a, st); break;
+    case 4: a.d == 128 ? launch_tiles<E, 4, true>(a, st) : launch_tiles<E, 4, false>(a, st); break;
+    case 5:
+    case 6: launch_tiles<E, 6, false>(a, st); break;
+    default: launch_tiles<E, 8, false>(a, st);
+  }
 }
 
 }  // namespace
@@ -167,12 +657,11 @@ int cv3_paged_extend(const float* q, int64_t ldq, int64_t n, int heads, int kv_h
   CV3_REQUIRE(apart(res, in), CV3_EINVAL, "out overlaps the caches, the tables, the lengths or the starts");
   ExtArgs a{q, ldq, k_cache, v_cache, tables, lengths, starts, out, ldo, pages, blocks, n,
             (int)std::min<int64_t>(window, INT32_MAX), (int)batch, (int)page, heads, kv_heads, heads / kv_heads, d,
-            scale * 1.4426950408889634f};
+            (int)(n * (heads / kv_heads) / kRows + batch), scale * 1.4426950408889634f};
   hipStream_t st = stream_of(s);
-  const dim3 grid((unsigned)ceil_div(n * heads, 4));
-  if (cache_type == CV3_F32) hipLaunchKernelGGL(k_extend_rows<float>, grid, dim3(256), 0, st, a);
-  else if (cache_type == CV3_F16) hipLaunchKernelGGL(k_extend_rows<_Float16>, grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(k_extend_rows<__bf16>, grid, dim3(256), 0, st, a);
+  if (cache_type == CV3_F32) extend_for<float>(a, st);
+  else if (cache_type == CV3_F16) extend_for<_Float16>(a, st);
+  else extend_for<__bf16>(a, st);
   CV3_LAUNCHED();
   return CV3_OK;
 }
