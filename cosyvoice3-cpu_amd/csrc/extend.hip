@@ -31,6 +31,9 @@ struct ExtArgs {
   int window;                  // keys that a query sees at most
   int batch, page, heads, kv_heads, group, d, slots;
   float scale;                 // times log2(e)
+  float* part;                 // [2 groups][rows of a tile][d + 2]: output, maximum, sum of a part of a row's keys
+  int2* pairs;                 // [slots][kv heads]
+  int groups, part_rows;
 };
 
 template <typename E>
@@ -608,9 +611,184 @@ __global__ __launch_bounds__(kThreads, ND <= 4 ? 2 : 1) void k_extend_whole(ExtA
   attend<E, ND, FULL>(a, it, t0, t1, t0, t1, nullptr, mem);
 }
 
+// A workgroup's share of the (slot, kv head, key tile) units, in that order.
+struct Plan {
+  int64_t before[kSplitSlots + 1];   // key tiles of one kv head in the slots ahead
+  int32_t slot[kSplitSlots];         // a sequence's first slot
+  int64_t sum[kThreads / 64];
+};
+// The last i of [0, n) with v[i] <= x; v[0] <= x.
+template <typename T>
+__device__ __forceinline__ int last_at(const T* v, int n, T x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (v[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// The units shared out evenly over `groups` workgroups by what the device holds: a long cache with few rows, a ragged
+// batch and a causal triangle all fill the machine, and a captured launch serves every length.  Every workgroup sums
+// over the slots by itself.  An item (slot, kv head) that one workgroup holds whole is written by it; of one that
+// crosses workgroups each leaves its rows' outputs, maxima and sums in `part` (slot 2 w, or 2 w + 1 where the item
+// begins inside w's share), and k_extend_join adds them up.  The workgroup that begins an item enters it into `pairs`:
+// its first part and last workgroup, or -1.  Shares that follow each other go to one XCD, whose L2 they share keys in.
+template <typename E, int ND, bool FULL>
+__global__ __launch_bounds__(kThreads, ND <= 4 ? 2 : 1) void k_extend_split(ExtArgs a) {
+  constexpr int KT = Shape<E, ND>::KT;
+  __shared__ union {
+    typename Shape<E, ND>::Mem mem;
+    Plan plan;
+  } lds;
+  Plan& p = lds.plan;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, slots = a.slots;
+  const int w = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
+  for (int b = tid; b < a.batch; b += kThreads)
+    p.slot[b] = slot_of(a, (int)min((int64_t)max(a.starts[b], 0), a.n), b);
+  __syncthreads();
+  constexpr int kEach = kSplitSlots / kThreads;
+  const int each = (slots + kThreads - 1) / kThreads;
+  int64_t mine[kEach], all = 0;
+#pragma unroll 1
+  for (int i = 0; i < each; ++i) {
+    const int s = tid * each + i;
+    int64_t units = 0;
+    if (s < slots && p.slot[0] <= s) {
+      const int b = last_at(p.slot, a.batch, (int32_t)s);
+      const Seq q = seq_of(a, b);
+      const int64_t row0 = (int64_t)(s - p.slot[b]) * kRows, rows = min((int64_t)q.count * a.group - row0, (int64_t)kRows);
+      if (row0 >= 0 && rows > 0) {
+        Item it{b, 0, q.first, q.base, q.len, (int)row0, (int)rows};
+        int t0, t1;
+        tiles_of<KT>(a, it, t0, t1);
+        units = t1 - t0;
+      }
+    }
+    mine[i] = units;
+    all += units;
+  }
+  int64_t up = all;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t u = __shfl_up(up, o, kWave);
+    if (lane >= o) up += u;
+  }
+  if (lane == 63) p.sum[wv] = up;
+  __syncthreads();
+  int64_t at = up - all, total = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) {
+    if (i < wv) at += p.sum[i];
+    total += p.sum[i];
+  }
+#pragma unroll 1
+  for (int i = 0; i < each; ++i) {
+    const int s = tid * each + i;
+    if (s < slots) p.before[s] = at;
+    at += mine[i];
+  }
+  __syncthreads();
+  total = uniform(total) * a.kv_heads;
+  const int64_t n = min((int64_t)a.groups, total);
+  if (w >= n) return;
+  const int64_t first = total * w / n, end = total * (w + 1) / n;
+  int slot = uniform(last_at(p.before, slots, first / a.kv_heads));
+  int64_t in = first - uniform(p.before[slot]) * a.kv_heads;          // the unit within the slot: [kv head][key tile]
+  int b = uniform(last_at(p.slot, a.batch, (int32_t)slot));
+  __syncthreads();                     // the plan's memory is the tiles' from here on
+
+  at = first;
+  while (at < end) {
+    Item it{};
+    int t0 = 0, t1 = 0;
+    const int tile = slot - slot_of(a, uniform((int)min((int64_t)max(a.starts[b], 0), a.n)), b);
+    if (item_of(a, b, tile, it)) tiles_of<KT>(a, it, t0, t1);
+    const int units = t1 - t0;
+    if (in >= (int64_t)units * a.kv_heads) {           // the next slot; of the next sequence, where it begins there
+      in -= (int64_t)units * a.kv_heads;
+      if (++slot >= slots) return;                     // lengths that changed under the call
+      while (b + 1 < a.batch && slot_of(a, uniform((int)min((int64_t)max(a.starts[b + 1], 0), a.n)), b + 1) <= slot) ++b;
+      continue;
+    }
+    it.kvh = (int)(in / units);
+    const int t = (int)(in - (int64_t)it.kvh * units), take = (int)min((int64_t)(units - t), end - at);
+    const int place = 2 * w + (at == first ? 0 : 1);
+    if (tid == 0 && t == 0) {
+      const bool whole = take == units;
+      a.pairs[(int64_t)slot * a.kv_heads + it.kvh] =
+          make_int2(whole ? -1 : place, whole ? 0 : (int)(((at + units) * n - 1) / total));
+    }
+    attend<E, ND, FULL>(a, it, t0 + t, t0 + t + take, t0, t1, a.part + (int64_t)place * a.part_rows * (a.d + 2), lds.mem);
+    __syncthreads();                   // before the next item's first page ids
+    at += take;
+    in += take;
+  }
+}
+
+// Rows of items that crossed workgroups, and zeros for those with no key to see: a wave a row at a time, eight rows each.
+constexpr int kJoinRows = 32;
+__global__ __launch_bounds__(kThreads) void k_extend_join(ExtArgs a) {
+  const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
+  const int slot = (int)(blockIdx.x / (unsigned)a.kv_heads), row0 = blockIdx.y * kJoinRows;
+  Item it;
+  if (!find_item(a, slot, it) || row0 >= it.rows) return;
+  it.kvh = (int)(blockIdx.x % (unsigned)a.kv_heads);
+  const bool none = it.hi_of(a, it.rows - 1) == 0;
+  const int2 pair = none ? make_int2(0, 0) : a.pairs[blockIdx.x];
+  if (pair.x < 0) return;              // written by the one workgroup that held it
+  const int w0 = min(pair.x >> 1, a.groups - 1), count = none ? 0 : min(pair.y, a.groups - 1) - w0 + 1;
+  for (int r = row0 + wv; r < min(row0 + kJoinRows, it.rows); r += kThreads / 64) {
+    const int flat = it.row0 + r, head = it.kvh * a.group + flat % a.group;
+    float* out = a.out + (int64_t)(it.first + flat / a.group) * a.ldo + (int64_t)head * a.d;
+    float x[4], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = 0.f;
+    constexpr int kAhead = 4;
+    for (int i = 0; i < count; i += kAhead) {
+      float y[kAhead][4], t[kAhead], l[kAhead], now = top;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int m = min(i + u, count - 1);
+        const float* src = a.part + ((int64_t)(m ? 2 * (w0 + m) : pair.x) * a.part_rows + r) * (a.d + 2);
+        t[u] = i + u < count ? src[a.d] : -INFINITY;
+        l[u] = src[a.d + 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[u][j] = 64 * j + lane < a.d ? src[64 * j + lane] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) now = fmaxf(now, t[u]);
+      const float f = weight_of(top, now);
+      sum *= f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] *= f;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (t[u] != -INFINITY) {
+          const float g = weight_of(t[u], now) * l[u];
+          sum += g;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] += g * y[u][j];
+        }
+      top = now;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (64 * j + lane < a.d) out[64 * j + lane] = top != -INFINITY ? x[j] / sum : 0.f;
+  }
+}
+
+constexpr int groups_of(int d) { return d <= 128 ? 512 : 256; }     // workgroups that the registers let run at once
+
 template <typename E, int ND, bool FULL>
 void launch_tiles(const ExtArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((k_extend_whole<E, ND, FULL>), dim3((unsigned)a.slots * a.kv_heads), dim3(kThreads), 0, st, a);
+  if (!a.part) {
+    hipLaunchKernelGGL((k_extend_whole<E, ND, FULL>), dim3((unsigned)a.slots * a.kv_heads), dim3(kThreads), 0, st, a);
+    return;
+  }
+  hipLaunchKernelGGL((k_extend_split<E, ND, FULL>), dim3(a.groups), dim3(kThreads), 0, st, a);
+  hipLaunchKernelGGL(k_extend_join, dim3((unsigned)a.slots * a.kv_heads, (unsigned)ceil_div(a.part_rows, kJoinRows)), dim3(kThreads),
+                     0, st, a);
 }
 
 template <typename E>
@@ -657,13 +835,27 @@ int cv3_paged_extend(const float* q, int64_t ldq, int64_t n, int heads, int kv_h
   CV3_REQUIRE(apart(res, in), CV3_EINVAL, "out overlaps the caches, the tables, the lengths or the starts");
   ExtArgs a{q, ldq, k_cache, v_cache, tables, lengths, starts, out, ldo, pages, blocks, n,
             (int)std::min<int64_t>(window, INT32_MAX), (int)batch, (int)page, heads, kv_heads, heads / kv_heads, d,
-            (int)(n * (heads / kv_heads) / kRows + batch), scale * 1.4426950408889634f};
+            (int)(n * (heads / kv_heads) / kRows + batch), scale * 1.4426950408889634f, nullptr, nullptr, 0, 0};
   hipStream_t st = stream_of(s);
+  const int64_t cap = blocks * page, items = (int64_t)a.slots * kv_heads;
+  const bool whole = a.slots > kSplitSlots || cap <= 256 || items >= 8192;
+  if (!whole) {
+    a.groups = groups_of(d);
+    a.part_rows = (int)std::min<int64_t>(kRows, n * a.group);
+    const size_t parts = (size_t)2 * a.groups * a.part_rows * (d + 2) * sizeof(float);      // a multiple of 8
+    void* work = nullptr;
+    const int rc = scratch_alloc(&work, parts + (size_t)items * sizeof(int2), st);
+    if (rc && rc != CV3_ENOMEM) return rc;     // without memory: one workgroup an item
+    a.part = (float*)work;
+    a.pairs = (int2*)((char*)work + parts);
+  }
   if (cache_type == CV3_F32) extend_for<float>(a, st);
   else if (cache_type == CV3_F16) extend_for<_Float16>(a, st);
   else extend_for<__bf16>(a, st);
-  CV3_LAUNCHED();
-  return CV3_OK;
+  const hipError_t err = hipGetLastError();
+  const int rc = a.part ? scratch_free(a.part, st) : CV3_OK;
+  CV3_REQUIRE(err == hipSuccess, CV3_EHIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return rc;
 }
 
 }  // extern "C"
