@@ -126,7 +126,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kRows = 128;          // (token, head) rows of a workgroup: 32 a wave
 constexpr int kThreads = 256;
 constexpr int kSplitSlots = 2048;   // tiles of rows whose keys may be shared out
-constexpr float kUp = 12.f, kSlack = 3.f;   // weights are held 2^12 up, and pass that by at most 2^3: below the largest float16
+// Weights are held 2^10 up against a reference that a row's largest score has passed by so little that the 32 of a lane
+// sum to no more than kMost, which float16 holds; so small planes end 2^-35 below the largest weight or lower.
+constexpr float kUp = 10.f, kMost = 60000.f;
 
 // How a cache's numbers become float16 operands.  float32: two planes, x 2^s = hi + lo within 2^-23 of x or 2^-25.
 // bfloat16: one plane that holds x 2^s whole, down to 2^-17 of the largest's.  float16: as it is.
@@ -163,7 +165,9 @@ __device__ __forceinline__ h2 half2_of(float a, float b) { return __builtin_conv
 // x = hi + lo
 __device__ __forceinline__ void split2(float a, float b, h2& hi, h2& lo) {
   hi = half2_of(a, b);
-  lo = half2_of(a - (float)hi[0], b - (float)hi[1]);
+  float minus = -1.f;                  // kept from folding: what is left is one mixed multiply-add each, exact
+  asm("" : "+s"(minus));
+  lo = half2_of(fmaf((float)hi[0], minus, a), fmaf((float)hi[1], minus, b));
 }
 __device__ __forceinline__ h4 join4(h2 a, h2 b) { return h4{a[0], a[1], b[0], b[1]}; }
 
@@ -224,8 +228,8 @@ struct Shape {
   static constexpr int KS = DP + 8, VS = KT + 8;       // strides: 16 rows 16 bytes apart lie in distinct banks
   static constexpr int BLOCKS = KT / 4 * (DP / 4), NB = (BLOCKS + kThreads - 1) / kThreads;
   struct Mem {
-    _Float16 k[N][KT * KS];                            // [key][channel]
-    _Float16 v[N][DP * VS];                            // [channel][key], keys in the order that the product takes them
+    alignas(16) _Float16 k[N][KT * KS];                // [key][channel]
+    alignas(16) _Float16 v[N][DP * VS];                // [channel][key], keys in the order that the product takes them
     int64_t off[KT];
     uint64_t mask;
     float mx[kThreads / 64][2];
@@ -486,23 +490,46 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       const float c = factor * down;
       // a score's terms are up to 2^30 c, and off by 2^-10 c where the small planes end: 2^-23 with 16 of them
       coarse = coarse || !(c <= (C::SCALED ? 0x1p-17f : 0x1p-8f));
-      float mx = sc[0][0];
+      // Weights against the reference so far, whose sum of positive numbers shows whether one of them is too large for
+      // float16.  Only then, and for rows that have met no key before, the tile's maximum is found and the reference moved.
+      h8 ph[KT / 16], pl[KT / 16];
+      float tile = 0.f;
+      auto weigh = [&]() {
+        const float ref = (top == -INFINITY ? 0.f : top) - kUp;
+        tile = 0.f;
 #pragma unroll
-      for (int u = 0; u < KT / 32; ++u)
+        for (int u = 0; u < KT / 16; ++u) {
+          float part_sum = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[u][r]);
-      {
+          for (int e = 0; e < 8; e += 2) {
+            const float p0 = exp2_fast(fmaf(sc[u / 2][8 * (u % 2) + e], c, -ref));
+            const float p1 = exp2_fast(fmaf(sc[u / 2][8 * (u % 2) + e + 1], c, -ref));
+            part_sum += p0 + p1;
+            h2 h, l;
+            split2(p0, p1, h, l);
+            ph[u][e] = h[0], ph[u][e + 1] = h[1];
+            pl[u][e] = l[0], pl[u][e + 1] = l[1];
+          }
+          tile += part_sum;
+        }
+      };
+      float f = 1.f;
+      weigh();
+      if (__any(!(tile <= kMost) || top == -INFINITY)) {
+        float mx = sc[0][0];
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[u][r]);
         const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
         mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
-      }
-      // the running maximum moves only when a score passes it by more than 2^kSlack
-      float f = 1.f;
-      if (__any(!(mx <= top + kSlack) && mx != -INFINITY)) {
         const float up = fmaxf(mx, top);
         f = weight_of(top, up);
         top = up;
         sum *= f;
+        weigh();
       }
+      sum += tile;
       if (C::SCALED && o_up != v_up) {
         f *= ldexpf(1.f, v_up - o_up);
         o_up = v_up;
@@ -513,33 +540,18 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[i][r] *= f;
       }
-      const float ref = (top == -INFINITY ? 0.f : top) - kUp;
 #pragma unroll
-      for (int u = 0; u < KT / 16; ++u) {
-        h8 ph, pl;
-        float part_sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float p0 = exp2_fast(fmaf(sc[u / 2][8 * (u % 2) + e], c, -ref));
-          const float p1 = exp2_fast(fmaf(sc[u / 2][8 * (u % 2) + e + 1], c, -ref));
-          part_sum += p0 + p1;
-          h2 h, l;
-          split2(p0, p1, h, l);
-          ph[e] = h[0], ph[e + 1] = h[1];
-          pl[e] = l[0], pl[e + 1] = l[1];
-        }
-        sum += part_sum;
+      for (int u = 0; u < KT / 16; ++u)
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
           const h8 vh = *(const h8*)&mem.v[0][(32 * i + n) * VS + 16 * u + 8 * g];
-          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph, o[i], 0, 0, 0);
-          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl, o[i], 0, 0, 0);
+          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[u], o[i], 0, 0, 0);
+          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[u], o[i], 0, 0, 0);
           if constexpr (N == 2) {
             const h8 vl = *(const h8*)&mem.v[1][(32 * i + n) * VS + 16 * u + 8 * g];
-            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[u], o[i], 0, 0, 0);
           }
         }
-      }
     }
   }
 
@@ -593,7 +605,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       if (64 * i + lane < d) to[64 * i + lane] = !x.there || (none && !whole) ? 0.f : x.o[i] / x.sum;
     if (!whole && lane == 0) {
       to[d] = none ? kNoScore : x.top;
-      to[d + 1] = x.sum * 0x1p12f;
+      to[d + 1] = x.sum * 0x1p10f;
     }
   }
 }
