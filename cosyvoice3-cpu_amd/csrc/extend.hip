@@ -29,6 +29,7 @@ struct ExtArgs {
   int64_t ldo;
   int64_t pages, blocks, n;
   int window;                  // keys that a query sees at most
+  uint32_t page_inv;           // (2^32 - 1) / page
   int batch, page, heads, kv_heads, group, d, slots;
   float scale;                 // times log2(e)
   float* part;                 // [2 groups][rows of a tile][d + 2]: output, maximum, sum of a part of a row's keys
@@ -161,15 +162,18 @@ struct Cell<_Float16> {
   static __device__ __forceinline__ void four(const uint2&, float*) {}
 };
 
+// x up = hi + lo, each rounded to float16 from the exact sum of product and addend (mixed multiply-adds; `zero` and `one`
+// are kept from folding, which would bring back a multiplication and two conversions).
+struct Exact {
+  float zero, one;
+  __device__ __forceinline__ Exact() {
+    zero = 0.f, one = 1.f;
+    asm("" : "+s"(zero), "+s"(one));
+  }
+  __device__ __forceinline__ _Float16 scaled(float x, float up) const { return (_Float16)fmaf(x, up, zero); }
+  static __device__ __forceinline__ _Float16 rest(float x, float up, _Float16 hi) { return (_Float16)fmaf(x, up, -(float)hi); }
+};
 __device__ __forceinline__ h2 half2_of(float a, float b) { return __builtin_convertvector((f32x2{a, b}), h2); }
-// x = hi + lo
-__device__ __forceinline__ void split2(float a, float b, h2& hi, h2& lo) {
-  hi = half2_of(a, b);
-  float minus = -1.f;                  // kept from folding: what is left is one mixed multiply-add each, exact
-  asm("" : "+s"(minus));
-  lo = half2_of(fmaf((float)hi[0], minus, a), fmaf((float)hi[1], minus, b));
-}
-__device__ __forceinline__ h4 join4(h2 a, h2 b) { return h4{a[0], a[1], b[0], b[1]}; }
 
 // 2^15 over the power of two above x: what brings numbers of at most x below the largest float16.
 __device__ __forceinline__ int up_of(float x) {
@@ -223,13 +227,22 @@ __device__ __forceinline__ bool find_item(const ExtArgs& a, int slot, Item& it) 
 template <typename E, int ND>
 struct Shape {
   static constexpr int DP = 32 * ND;                   // channels, padded
-  static constexpr int KT = ND <= 4 ? 64 : 32;         // keys of a tile
   static constexpr int N = Cell<E>::N;
-  static constexpr int KS = DP + 8, VS = KT + 8;       // strides: 16 rows 16 bytes apart lie in distinct banks
+  // Keys of a tile: 64 where the registers hold what a thread fetches of it ahead (8 x 800 queries over 5800 keys, 32 on 8
+  // heads of 128: float32 2.98 ms with 64, 2.39 with 32; bfloat16 1.93 and 1.50; float16, not widened, 1.25 and 1.29).
+  static constexpr int KT = ND <= 2 || (ND <= 4 && N == 1 && !Cell<E>::SCALED) ? 64 : 32;
+  static constexpr int KS = DP + 8;                    // 16 rows, each this much on, lie in distinct banks
   static constexpr int BLOCKS = KT / 4 * (DP / 4), NB = (BLOCKS + kThreads - 1) / kThreads;
+  // Where eight keys of a channel lie: step u takes keys 16 u + {0 .. 3, 8 .. 11} and {4 .. 7, 12 .. 15}, run r = 2 u + 0
+  // and 1.  Runs are exchanged by channel bits so that 16 channels' reads of a run fall into distinct banks, and likewise
+  // the writes of 16 threads, whose channels are 4 apart.
+  static __device__ __forceinline__ int v_at(int channel, int run) {
+    const int turn = KT == 64 ? (channel >> 1 & 7) ^ (channel >> 4 & 1) : (channel >> 2 & 3) ^ (channel >> 4 & 3);
+    return channel * KT + 8 * (run ^ turn);
+  }
   struct Mem {
     alignas(16) _Float16 k[N][KT * KS];                // [key][channel]
-    alignas(16) _Float16 v[N][DP * VS];                // [channel][key], keys in the order that the product takes them
+    alignas(16) _Float16 v[N][DP * KT];                // [channel][key], see v_at
     int64_t off[KT];
     uint64_t mask;
     float mx[kThreads / 64][2];
@@ -252,7 +265,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
   typedef Shape<E, ND> S;
   typedef Cell<E> C;
   typedef typename C::Raw Raw;
-  constexpr int KT = S::KT, DP = S::DP, N = S::N, KS = S::KS, VS = S::VS, NB = S::NB, CG = DP / 4;
+  constexpr int KT = S::KT, DP = S::DP, N = S::N, KS = S::KS, NB = S::NB, CG = DP / 4;
   const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), n = lane & 31, g = lane >> 5;
   const int d = FULL ? DP : a.d;
   const int row = wv * 32 + n;
@@ -266,6 +279,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
   const int w_lo = Item::lo_of(a, s_hi), s_lo = Item::lo_of(a, w_hi);
   const float* q = a.q + (int64_t)tok * a.ldq + (int64_t)head * d;
 
+  const Exact exact;
   // the row's channels 16 s + 8 g .. + 8, in two planes
   h8 qh[DP / 16], ql[DP / 16];
   float factor;                        // of the row's scores: |scale| log2(e) over its power of two
@@ -288,14 +302,13 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     big = fmaxf(big, __shfl_xor(big, 32, kWave));
     const int up = up_of(big);
     factor = ldexpf(fabsf(a.scale), -up);
+    const float unit = ldexpf(1.f, up);
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        h2 h, l;
-        split2(ldexpf(x[s][e], up), ldexpf(x[s][e + 1], up), h, l);
-        qh[s][e] = h[0], qh[s][e + 1] = h[1];
-        ql[s][e] = l[0], ql[s][e + 1] = l[1];
+      for (int e = 0; e < 8; ++e) {
+        qh[s][e] = exact.scaled(x[s][e], unit);
+        ql[s][e] = Exact::rest(x[s][e], unit, qh[s][e]);
       }
   }
 
@@ -308,8 +321,9 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     in = 0;
     const int key = t * KT + tid;
     if (tid < KT && t < t1 && key < it.len) {
-      const uint32_t blk = (uint32_t)key / (uint32_t)a.page;
+      uint32_t blk = __umulhi((uint32_t)key, a.page_inv);          // the quotient, or one less
       in = (uint32_t)key - blk * (uint32_t)a.page;
+      if (in >= (uint32_t)a.page) ++blk, in -= (uint32_t)a.page;
       id = table[blk];
     }
   };
@@ -323,26 +337,35 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
   };
   // this thread's blocks of 4 keys x 4 channels
   Raw kr[NB][4], vr[NB][4];
+  constexpr uint64_t kAll = ~(uint64_t)0 >> (64 - KT);
   uint64_t mask = 0;
   auto fetch = [&]() {
     mask = mem.mask;
     mask = (uint64_t)uniform((int64_t)mask);
-    const bool all = mask == (KT == 64 ? ~(uint64_t)0 : ((uint64_t)1 << (KT & 63)) - 1);
+    const bool all = mask == kAll;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int at = tid + j * kThreads, cg = at % CG, kg = at / CG;
       const bool on = (S::BLOCKS % kThreads == 0 || at < S::BLOCKS) && (FULL || 4 * cg < d);
+      int64_t off[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t off = on ? mem.off[4 * kg + i] : -1;
-        kr[j][i] = vr[j][i] = Raw{};
-        if (FULL && S::BLOCKS % kThreads == 0 && all) {
-          kr[j][i] = *(const Raw*)(kc + off + 4 * cg);
-          vr[j][i] = *(const Raw*)(vc + off + 4 * cg);
-        } else if (off >= 0) {
-          kr[j][i] = *(const Raw*)(kc + off + 4 * cg);
-          vr[j][i] = *(const Raw*)(vc + off + 4 * cg);
+      for (int i = 0; i < 4; ++i) off[i] = mem.off[(S::BLOCKS % kThreads == 0 ? 4 * kg : 4 * kg % KT) + i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kr[j][i] = vr[j][i] = Raw{};
+      if (all) {
+        if (on) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) kr[j][i] = *(const Raw*)(kc + off[i] + 4 * cg);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vr[j][i] = *(const Raw*)(vc + off[i] + 4 * cg);
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (on && off[i] >= 0) {
+            kr[j][i] = *(const Raw*)(kc + off[i] + 4 * cg);
+            vr[j][i] = *(const Raw*)(vc + off[i] + 4 * cg);
+          }
       }
     }
   };
@@ -405,22 +428,28 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
         for (int j = 0; j < NB; ++j) {
           const int at = tid + j * kThreads, cg = at % CG, kg = at / CG;
           if (S::BLOCKS % kThreads != 0 && at >= S::BLOCKS) continue;
-          const int slot = 16 * (kg >> 2) + 8 * (kg & 1) + 4 * (kg >> 1 & 1);
+          const int run = 2 * (kg >> 2) + (kg & 1), half = 4 * (kg >> 1 & 1);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            h2 h0, l0, h1, l1;
-            split2(kx[j][i][0] * ku, kx[j][i][1] * ku, h0, l0);
-            split2(kx[j][i][2] * ku, kx[j][i][3] * ku, h1, l1);
-            *(h4*)&mem.k[0][(4 * kg + i) * KS + 4 * cg] = join4(h0, h1);
-            if constexpr (N == 2) *(h4*)&mem.k[1][(4 * kg + i) * KS + 4 * cg] = join4(l0, l1);
+            h4 h, l;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              h[c] = exact.scaled(kx[j][i][c], ku);
+              if constexpr (N == 2) l[c] = Exact::rest(kx[j][i][c], ku, h[c]);
+            }
+            *(h4*)&mem.k[0][(4 * kg + i) * KS + 4 * cg] = h;
+            if constexpr (N == 2) *(h4*)&mem.k[1][(4 * kg + i) * KS + 4 * cg] = l;
           }
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            h2 h0, l0, h1, l1;
-            split2(vx[j][0][c] * vu, vx[j][1][c] * vu, h0, l0);
-            split2(vx[j][2][c] * vu, vx[j][3][c] * vu, h1, l1);
-            *(h4*)&mem.v[0][(4 * cg + c) * VS + slot] = join4(h0, h1);
-            if constexpr (N == 2) *(h4*)&mem.v[1][(4 * cg + c) * VS + slot] = join4(l0, l1);
+            h4 h, l;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              h[i] = exact.scaled(vx[j][i][c], vu);
+              if constexpr (N == 2) l[i] = Exact::rest(vx[j][i][c], vu, h[i]);
+            }
+            *(h4*)&mem.v[0][S::v_at(4 * cg + c, run) + half] = h;
+            if constexpr (N == 2) *(h4*)&mem.v[1][S::v_at(4 * cg + c, run) + half] = l;
           }
         }
       } else {
@@ -428,7 +457,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
         for (int j = 0; j < NB; ++j) {
           const int at = tid + j * kThreads, cg = at % CG, kg = at / CG;
           if (S::BLOCKS % kThreads != 0 && at >= S::BLOCKS) continue;
-          const int slot = 16 * (kg >> 2) + 8 * (kg & 1) + 4 * (kg >> 1 & 1);
+          const int run = 2 * (kg >> 2) + (kg & 1), half = 4 * (kg >> 1 & 1);
           uint32_t x[4][2];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -439,7 +468,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
 #pragma unroll
           for (int c = 0; c < 4; ++c) {      // 4 x 4 two-byte values turned by byte permutations
             const uint32_t sel = c % 2 ? 0x07060302u : 0x05040100u;
-            *(uint2*)&mem.v[0][(4 * cg + c) * VS + slot] = make_uint2(__builtin_amdgcn_perm(x[1][c / 2], x[0][c / 2], sel),
+            *(uint2*)&mem.v[0][S::v_at(4 * cg + c, run) + half] = make_uint2(__builtin_amdgcn_perm(x[1][c / 2], x[0][c / 2], sel),
                                                                      __builtin_amdgcn_perm(x[3][c / 2], x[2][c / 2], sel));
           }
         }
@@ -459,19 +488,24 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[u][r] = 0.f;
 #pragma unroll
-      for (int s = 0; s < DP / 16; ++s)
+      for (int s = 0; s < DP / 16; ++s) {
+        // products of one accumulator are kept apart: one that follows on another of the same waits for it
+        h8 kx8[N][KT / 32];
 #pragma unroll
-        for (int u = 0; u < KT / 32; ++u) {
-          const h8 kh = *(const h8*)&mem.k[0][(32 * u + n) * KS + 16 * s + 8 * g];
-          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[s], sc[u], 0, 0, 0);
-          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[s], sc[u], 0, 0, 0);
-          if constexpr (N == 2) {
-            const h8 kl = *(const h8*)&mem.k[1][(32 * u + n) * KS + 16 * s + 8 * g];
-            sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[s], sc[u], 0, 0, 0);
-          }
+        for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+          for (int j = 0; j < N; ++j) kx8[j][u] = *(const h8*)&mem.k[j][(32 * u + n) * KS + 16 * s + 8 * g];
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx8[0][u], qh[s], sc[u], 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx8[0][u], ql[s], sc[u], 0, 0, 0);
+        if constexpr (N == 2) {
+#pragma unroll
+          for (int u = 0; u < KT / 32; ++u) sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx8[1][u], qh[s], sc[u], 0, 0, 0);
         }
+      }
       // register r of sc[u]: key 32 u + 8 (r / 4) + 4 g + r % 4
-      const bool every = now == (KT == 64 ? ~(uint64_t)0 : ((uint64_t)1 << (KT & 63)) - 1) && k0 + KT <= s_hi && k0 >= s_lo;
+      const bool every = now == kAll && k0 + KT <= s_hi && k0 >= s_lo;
       if (every) {
         there = true;
       } else {
@@ -490,68 +524,73 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       const float c = factor * down;
       // a score's terms are up to 2^30 c, and off by 2^-10 c where the small planes end: 2^-23 with 16 of them
       coarse = coarse || !(c <= (C::SCALED ? 0x1p-17f : 0x1p-8f));
-      // Weights against the reference so far, whose sum of positive numbers shows whether one of them is too large for
-      // float16.  Only then, and for rows that have met no key before, the tile's maximum is found and the reference moved.
-      h8 ph[KT / 16], pl[KT / 16];
-      float tile = 0.f;
-      auto weigh = [&]() {
-        const float ref = (top == -INFINITY ? 0.f : top) - kUp;
-        tile = 0.f;
-#pragma unroll
-        for (int u = 0; u < KT / 16; ++u) {
-          float part_sum = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float p0 = exp2_fast(fmaf(sc[u / 2][8 * (u % 2) + e], c, -ref));
-            const float p1 = exp2_fast(fmaf(sc[u / 2][8 * (u % 2) + e + 1], c, -ref));
-            part_sum += p0 + p1;
-            h2 h, l;
-            split2(p0, p1, h, l);
-            ph[u][e] = h[0], ph[u][e + 1] = h[1];
-            pl[u][e] = l[0], pl[u][e + 1] = l[1];
-          }
-          tile += part_sum;
-        }
-      };
-      float f = 1.f;
-      weigh();
-      if (__any(!(tile <= kMost) || top == -INFINITY)) {
-        float mx = sc[0][0];
-#pragma unroll
-        for (int u = 0; u < KT / 32; ++u)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[u][r]);
-        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
-        const float up = fmaxf(mx, top);
-        f = weight_of(top, up);
-        top = up;
-        sum *= f;
-        weigh();
-      }
-      sum += tile;
       if (C::SCALED && o_up != v_up) {
-        f *= ldexpf(1.f, v_up - o_up);
+        const float f = ldexpf(1.f, v_up - o_up);
         o_up = v_up;
-      }
-      if (__any(f != 1.f)) {
 #pragma unroll
         for (int i = 0; i < ND; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[i][r] *= f;
       }
+      // Half by half, 32 keys: weights against the reference so far, whose sum of positive numbers shows whether one of
+      // them is too large for float16.  Only then, and for rows that have met no key before, the largest score is found
+      // and the reference moved.  The products of one half run beside the weights of the next.
 #pragma unroll
-      for (int u = 0; u < KT / 16; ++u)
+      for (int w = 0; w < KT / 32; ++w) {
+        h8 ph[2], pl[2];
+        float part_sum;
+        auto weigh = [&]() {
+          const float ref = (top == -INFINITY ? 0.f : top) - kUp;
+          part_sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < ND; ++i) {
-          const h8 vh = *(const h8*)&mem.v[0][(32 * i + n) * VS + 16 * u + 8 * g];
-          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[u], o[i], 0, 0, 0);
-          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[u], o[i], 0, 0, 0);
+          for (int u = 0; u < 2; ++u) {
+            float x = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const float p0 = exp2_fast(fmaf(sc[w][8 * u + e], c, -ref)), p1 = exp2_fast(fmaf(sc[w][8 * u + e + 1], c, -ref));
+              x += p0 + p1;
+              const h2 h = half2_of(p0, p1);
+              ph[u][e] = h[0], ph[u][e + 1] = h[1];
+              pl[u][e] = Exact::rest(p0, exact.one, h[0]), pl[u][e + 1] = Exact::rest(p1, exact.one, h[1]);
+            }
+            part_sum += x;
+          }
+        };
+        weigh();
+        if (__any(!(part_sum <= kMost) || top == -INFINITY)) {
+          float mx = sc[w][0];
+#pragma unroll
+          for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[w][r]);
+          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+          mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
+          const float up = fmaxf(mx, top), f = weight_of(top, up);
+          top = up;
+          sum *= f;
+#pragma unroll
+          for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][r] *= f;
+          weigh();
+        }
+        sum += part_sum;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          // products of one accumulator are kept apart, as above
+          h8 vx8[N][ND];
+#pragma unroll
+          for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) vx8[j][i] = *(const h8*)&mem.v[j][S::v_at(32 * i + n, 4 * w + 2 * u + g)];
+#pragma unroll
+          for (int i = 0; i < ND; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx8[0][i], ph[u], o[i], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < ND; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx8[0][i], pl[u], o[i], 0, 0, 0);
           if constexpr (N == 2) {
-            const h8 vl = *(const h8*)&mem.v[1][(32 * i + n) * VS + 16 * u + 8 * g];
-            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[u], o[i], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < ND; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx8[1][i], ph[u], o[i], 0, 0, 0);
           }
         }
+      }
     }
   }
 
@@ -846,7 +885,7 @@ int cv3_paged_extend(const float* q, int64_t ldq, int64_t n, int heads, int kv_h
   const Run res[] = {{out, 4.0 * ((n - 1) * (double)ldo + (double)heads * d)}};
   CV3_REQUIRE(apart(res, in), CV3_EINVAL, "out overlaps the caches, the tables, the lengths or the starts");
   ExtArgs a{q, ldq, k_cache, v_cache, tables, lengths, starts, out, ldo, pages, blocks, n,
-            (int)std::min<int64_t>(window, INT32_MAX), (int)batch, (int)page, heads, kv_heads, heads / kv_heads, d,
+            (int)std::min<int64_t>(window, INT32_MAX), (uint32_t)(0xffffffffu / (uint32_t)page), (int)batch, (int)page, heads, kv_heads, heads / kv_heads, d,
             (int)(n * (heads / kv_heads) / kRows + batch), scale * 1.4426950408889634f, nullptr, nullptr, 0, 0};
   hipStream_t st = stream_of(s);
   const int64_t cap = blocks * page, items = (int64_t)a.slots * kv_heads;
