@@ -32,9 +32,12 @@ struct ExtArgs {
   uint32_t page_inv;           // (2^32 - 1) / page
   int batch, page, heads, kv_heads, group, d, slots;
   float scale;                 // times log2(e)
-  float* part;                 // [2 groups][rows of a tile][d + 2]: output, maximum, sum of a part of a row's keys
-  int2* pairs;                 // [slots][kv heads]
-  int groups, part_rows;
+  float* part;                 // [places][rows of a tile][d]: outputs of parts of the rows' keys
+  float2* part_ml;             // [places][rows of a tile]: their maxima and sums
+  struct Piece* pieces;        // parts of items, a workgroup each
+  struct Piece* cuts;          // the first part of every item that has several
+  int* counts;                 // of cuts and pieces
+  int groups, part_rows, pieces_most, places, cuts_most;
 };
 
 template <typename E>
@@ -124,9 +127,11 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kRows = 128;          // (token, head) rows of a workgroup: 32 a wave
-constexpr int kThreads = 256;
-constexpr int kSplitSlots = 2048;   // tiles of rows whose keys may be shared out
+constexpr int kWaveRows = 32;       // (token, head) rows of a wave
+constexpr int kSplitSlots = 1024;   // tiles of rows whose keys may be shared out
+constexpr int kWholeKeys = 1024;    // tables up to here are not worth a plan: 12 prompts of up to 900 tokens 68 us without, 90 with
+constexpr int kFewRows = 48;        // rows a sequence, on average, that one wave takes
+
 // Weights are held 2^10 up against a reference that a row's largest score has passed by so little that the 32 of a lane
 // sum to no more than kMost, which float16 holds; so small planes end 2^-35 below the largest weight or lower.
 constexpr float kUp = 10.f, kMost = 60000.f;
@@ -180,7 +185,8 @@ __device__ __forceinline__ int up_of(float x) {
   return x > 0.f && x < INFINITY ? min(15 - __builtin_amdgcn_frexp_expf(x), 126) : 15;
 }
 
-// A tile of rows: rows row0 .. row0 + rows of sequence b's count * group (token, head of the group) rows, for one kv head.
+// A tile of rows, a workgroup's: rows row0 .. row0 + rows of sequence b's count * group (token, head of the group) rows,
+// for one kv head.
 struct Item {
   int b, kvh, first, base, len, row0, rows;
   __device__ __forceinline__ int hi_of(const ExtArgs& a, int r) const {     // keys seen: [lo, hi)
@@ -189,11 +195,19 @@ struct Item {
   static __device__ __forceinline__ int lo_of(const ExtArgs& a, int hi) { return max(0, hi - a.window); }
 };
 
-// Slots: sequence b's tiles are those from floor(starts[b] group / 128) + b on, so that no two sequences share one.
+// Slots: sequence b's tiles of W waves are those from floor(starts[b] group / (32 W)) + b on, so that no two sequences
+// share one.
+template <int W>
 __device__ __forceinline__ int slot_of(const ExtArgs& a, int first, int b) {
-  return (int)((int64_t)first * a.group / kRows) + b;
+  return (int)((int64_t)first * a.group / (kWaveRows * W)) + b;
 }
+template <int W>
+__device__ __forceinline__ int first_slot(const ExtArgs& a, int b) {
+  return slot_of<W>(a, (int)min((int64_t)max(a.starts[b], 0), a.n), b);
+}
+template <int W>
 __device__ __forceinline__ bool item_of(const ExtArgs& a, int b, int tile, Item& it) {
+  constexpr int kRows = kWaveRows * W;
   const Seq s = seq_of(a, b);
   it.b = b;
   it.first = uniform(s.first), it.base = uniform(s.base), it.len = uniform(s.len);
@@ -212,27 +226,29 @@ __device__ __forceinline__ void tiles_of(const ExtArgs& a, const Item& it, int& 
   if (hi == 0) t1 = t0;
 }
 // The sequence of a slot, by every thread of the workgroup alike: how many begin at or before it.
+template <int W, int WAVES = W>
 __device__ __forceinline__ bool find_item(const ExtArgs& a, int slot, Item& it) {
   int before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+  for (int b0 = 0; b0 < a.batch; b0 += 64 * WAVES) {
     const int b = b0 + (int)threadIdx.x;
-    const bool at = b < a.batch && slot_of(a, (int)min((int64_t)max(a.starts[b], 0), a.n), b) <= slot;
-    before += __syncthreads_count(at);
+    before += __syncthreads_count(b < a.batch && first_slot<W>(a, b) <= slot);
   }
   if (before == 0) return false;
   const int b = uniform(before - 1);
-  return item_of(a, b, slot - uniform(slot_of(a, (int)min((int64_t)max(a.starts[b], 0), a.n), b)), it);
+  return item_of<W>(a, b, slot - uniform(first_slot<W>(a, b)), it);
 }
 
-template <typename E, int ND>
+template <typename E, int ND, int W>
 struct Shape {
+  static constexpr int T = 64 * W;                     // threads
   static constexpr int DP = 32 * ND;                   // channels, padded
   static constexpr int N = Cell<E>::N;
   // Keys of a tile: 64 where the registers hold what a thread fetches of it ahead (8 x 800 queries over 5800 keys, 32 on 8
   // heads of 128: float32 2.98 ms with 64, 2.39 with 32; bfloat16 1.93 and 1.50; float16, not widened, 1.25 and 1.29).
-  static constexpr int KT = ND <= 2 || (ND <= 4 && N == 1 && !Cell<E>::SCALED) ? 64 : 32;
+  // One wave alone fetches all of a tile: 32.
+  static constexpr int KT = W > 1 && (ND <= 2 || (ND <= 4 && N == 1 && !Cell<E>::SCALED)) ? 64 : 32;
   static constexpr int KS = DP + 8;                    // 16 rows, each this much on, lie in distinct banks
-  static constexpr int BLOCKS = KT / 4 * (DP / 4), NB = (BLOCKS + kThreads - 1) / kThreads;
+  static constexpr int BLOCKS = KT / 4 * (DP / 4), NB = (BLOCKS + T - 1) / T;
   // Where eight keys of a channel lie: step u takes keys 16 u + {0 .. 3, 8 .. 11} and {4 .. 7, 12 .. 15}, run r = 2 u + 0
   // and 1.  Runs are exchanged by channel bits so that 16 channels' reads of a run fall into distinct banks, and likewise
   // the writes of 16 threads, whose channels are 4 apart.
@@ -245,7 +261,7 @@ struct Shape {
     alignas(16) _Float16 v[N][DP * KT];                // [channel][key], see v_at
     int64_t off[KT];
     uint64_t mask;
-    float mx[kThreads / 64][2];
+    float mx[W][2];
   };
 };
 
@@ -259,31 +275,32 @@ struct Shape {
 // and 3.  Keys are scaled by a power of two a tile, values by one that only grows over the tiles.  What that loses, small
 // numbers beside large ones, is looked for: a row whose scores could be off (their factor is large), whose outputs are
 // below 2^-15 of the largest value, or whose results are not finite is formed again in float32 (RowSum).
-template <typename E, int ND, bool FULL>
-__device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0, int t1, int whole_t0, int whole_t1,
-                                       float* part, typename Shape<E, ND>::Mem& mem) {
-  typedef Shape<E, ND> S;
+template <typename E, int ND, bool FULL, int W>
+__device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0, int t1, bool whole, float* part,
+                                       float2* part_ml, typename Shape<E, ND, W>::Mem& mem) {
+  typedef Shape<E, ND, W> S;
   typedef Cell<E> C;
   typedef typename C::Raw Raw;
   constexpr int KT = S::KT, DP = S::DP, N = S::N, KS = S::KS, NB = S::NB, CG = DP / 4;
   const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), n = lane & 31, g = lane >> 5;
   const int d = FULL ? DP : a.d;
-  const int row = wv * 32 + n;
+  const int row = wv * kWaveRows + n;
   const bool valid = row < it.rows;
-  const int flat = it.row0 + (valid ? row : 0);
-  const int tok = it.first + flat / a.group, head = it.kvh * a.group + flat % a.group;
+  auto token_of = [&](int r) { return it.first + (it.row0 + r) / a.group; };
+  auto head_of = [&](int r) { return it.kvh * a.group + (it.row0 + r) % a.group; };
   const int hi = valid ? it.hi_of(a, row) : 0, lo = Item::lo_of(a, hi);
   // of the wave: keys that any of its rows sees [w_lo, w_hi), and that all of them see [s_lo, s_hi)
-  const bool active = wv * 32 < it.rows;
-  const int w_hi = active ? it.hi_of(a, min(it.rows, wv * 32 + 32) - 1) : 0, s_hi = active ? it.hi_of(a, wv * 32) : 0;
+  const bool active = wv * kWaveRows < it.rows;
+  const int w_hi = active ? it.hi_of(a, min(it.rows, (wv + 1) * kWaveRows) - 1) : 0;
+  const int s_hi = active ? it.hi_of(a, wv * kWaveRows) : 0;
   const int w_lo = Item::lo_of(a, s_hi), s_lo = Item::lo_of(a, w_hi);
-  const float* q = a.q + (int64_t)tok * a.ldq + (int64_t)head * d;
 
   const Exact exact;
   // the row's channels 16 s + 8 g .. + 8, in two planes
   h8 qh[DP / 16], ql[DP / 16];
   float factor;                        // of the row's scores: |scale| log2(e) over its power of two
   {
+    const float* q = a.q + (int64_t)token_of(valid ? row : 0) * a.ldq + (int64_t)head_of(valid ? row : 0) * d;
     float x[DP / 16][8], big = 0.f;
     const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
@@ -345,11 +362,11 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     const bool all = mask == kAll;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const int at = tid + j * kThreads, cg = at % CG, kg = at / CG;
-      const bool on = (S::BLOCKS % kThreads == 0 || at < S::BLOCKS) && (FULL || 4 * cg < d);
+      const int at = tid + j * S::T, cg = at % CG, kg = at / CG;
+      const bool on = (S::BLOCKS % S::T == 0 || at < S::BLOCKS) && (FULL || 4 * cg < d);
       int64_t off[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) off[i] = mem.off[(S::BLOCKS % kThreads == 0 ? 4 * kg : 4 * kg % KT) + i];
+      for (int i = 0; i < 4; ++i) off[i] = mem.off[(S::BLOCKS % S::T == 0 ? 4 * kg : 4 * kg % KT) + i];
 #pragma unroll
       for (int i = 0; i < 4; ++i) kr[j][i] = vr[j][i] = Raw{};
       if (all) {
@@ -415,7 +432,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       if constexpr (C::SCALED) {
         float km = 0.f;
 #pragma unroll
-        for (int w = 0; w < kThreads / 64; ++w) {
+        for (int w = 0; w < W; ++w) {
           km = fmaxf(km, mem.mx[w][0]);
           v_big = fmaxf(v_big, mem.mx[w][1]);
         }
@@ -426,8 +443,8 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
         const float ku = ldexpf(1.f, up), vu = ldexpf(1.f, v_up);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-          const int at = tid + j * kThreads, cg = at % CG, kg = at / CG;
-          if (S::BLOCKS % kThreads != 0 && at >= S::BLOCKS) continue;
+          const int at = tid + j * S::T, cg = at % CG, kg = at / CG;
+          if (S::BLOCKS % S::T != 0 && at >= S::BLOCKS) continue;
           const int run = 2 * (kg >> 2) + (kg & 1), half = 4 * (kg >> 1 & 1);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -455,8 +472,8 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       } else {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-          const int at = tid + j * kThreads, cg = at % CG, kg = at / CG;
-          if (S::BLOCKS % kThreads != 0 && at >= S::BLOCKS) continue;
+          const int at = tid + j * S::T, cg = at % CG, kg = at / CG;
+          if (S::BLOCKS % S::T != 0 && at >= S::BLOCKS) continue;
           const int run = 2 * (kg >> 2) + (kg & 1), half = 4 * (kg >> 1 & 1);
           uint32_t x[4][2];
 #pragma unroll
@@ -610,10 +627,12 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
   big = fmaxf(big, __shfl_xor(big, 32, kWave));
   odd = odd || coarse || !(sum > 0.f && sum < INFINITY) || (C::SCALED && big < 1.f && v_big > 0.f);
   odd = __shfl_xor((int)odd, 32, kWave) || odd;
-  const bool again = valid && there && odd, whole = t0 == whole_t0 && t1 == whole_t1;
+  const bool again = valid && there && odd;
   const float unit = C::SCALED ? ldexpf(1.f, -o_up) : 1.f;
-  float* dst = whole ? a.out + (int64_t)tok * a.ldo + (int64_t)head * d : part + (int64_t)row * (d + 2);
   if (valid && !again) {
+    int r = row;
+    asm volatile("" : "+v"(r));        // token and head again, rather than held over the keys
+    float* dst = whole ? a.out + (int64_t)token_of(r) * a.ldo + (int64_t)head_of(r) * d : part + (int64_t)row * d;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
@@ -624,53 +643,66 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
         for (int e = 0; e < 4; ++e) x.v[e] = there ? o[i][r + e] * unit : 0.f;
         if (FULL || c < d) *(f32x4u*)(dst + c) = x;
       }
-    if (!whole && g == 0) {
-      dst[d] = there ? top : -INFINITY;
-      dst[d + 1] = there ? sum : 0.f;
-    }
+    if (!whole && g == 0) part_ml[row] = make_float2(there ? top : -INFINITY, there ? sum : 0.f);
   }
   uint64_t rest = __ballot(again && g == 0);
   while (rest) {
     const int r = uniform(__ffsll((unsigned long long)rest) - 1);
     rest &= rest - 1;
-    const int r_tok = uniform(__shfl(tok, r, kWave)), r_head = uniform(__shfl(head, r, kWave));
+    const int r_tok = token_of(wv * kWaveRows + r), r_head = head_of(wv * kWaveRows + r);
     const int r_hi = min(uniform(__shfl(hi, r, kWave)), t1 * KT), r_lo = max(uniform(__shfl(lo, r, kWave)), t0 * KT);
     RowSum<E> x;
     x.run(a, it.b, it.kvh, a.q + (int64_t)r_tok * a.ldq + (int64_t)r_head * d, r_lo, r_hi);
     const bool none = x.there && x.top == -INFINITY;       // scores of -inf alone
-    float* to = whole ? a.out + (int64_t)r_tok * a.ldo + (int64_t)r_head * d : part + (int64_t)(wv * 32 + r) * (d + 2);
+    float* to = whole ? a.out + (int64_t)r_tok * a.ldo + (int64_t)r_head * d : part + (int64_t)(wv * kWaveRows + r) * d;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (64 * i + lane < d) to[64 * i + lane] = !x.there || (none && !whole) ? 0.f : x.o[i] / x.sum;
-    if (!whole && lane == 0) {
-      to[d] = none ? kNoScore : x.top;
-      to[d + 1] = x.sum * 0x1p10f;
-    }
+    if (!whole && lane == 0) part_ml[wv * kWaveRows + r] = make_float2(none ? kNoScore : x.top, x.sum * 0x1p10f);
   }
 }
 
-// One workgroup a (tile of rows, kv head).
-template <typename E, int ND, bool FULL>
-__global__ __launch_bounds__(kThreads, ND <= 4 ? 2 : 1) void k_extend_whole(ExtArgs a) {
-  __shared__ typename Shape<E, ND>::Mem mem;
-  Item it;
-  // the last tiles of a sequence see the most keys: they go first
-  if (!find_item(a, a.slots - 1 - (int)(blockIdx.x / (unsigned)a.kv_heads), it)) return;
-  it.kvh = (int)(blockIdx.x % (unsigned)a.kv_heads);
-  int t0, t1;
-  tiles_of<Shape<E, ND>::KT>(a, it, t0, t1);
-  attend<E, ND, FULL>(a, it, t0, t1, t0, t1, nullptr, mem);
+// Waves a SIMD that the registers are held to: a third one, where it fits, works while the others wait at their barriers
+// (float16, 14 on 2 heads of 64: 3.39 -> 2.84 ms at 8 x 800 queries over 5800 keys; with float32 the spills cost more).
+template <typename E, int ND>
+constexpr int simd_waves() {
+  return ND > 4 ? 1 : ND == 2 && Cell<E>::N == 1 && !Cell<E>::SCALED ? 3 : 2;
 }
 
-// A workgroup's share of the (slot, kv head, key tile) units, in that order.
-struct Plan {
-  int64_t before[kSplitSlots + 1];   // key tiles of one kv head in the slots ahead
-  int32_t slot[kSplitSlots];         // a sequence's first slot
-  int64_t sum[kThreads / 64];
+// One workgroup a (tile of rows, kv head).
+template <typename E, int ND, bool FULL, int W>
+__global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_whole(ExtArgs a) {
+  __shared__ typename Shape<E, ND, W>::Mem mem;
+  Item it;
+  // the last tiles of a sequence see the most keys: they go first
+  if (!find_item<W>(a, a.slots - 1 - (int)(blockIdx.x / (unsigned)a.kv_heads), it)) return;
+  it.kvh = (int)(blockIdx.x % (unsigned)a.kv_heads);
+  int t0, t1;
+  tiles_of<Shape<E, ND, W>::KT>(a, it, t0, t1);
+  attend<E, ND, FULL, W>(a, it, t0, t1, true, nullptr, nullptr, mem);
+}
+
+// A workgroup's part of an item (slot, kv head): `part` of `parts` equal runs of its key tiles.  Parts of one item have
+// places that follow each other; parts 0: nothing to do.
+struct Piece {
+  int b, kvh, tile, part, parts, place, pad[2];
 };
+
+// One value of a wave's 64, by lane exchanges within rows of 16 and four lane reads.
+template <typename F>
+__device__ __forceinline__ uint32_t wave_fold(uint32_t v, F f) {
+  v = f(v, dpp32<kDppXor1>(v));
+  v = f(v, dpp32<kDppXor2>(v));
+  v = f(v, dpp32<kDppHalfMirror>(v));
+  v = f(v, dpp32<kDppMirror>(v));
+  return f(f((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16)),
+           f((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
+}
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
+  return wave_fold(v, [](uint32_t x, uint32_t y) { return x + y; });
+}
 // The last i of [0, n) with v[i] <= x; v[0] <= x.
-template <typename T>
-__device__ __forceinline__ int last_at(const T* v, int n, T x) {
+__device__ __forceinline__ int last_at(const int32_t* v, int n, int x) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -679,179 +711,352 @@ __device__ __forceinline__ int last_at(const T* v, int n, T x) {
   return lo;
 }
 
-// The units shared out evenly over `groups` workgroups by what the device holds: a long cache with few rows, a ragged
-// batch and a causal triangle all fill the machine, and a captured launch serves every length.  Every workgroup sums
-// over the slots by itself.  An item (slot, kv head) that one workgroup holds whole is written by it; of one that
-// crosses workgroups each leaves its rows' outputs, maxima and sums in `part` (slot 2 w, or 2 w + 1 where the item
-// begins inside w's share), and k_extend_join adds them up.  The workgroup that begins an item enters it into `pairs`:
-// its first part and last workgroup, or -1.  Shares that follow each other go to one XCD, whose L2 they share keys in.
-template <typename E, int ND, bool FULL>
-__global__ __launch_bounds__(kThreads, ND <= 4 ? 2 : 1) void k_extend_split(ExtArgs a) {
-  constexpr int KT = Shape<E, ND>::KT;
-  __shared__ union {
-    typename Shape<E, ND>::Mem mem;
-    Plan plan;
-  } lds;
-  Plan& p = lds.plan;
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, slots = a.slots;
-  const int w = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
-  for (int b = tid; b < a.batch; b += kThreads)
-    p.slot[b] = slot_of(a, (int)min((int64_t)max(a.starts[b], 0), a.n), b);
+// The keys of long items shared out by what the device holds, so that a long cache with few rows, a ragged batch and a
+// causal triangle all fill the machine and a captured launch serves every length.  Items are cut into equal parts of at
+// most `most` key tiles, a workgroup each.  `most` is the size with the least estimate of: no cut; the least of a few
+// sizes whose parts all run at once (`groups` do); half a workgroup's mean load.  A part is charged kPartCost tiles for
+// its start and end, and kCutCost more where it has to be joined (some 2 us a tile); what runs in several rounds half of
+// the largest part for the last.
+//
+// One workgroup, a thread a slot: bound by the chain of its loads, searches and sums.  (Done by every workgroup of
+// k_extend_split for itself it took 4 - 9 us of each, and registers of the products.)
+constexpr int kPlanThreads = kSplitSlots, kTries = 9, kPartCost = 2, kCutCost = 3;
+template <int KT, int W>
+__global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
+  constexpr int kRows = kWaveRows * W, kWaves = kPlanThreads / 64, kSums = kTries + 1;
+  __shared__ int32_t s_slot[kSplitSlots];           // a sequence's first slot
+  __shared__ int32_t s_pieces[kSplitSlots];         // parts of the slots ahead
+  __shared__ int32_t s_places[kSplitSlots];         // of them those of cut items
+  __shared__ int32_t s_cuts[kSplitSlots];           // items that are cut, of the slots ahead
+  __shared__ int32_t s_parts[kSplitSlots];
+  __shared__ uint32_t s_red[kWaves][kSums];
+  __shared__ uint64_t s_up[kWaves];
+  __shared__ float s_load, s_items, s_inv;
+  __shared__ uint32_t s_top;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, slots = a.slots, hk = a.kv_heads;
+  for (int b = tid; b < a.batch; b += kPlanThreads) s_slot[b] = first_slot<W>(a, b);
   __syncthreads();
-  constexpr int kEach = kSplitSlots / kThreads;
-  const int each = (slots + kThreads - 1) / kThreads;
-  int64_t mine[kEach], all = 0;
-#pragma unroll 1
-  for (int i = 0; i < each; ++i) {
-    const int s = tid * each + i;
-    int64_t units = 0;
-    if (s < slots && p.slot[0] <= s) {
-      const int b = last_at(p.slot, a.batch, (int32_t)s);
-      const Seq q = seq_of(a, b);
-      const int64_t row0 = (int64_t)(s - p.slot[b]) * kRows, rows = min((int64_t)q.count * a.group - row0, (int64_t)kRows);
-      if (row0 >= 0 && rows > 0) {
-        Item it{b, 0, q.first, q.base, q.len, (int)row0, (int)rows};
-        int t0, t1;
-        tiles_of<KT>(a, it, t0, t1);
-        units = t1 - t0;
-      }
+  const int s = slots - 1 - tid;                    // the last slots first: they see the most keys
+  int mine = 0;                                     // key tiles of this thread's slot, for one kv head
+  if (s >= 0 && s_slot[0] <= s) {
+    const int b = last_at(s_slot, a.batch, s);
+    const Seq q = seq_of(a, b);
+    const int64_t row0 = (int64_t)(s - s_slot[b]) * kRows, rows = min((int64_t)q.count * a.group - row0, (int64_t)kRows);
+    if (row0 >= 0 && rows > 0) {
+      Item one{b, 0, q.first, q.base, q.len, (int)row0, (int)rows};
+      int u0, u1;
+      tiles_of<KT>(a, one, u0, u1);
+      mine = max(u1 - u0, 1);          // rows with no key to see are written too: a part with nothing in it
     }
-    mine[i] = units;
-    all += units;
   }
-  int64_t up = all;
+  {
+    const uint32_t lo = wave_sum_u32((uint32_t)mine & 0xffff), hi = wave_sum_u32((uint32_t)mine >> 16), n = __popcll(__ballot(mine > 0));
+    const uint32_t top = wave_fold((uint32_t)mine, [](uint32_t x, uint32_t y) { return max(x, y); });
+    if (lane == 0) s_red[wv][0] = lo, s_red[wv][1] = hi, s_red[wv][2] = n, s_red[wv][3] = top;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    float units = 0.f, n = 0.f;
+    uint32_t top = 1;
+    for (int w = 0; w < kWaves; ++w) {
+      units += (float)s_red[w][0] + 65536.f * (float)s_red[w][1];
+      n += (float)s_red[w][2];
+      top = max(top, s_red[w][3]);
+    }
+    s_load = units * (float)hk / (float)a.groups, s_items = n * (float)hk, s_top = top;
+  }
+  __syncthreads();
+  const float load = s_load, least = fmaxf(ceilf(load), 1.f);
+  auto size_of = [&](int k) { return k < kTries ? ceilf(least * (1.f + (float)k / (kTries - 1))) : fmaxf(ceilf(0.5f * load), 1.f); };
+  auto parts_of = [](int n, float inv) { return n > 0 ? 1 + (int)((float)(n - 1) * inv) : 0; };
+#pragma unroll
+  for (int k = 0; k < kSums; ++k) {
+    const uint32_t need = wave_sum_u32((uint32_t)parts_of(mine, 1.f / size_of(k)));
+    if (lane == 0) s_red[wv][k] = need;
+  }
+  __syncthreads();
+  if (wv == 0) {
+    // a candidate a lane; the last lane: no cut
+    const float groups = (float)a.groups, top = (float)s_top, whole = s_items, cost = kPartCost + kCutCost;
+    float est = INFINITY, size = top;
+    if (lane < kSums) {
+      uint32_t need = 0;
+      for (int w = 0; w < kWaves; ++w) need += s_red[w][lane];
+      const float n = (float)need * (float)hk;
+      size = size_of(lane);
+      est = n <= groups ? size + cost : lane < kTries ? INFINITY : load + cost * n / groups + 0.5f * size;
+      if (size >= top) est = INFINITY;
+    } else if (lane == kSums) {
+      est = whole <= groups ? top + kPartCost : load + kPartCost * whole / groups + 0.5f * top;
+    }
+    const float best = -wave_max_dpp(-est);
+    const int pick = __ffsll((unsigned long long)__ballot(est == best)) - 1;
+    size = __shfl(size, pick, kWave);
+    if (lane == 0) s_inv = 1.f / size;
+  }
+  __syncthreads();
+  // parts, parts of cut items, and cut items of the slots ahead, 21 bits each: there are at most 2^10 and 3 groups
+  const int parts = parts_of(mine, s_inv);
+  const uint64_t n = parts > 1 ? (uint64_t)parts | (uint64_t)parts << 21 | (uint64_t)1 << 42 : (uint64_t)parts;
+  uint64_t up = n;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t u = __shfl_up(up, o, kWave);
+    const uint64_t u = __shfl_up((unsigned long long)up, o, kWave);
     if (lane >= o) up += u;
   }
-  if (lane == 63) p.sum[wv] = up;
+  if (lane == 63) s_up[wv] = up;
   __syncthreads();
-  int64_t at = up - all, total = 0;
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) {
-    if (i < wv) at += p.sum[i];
-    total += p.sum[i];
+  uint64_t all = 0;
+  up -= n;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wv) up += s_up[w];
+    all += s_up[w];
   }
-#pragma unroll 1
-  for (int i = 0; i < each; ++i) {
-    const int s = tid * each + i;
-    if (s < slots) p.before[s] = at;
-    at += mine[i];
-  }
+  constexpr uint64_t kField = (1 << 21) - 1;
+  s_pieces[tid] = (int)(up & kField) * hk, s_places[tid] = (int)(up >> 21 & kField) * hk, s_cuts[tid] = (int)(up >> 42) * hk;
+  s_parts[tid] = parts;
   __syncthreads();
-  total = uniform(total) * a.kv_heads;
-  const int64_t n = min((int64_t)a.groups, total);
-  if (w >= n) return;
-  const int64_t first = total * w / n, end = total * (w + 1) / n;
-  int slot = uniform(last_at(p.before, slots, first / a.kv_heads));
-  int64_t in = first - uniform(p.before[slot]) * a.kv_heads;          // the unit within the slot: [kv head][key tile]
-  int b = uniform(last_at(p.slot, a.batch, (int32_t)slot));
-  __syncthreads();                     // the plan's memory is the tiles' from here on
-
-  at = first;
-  while (at < end) {
-    Item it{};
-    int t0 = 0, t1 = 0;
-    const int tile = slot - slot_of(a, uniform((int)min((int64_t)max(a.starts[b], 0), a.n)), b);
-    if (item_of(a, b, tile, it)) tiles_of<KT>(a, it, t0, t1);
-    const int units = t1 - t0;
-    if (in >= (int64_t)units * a.kv_heads) {           // the next slot; of the next sequence, where it begins there
-      in -= (int64_t)units * a.kv_heads;
-      if (++slot >= slots) return;                     // lengths that changed under the call
-      while (b + 1 < a.batch && slot_of(a, uniform((int)min((int64_t)max(a.starts[b + 1], 0), a.n)), b + 1) <= slot) ++b;
-      continue;
-    }
-    it.kvh = (int)(in / units);
-    const int t = (int)(in - (int64_t)it.kvh * units), take = (int)min((int64_t)(units - t), end - at);
-    const int place = 2 * w + (at == first ? 0 : 1);
-    if (tid == 0 && t == 0) {
-      const bool whole = take == units;
-      a.pairs[(int64_t)slot * a.kv_heads + it.kvh] =
-          make_int2(whole ? -1 : place, whole ? 0 : (int)(((at + units) * n - 1) / total));
-    }
-    attend<E, ND, FULL>(a, it, t0 + t, t0 + t + take, t0, t1, a.part + (int64_t)place * a.part_rows * (a.d + 2), lds.mem);
-    __syncthreads();                   // before the next item's first page ids
-    at += take;
-    in += take;
+  const int count = min((int)(all & kField) * hk, a.pieces_most);
+  if (tid == 0) a.counts[0] = min((int)(all >> 42) * hk, a.cuts_most), a.counts[1] = count;
+  for (int w = tid; w < count; w += kPlanThreads) {
+    const int at = last_at(s_pieces, min(slots, kSplitSlots), w), slot = slots - 1 - at, b = last_at(s_slot, a.batch, slot);
+    const int of = s_parts[at], in = w - s_pieces[at], kvh = in / of, part = in - kvh * of, place = s_places[at] + in;
+    const int cut = s_cuts[at] + kvh;
+    Piece one{b, kvh, slot - s_slot[b], part, of, place, {0, 0}};
+    if (of > 1 && (place >= a.places || cut >= a.cuts_most)) one.parts = 0;      // starts that do not rise
+    a.pieces[w] = one;
+    if (one.parts > 1 && part == 0) a.cuts[cut] = one;
   }
 }
 
-// Rows of items that crossed workgroups, and zeros for those with no key to see: a wave a row at a time, eight rows each.
-constexpr int kJoinRows = 32;
-__global__ __launch_bounds__(kThreads) void k_extend_join(ExtArgs a) {
-  const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
-  const int slot = (int)(blockIdx.x / (unsigned)a.kv_heads), row0 = blockIdx.y * kJoinRows;
+// Of a cut item each workgroup leaves its rows' outputs, maxima and sums (`part`, `part_ml`).
+template <typename E, int ND, bool FULL, int W>
+__global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_split(ExtArgs a) {
+  typedef Shape<E, ND, W> S;
+  __shared__ typename S::Mem mem;
+  // pieces that follow each other share keys: they go to one XCD's L2 where all run at once
+  const int count = a.counts[1], eighth = (count + 7) / 8, in_eighth = (int)(blockIdx.x / 8);
+  const int w = count <= a.groups ? (int)(blockIdx.x % 8) * eighth + in_eighth : (int)blockIdx.x;
+  if (w >= count || (count <= a.groups && in_eighth >= eighth)) return;
+  const Piece p = a.pieces[w];
   Item it;
-  if (!find_item(a, slot, it) || row0 >= it.rows) return;
-  it.kvh = (int)(blockIdx.x % (unsigned)a.kv_heads);
-  const bool none = it.hi_of(a, it.rows - 1) == 0;
-  const int2 pair = none ? make_int2(0, 0) : a.pairs[blockIdx.x];
-  if (pair.x < 0) return;              // written by the one workgroup that held it
-  const int w0 = min(pair.x >> 1, a.groups - 1), count = none ? 0 : min(pair.y, a.groups - 1) - w0 + 1;
-  for (int r = row0 + wv; r < min(row0 + kJoinRows, it.rows); r += kThreads / 64) {
-    const int flat = it.row0 + r, head = it.kvh * a.group + flat % a.group;
-    float* out = a.out + (int64_t)(it.first + flat / a.group) * a.ldo + (int64_t)head * a.d;
-    float x[4], top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = 0.f;
-    constexpr int kAhead = 4;
-    for (int i = 0; i < count; i += kAhead) {
-      float y[kAhead][4], t[kAhead], l[kAhead], now = top;
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int m = min(i + u, count - 1);
-        const float* src = a.part + ((int64_t)(m ? 2 * (w0 + m) : pair.x) * a.part_rows + r) * (a.d + 2);
-        t[u] = i + u < count ? src[a.d] : -INFINITY;
-        l[u] = src[a.d + 1];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[u][j] = 64 * j + lane < a.d ? src[64 * j + lane] : 0.f;
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) now = fmaxf(now, t[u]);
-      const float f = weight_of(top, now);
-      sum *= f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] *= f;
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (t[u] != -INFINITY) {
-          const float g = weight_of(t[u], now) * l[u];
-          sum += g;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] += g * y[u][j];
-        }
-      top = now;
+  const int parts = uniform(p.parts), part = uniform(p.part);
+  if (parts < 1 || !item_of<W>(a, uniform(p.b), uniform(p.tile), it)) return;
+  it.kvh = uniform(p.kvh);
+  int t0, t1;
+  tiles_of<S::KT>(a, it, t0, t1);
+  const int64_t place = uniform(p.place);
+  const int from = t0 + (int)((int64_t)(t1 - t0) * part / parts), to = t0 + (int)((int64_t)(t1 - t0) * (part + 1) / parts);
+  attend<E, ND, FULL, W>(a, it, from, to, parts == 1, a.part + place * a.part_rows * a.d, a.part_ml + place * a.part_rows, mem);
+}
+
+// Few rows a sequence: a wave each has 32 rows and one of `parts` runs of every item's keys, cut alike whatever their
+// lengths (the host knows no more), so that no plan has to come first.
+template <typename E, int ND, bool FULL>
+__global__ __launch_bounds__(64, (simd_waves<E, ND>())) void k_extend_few(ExtArgs a, int parts) {
+  typedef Shape<E, ND, 1> S;
+  __shared__ typename S::Mem mem;
+  const int item = (int)(blockIdx.x / (unsigned)parts), part = (int)(blockIdx.x % (unsigned)parts);
+  Item it;
+  if (!find_item<1>(a, item / a.kv_heads, it)) return;
+  it.kvh = item % a.kv_heads;
+  int t0, t1;
+  tiles_of<S::KT>(a, it, t0, t1);
+  const int from = t0 + (int)((int64_t)(t1 - t0) * part / parts), to = t0 + (int)((int64_t)(t1 - t0) * (part + 1) / parts);
+  attend<E, ND, FULL, 1>(a, it, from, to, parts == 1, a.part + (int64_t)blockIdx.x * a.part_rows * a.d,
+                         a.part_ml + (int64_t)blockIdx.x * a.part_rows, mem);
+}
+
+// The parts of an item's rows.  A wave reads four channels a lane, so several parts at a time, then joins its lanes; with
+// many parts the waves share them, with few each takes rows of its own.  parts 0: the items are those of `cuts`.
+constexpr int kJoinAhead = 4, kJoinFew = 32, kJoinGroups = 2048;
+template <int LP, int W>                         // lanes of a part: a power of two with 4 LP >= d
+__global__ __launch_bounds__(256) void k_extend_join(ExtArgs a, int parts, int rows) {
+  constexpr int PP = 64 / LP;                    // parts of one load
+  __shared__ float s_o[4][256], s_ml[4][2];
+  const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6), c4 = 4 * (lane % LP), sub = lane / LP;
+  const int row_groups = (a.part_rows + rows - 1) / rows;        // `rows` at a time
+  const int tasks = (parts ? a.slots * a.kv_heads : a.counts[0]) * row_groups;
+  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+    const int item = task / row_groups;
+    Item it;
+    int64_t first;
+    int count;
+    if (parts) {
+      if (!find_item<W, 4>(a, item / a.kv_heads, it)) continue;
+      it.kvh = item % a.kv_heads;
+      first = (int64_t)item * parts;
+      count = parts;
+    } else {
+      const Piece cut = a.cuts[item];
+      if (!item_of<W>(a, uniform(cut.b), uniform(cut.tile), it)) continue;
+      it.kvh = uniform(cut.kvh);
+      first = uniform(cut.place);
+      count = uniform(cut.parts);
     }
+    const int row0 = task % row_groups * rows, end = min(row0 + rows, it.rows);
+    const bool few = count <= kJoinFew;
+    const int step = few ? PP : 4 * PP;
+    for (int r = few ? row0 + wv : row0; r < end; r += few ? 4 : 1) {
+      f32x4u x{};
+      float top = -INFINITY, sum = 0.f;
+      for (int i = (few ? 0 : wv * PP) + sub; __any(i < count); i += step * kJoinAhead) {
+        f32x4u y[kJoinAhead];
+        float2 ml[kJoinAhead];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (64 * j + lane < a.d) out[64 * j + lane] = top != -INFINITY ? x[j] / sum : 0.f;
+        for (int u = 0; u < kJoinAhead; ++u) {
+          const int m = i + u * step;
+          const int64_t at = (first + min(m, count - 1)) * a.part_rows + r;
+          ml[u] = a.part_ml[at];
+          y[u] = f32x4u{};
+          if (c4 < a.d) y[u] = *(const f32x4u*)(a.part + at * a.d + c4);
+          if (m >= count) ml[u].x = -INFINITY;
+        }
+        float now = top;
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; ++u) now = fmaxf(now, ml[u].x);
+        const float f = weight_of(top, now);
+        sum *= f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.v[j] *= f;
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; ++u)
+          if (ml[u].x != -INFINITY) {
+            const float g = weight_of(ml[u].x, now) * ml[u].y;
+            sum += g;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.v[j] += g * y[u].v[j];
+          }
+        top = now;
+      }
+      auto join = [&](float t, float l, const f32x4u& o) {
+        const float now = fmaxf(top, t), f = weight_of(top, now), g = weight_of(t, now);
+        sum = f * sum + g * l;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.v[j] = f * x.v[j] + g * o.v[j];
+        top = now;
+      };
+#pragma unroll
+      for (int o = LP; o < 64; o <<= 1) {
+        f32x4u y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y.v[j] = __shfl_xor(x.v[j], o, kWave);
+        join(__shfl_xor(top, o, kWave), __shfl_xor(sum, o, kWave), y);
+      }
+      const int flat = it.row0 + r, head = it.kvh * a.group + flat % a.group;
+      float* out = a.out + (int64_t)(it.first + flat / a.group) * a.ldo + (int64_t)head * a.d;
+      if (!few) {
+        __syncthreads();
+        if (sub == 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s_o[wv][c4 + j] = x.v[j];
+        }
+        if (lane == 0) s_ml[wv][0] = top, s_ml[wv][1] = sum;
+        __syncthreads();
+        if (wv != 0) continue;
+#pragma unroll
+        for (int u = 1; u < 4; ++u) {
+          f32x4u y;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y.v[j] = s_o[u][c4 + j];
+          join(s_ml[u][0], s_ml[u][1], y);
+        }
+      }
+      if (sub == 0 && c4 < a.d) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.v[j] = top != -INFINITY ? x.v[j] / sum : 0.f;
+        *(f32x4u*)(out + c4) = x;
+      }
+    }
   }
 }
 
-constexpr int groups_of(int d) { return d <= 128 ? 512 : 256; }     // workgroups that the registers let run at once
+template <int ND, int W>
+void launch_join(const ExtArgs& a, int64_t items, int parts, hipStream_t st) {
+  const int rows = parts > kJoinFew ? 1 : 4;
+  const dim3 grid((unsigned)std::min<int64_t>(items * ceil_div(a.part_rows, rows), kJoinGroups)), block(256);
+  if (ND == 2) hipLaunchKernelGGL((k_extend_join<16, W>), grid, block, 0, st, a, parts, rows);
+  else if (ND <= 4) hipLaunchKernelGGL((k_extend_join<32, W>), grid, block, 0, st, a, parts, rows);
+  else hipLaunchKernelGGL((k_extend_join<64, W>), grid, block, 0, st, a, parts, rows);
+}
+
+// Scratch for `rows` rows of parts and `more` bytes behind them.  1: there is none.
+int part_scratch(ExtArgs& a, int64_t rows, size_t more, void** work, void** behind, hipStream_t st) {
+  const int rc = scratch_alloc(work, (size_t)rows * (a.d * 4 + 8) + more, st);
+  if (rc) {
+    *work = nullptr;
+    return rc;
+  }
+  a.part = (float*)*work;
+  a.part_ml = (float2*)(a.part + rows * a.d);
+  *behind = a.part_ml + rows;
+  return CV3_OK;
+}
 
 template <typename E, int ND, bool FULL>
-void launch_tiles(const ExtArgs& a, hipStream_t st) {
-  if (!a.part) {
-    hipLaunchKernelGGL((k_extend_whole<E, ND, FULL>), dim3((unsigned)a.slots * a.kv_heads), dim3(kThreads), 0, st, a);
-    return;
+int run_tiles(ExtArgs a, hipStream_t st) {
+  constexpr int W = 4, kAtOnce = 256 * simd_waves<E, ND>() * 4;     // waves that the registers let run at once
+  const int64_t cap = a.blocks * a.page, rows = a.n * a.group;
+  void *work = nullptr, *behind;
+  int rc = CV3_OK;
+  const bool few = rows <= kFewRows * a.batch;
+  if (few && ND == 2) {
+    constexpr int KT = Shape<E, ND, 1>::KT;
+    a.slots = (int)(rows / kWaveRows + a.batch);
+    a.part_rows = (int)std::min<int64_t>(kWaveRows, rows);
+    const int64_t items = (int64_t)a.slots * a.kv_heads;
+    // enough waves to fill the machine twice, but parts of 8 tiles where there would be more than 16 of them
+    const int64_t tiles = ceil_div(cap, KT), most = tiles <= 16 ? tiles : std::max<int64_t>(16, tiles / 8);
+    int64_t parts = std::max<int64_t>(1, std::min(ceil_div(2 * kAtOnce, items), most));
+    if (parts > 1) {
+      rc = part_scratch(a, items * parts * a.part_rows, 0, &work, &behind, st);
+      if (rc && rc != CV3_ENOMEM) return rc;
+      if (rc) parts = 1;               // without memory: one wave an item
+    }
+    if constexpr (ND == 2)
+      hipLaunchKernelGGL((k_extend_few<E, ND, FULL>), dim3((unsigned)(items * parts)), dim3(64), 0, st, a, (int)parts);
+    if (work) launch_join<ND, 1>(a, items, (int)parts, st);
+  } else {
+    a.slots = (int)(rows / (kWaveRows * W) + a.batch);
+    const int64_t items = (int64_t)a.slots * a.kv_heads;
+    if (a.slots <= kSplitSlots && cap > (few ? kWholeKeys / 4 : kWholeKeys)) {
+      a.groups = kAtOnce / W;
+      a.part_rows = (int)std::min<int64_t>(kWaveRows * W, rows);
+      // parts of no more than half a mean load: items and 2 groups of them, 4 groups of those in cut items
+      a.pieces_most = (int)items + 2 * a.groups;
+      a.places = 4 * a.groups;
+      a.cuts_most = (int)std::min<int64_t>(items, 2 * a.groups);
+      const size_t lists = (size_t)(a.pieces_most + a.cuts_most) * sizeof(Piece) + 16;
+      rc = part_scratch(a, (int64_t)a.places * a.part_rows, lists, &work, &behind, st);
+      if (rc && rc != CV3_ENOMEM) return rc;
+      a.pieces = (Piece*)behind;
+      a.cuts = a.pieces + a.pieces_most;
+      a.counts = (int*)(a.cuts + a.cuts_most);
+    }
+    if (work) {
+      hipLaunchKernelGGL((k_extend_plan<Shape<E, ND, W>::KT, W>), dim3(1), dim3(kPlanThreads), 0, st, a);
+      hipLaunchKernelGGL((k_extend_split<E, ND, FULL, W>), dim3((unsigned)a.pieces_most), dim3(64 * W), 0, st, a);
+      launch_join<ND, W>(a, a.cuts_most, 0, st);
+    } else {                           // short tables, very many tiles, or no memory: one workgroup an item
+      hipLaunchKernelGGL((k_extend_whole<E, ND, FULL, W>), dim3((unsigned)items), dim3(64 * W), 0, st, a);
+    }
   }
-  hipLaunchKernelGGL((k_extend_split<E, ND, FULL>), dim3(a.groups), dim3(kThreads), 0, st, a);
-  hipLaunchKernelGGL(k_extend_join, dim3((unsigned)a.slots * a.kv_heads, (unsigned)ceil_div(a.part_rows, kJoinRows)), dim3(kThreads),
-                     0, st, a);
+  const hipError_t err = hipGetLastError();
+  rc = work ? scratch_free(work, st) : CV3_OK;
+  CV3_REQUIRE(err == hipSuccess, CV3_EHIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return rc;
 }
 
 template <typename E>
-void extend_for(const ExtArgs& a, hipStream_t st) {
+int extend_for(const ExtArgs& a, hipStream_t st) {
   switch ((a.d + 31) / 32) {
     case 1:
-    case 2: a.d == 64 ? launch_tiles<E, 2, true>(a, st) : launch_tiles<E, 2, false>(a, st); break;
-    case 3: launch_tiles<E, 3, false>(a, st); break;
-    case 4: a.d == 128 ? launch_tiles<E, 4, true>(a, st) : launch_tiles<E, 4, false>(a, st); break;
+    case 2: return a.d == 64 ? run_tiles<E, 2, true>(a, st) : run_tiles<E, 2, false>(a, st);
+    case 3: return run_tiles<E, 3, false>(a, st);
+    case 4: return a.d == 128 ? run_tiles<E, 4, true>(a, st) : run_tiles<E, 4, false>(a, st);
     case 5:
-    case 6: launch_tiles<E, 6, false>(a, st); break;
-    default: launch_tiles<E, 8, false>(a, st);
+    case 6: return run_tiles<E, 6, false>(a, st);
+    default: return run_tiles<E, 8, false>(a, st);
   }
 }
 
@@ -886,27 +1091,11 @@ int cv3_paged_extend(const float* q, int64_t ldq, int64_t n, int heads, int kv_h
   CV3_REQUIRE(apart(res, in), CV3_EINVAL, "out overlaps the caches, the tables, the lengths or the starts");
   ExtArgs a{q, ldq, k_cache, v_cache, tables, lengths, starts, out, ldo, pages, blocks, n,
             (int)std::min<int64_t>(window, INT32_MAX), (uint32_t)(0xffffffffu / (uint32_t)page), (int)batch, (int)page, heads, kv_heads, heads / kv_heads, d,
-            (int)(n * (heads / kv_heads) / kRows + batch), scale * 1.4426950408889634f, nullptr, nullptr, 0, 0};
+            0, scale * 1.4426950408889634f};
   hipStream_t st = stream_of(s);
-  const int64_t cap = blocks * page, items = (int64_t)a.slots * kv_heads;
-  const bool whole = a.slots > kSplitSlots || cap <= 256 || items >= 8192;
-  if (!whole) {
-    a.groups = groups_of(d);
-    a.part_rows = (int)std::min<int64_t>(kRows, n * a.group);
-    const size_t parts = (size_t)2 * a.groups * a.part_rows * (d + 2) * sizeof(float);      // a multiple of 8
-    void* work = nullptr;
-    const int rc = scratch_alloc(&work, parts + (size_t)items * sizeof(int2), st);
-    if (rc && rc != CV3_ENOMEM) return rc;     // without memory: one workgroup an item
-    a.part = (float*)work;
-    a.pairs = (int2*)((char*)work + parts);
-  }
-  if (cache_type == CV3_F32) extend_for<float>(a, st);
-  else if (cache_type == CV3_F16) extend_for<_Float16>(a, st);
-  else extend_for<__bf16>(a, st);
-  const hipError_t err = hipGetLastError();
-  const int rc = a.part ? scratch_free(a.part, st) : CV3_OK;
-  CV3_REQUIRE(err == hipSuccess, CV3_EHIP, "kernel launch failed: %s", hipGetErrorString(err));
-  return rc;
+  if (cache_type == CV3_F32) return extend_for<float>(a, st);
+  if (cache_type == CV3_F16) return extend_for<_Float16>(a, st);
+  return extend_for<__bf16>(a, st);
 }
 
 }  // extern "C"
