@@ -13,6 +13,8 @@ using namespace cv3;
 
 namespace {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));     // 16 bytes
+
 constexpr int kForks = 4096, kForkRows = 65536;   // forks of a call, sequences of its tables
 constexpr int kForkGroups = 2048;                 // workgroups of a fork's copies, about
 constexpr int kThreads = 256, kAhead = 4;         // 16-byte vectors of a thread in flight
@@ -25,8 +27,8 @@ struct ForkArgs {
   const int32_t* free_pages;
   const int32_t* taken;
   int32_t* taken_out;
-  uint4* k;
-  uint4* v;
+  u32x4* k;
+  u32x4* v;
   int64_t pages, blocks, free_count, layers;
   int forks, rows, kv_heads, page, row_vecs;
 };
@@ -51,58 +53,80 @@ __global__ __launch_bounds__(kThreads) void k_fork(ForkArgs a) {
   for (int w = tid; w < 3 * words; w += kThreads) s_bits[w] = 0;
   if (tid == 0) s_before = s_all = 0;
   __syncthreads();
-  for (int f = tid; f < a.forks; f += kThreads) {
-    const uint32_t p = (uint32_t)a.parents[f], c = (uint32_t)a.children[f];
-    if (p < (uint32_t)a.rows) atomicOr(&parent[p >> 5], 1u << (p & 31));
-    if (c < (uint32_t)a.rows && atomicOr(&child[c >> 5], 1u << (c & 31)) >> (c & 31) & 1)
-      atomicOr(&again[c >> 5], 1u << (c & 31));
+  // this fork's numbers and every fork's, together; the lengths of kForksEach x 256 of them at a time
+  constexpr int kForksEach = 4;
+  const uint32_t p = a.forks ? (uint32_t)a.parents[i] : ~0u, c = a.forks ? (uint32_t)a.children[i] : ~0u;
+  const int len = p < (uint32_t)a.rows ? held_of(a.lengths, p, a.blocks, a.page) : 0, full = len / a.page, rest = len - full * a.page;
+  const int32_t* from = a.tables + (int64_t)(p < (uint32_t)a.rows ? p : 0) * a.blocks;
+  const int32_t source = rest ? from[full] : -1;
+  uint32_t ps[kForksEach], cs[kForksEach];
+  int part[kForksEach];
+  const bool once = a.forks <= kForksEach * kThreads;
+#pragma unroll
+  for (int e = 0; e < kForksEach; ++e) {
+    const int f = tid + e * kThreads;
+    ps[e] = f < a.forks ? (uint32_t)a.parents[f] : ~0u;
+    cs[e] = f < a.forks ? (uint32_t)a.children[f] : ~0u;
   }
+#pragma unroll
+  for (int e = 0; e < kForksEach; ++e) part[e] = ps[e] < (uint32_t)a.rows ? held_of(a.lengths, ps[e], a.blocks, a.page) % a.page : 0;
+  auto enter = [&](uint32_t fp, uint32_t fc) {
+    if (fp < (uint32_t)a.rows) atomicOr(&parent[fp >> 5], 1u << (fp & 31));
+    if (fc < (uint32_t)a.rows && atomicOr(&child[fc >> 5], 1u << (fc & 31)) >> (fc & 31) & 1)
+      atomicOr(&again[fc >> 5], 1u << (fc & 31));
+  };
+#pragma unroll
+  for (int e = 0; e < kForksEach; ++e) enter(ps[e], cs[e]);
+  for (int f = tid + kForksEach * kThreads; f < a.forks; f += kThreads) enter((uint32_t)a.parents[f], (uint32_t)a.children[f]);
   __syncthreads();
-  auto made = [&](uint32_t p, uint32_t c) {
-    return p < (uint32_t)a.rows && c < (uint32_t)a.rows && !((parent[c >> 5] | again[c >> 5]) >> (c & 31) & 1);
+  auto made = [&](uint32_t fp, uint32_t fc) {
+    return fp < (uint32_t)a.rows && fc < (uint32_t)a.rows && !((parent[fc >> 5] | again[fc >> 5]) >> (fc & 31) & 1);
   };
   int before = 0, all = 0;
-  for (int f = tid; f < a.forks; f += kThreads) {
-    const uint32_t p = (uint32_t)a.parents[f];
-    if (made(p, (uint32_t)a.children[f]) && held_of(a.lengths, p, a.blocks, a.page) % a.page) {
+  auto count = [&](int f, uint32_t fp, uint32_t fc, int rows_of_last) {
+    if (rows_of_last && made(fp, fc)) {
       ++all;
       if (f < i) ++before;
     }
-  }
+  };
+#pragma unroll
+  for (int e = 0; e < kForksEach; ++e) count(tid + e * kThreads, ps[e], cs[e], part[e]);
+  if (!once)
+    for (int f = tid + kForksEach * kThreads; f < a.forks; f += kThreads) {
+      const uint32_t fp = (uint32_t)a.parents[f];
+      count(f, fp, (uint32_t)a.children[f], fp < (uint32_t)a.rows ? held_of(a.lengths, fp, a.blocks, a.page) % a.page : 0);
+    }
   if (before) atomicAdd(&s_before, before);
   if (all) atomicAdd(&s_all, all);
   __syncthreads();
   const int64_t taken = a.taken[0];
   if (blockIdx.x == 0 && i == 0 && tid == 0) a.taken_out[0] = (int32_t)min(taken + s_all, (int64_t)INT32_MAX);
-  const uint32_t p = (uint32_t)a.parents[i], c = (uint32_t)a.children[i];
   if (!made(p, c)) return;
-  const int len = held_of(a.lengths, p, a.blocks, a.page), full = len / a.page, rest = len - full * a.page;
   const int64_t at = taken + s_before;
   const int32_t to = rest && at >= 0 && at < a.free_count ? a.free_pages[at] : -1;
-  const int32_t* from = a.tables + (int64_t)p * a.blocks;
   if (blockIdx.x == 0) {
     for (int64_t b = tid; b < a.blocks; b += kThreads)
       a.tables[(int64_t)c * a.blocks + b] = b < full ? from[b] : b == full ? to : -1;
     if (tid == 0) a.lengths[c] = len;
   }
   if (!rest) return;
-  const int32_t source = from[full];
   if ((uint32_t)source >= (uint64_t)a.pages || (uint32_t)to >= (uint64_t)a.pages || source == to) return;
-  // rows [0, rest) of every (layer, k or v, kv head)
-  const uint32_t run = (uint32_t)rest * a.row_vecs;
+  // rows [0, rest) of every (layer, kv head, k or v): runs that follow each other, 16 bytes a thread
+  const uint32_t run = (uint32_t)rest * a.row_vecs, runs = (uint32_t)(a.layers * 2 * a.kv_heads);
   const int64_t head_vecs = (int64_t)a.page * a.row_vecs, page_vecs = head_vecs * a.kv_heads;
-  const int64_t vecs = a.layers * 2 * a.kv_heads * run, step = (int64_t)gridDim.x * kThreads;
+  const int64_t vecs = (int64_t)runs * run, step = (int64_t)gridDim.x * kThreads;
   for (int64_t x0 = (int64_t)blockIdx.x * kThreads + tid; x0 < vecs; x0 += step * kAhead) {
-    uint4 got[kAhead];
-    uint4* dst[kAhead];
+    u32x4 got[kAhead];
+    u32x4* dst[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int64_t x = x0 + u * step;
       dst[u] = nullptr;
+      got[u] = u32x4{};
       if (x >= vecs) continue;
-      const uint32_t which = (uint32_t)(x / run), vec = (uint32_t)(x - (int64_t)which * run);     // [layer][kv head][k or v]
+      const uint32_t which = vecs <= UINT32_MAX ? (uint32_t)x / run : (uint32_t)(x / run), vec = (uint32_t)(x - (int64_t)which * run);
       const uint32_t head = which >> 1, layer = head / (uint32_t)a.kv_heads;
-      uint4* base = (which & 1 ? a.v : a.k) + (int64_t)layer * a.pages * page_vecs +
+      u32x4* base = (which & 1 ? a.v : a.k) + (int64_t)layer * a.pages * page_vecs +
                     (int64_t)(head - layer * a.kv_heads) * head_vecs + vec;
       got[u] = base[source * page_vecs];
       dst[u] = base + to * page_vecs;
@@ -121,8 +145,9 @@ constexpr int64_t kPagesMost = 1 << 24;       // pages of a cache
 constexpr int kRange = 8192;                  // pages of a workgroup of the list
 constexpr int kRanges = (int)(kPagesMost / kRange);
 constexpr int kListThreads = 1024;
-// One workgroup does it all up to here: its bits lie in LDS.
-constexpr int64_t kOnePages = 1 << 17, kOneEntries = 1 << 18;
+// Up to here one launch does it: bits and lengths lie in LDS, and every workgroup goes over all entries.
+constexpr int64_t kOnePages = 1 << 17, kOneEntries = 1 << 16;
+constexpr int kOneRows = 4096, kOneShare = 4096;        // pages that a workgroup lists
 
 struct HeldArgs {
   const int32_t* tables;
@@ -136,16 +161,8 @@ struct HeldArgs {
   int page;
 };
 
-// The held pages' bits by the waves, a row of the table each; `first` and `step` in waves.
-__device__ __forceinline__ void mark(const HeldArgs& a, uint32_t* bits, int64_t first, int64_t step) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t r = first; r < a.rows; r += step) {
-    const int live = live_of(a.lengths, r, a.blocks, a.page);
-    for (int b = lane; b < live; b += 64) {
-      const uint32_t id = (uint32_t)a.tables[r * a.blocks + b];
-      if (id < (uint64_t)a.pages) atomicOr(&bits[id >> 5], 1u << (id & 31));
-    }
-  }
+__device__ __forceinline__ void hold(const HeldArgs& a, uint32_t* bits, uint32_t id) {
+  if (id < (uint64_t)a.pages) atomicOr(&bits[id >> 5], 1u << (id & 31));
 }
 
 // Lists the pages of [p0, p1) that are asked for, from place `at` on; `scan` is LDS, a word a wave.
@@ -162,12 +179,19 @@ __device__ __forceinline__ void list_range(const HeldArgs& a, const uint32_t* bi
     const bool held = bits[p >> 5] >> (p & 31) & 1;
     return held == (a.rank != nullptr);
   };
+  // the run's words, a lane each: pages past p1 lie in its last word alone
   int mine = 0;
-  for (int64_t s = s0; s < s1; ++s) mine += __popcll(__ballot(listed(p0 + s * 64 + lane)));
+  for (int64_t w = (p0 + s0 * 64) / 32 + lane; w * 32 < min(p0 + s1 * 64, p1); w += 64) {
+    const int64_t in = p1 - w * 32;
+    mine += __popc((a.rank ? bits[w] : ~bits[w]) & (in >= 32 ? ~0u : (1u << in) - 1));
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o, kWave);
   if (lane == 0) scan[wv] = mine;
   __syncthreads();
   int32_t place = at;
   for (int w = 0; w < wv; ++w) place += scan[w];
+#pragma unroll 4
   for (int64_t s = s0; s < s1; ++s) {
     const int64_t p = p0 + s * 64 + lane;
     const bool on = listed(p);
@@ -181,28 +205,70 @@ __device__ __forceinline__ void list_range(const HeldArgs& a, const uint32_t* bi
   }
 }
 
+// Small caches, in one launch: every workgroup marks all held pages in its LDS, every entry of the tables a thread's,
+// kEntriesAhead of them in flight (bound by its instructions: a dozen an entry), and lists a share of the pages.
+constexpr int kEntriesAhead = 8;
 __global__ __launch_bounds__(kListThreads) void k_held_one(HeldArgs a) {
   extern __shared__ uint32_t s_bits[];
-  __shared__ int32_t s_scan[kListThreads / 64];
-  const int words = (int)ceil_div(a.pages, 32), tid = threadIdx.x;
+  __shared__ int32_t s_live[kOneRows];
+  __shared__ int32_t s_scan[kListThreads / 64], s_before[kListThreads / 64], s_all[kListThreads / 64];
+  const int words = (int)ceil_div(a.pages, 32), tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const uint32_t blocks = (uint32_t)a.blocks, entries = (uint32_t)(a.rows * a.blocks);
+  for (int r = tid; r < a.rows; r += kListThreads) s_live[r] = live_of(a.lengths, r, a.blocks, a.page);
   for (int w = tid; w < words; w += kListThreads) s_bits[w] = 0;
   __syncthreads();
-  mark(a, s_bits, uniform(tid >> 6), kListThreads / 64);
+  const uint32_t rows_on = kListThreads / blocks, on = kListThreads - rows_on * blocks;
+  uint32_t row = (uint32_t)tid / blocks, col = (uint32_t)tid - row * blocks;
+  for (uint32_t e = tid; e < entries; e += kListThreads * kEntriesAhead) {
+    uint32_t id[kEntriesAhead];
+#pragma unroll
+    for (int i = 0; i < kEntriesAhead; ++i) {
+      const uint32_t at = e + i * kListThreads;
+      id[i] = 0xffffffffu;
+      if (at < entries && (int)col < s_live[row]) id[i] = (uint32_t)a.tables[at];
+      row += rows_on, col += on;
+      if (col >= blocks) ++row, col -= blocks;
+    }
+#pragma unroll
+    for (int i = 0; i < kEntriesAhead; ++i) hold(a, s_bits, id[i]);
+  }
   __syncthreads();
-  list_range<kListThreads>(a, s_bits, 0, a.pages, 0, s_scan);
-  int32_t all = 0;
-  for (int w = 0; w < kListThreads / 64; ++w) all += s_scan[w];
-  if (tid == 0) a.count[0] = all;
+  // this workgroup's share, and what is listed ahead of it
+  const int64_t each = ceil_div(ceil_div(a.pages, 64), gridDim.x) * 64, p0 = min((int64_t)blockIdx.x * each, a.pages);
+  int before = 0, all = 0;
+  for (int w = tid; w < words; w += kListThreads) {
+    const int64_t in = a.pages - (int64_t)w * 32;
+    const int n = __popc((a.rank ? s_bits[w] : ~s_bits[w]) & (in >= 32 ? ~0u : (1u << in) - 1));
+    all += n;
+    if ((int64_t)w * 32 < p0) before += n;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    before += __shfl_xor(before, o, kWave);
+    all += __shfl_xor(all, o, kWave);
+  }
+  if (lane == 0) s_before[wv] = before, s_all[wv] = all;
+  __syncthreads();
+  before = all = 0;
+  for (int w = 0; w < kListThreads / 64; ++w) before += s_before[w], all += s_all[w];
+  list_range<kListThreads>(a, s_bits, p0, min(p0 + each, a.pages), before, s_scan);
+  if (blockIdx.x == 0 && tid == 0) a.count[0] = all;
   if (!a.rank)
-    for (int64_t i = all + tid; i < a.pages; i += kListThreads) a.list[i] = -1;
+    for (int64_t i = max((int64_t)all, p0) + tid; i < min(p0 + each, a.pages); i += kListThreads) a.list[i] = -1;
 }
 
 __global__ __launch_bounds__(kThreads) void k_held_clear(HeldArgs a) {
   const int64_t words = ceil_div(a.pages, 32);
   for (int64_t w = (int64_t)blockIdx.x * kThreads + threadIdx.x; w < words; w += (int64_t)gridDim.x * kThreads) a.bits[w] = 0;
 }
-__global__ __launch_bounds__(kThreads) void k_held_mark(HeldArgs a) {
-  mark(a, a.bits, (int64_t)blockIdx.x * (kThreads / 64) + uniform((int)threadIdx.x >> 6), (int64_t)gridDim.x * (kThreads / 64));
+__global__ __launch_bounds__(kThreads) void k_held_mark(HeldArgs a) {       // a wave a row of the table
+  const int lane = threadIdx.x & 63;
+  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 64) + uniform((int)threadIdx.x >> 6); r < a.rows;
+       r += (int64_t)gridDim.x * (kThreads / 64)) {
+    const int live = live_of(a.lengths, r, a.blocks, a.page);
+#pragma unroll 4
+    for (int b = lane; b < live; b += 64) hold(a, a.bits, (uint32_t)a.tables[r * a.blocks + b]);
+  }
 }
 __global__ __launch_bounds__(kThreads) void k_held_count(HeldArgs a) {
   __shared__ int32_t s_sum[kThreads / 64];
@@ -248,13 +314,13 @@ __global__ __launch_bounds__(kThreads) void k_held_list(HeldArgs a) {
 
 // The lists of k_held_one or the four kernels; scratch for bits and counts is the caller's.
 int64_t held_scratch(int64_t rows, int64_t blocks, int64_t pages) {
-  if (pages <= kOnePages && rows * blocks <= kOneEntries) return 0;
+  if (pages <= kOnePages && rows <= kOneRows && rows * blocks <= kOneEntries) return 0;
   return 4 * (ceil_div(pages, 32) + kRanges);
 }
 void list_held(HeldArgs a, void* work, hipStream_t st) {
   const int64_t words = ceil_div(a.pages, 32);
   if (!work) {
-    hipLaunchKernelGGL(k_held_one, dim3(1), dim3(kListThreads), (size_t)words * 4, st, a);
+    hipLaunchKernelGGL(k_held_one, dim3((unsigned)ceil_div(a.pages, kOneShare)), dim3(kListThreads), (size_t)words * 4, st, a);
     return;
   }
   a.bits = (uint32_t*)work;
@@ -278,15 +344,16 @@ struct MoveArgs {
   const int32_t* list;
   const int32_t* rank;
   const int32_t* used;
-  const uint4* k;
-  const uint4* v;
-  uint4* k_new;
-  uint4* v_new;
+  const u32x4* k;
+  const u32x4* v;
+  u32x4* k_new;
+  u32x4* v_new;
   int64_t rows, blocks, pages, pages_new, layers, page_vecs;
-  int page, table_groups;
+  int page, table_groups, most;      // most: pages that may be held
 };
 
 // The first table_groups workgroups turn the tables, the others copy: a wave a run of one page in one layer, its K or V.
+constexpr int kMoveAhead = 8;
 __global__ __launch_bounds__(kThreads) void k_move_pages(MoveArgs a) {
   const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
   constexpr int kWaves = kThreads / 64;
@@ -305,22 +372,21 @@ __global__ __launch_bounds__(kThreads) void k_move_pages(MoveArgs a) {
     }
     return;
   }
-  const int64_t n = min((int64_t)a.used[0], a.pages_new), units = n * a.layers * 2;
-  const int64_t step = (int64_t)(gridDim.x - a.table_groups) * kWaves;
-  for (int64_t u = (int64_t)(blockIdx.x - a.table_groups) * kWaves + wv; u < units; u += step) {
-    const int64_t plane = u / n, to = u - plane * n, layer = plane >> 1;
-    const int64_t from = a.list[to];
-    const uint4* src = (plane & 1 ? a.v : a.k) + (layer * a.pages + from) * a.page_vecs;
-    uint4* dst = (plane & 1 ? a.v_new : a.k_new) + (layer * a.pages_new + to) * a.page_vecs;
-    for (int64_t x0 = lane; x0 < a.page_vecs; x0 += 64 * kAhead) {
-      uint4 got[kAhead];
+  // a wave a (plane, page): as many pages as there may be, so that the list is read beside its length
+  const uint32_t at = (blockIdx.x - a.table_groups) * kWaves + wv, plane = at / (uint32_t)a.most;
+  const int64_t to = at - plane * (uint32_t)a.most, layer = plane >> 1;
+  if (layer >= a.layers) return;
+  const int64_t n = min((int64_t)a.used[0], a.pages_new), from = a.list[to];
+  if (to >= n) return;
+  const u32x4* src = (plane & 1 ? a.v : a.k) + (layer * a.pages + from) * a.page_vecs;
+  u32x4* dst = (plane & 1 ? a.v_new : a.k_new) + (layer * a.pages_new + to) * a.page_vecs;
+  for (int64_t x0 = lane; x0 < a.page_vecs; x0 += 64 * kMoveAhead) {
+    u32x4 got[kMoveAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (x0 + 64 * i < a.page_vecs) got[i] = src[x0 + 64 * i];
+    for (int i = 0; i < kMoveAhead; ++i) got[i] = src[min(x0 + 64 * i, a.page_vecs - 1)];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (x0 + 64 * i < a.page_vecs) dst[x0 + 64 * i] = got[i];
-    }
+    for (int i = 0; i < kMoveAhead; ++i)
+      if (x0 + 64 * i < a.page_vecs) dst[x0 + 64 * i] = got[i];
   }
 }
 
@@ -355,7 +421,7 @@ int cv3_paged_fork(const int32_t* parents, const int32_t* children, int64_t fork
   const Run out[] = {{tables, 4 * n * blocks}, {lengths, 4 * n}, {taken_out, 4}, {k_cache, cache}, {v_cache, cache}};
   CV3_REQUIRE(apart(out, in), CV3_EINVAL, "tables, lengths, caches and the count of pages overlap each other or the inputs");
   const int row_vecs = d * elem_size(cache_type) / 16;
-  ForkArgs a{parents, children, tables, lengths, free_pages, taken, taken_out, (uint4*)k_cache, (uint4*)v_cache, pages,
+  ForkArgs a{parents, children, tables, lengths, free_pages, taken, taken_out, (u32x4*)k_cache, (u32x4*)v_cache, pages,
              blocks, free_count, layers, (int)forks, (int)rows, kv_heads, (int)page, row_vecs};
   CV3_REQUIRE((double)layers * 2 * kv_heads < 2147483648.0, CV3_EINVAL, "bad cache shape");
   // at least one workgroup, so that the pages taken are passed on
@@ -406,6 +472,8 @@ int cv3_paged_compact(const int32_t* tables, int64_t rows, int64_t blocks, const
   const Run in[] = {{tables, 4 * n * blocks}, {lengths, 4 * n}, {k_cache, one * pages}, {v_cache, one * pages}};
   const Run out[] = {{tables_new, 4 * n * blocks}, {used, 4}, {k_new, one * pages_new}, {v_new, one * pages_new}};
   CV3_REQUIRE(apart(out, in), CV3_EINVAL, "the new cache, its tables and their count overlap each other or what is read");
+  CV3_REQUIRE((double)std::min({(double)pages, (double)pages_new, n * blocks}) * layers * 2 / 4 < kLaunchBlocks, CV3_EINVAL,
+              "%lld pages of %lld layers are too many for one call", (long long)pages, (long long)layers);
   hipStream_t st = stream_of(s);
   const int64_t bits = held_scratch(rows, blocks, pages);
   void* work = nullptr;
@@ -413,13 +481,12 @@ int cv3_paged_compact(const int32_t* tables, int64_t rows, int64_t blocks, const
   int32_t *list = (int32_t*)work, *rank = list + pages;
   list_held(HeldArgs{tables, lengths, nullptr, nullptr, list, rank, used, rows, blocks, pages, (int)page},
             bits ? (void*)(rank + pages) : nullptr, st);
-  const int64_t most = std::min({pages, pages_new, rows * blocks}) * layers * 2;      // runs to copy, at most
-  MoveArgs a{tables, lengths, tables_new, list, rank, used, (const uint4*)k_cache, (const uint4*)v_cache, (uint4*)k_new,
-             (uint4*)v_new, rows, blocks, pages, pages_new, layers, kv_heads * page * row_vecs, (int)page,
-             (int)std::min<int64_t>(ceil_div(rows, kThreads / 64), 256)};
-  const int64_t copies = std::min<int64_t>(ceil_div(most, kThreads / 64), 4096);
-  if (a.table_groups + copies > 0)
-    hipLaunchKernelGGL(k_move_pages, dim3((unsigned)(a.table_groups + copies)), dim3(kThreads), 0, st, a);
+  const int64_t most = std::min({pages, pages_new, rows * blocks});       // pages to copy; the list is as long as the cache
+  const int64_t copies = ceil_div(most * layers * 2, kThreads / 64), tables_by = std::min<int64_t>(ceil_div(rows, kThreads / 64), 256);
+  MoveArgs a{tables, lengths, tables_new, list, rank, used, (const u32x4*)k_cache, (const u32x4*)v_cache, (u32x4*)k_new,
+             (u32x4*)v_new, rows, blocks, pages, pages_new, layers, kv_heads * page * row_vecs, (int)page, (int)tables_by, (int)most};
+  if (copies + tables_by > 0)
+    hipLaunchKernelGGL(k_move_pages, dim3((unsigned)(copies + tables_by)), dim3(kThreads), 0, st, a);
   const hipError_t err = hipGetLastError();
   const int rc = scratch_free(work, st);
   CV3_REQUIRE(err == hipSuccess, CV3_EHIP, "kernel launch failed: %s", hipGetErrorString(err));

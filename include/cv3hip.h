@@ -649,8 +649,8 @@ int cv3_paged_fork(const int32_t* parents, const int32_t* children, int64_t fork
                    int64_t layers, int64_t pages, int kv_heads, int64_t page, int d, cv3_stream_t s);
 /* The ids of [0, pages) that none of the first ceil(lengths[b] / page) entries of a table names, ascending, into
  * free_pages [pages], -1 behind the last; *count of them.  That is what a sequence held that has ended (length 0), and
- * what cv3_paged_tables and cv3_paged_fork take from.  At most 2^24 pages.  More than 131072 pages or 262144 table
- * entries take scratch of the allocator (CV3_ENOMEM where a capture finds none). */
+ * what cv3_paged_tables and cv3_paged_fork take from.  At most 2^24 pages.  More than 131072 pages, 65536 table entries
+ * or 4096 tables take scratch of the allocator (CV3_ENOMEM where a capture finds none). */
 int cv3_paged_free(const int32_t* tables, int64_t rows, int64_t blocks, const int32_t* lengths, int64_t page,
                    int64_t pages, int32_t* free_pages, int32_t* count, cv3_stream_t s);
 /* The pages that the tables' first ceil(lengths[b] / page) entries name, each once and in the order of their ids, copied
