@@ -604,9 +604,11 @@ class DeviceQwen2:
             self._batch = {n: (w, w.rows if rows is None else rows, *made[n]) for n, (w, _, rows) in parts.items() if made}
         return self._batch
 
-    def _paged_layers(self, x: DeviceArray, pos, slots, tables, lengths, cos, sin, k: DeviceArray, v: DeviceArray):
+    def _paged_layers(self, x: DeviceArray, pos, slots, tables, lengths, cos, sin, k: DeviceArray, v: DeviceArray,
+                      starts=None):
         """The body over rows of any sequences (qwen2.py:139-179): each row's k and v go to its slot, and it sees the
-        ``lengths`` keys of its own table row.  Returns the residual stream."""
+        ``lengths`` keys of its own table row.  With ``starts`` the rows are several tokens of each sequence, the last at
+        ``lengths`` - 1, and each sees its sequence up to itself.  Returns the residual stream."""
         t = x.shape[0]
         D, H, R, I = self.hidden, self.heads, self.qkv.rows, self.inter
         h, n, qkv = x.copy(), DeviceArray((t, D)), DeviceArray((t, R))
@@ -631,7 +633,10 @@ class DeviceQwen2:
             else:
                 self._linear(n.ptr, t, self.qkv, l, qkv.ptr, R, bias=bias)
             paged.append(qkv, H, pos, slots, cos, sin, kl, vl, out=q)
-            paged.attention(q, kl, vl, tables, lengths, out=att)
+            if starts is None:
+                paged.attention(q, kl, vl, tables, lengths, out=att)
+            else:
+                paged.extend(q, kl, vl, tables, lengths, starts, out=att)
             if not planes:
                 self._after_attention(l, t, att, h, n, u, a, res, swiglu)
                 continue
@@ -642,6 +647,28 @@ class DeviceQwen2:
             _lib.call("binary", 2, a.ptr, u.ptr, a.ptr, t * I, 0.0, 0.0, None)       # silu(gate) * up
             linear("down", a.ptr, h.ptr, D, None, res)
         return h
+
+    def _ragged(self, x, before, new, tables: DeviceArray, slots, pos, cos, sin, k: DeviceArray, v: DeviceArray):
+        """The body over ``new`` tokens of each sequence, after the ``before`` it holds (both the host's), in parts of rows
+        that one launch serves: a sequence's earlier keys are in the cache, wherever the cut is.  ``x(t0, t1)`` are the
+        rows' embeddings on the device.  Yields (t0, t1, residual stream)."""
+        ends = np.cumsum(new, dtype=np.int64)
+        begins, part = ends - new, min(_PROMPT_ROWS, (2**23 - 1) // self.heads)
+        for t0 in range(0, int(ends[-1]), part):
+            t1 = min(t0 + part, int(ends[-1]))
+            at = np.flatnonzero((begins < t1) & (ends > t0))
+            r = slice(int(at[0]), int(at[-1]) + 1)
+            starts = np.clip(np.append(begins[r], ends[r][-1]), t0, t1) - t0
+            upto = before[r] + np.minimum(ends[r], t1) - begins[r]
+            yield t0, t1, self._paged_layers(x(t0, t1), pos.rows(t0, t1), slots.rows(t0, t1), tables.rows(r.start, r.stop),
+                                             to_device(upto.astype(np.int32)), cos, sin, k, v,
+                                             to_device(starts.astype(np.int32)))
+
+    def _embedded(self, ids: DeviceArray, out: DeviceArray) -> DeviceArray:
+        """Rows of the speech embedding for device ids (int64)."""
+        kind, q, sc, sdt, kp, block, n = self.emb.layer(0)
+        _lib.call("embedding", kind, q, sc, sdt, n, self.hidden, kp, block, ids.ptr, ids.size, out.ptr, None)
+        return out
 
     @staticmethod
     def _reserve(held, beams: int, new: int, page: int):
@@ -714,16 +741,12 @@ class DeviceQwen2:
         k, v = paged.new_cache(pages, self.kv_heads, page, dh, cache, layers=self.layers)
         own, tables = to_device(own_h), to_device(own_h)
         # the prompts: every token a row that sees its own sequence up to itself
-        rows = np.repeat(np.arange(r), held)
-        _, slots, pos = self._slots(to_device(np.zeros(r, np.int32)), to_device(held), held, page, to_device(own_h[:, 0]))
-        upto = np.concatenate([np.arange(1, n + 1) for n in held]).astype(np.int32)
+        first = to_device(own_h[:, 0])
+        _, slots, pos = self._slots(to_device(np.zeros(r, np.int32)), to_device(held), held, page, first)
         ends, every = np.cumsum(held, dtype=np.int64), np.concatenate(xs).astype(np.float32)
         last = DeviceArray((r * w, self.hidden))
-        part = min(_PROMPT_ROWS, (2**23 - 1) // self.heads)
-        for t0 in range(0, len(rows), part):       # a row's earlier keys are in the cache, wherever the cut is
-            t1 = min(t0 + part, len(rows))
-            h = self._paged_layers(to_device(every[t0:t1]), pos.rows(t0, t1), slots.rows(t0, t1),
-                                   to_device(own_h[rows[t0:t1], 0]), to_device(upto[t0:t1]), cos, sin, k, v)
+        for t0, t1, h in self._ragged(lambda t0, t1: to_device(every[t0:t1]), np.zeros(r, np.int64), held, first, slots, pos,
+                                      cos, sin, k, v):
             for i in np.flatnonzero((ends > t0) & (ends <= t1)):
                 for j in range(w):
                     _lib.call("copy_d2d", last.ptr + (int(i) * w + j) * self.hidden * 4,
@@ -745,8 +768,7 @@ class DeviceQwen2:
             for r0 in range(0, r if w > 1 else 0, _TABLE_ROWS):
                 r1 = min(r0 + _TABLE_ROWS, r)
                 paged.beam_reorder(parents.rows(r0, r1), tables.rows(r0, r1), own.rows(r0, r1), (held + i)[r0:r1], k, v)
-            kind, q, sc, sdt, kp, block, n = self.emb.layer(0)
-            _lib.call("embedding", kind, q, sc, sdt, n, self.hidden, kp, block, chosen.ptr, r * w, x.ptr, None)
+            self._embedded(chosen, x)
             lengths, slots, pos = self._slots(lengths, ones, each, page, own.reshape(r * w, blocks))
             h = self._paged_layers(x, pos, slots, tables.reshape(r * w, blocks), lengths, cos, sin, k, v)
             logits = self._head(h)
@@ -760,3 +782,104 @@ class DeviceQwen2:
             ends = [j for j, t in enumerate(tokens) if stop[0] <= t < stop[1]]
             out.append((tokens[:ends[0]] if ends else tokens, float(best[i, 0])))
         return out
+
+    # -- given continuations of several prompts ----
+    def score_batch(self, prompts, continuations, top: int = 0, page: int = 16, cache: str = "float32"):
+        """What given speech tokens are worth after their prompts: for each of several prompts ((T, hidden) embeddings, of
+        any lengths) a list of continuations, each a list of token ids.  Returns as many lists, of (logprobs (n,), entropy
+        (n,), ids (n, top) int64, values (n, top)) a continuation: each token's log probability after all before it, the
+        entropy in nats of the distribution that it comes from, and that one's ``top`` (0 to 32) best tokens with their
+        log probabilities, best first.
+
+        A prompt is run once; its continuations go on from its cache (whole pages shared, a part-filled last one copied
+        for each), and the tokens of all of them are rows of the same passes over the weights.  The cache is as in
+        ``generate_batch``; prompts and continuations are taken 4096 sequences at a time."""
+        xs = [x.numpy() if isinstance(x, DeviceArray) else np.asarray(x, np.float32) for x in prompts]
+        if any(x.ndim != 2 or x.shape[1] != self.hidden or x.shape[0] < 1 for x in xs):
+            raise ValueError(f"prompts are (T, {self.hidden}) embeddings")
+        texts = [[np.asarray(c) for c in cs] for cs in continuations]
+        if len(texts) != len(xs):
+            raise ValueError(f"{len(texts)} lists of continuations for {len(xs)} prompts")
+        known = min(self.vocab, self.emb.rows)
+        for c in (c for cs in texts for c in cs):
+            if c.ndim != 1 or c.size and (c.dtype.kind not in "iu" or int(c.min()) < 0 or int(c.max()) >= known):
+                raise ValueError(f"continuations are lists of token ids below {known}")
+        if not 0 <= top <= min(32, self.vocab) or not 1 <= page <= 65536:
+            raise ValueError("scores take 0 to 32 alternatives and pages of 1 to 65536 keys")
+        if cache not in ("float32", "float16", "bfloat16"):
+            raise ValueError(f"a cache is float32, float16 or bfloat16, not {cache}")
+        none = tuple(np.zeros(s, t) for s, t in ((0, np.float32), (0, np.float32), ((0, top), np.int64), ((0, top), np.float32)))
+        out = [[none] * len(cs) for cs in texts]
+        group, size = [], 0                 # (prompt, its continuations) of one pass
+        for i, cs in enumerate(texts):
+            some = [j for j, c in enumerate(cs) if c.size]
+            while some:
+                if size + 2 > _TABLE_ROWS:
+                    self._score_group(xs, texts, group, top, page, cache, out)
+                    group, size = [], 0
+                take, some = some[:_TABLE_ROWS - size - 1], some[_TABLE_ROWS - size - 1:]
+                group.append((i, take))
+                size += 1 + len(take)
+        if group:
+            self._score_group(xs, texts, group, top, page, cache, out)
+        return out
+
+    def _score_group(self, xs, texts, group, top: int, page: int, cache: str, out):
+        """score_batch of up to 4096 sequences: the prompts are the first rows of the tables, their continuations the
+        others."""
+        r, D = len(group), self.hidden
+        of = np.array([p for p, (_, js) in enumerate(group) for _ in js], np.int32)      # each continuation's prompt
+        ids = [texts[i][j].astype(np.int64) for i, js in group for j in js]
+        held = np.array([xs[i].shape[0] for i, _ in group], np.int64)
+        count = np.array([c.size for c in ids], np.int64)
+        # what a continuation adds to the cache: all but its last token
+        total = held[of] + count - 1
+        pages = int((-(-held // page)).sum() + (-(-total // page) - held[of] // page).sum())
+        cos, sin = (to_device(a) for a in rope_tables(self.head_dim, self.theta, int(total.max())))
+        k, v = paged.new_cache(pages, self.kv_heads, page, self.head_dim, cache, layers=self.layers)
+        n = r + len(ids)
+        tables = to_device(np.full((n, int((-(-total // page)).max())), -1, np.int32))
+        free = to_device(np.arange(pages, dtype=np.int32))
+        row = 4 * D
+        states = DeviceArray((int(count.sum()), D))         # the residual stream that each token is drawn from
+        ends = np.cumsum(count)
+
+        def run(lengths, before, new, taken, x, keep):
+            lengths, taken, _, slots, pos = paged.block_tables(lengths, to_device(new.astype(np.int32)), page, free, taken,
+                                                               tables, tokens=int(new.sum()))
+            for t0, t1, h in self._ragged(x, before, new, tables, slots, pos, cos, sin, k, v) if new.any() else ():
+                keep(t0, t1, h)
+            return lengths, taken
+
+        every = np.concatenate([xs[i] for i, _ in group]).astype(np.float32)
+        last = np.cumsum(held) - 1
+
+        def keep_last(t0, t1, h):
+            for c in np.flatnonzero((last[of] >= t0) & (last[of] < t1)):
+                _lib.call("copy_d2d", states.ptr + int(ends[c] - count[c]) * row, h.ptr + int(last[of[c]] - t0) * row, row, None)
+
+        zero = np.zeros(n, np.int64)
+        lengths, taken = run(to_device(zero.astype(np.int32)), zero, np.append(held, zero[r:]), to_device(np.zeros(1, np.int32)),
+                             lambda t0, t1: to_device(every[t0:t1]), keep_last)
+        taken = paged.fork(to_device(of), to_device(np.arange(r, n, dtype=np.int32)), tables, lengths, free, taken, k, v)
+        fed = np.concatenate([c[:-1] for c in ids])
+        at = np.cumsum(count - 1)                           # each continuation's end among the tokens that are fed
+
+        def keep_all(t0, t1, h):
+            for c in np.flatnonzero((at - count + 1 < t1) & (at > t0)):
+                a, b = max(int(at[c] - count[c] + 1), t0), min(int(at[c]), t1)
+                _lib.call("copy_d2d", states.ptr + int(ends[c] - (at[c] - a)) * row, h.ptr + (a - t0) * row, (b - a) * row, None)
+
+        run(lengths, np.append(held, held[of]), np.append(zero[:r], count - 1), taken,
+            lambda t0, t1: self._embedded(to_device(fed[t0:t1]), DeviceArray((t1 - t0, D))), keep_all)
+        tokens, found = np.concatenate(ids), []
+        for t0 in range(0, len(tokens), _PROMPT_ROWS):
+            t1 = min(t0 + _PROMPT_ROWS, len(tokens))
+            got = paged.token_logprobs(self._head(states.rows(t0, t1)), to_device(tokens[t0:t1]), top)
+            found.append([g.numpy() for g in got])
+        found = [np.concatenate(f) for f in zip(*found)]
+        c = 0
+        for i, js in group:
+            for j in js:
+                out[i][j] = tuple(f[ends[c] - count[c]:ends[c]].copy() for f in found)
+                c += 1
