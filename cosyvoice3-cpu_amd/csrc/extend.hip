@@ -129,7 +129,10 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWaveRows = 32;       // (token, head) rows of a wave
 constexpr int kSplitSlots = 1024;   // tiles of rows whose keys may be shared out
-constexpr int kWholeKeys = 1024;    // tables up to here are not worth a plan: 12 prompts of up to 900 tokens 68 us without, 90 with
+constexpr int kWholeKeys = 1024;    // tables up to here are not worth a plan: 12 prompts of up to 900 tokens 50 us without, 90 with
+// Items from which their order counts, more than one a compute unit: 12 prompts of up to 900 tokens 66 us by slots, 50 with
+// the longest first, 16 of 1000 156 and 136; where all are alike (24 x 60 queries over 360 keys) 52 and 53.
+constexpr int kOrderItems = 256;
 constexpr int kFewRows = 48;        // rows a sequence, on average, that one wave takes
 
 // Weights are held 2^10 up against a reference that a row's largest score has passed by so little that the 32 of a lane
@@ -236,6 +239,50 @@ __device__ __forceinline__ bool find_item(const ExtArgs& a, int slot, Item& it) 
   if (before == 0) return false;
   const int b = uniform(before - 1);
   return item_of<W>(a, b, slot - uniform(first_slot<W>(a, b)), it);
+}
+
+// One value of a wave's 64, by lane exchanges within rows of 16 and four lane reads.
+template <typename F>
+__device__ __forceinline__ uint32_t wave_fold(uint32_t v, F f) {
+  v = f(v, dpp32<kDppXor1>(v));
+  v = f(v, dpp32<kDppXor2>(v));
+  v = f(v, dpp32<kDppHalfMirror>(v));
+  v = f(v, dpp32<kDppMirror>(v));
+  return f(f((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16)),
+           f((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
+}
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
+  return wave_fold(v, [](uint32_t x, uint32_t y) { return x + y; });
+}
+// Item `at` of up to 64 sequences in the order of their last key's tile, the furthest first: a sequence a lane, the level
+// by bisection of how many lie at or above it, by every wave for itself.
+template <int KT, int W>
+__device__ __forceinline__ bool find_by_keys(const ExtArgs& a, int at, Item& it) {
+  constexpr int kRows = kWaveRows * W;
+  const int lane = threadIdx.x & 63;
+  const Seq s = lane < a.batch ? seq_of(a, lane) : Seq{};
+  const int all = (s.count * a.group + kRows - 1) / kRows;
+  // how many of the sequence's tiles of rows see a key past L tiles of keys: its last ones
+  auto past = [&](int L) {
+    const int64_t x = (int64_t)L * KT - s.base;      // tokens before the first that does
+    return L < 0 || x <= 0 ? all : x >= s.count ? 0 : all - (int)x * a.group / kRows;
+  };
+  int lo = -1, hi = (int)((a.blocks * a.page + KT - 1) / KT);
+  if ((uint32_t)at >= wave_sum_u32((uint32_t)all)) return false;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (wave_sum_u32((uint32_t)past(mid)) > (uint32_t)at) lo = mid; else hi = mid;
+  }
+  const int above = past(hi), mine = past(lo) - above;
+  int up = mine, before = (int)wave_sum_u32((uint32_t)above);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(up, o, kWave);
+    if (lane >= o) up += u;
+  }
+  before += up - mine;                       // items ahead of this sequence's at the level
+  const int b = uniform(__ffsll((unsigned long long)__ballot(at >= before && at < before + mine)) - 1);
+  return item_of<W>(a, b, __builtin_amdgcn_readlane(all - above - 1 - (at - before), b), it);
 }
 
 template <typename E, int ND, int W>
@@ -671,11 +718,12 @@ constexpr int simd_waves() {
 
 // One workgroup a (tile of rows, kv head).
 template <typename E, int ND, bool FULL, int W>
-__global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_whole(ExtArgs a) {
+__global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_whole(ExtArgs a, bool by_keys) {
   __shared__ typename Shape<E, ND, W>::Mem mem;
   Item it;
-  // the last tiles of a sequence see the most keys: they go first
-  if (!find_item<W>(a, a.slots - 1 - (int)(blockIdx.x / (unsigned)a.kv_heads), it)) return;
+  // what sees the most keys goes first, or at least the last tiles of each sequence
+  const int at = (int)(blockIdx.x / (unsigned)a.kv_heads);
+  if (!(by_keys ? find_by_keys<Shape<E, ND, W>::KT, W>(a, at, it) : find_item<W>(a, a.slots - 1 - at, it))) return;
   it.kvh = (int)(blockIdx.x % (unsigned)a.kv_heads);
   int t0, t1;
   tiles_of<Shape<E, ND, W>::KT>(a, it, t0, t1);
@@ -688,19 +736,6 @@ struct Piece {
   int b, kvh, tile, part, parts, place, pad[2];
 };
 
-// One value of a wave's 64, by lane exchanges within rows of 16 and four lane reads.
-template <typename F>
-__device__ __forceinline__ uint32_t wave_fold(uint32_t v, F f) {
-  v = f(v, dpp32<kDppXor1>(v));
-  v = f(v, dpp32<kDppXor2>(v));
-  v = f(v, dpp32<kDppHalfMirror>(v));
-  v = f(v, dpp32<kDppMirror>(v));
-  return f(f((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16)),
-           f((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
-}
-__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
-  return wave_fold(v, [](uint32_t x, uint32_t y) { return x + y; });
-}
 // The last i of [0, n) with v[i] <= x; v[0] <= x.
 __device__ __forceinline__ int last_at(const int32_t* v, int n, int x) {
   int lo = 0, hi = n;
@@ -1038,7 +1073,8 @@ int run_tiles(ExtArgs a, hipStream_t st) {
       hipLaunchKernelGGL((k_extend_split<E, ND, FULL, W>), dim3((unsigned)a.pieces_most), dim3(64 * W), 0, st, a);
       launch_join<ND, W>(a, a.cuts_most, 0, st);
     } else {                           // short tables, very many tiles, or no memory: one workgroup an item
-      hipLaunchKernelGGL((k_extend_whole<E, ND, FULL, W>), dim3((unsigned)items), dim3(64 * W), 0, st, a);
+      hipLaunchKernelGGL((k_extend_whole<E, ND, FULL, W>), dim3((unsigned)items), dim3(64 * W), 0, st, a,
+                         a.batch > 1 && a.batch <= 64 && items > kOrderItems);
     }
   }
   const hipError_t err = hipGetLastError();

@@ -145,6 +145,18 @@ def test_extend_large_batches(paged, batch):
     check(paged, rng.integers(0, 5, batch), rng.integers(0, 60, batch), 4, 2, 32, 16, "bfloat16")
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("h,kv,d", [(64, 32, 8), (48, 16, 64), (32, 8, 128), (40, 10, 160)])
+def test_extend_many_tiles_of_short_tables(paged, h, kv, d, kind):
+    """More tiles of rows than run at once, taken by their last keys: sequences of any order and size, some of nothing,
+    one with more tokens than keys, windows; and as many sequences as are ordered, and one more."""
+    check(paged, [30, 0, 290, 1, 200, 290, 0, 77, 128, 3], [0, 9, 64, 400, 0, 64, 0, 20, -60, 300], h, kv, d, 16, kind, pad=(4, 5))
+    check(paged, [30, 290, 200, 77, 128], [350, 64, 0, 20, 500], h, kv, d, 24, kind, window=100)
+    rng = np.random.default_rng(d)
+    for batch in (64, 65):
+        check(paged, rng.integers(0, 30, batch), rng.integers(0, 100, batch), h, kv, d, 16, kind, seed=batch)
+
+
 def test_extend_scales(paged):
     """Any scale: none, negative, large; scores of hundreds."""
     for kind in TYPES:
