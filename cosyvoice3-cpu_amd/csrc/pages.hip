@@ -16,8 +16,10 @@ namespace {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));     // 16 bytes
 
 constexpr int kForks = 4096, kForkRows = 65536;   // forks of a call, sequences of its tables
-constexpr int kForkGroups = 2048;                 // workgroups of a fork's copies, about
-constexpr int kThreads = 256, kAhead = 4;         // 16-byte vectors of a thread in flight
+// Workgroups of a call's copies, about, and 16-byte vectors of a thread in flight: what every workgroup does before its
+// copies is most of a small call.
+constexpr int kForkGroups = 1024, kForkAhead = 6;
+constexpr int kThreads = 256;
 
 struct ForkArgs {
   const int32_t* parents;
@@ -115,11 +117,11 @@ __global__ __launch_bounds__(kThreads) void k_fork(ForkArgs a) {
   const uint32_t run = (uint32_t)rest * a.row_vecs, runs = (uint32_t)(a.layers * 2 * a.kv_heads);
   const int64_t head_vecs = (int64_t)a.page * a.row_vecs, page_vecs = head_vecs * a.kv_heads;
   const int64_t vecs = (int64_t)runs * run, step = (int64_t)gridDim.x * kThreads;
-  for (int64_t x0 = (int64_t)blockIdx.x * kThreads + tid; x0 < vecs; x0 += step * kAhead) {
-    u32x4 got[kAhead];
-    u32x4* dst[kAhead];
+  for (int64_t x0 = (int64_t)blockIdx.x * kThreads + tid; x0 < vecs; x0 += step * kForkAhead) {
+    u32x4 got[kForkAhead];
+    u32x4* dst[kForkAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < kForkAhead; ++u) {
       const int64_t x = x0 + u * step;
       dst[u] = nullptr;
       got[u] = u32x4{};
@@ -132,7 +134,7 @@ __global__ __launch_bounds__(kThreads) void k_fork(ForkArgs a) {
       dst[u] = base + to * page_vecs;
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
+    for (int u = 0; u < kForkAhead; ++u)
       if (dst[u]) *dst[u] = got[u];
   }
 }
@@ -426,7 +428,10 @@ int cv3_paged_fork(const int32_t* parents, const int32_t* children, int64_t fork
   CV3_REQUIRE((double)layers * 2 * kv_heads < 2147483648.0, CV3_EINVAL, "bad cache shape");
   // at least one workgroup, so that the pages taken are passed on
   const int64_t vecs = layers * 2 * kv_heads * page * row_vecs, count = std::max<int64_t>(forks, 1);
-  const int64_t each = std::max<int64_t>(1, std::min(ceil_div(vecs, kThreads * kAhead), ceil_div(kForkGroups, count)));
+  // where it may be, a multiple of the XCDs: children of one parent then find its rows in their L2 (84 forks of 12 parents,
+  // 24 layers of 2 x 80 float32, 23 us with 13 workgroups each, 19 with 16)
+  const int64_t share = std::max<int64_t>(1, kForkGroups / count);
+  const int64_t each = std::max<int64_t>(1, std::min(ceil_div(vecs, kThreads * kForkAhead), share >= 8 ? (share + 4) / 8 * 8 : share));
   if (forks == 0) a.rows = 0;
   hipLaunchKernelGGL(k_fork, dim3((unsigned)each, (unsigned)count), dim3(kThreads), (size_t)3 * ((a.rows + 31) / 32) * 4,
                      stream_of(s), a);

@@ -257,6 +257,8 @@ __global__ __launch_bounds__(kThreads) void k_score_join(ScoreArgs a) {
   }
 }
 
+// Up to 2048 and 4096 logits a row, slices as long: 2000 rows of 2000 15.6 us with 32 logits a thread, 11.6 with 8; 1000 of
+// 4000 10.4 and 8.7 with 16; 3 of 2000 6.7 and 6.9.
 template <int E>
 void launch_slices(const ScoreArgs& a, int64_t rows, hipStream_t st) {
   const dim3 grid((unsigned)(rows * a.slices)), block(kThreads);
@@ -289,7 +291,9 @@ int cv3_token_logprobs(const float* logits, int64_t rows, int64_t vocab, const i
   a.slices = (int)ceil_div(vocab, a.slice);
   hipStream_t st = stream_of(s);
   if (a.slices == 1) {
-    launch_slices<32>(a, rows, st);
+    if (vocab <= 8 * kThreads) launch_slices<8>(a, rows, st);
+    else if (vocab <= 16 * kThreads) launch_slices<16>(a, rows, st);
+    else launch_slices<32>(a, rows, st);
     CV3_LAUNCHED();
     return CV3_OK;
   }

@@ -65,7 +65,8 @@ def check(paged, x, tokens, top):
 
 SIZES = [(1, 1, 1), (1, 6761, 5), (6, 6761, 0), (70, 6761, 32), (3, 2, 2), (5, 255, 16), (4, 256, 8), (7, 257, 9), (2, 32, 32),
          (3, 1023, 1), (2, 8191, 8), (2, 8192, 8), (2, 8193, 8), (3, 16385, 32), (5, 128000, 5), (1, 151936, 20),
-         (2, 1 << 19, 32), (2, (1 << 19) - 1, 0), (2000, 300, 3), (300, 20001, 2)]
+         (2, 1 << 19, 32), (2, (1 << 19) - 1, 0), (2000, 300, 3), (300, 20001, 2),
+         (4, 2047, 5), (3, 2048, 32), (3, 2049, 32), (2, 4095, 0), (2, 4096, 8), (2, 4097, 9)]
 
 
 @pytest.mark.parametrize("rows,vocab,top", SIZES)
@@ -79,7 +80,7 @@ def test_scores(paged, rows, vocab, top):
     check(paged, 10.0 * x, tokens, top)
 
 
-@pytest.mark.parametrize("vocab", [40, 6761, 20000])
+@pytest.mark.parametrize("vocab", [40, 2048, 4000, 6761, 20000])
 def test_scores_of_equal_logits(paged, vocab):
     """Ties go to the lower token, wherever their slices lie; more equal logits than the list of a slice holds."""
     rng = np.random.default_rng(vocab)
@@ -89,7 +90,7 @@ def test_scores_of_equal_logits(paged, vocab):
         check(paged, x, [0, vocab - 1, vocab // 2, 1, vocab - 1, 0], top)
 
 
-@pytest.mark.parametrize("vocab", [64, 6761, 20000])
+@pytest.mark.parametrize("vocab", [64, 2047, 4095, 6761, 20000])
 def test_scores_that_are_no_numbers(paged, vocab):
     """-inf (a banned token) adds nothing; a NaN, +inf, or -inf alone makes its own row NaN."""
     rng = np.random.default_rng(vocab + 1)
