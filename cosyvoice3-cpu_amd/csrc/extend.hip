@@ -129,11 +129,14 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWaveRows = 32;       // (token, head) rows of a wave
 constexpr int kSplitSlots = 1024;   // tiles of rows whose keys may be shared out
-constexpr int kWholeKeys = 1024;    // tables up to here are not worth a plan: 12 prompts of up to 900 tokens 50 us without, 90 with
+// Tables up to here are not worth a plan: 12 prompts of up to 900 tokens 50 us without, 90 with.
+constexpr int kWholeKeys = 1024;
 // Items from which their order counts, more than one a compute unit: 12 prompts of up to 900 tokens 66 us by slots, 50 with
 // the longest first, 16 of 1000 156 and 136; where all are alike (24 x 60 queries over 360 keys) 52 and 53.
 constexpr int kOrderItems = 256;
-constexpr int kFewRows = 48;        // rows a sequence, on average, that one wave takes
+// Rows a sequence, on average, that one wave takes: 4 tokens of 7 heads a kv head over 504 keys 12 us, 16 with four waves.
+// For d > 64 one wave fetches too slowly (8 x 9 queries over 709 keys, 4 heads of 128 a kv head, 65 us against 35).
+constexpr int kFewRows = 48;
 
 // Weights are held 2^10 up against a reference that a row's largest score has passed by so little that the 32 of a lane
 // sum to no more than kMost, which float16 holds; so small planes end 2^-35 below the largest weight or lower.
@@ -322,6 +325,12 @@ struct Shape {
 // and 3.  Keys are scaled by a power of two a tile, values by one that only grows over the tiles.  What that loses, small
 // numbers beside large ones, is looked for: a row whose scores could be off (their factor is large), whose outputs are
 // below 2^-15 of the largest value, or whose results are not finite is formed again in float32 (RowSum).
+//
+// Bound by the matrix cores and the vector units, which share a wave's time: of 3870 cycles a tile of 64 keys (float16,
+// d = 64, two workgroups a CU) the products with their operands take about half, exponentials and planes of the weights a
+// quarter, addresses and loads 750, barriers 430; float32 widens its tile for another 1000.  500 queries over 60501 keys
+// (14 on 2 heads, float16) 260 us, 420 TFLOP/s of 4 d flops a score: twice that in products, where a library's large
+// product of float16 reaches 1060.  12 slices of up to 800 over 5800 keys (32 on 8 heads of 128, bfloat16) 690 us, 385.
 template <typename E, int ND, bool FULL, int W>
 __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0, int t1, bool whole, float* part,
                                        float2* part_ml, typename Shape<E, ND, W>::Mem& mem) {
@@ -710,13 +719,14 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
 }
 
 // Waves a SIMD that the registers are held to: a third one, where it fits, works while the others wait at their barriers
-// (float16, 14 on 2 heads of 64: 3.39 -> 2.84 ms at 8 x 800 queries over 5800 keys; with float32 the spills cost more).
+// (float16, 14 on 2 heads of 64, 8 x 800 queries over 5800 keys: 339 -> 284 us; with float32 the spills cost more).
 template <typename E, int ND>
 constexpr int simd_waves() {
   return ND > 4 ? 1 : ND == 2 && Cell<E>::N == 1 && !Cell<E>::SCALED ? 3 : 2;
 }
 
-// One workgroup a (tile of rows, kv head).
+// One workgroup a (tile of rows, kv head).  12 prompts of up to 900 tokens (14 on 2 heads of 64, float32) 49 us, where the
+// 15 tiles of the longest, 1.5 us each in a workgroup that has its CU alone, take half of it.
 template <typename E, int ND, bool FULL, int W>
 __global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_whole(ExtArgs a, bool by_keys) {
   __shared__ typename Shape<E, ND, W>::Mem mem;
@@ -753,7 +763,7 @@ __device__ __forceinline__ int last_at(const int32_t* v, int n, int x) {
 // its start and end, and kCutCost more where it has to be joined (some 2 us a tile); what runs in several rounds half of
 // the largest part for the last.
 //
-// One workgroup, a thread a slot: bound by the chain of its loads, searches and sums.  (Done by every workgroup of
+// One workgroup, a thread a slot: 8 - 9.5 us, the chain of its loads, searches and sums.  (Done by every workgroup of
 // k_extend_split for itself it took 4 - 9 us of each, and registers of the products.)
 constexpr int kPlanThreads = kSplitSlots, kTries = 9, kPartCost = 2, kCutCost = 3;
 template <int KT, int W>
@@ -864,7 +874,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
   }
 }
 
-// Of a cut item each workgroup leaves its rows' outputs, maxima and sums (`part`, `part_ml`).
+// Of a cut item each workgroup leaves its rows' outputs, maxima and sums (`part`, `part_ml`).  The two cases named at
+// `attend`: 254 - 270 and 688 - 745 us, beside them the plan and 8 and 38 us of joins.
 template <typename E, int ND, bool FULL, int W>
 __global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_split(ExtArgs a) {
   typedef Shape<E, ND, W> S;
@@ -886,7 +897,8 @@ __global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_split(
 }
 
 // Few rows a sequence: a wave each has 32 rows and one of `parts` runs of every item's keys, cut alike whatever their
-// lengths (the host knows no more), so that no plan has to come first.
+// lengths (the host knows no more), so that no plan has to come first.  4 queries over 504 keys (14 on 2 heads of 64, float32) 7.7 us
+// and 4.3 of joining: launches and memory latencies.
 template <typename E, int ND, bool FULL>
 __global__ __launch_bounds__(64, (simd_waves<E, ND>())) void k_extend_few(ExtArgs a, int parts) {
   typedef Shape<E, ND, 1> S;
@@ -903,7 +915,8 @@ __global__ __launch_bounds__(64, (simd_waves<E, ND>())) void k_extend_few(ExtArg
 }
 
 // The parts of an item's rows.  A wave reads four channels a lane, so several parts at a time, then joins its lanes; with
-// many parts the waves share them, with few each takes rows of its own.  parts 0: the items are those of `cuts`.
+// many parts the waves share them, with few each takes rows of its own.  parts 0: the items are those of `cuts`.  Bound by
+// the parts' bytes: 38 us for some 100 MB (12 ragged slices, 32 heads of 128).
 constexpr int kJoinAhead = 4, kJoinFew = 32, kJoinGroups = 2048;
 template <int LP, int W>                         // lanes of a part: a power of two with 4 LP >= d
 __global__ __launch_bounds__(256) void k_extend_join(ExtArgs a, int parts, int rows) {
@@ -1015,7 +1028,7 @@ void launch_join(const ExtArgs& a, int64_t items, int parts, hipStream_t st) {
   else hipLaunchKernelGGL((k_extend_join<64, W>), grid, block, 0, st, a, parts, rows);
 }
 
-// Scratch for `rows` rows of parts and `more` bytes behind them.  1: there is none.
+// Scratch for `rows` rows of parts and `more` bytes behind them; CV3_ENOMEM, which callers live without: there is none.
 int part_scratch(ExtArgs& a, int64_t rows, size_t more, void** work, void** behind, hipStream_t st) {
   const int rc = scratch_alloc(work, (size_t)rows * (a.d * 4 + 8) + more, st);
   if (rc) {

@@ -55,6 +55,9 @@ __device__ __forceinline__ void store_top(const ScoreArgs& a, int64_t row, int r
 // A key is the logit's rank over the complement of its token, so no two are equal and equal logits go by the lower
 // token.  Where more pass than the list holds (many equal logits) or the bar is -inf, the bar is set by whole keys:
 // what passes it lies in W groups, at most 4 W E keys.  W is the most that `top` may be, 0 where none are asked for.
+//
+// Bound by HBM where there is much, each logit read once: 500 rows of 128000 45.8 us, 5.6 TB/s; 6 of 6761 6.0 us, the chain
+// load, maximum, bar, sums, ranking.
 template <int E, int W>
 __global__ __launch_bounds__(kThreads) void k_score_slices(ScoreArgs a) {
   constexpr int kMost = W ? std::max(4 * W * E, kList) : 1;
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void k_score_slices(ScoreArgs a) {
 }
 
 // The slices of a row, one workgroup each: sums over the largest of their maxima, and the best of their sorted lists.
-// The W-th best of the lists' heads is a bar that at most W lists pass.
+// The W-th best of the lists' heads is a bar that at most W lists pass.  500 rows of 16 slices: 4.8 us, a launch and its chain.
 __global__ __launch_bounds__(kThreads) void k_score_join(ScoreArgs a) {
   __shared__ uint64_t s_list[kTop * 64];
   __shared__ uint64_t s_pass[kTop * kTop];

@@ -24,8 +24,8 @@ as NumPy arrays where the first argument was one.  ``out`` takes the results' ar
 Calls are enqueued on the calling thread's stream and do not synchronise; lengths, page ids and slots are
 read on the device and checked there.
 
-``attention`` and ``extend`` over long caches, ``beam_select``, ``compact``, and ``token_logprobs`` and ``free_pages``
-of large inputs take scratch from the allocator.  Captured into a graph they take it from the allocator's cache, and
+``attention`` and ``extend`` over long caches, ``beam_select``, ``compact``, ``token_logprobs`` of more than 8192 logits a
+row, and ``free_pages`` of more than 131072 pages, 65536 table entries or 4096 tables take scratch from the allocator.  Captured into a graph they take it from the allocator's cache, and
 the graph keeps it: run them once eagerly before each capture.  Where the cache has none, ``attention`` and ``extend``
 run without splitting a sequence's keys over workgroups, which is slow for few long sequences; the others raise
 ``ScratchError``.
@@ -267,8 +267,8 @@ def extend(q, k_cache: DeviceArray, v_cache: DeviceArray, tables, lengths, start
     they are (zeros in an array that the call makes).  A query with no key to see gives zeros, one whose scores are
     all -inf NaN (0 / 0); what lies in rows that are not seen reaches nothing.  Queries and weights enter the products
     with 22 bits of the largest in their row or tile, float32 keys and values too, and sums are float32: the error is
-    that of float32 arithmetic but for values 2^17 times smaller than others of the same sequence and head, whose last
-    bits are lost beside those.  Outputs that are not finite are formed again in float32."""
+    that of float32 arithmetic.  Rows where that would lose more (outputs far smaller than the largest value, very large
+    scores, results that are not finite) are formed again in float32, one after the other.  ``out`` may be ``q``."""
     kind = _cache(k_cache, v_cache)
     pages, kv_heads, page, d = k_cache.shape
     first = q
