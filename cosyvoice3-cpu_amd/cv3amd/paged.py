@@ -355,6 +355,8 @@ def free_pages(tables, lengths, page: int, pages: int, out=None):
     if tables.ndim != 2:
         raise ValueError(f"tables are (sequences, blocks), got {tables.shape}")
     rows, blocks = tables.shape
+    if pages < 1:
+        raise ValueError(f"a cache of {pages} pages")
     lengths, out = _in(lengths, _I32, "lengths", (rows,)), _outs(out, 2)
     free, count = _out(out[0], (pages,), _I32, "free"), _out(out[1], (1,), _I32, "count")
     _lib.call("paged_free", tables.ptr, rows, blocks, lengths.ptr, page, pages, free.ptr, count.ptr, None)

@@ -444,3 +444,46 @@ def test_calls_on_an_explicit_stream(gpu, paged):
     assert count.numpy()[0] == (~used_ref).sum() and used.numpy()[0] == used_ref.sum()
     for k, x in zip(want[3], new):
         assert np.array_equal(x.numpy()[:, :used_ref.sum()], k[:, used_ref])
+
+
+def test_two_graphs_with_scratch_of_their_own(gpu, paged):
+    """A compaction and an extension that splits its keys, each captured twice, replayed in turn over other contents with
+    eager calls between: no graph finds another's lists or parts."""
+    from cv3amd import device
+    rng = np.random.default_rng(12)
+    rows, blocks, page, kv, d, pages, h, n = 3, 300, 8, 2, 64, 1000, 4, 40
+    k, v = (dev(rng.normal(size=(pages, kv, page, d)).astype(np.float32)) for _ in range(2))
+    tables = [dev(rng.permutation(pages).astype(I32)[:rows * blocks].reshape(rows, blocks)) for _ in range(2)]
+    lengths = [dev(np.array(x, I32)) for x in ([2400, 100, 1999], [7, 2000, 0])]
+    starts, q = dev(np.array([0, 20, 40, 40], I32)), [dev(rng.normal(size=(n, h, d)).astype(np.float32)) for _ in range(2)]
+
+    def outs():
+        return dict(out=dev(np.zeros((n, h, d), np.float32)), k=dev(np.zeros((400, kv, page, d), np.float32)),
+                    v=dev(np.zeros((400, kv, page, d), np.float32)), t=dev(np.zeros((rows, blocks), I32)), used=dev(np.zeros(1, I32)))
+
+    def step(i, o):
+        paged.extend(q[i], k, v, tables[i], lengths[i], starts, out=o["out"])
+        paged.compact(tables[i], lengths[i], k, v, o["k"], o["v"], out=(o["t"], o["used"]))
+
+    def numbers(o):
+        return {name: x.numpy() for name, x in o.items()}
+
+    want, held, graphs = [], [outs(), outs()], []
+    for i in range(2):
+        o = outs()
+        step(i, o)
+        want.append(numbers(o))
+        assert 0 < int(want[i]["used"][0]) and not np.array_equal(want[0]["t"], np.zeros((rows, blocks)))
+    for i in range(2):
+        step(i, held[i])                         # so that the allocator has the scratch that the capture takes
+        graphs.append(device.Graph())
+        with graphs[i]:
+            step(i, held[i])
+    for i in (0, 1, 1, 0, 0, 1):
+        for name in ("out", "t", "used"):
+            held[i][name].copy_from(np.zeros_like(want[i][name]))
+        graphs[i].launch()
+        step(1 - i, outs())
+        got = numbers(held[i])
+        for name, x in want[i].items():
+            assert np.array_equal(got[name], x), (i, name)

@@ -125,3 +125,38 @@ def test_refusals(gpu):
                 dict(prompts=x, continuations=[[[1]]], cache="int8")):
         with pytest.raises(ValueError):
             d.score_batch(**bad)
+
+
+def test_the_objects_own_cache_is_left(gpu):
+    from cv3amd.qwen2 import DeviceQwen2
+    lm, store = setup("per_channel")
+    d = DeviceQwen2(store, cap=64)
+    rng = np.random.default_rng(27)
+    xs = prompts(rng, (20, 7))
+    d.prefill(xs[0], 0)
+    d.score_batch(xs, [tokens(rng, 5), tokens(rng, 3, 3)], 1)
+    assert d.generate_after_prefill(1, graph=False)[0] == int(logp(lm, xs[0], []).argmax())
+
+
+def test_two_calls_at_once(gpu):
+    """Two threads, each with its own stream, answer as a call alone."""
+    import threading
+    from cv3amd.qwen2 import DeviceQwen2
+    _, store = setup("per_channel")
+    d = DeviceQwen2(store, cap=64)
+    rng = np.random.default_rng(28)
+    xs = prompts(rng, (21, 8, 30))
+    texts = [tokens(rng, 9, 2), tokens(rng, 17), tokens(rng, 1, 30)]
+    got = [None, None]
+
+    def one(i):
+        got[i] = d.score_batch(xs, texts, 4)
+
+    threads = [threading.Thread(target=one, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for want, a, b in zip(d.score_batch(xs, texts, 4), *got):
+        for w, x, y in zip(want, a, b):
+            assert all(np.array_equal(i, j) and np.array_equal(i, k) for i, j, k in zip(w, x, y))

@@ -128,6 +128,8 @@ def test_python_checks_types_and_shapes():
         (ValueError, lambda: paged.free_pages(t, d((4,), i32), 16, 50)),
         (ValueError, lambda: paged.free_pages(t, n, 16, 50, out=(d((49,), i32), d((1,), i32)))),
         (TypeError, lambda: paged.free_pages(d((3, 4)), n, 16, 50)),
+        (ValueError, lambda: paged.free_pages(t, n, 16, 0)),
+        (ValueError, lambda: paged.free_pages(t, n, 16, -1)),
         (ValueError, lambda: paged.compact(t, n, k, v, d((5, 2, 8, 64)), d((5, 2, 8, 64)))),
         (ValueError, lambda: paged.compact(t, n, k, v, d((1, 5, 2, 16, 64)), d((1, 5, 2, 16, 64)))),
         (ValueError, lambda: paged.compact(t, n, k, v, d((5, 2, 16, 64), np.float16), d((5, 2, 16, 64), np.float16))),
