@@ -131,6 +131,10 @@ constexpr int kWaveRows = 32;       // (token, head) rows of a wave
 constexpr int kSplitSlots = 1024;   // tiles of rows whose keys may be shared out
 // Tables up to here are not worth a plan: 12 prompts of up to 900 tokens 50 us without, 90 with.
 constexpr int kWholeKeys = 1024;
+// And up to here where items nearly fill the machine and are taken in their order: 24 ragged slices of up to 300 queries over
+// 2300 keys (14 on 2 heads of 64, float32) 118 us planned, 95 whole; 2 prompts of 1500 over 3000 (20 on 4 of 80, bfloat16) 219
+// and 168; with half as many items (a prompt of 2000, 14 on 2 heads, float32) 63 and 80.
+constexpr int kOrderKeys = 4096;
 // Items from which their order counts, more than one a compute unit: 12 prompts of up to 900 tokens 66 us by slots, 50 with
 // the longest first, 16 of 1000 156 and 136; where all are alike (24 x 60 queries over 360 keys) 52 and 53.
 constexpr int kOrderItems = 256;
@@ -330,7 +334,7 @@ struct Shape {
 // d = 64, two workgroups a CU) the products with their operands take about half, exponentials and planes of the weights a
 // quarter, addresses and loads 750, barriers 430; float32 widens its tile for another 1000.  500 queries over 60501 keys
 // (14 on 2 heads, float16) 260 us, 420 TFLOP/s of 4 d flops a score: twice that in products, where a library's large
-// product of float16 reaches 1060.  12 slices of up to 800 over 5800 keys (32 on 8 heads of 128, bfloat16) 690 us, 385.
+// product of float16 reaches 1060.  12 slices of up to 800 over 5800 keys (32 on 8 heads of 128, bfloat16) 645 us, 415.
 template <typename E, int ND, bool FULL, int W>
 __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0, int t1, bool whole, float* part,
                                        float2* part_ml, typename Shape<E, ND, W>::Mem& mem) {
@@ -761,11 +765,13 @@ __device__ __forceinline__ int last_at(const int32_t* v, int n, int x) {
 // most `most` key tiles, a workgroup each.  `most` is the size with the least estimate of: no cut; the least of a few
 // sizes whose parts all run at once (`groups` do); half a workgroup's mean load.  A part is charged kPartCost tiles for
 // its start and end, and kCutCost more where it has to be joined (some 2 us a tile); what runs in several rounds half of
-// the largest part for the last.
+// the largest part for the last.  Where nothing is cut and items are more than run at once, they go by their size, the
+// largest first in kSizes steps, and the last round costs a step: 12 ragged slices of up to 800 queries over 5800 keys
+// (32 on 8 heads of 128, bfloat16) 700 us with the larger items cut in half, 645 so (640 in 16 or 32 steps).
 //
-// One workgroup, a thread a slot: 8 - 9.5 us, the chain of its loads, searches and sums.  (Done by every workgroup of
+// One workgroup, a thread a slot: 8 - 12 us, the chain of its loads, searches and sums.  (Done by every workgroup of
 // k_extend_split for itself it took 4 - 9 us of each, and registers of the products.)
-constexpr int kPlanThreads = kSplitSlots, kTries = 9, kPartCost = 2, kCutCost = 3;
+constexpr int kPlanThreads = kSplitSlots, kTries = 9, kPartCost = 2, kCutCost = 3, kSizes = 8;
 template <int KT, int W>
 __global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
   constexpr int kRows = kWaveRows * W, kWaves = kPlanThreads / 64, kSums = kTries + 1;
@@ -776,8 +782,11 @@ __global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
   __shared__ int32_t s_parts[kSplitSlots];
   __shared__ uint32_t s_red[kWaves][kSums];
   __shared__ uint64_t s_up[kWaves];
+  __shared__ int32_t s_tile[kSplitSlots];           // slots in their order
+  __shared__ int32_t s_size[kWaves][kSizes];
   __shared__ float s_load, s_items, s_inv;
   __shared__ uint32_t s_top;
+  __shared__ bool s_sort;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, slots = a.slots, hk = a.kv_heads;
   for (int b = tid; b < a.batch; b += kPlanThreads) s_slot[b] = first_slot<W>(a, b);
   __syncthreads();
@@ -832,16 +841,37 @@ __global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
       est = n <= groups ? size + cost : lane < kTries ? INFINITY : load + cost * n / groups + 0.5f * size;
       if (size >= top) est = INFINITY;
     } else if (lane == kSums) {
-      est = whole <= groups ? top + kPartCost : load + kPartCost * whole / groups + 0.5f * top;
+      est = whole <= groups ? top + kPartCost : fmaxf(top, load + top / kSizes) + kPartCost * whole / groups;
     }
     const float best = -wave_max_dpp(-est);
     const int pick = __ffsll((unsigned long long)__ballot(est == best)) - 1;
     size = __shfl(size, pick, kWave);
-    if (lane == 0) s_inv = 1.f / size;
+    if (lane == 0) s_inv = 1.f / size, s_sort = pick == kSums && whole > groups;
   }
   __syncthreads();
+  int parts = parts_of(mine, s_inv), slot = s;
+  if (s_sort) {
+    const int of = mine > 0 ? (int)((uint32_t)(s_top - mine) * (uint64_t)kSizes / s_top) : kSizes - 1;
+    int rank = 0;
+#pragma unroll
+    for (int i = 0; i < kSizes; ++i) {
+      const uint64_t m = __ballot(of == i);
+      if (lane == 0) s_size[wv][i] = __popcll(m);
+      if (of == i) rank = __popcll(m & (((uint64_t)1 << lane) - 1));
+    }
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+      for (int i = 0; i < kSizes; ++i)
+        if (i < of || (i == of && w < wv)) rank += s_size[w][i];
+    s_tile[rank] = s;
+    s_parts[rank] = parts;
+    __syncthreads();
+    slot = s_tile[tid], parts = s_parts[tid];
+    __syncthreads();
+  }
+  s_tile[tid] = slot;
   // parts, parts of cut items, and cut items of the slots ahead, 21 bits each: there are at most 2^10 and 3 groups
-  const int parts = parts_of(mine, s_inv);
   const uint64_t n = parts > 1 ? (uint64_t)parts | (uint64_t)parts << 21 | (uint64_t)1 << 42 : (uint64_t)parts;
   uint64_t up = n;
 #pragma unroll
@@ -864,7 +894,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
   const int count = min((int)(all & kField) * hk, a.pieces_most);
   if (tid == 0) a.counts[0] = min((int)(all >> 42) * hk, a.cuts_most), a.counts[1] = count;
   for (int w = tid; w < count; w += kPlanThreads) {
-    const int at = last_at(s_pieces, min(slots, kSplitSlots), w), slot = slots - 1 - at, b = last_at(s_slot, a.batch, slot);
+    const int at = last_at(s_pieces, min(slots, kSplitSlots), w), slot = s_tile[at], b = last_at(s_slot, a.batch, slot);
     const int of = s_parts[at], in = w - s_pieces[at], kvh = in / of, part = in - kvh * of, place = s_places[at] + in;
     const int cut = s_cuts[at] + kvh;
     Piece one{b, kvh, slot - s_slot[b], part, of, place, {0, 0}};
@@ -875,7 +905,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
 }
 
 // Of a cut item each workgroup leaves its rows' outputs, maxima and sums (`part`, `part_ml`).  The two cases named at
-// `attend`: 254 - 270 and 688 - 745 us, beside them the plan and 8 and 38 us of joins.
+// `attend`: 243 - 270 and 676 - 730 us traced, beside them the plan and 8 and 5 us of joins.
 template <typename E, int ND, bool FULL, int W>
 __global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_split(ExtArgs a) {
   typedef Shape<E, ND, W> S;
@@ -916,7 +946,7 @@ __global__ __launch_bounds__(64, (simd_waves<E, ND>())) void k_extend_few(ExtArg
 
 // The parts of an item's rows.  A wave reads four channels a lane, so several parts at a time, then joins its lanes; with
 // many parts the waves share them, with few each takes rows of its own.  parts 0: the items are those of `cuts`.  Bound by
-// the parts' bytes: 38 us for some 100 MB (12 ragged slices, 32 heads of 128).
+// the parts' bytes: 38 us for some 100 MB, 8 for 500 queries in 14 heads over 60501 keys, 4.3 for 4.
 constexpr int kJoinAhead = 4, kJoinFew = 32, kJoinGroups = 2048;
 template <int LP, int W>                         // lanes of a part: a power of two with 4 LP >= d
 __global__ __launch_bounds__(256) void k_extend_join(ExtArgs a, int parts, int rows) {
@@ -1067,8 +1097,10 @@ int run_tiles(ExtArgs a, hipStream_t st) {
   } else {
     a.slots = (int)(rows / (kWaveRows * W) + a.batch);
     const int64_t items = (int64_t)a.slots * a.kv_heads;
-    if (a.slots <= kSplitSlots && cap > (few ? kWholeKeys / 4 : kWholeKeys)) {
-      a.groups = kAtOnce / W;
+    a.groups = kAtOnce / W;
+    const bool ordered = a.batch <= 64;
+    const int64_t whole = few ? kWholeKeys / 4 : ordered && 4 * items >= 3 * a.groups ? kOrderKeys : kWholeKeys;
+    if (a.slots <= kSplitSlots && cap > whole) {
       a.part_rows = (int)std::min<int64_t>(kWaveRows * W, rows);
       // parts of no more than half a mean load: items and 2 groups of them, 4 groups of those in cut items
       a.pieces_most = (int)items + 2 * a.groups;
@@ -1087,7 +1119,7 @@ int run_tiles(ExtArgs a, hipStream_t st) {
       launch_join<ND, W>(a, a.cuts_most, 0, st);
     } else {                           // short tables, very many tiles, or no memory: one workgroup an item
       hipLaunchKernelGGL((k_extend_whole<E, ND, FULL, W>), dim3((unsigned)items), dim3(64 * W), 0, st, a,
-                         a.batch > 1 && a.batch <= 64 && items > kOrderItems);
+                         ordered && a.batch > 1 && items > kOrderItems);
     }
   }
   const hipError_t err = hipGetLastError();

@@ -157,6 +157,17 @@ def test_extend_many_tiles_of_short_tables(paged, h, kv, d, kind):
         check(paged, rng.integers(0, 30, batch), rng.integers(0, 100, batch), h, kv, d, 16, kind, seed=batch)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+def test_extend_of_planned_sequences_in_their_order(paged, kind):
+    """More items than run at once, over tables past those that go without a plan: uncut, the largest first; with one
+    sequence so long that it is cut; and with windows, which leave nearly equal items."""
+    new, held = [300, 0, 7, 260, 300, 130, 1, 300, 40], [4200, 5, 0, 1000, 0, 2500, 300, 3000, 64]
+    check(paged, new, held, 48, 16, 64, 32, kind, pad=(2, 3))
+    check(paged, [200] * 6 + [60], [0] * 6 + [20000], 64, 16, 64, 64, kind)
+    check(paged, new, held, 48, 16, 64, 32, kind, window=200)
+    check(paged, [30] * 70, [50] * 69 + [4500], 32, 16, 64, 16, kind)          # more sequences than are ordered by lane
+
+
 def test_extend_scales(paged):
     """Any scale: none, negative, large; scores of hundreds."""
     for kind in TYPES:
