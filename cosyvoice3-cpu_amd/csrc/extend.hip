@@ -36,7 +36,7 @@ struct ExtArgs {
   float2* part_ml;             // [places][rows of a tile]: their maxima and sums
   struct Piece* pieces;        // parts of items, a workgroup each
   struct Piece* cuts;          // the first part of every item that has several
-  int* counts;                 // of cuts and pieces
+  int* counts;                 // of cuts and pieces; whether these are sorted
   int groups, part_rows, pieces_most, places, cuts_most;
 };
 
@@ -131,10 +131,11 @@ constexpr int kWaveRows = 32;       // (token, head) rows of a wave
 constexpr int kSplitSlots = 1024;   // tiles of rows whose keys may be shared out
 // Tables up to here are not worth a plan: 12 prompts of up to 900 tokens 50 us without, 90 with.
 constexpr int kWholeKeys = 1024;
-// And up to here where items nearly fill the machine and are taken in their order: 24 ragged slices of up to 300 queries over
-// 2300 keys (14 on 2 heads of 64, float32) 118 us planned, 95 whole; 2 prompts of 1500 over 3000 (20 on 4 of 80, bfloat16) 219
-// and 168; with half as many items (a prompt of 2000, 14 on 2 heads, float32) 63 and 80.
-constexpr int kOrderKeys = 4096;
+// And up to here where items nearly fill the machine and are taken in their order: 8 ragged prompts of up to 2000 tokens (14
+// on 2 heads of 64, float32) 117 us planned, 99 whole.  Further up one long sequence among short ones would be the last by
+// far (a slice of 500 over 4000 keys among 16 prompts of 500: 100 planned, 160 whole), with fewer items the machine is not
+// full (a prompt of 2000: 63 and 80).
+constexpr int kOrderKeys = 2048;
 // Items from which their order counts, more than one a compute unit: 12 prompts of up to 900 tokens 66 us by slots, 50 with
 // the longest first, 16 of 1000 156 and 136; where all are alike (24 x 60 queries over 360 keys) 52 and 53.
 constexpr int kOrderItems = 256;
@@ -334,7 +335,7 @@ struct Shape {
 // d = 64, two workgroups a CU) the products with their operands take about half, exponentials and planes of the weights a
 // quarter, addresses and loads 750, barriers 430; float32 widens its tile for another 1000.  500 queries over 60501 keys
 // (14 on 2 heads, float16) 260 us, 420 TFLOP/s of 4 d flops a score: twice that in products, where a library's large
-// product of float16 reaches 1060.  12 slices of up to 800 over 5800 keys (32 on 8 heads of 128, bfloat16) 645 us, 415.
+// product of float16 reaches 1060.  12 slices of up to 800 over 5800 keys (32 on 8 heads of 128, bfloat16) 650 us, 410.
 template <typename E, int ND, bool FULL, int W>
 __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0, int t1, bool whole, float* part,
                                        float2* part_ml, typename Shape<E, ND, W>::Mem& mem) {
@@ -765,13 +766,16 @@ __device__ __forceinline__ int last_at(const int32_t* v, int n, int x) {
 // most `most` key tiles, a workgroup each.  `most` is the size with the least estimate of: no cut; the least of a few
 // sizes whose parts all run at once (`groups` do); half a workgroup's mean load.  A part is charged kPartCost tiles for
 // its start and end, and kCutCost more where it has to be joined (some 2 us a tile); what runs in several rounds half of
-// the largest part for the last.  Where nothing is cut and items are more than run at once, they go by their size, the
-// largest first in kSizes steps, and the last round costs a step: 12 ragged slices of up to 800 queries over 5800 keys
-// (32 on 8 heads of 128, bfloat16) 700 us with the larger items cut in half, 645 so (640 in 16 or 32 steps).
+// the largest part for the last.  A tile takes kAlone of its time in a workgroup that shares its CU with none, which is how
+// long items end.  Where nothing is cut, and items are more than run at once or the largest kUneven of their mean, they go by
+// size, the largest first in kSizes steps: 12 ragged slices of up to 800 queries over 5800 keys (32 on 8 heads of 128,
+// bfloat16) 710 us with the larger items cut in half, 655 so; the same of float16, 14 on 2 heads of 64, 188 and 176, but 248
+// uncut by slots.  4 slices of 500 over 2500 (20 on 4 heads of 80, float32), nearly alike, lose by it: 200 and 219.
 //
 // One workgroup, a thread a slot: 8 - 12 us, the chain of its loads, searches and sums.  (Done by every workgroup of
 // k_extend_split for itself it took 4 - 9 us of each, and registers of the products.)
 constexpr int kPlanThreads = kSplitSlots, kTries = 9, kPartCost = 2, kCutCost = 3, kSizes = 8;
+constexpr float kAlone = 0.55f, kUneven = 1.25f;
 template <int KT, int W>
 __global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
   constexpr int kRows = kWaveRows * W, kWaves = kPlanThreads / 64, kSums = kTries + 1;
@@ -841,12 +845,12 @@ __global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
       est = n <= groups ? size + cost : lane < kTries ? INFINITY : load + cost * n / groups + 0.5f * size;
       if (size >= top) est = INFINITY;
     } else if (lane == kSums) {
-      est = whole <= groups ? top + kPartCost : fmaxf(top, load + top / kSizes) + kPartCost * whole / groups;
+      est = fmaxf(kAlone * top, whole <= groups ? load : load + top / kSizes) + kPartCost * fmaxf(whole / groups, 1.f);
     }
     const float best = -wave_max_dpp(-est);
     const int pick = __ffsll((unsigned long long)__ballot(est == best)) - 1;
     size = __shfl(size, pick, kWave);
-    if (lane == 0) s_inv = 1.f / size, s_sort = pick == kSums && whole > groups;
+    if (lane == 0) s_inv = 1.f / size, s_sort = pick == kSums && (whole > groups || top * whole > kUneven * load * groups);
   }
   __syncthreads();
   int parts = parts_of(mine, s_inv), slot = s;
@@ -892,7 +896,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
   s_parts[tid] = parts;
   __syncthreads();
   const int count = min((int)(all & kField) * hk, a.pieces_most);
-  if (tid == 0) a.counts[0] = min((int)(all >> 42) * hk, a.cuts_most), a.counts[1] = count;
+  if (tid == 0) a.counts[0] = min((int)(all >> 42) * hk, a.cuts_most), a.counts[1] = count, a.counts[2] = s_sort;
   for (int w = tid; w < count; w += kPlanThreads) {
     const int at = last_at(s_pieces, min(slots, kSplitSlots), w), slot = s_tile[at], b = last_at(s_slot, a.batch, slot);
     const int of = s_parts[at], in = w - s_pieces[at], kvh = in / of, part = in - kvh * of, place = s_places[at] + in;
@@ -910,10 +914,11 @@ template <typename E, int ND, bool FULL, int W>
 __global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_split(ExtArgs a) {
   typedef Shape<E, ND, W> S;
   __shared__ typename S::Mem mem;
-  // pieces that follow each other share keys: they go to one XCD's L2 where all run at once
+  // pieces that follow each other share keys: they go to one XCD's L2 where all run at once and are alike
   const int count = a.counts[1], eighth = (count + 7) / 8, in_eighth = (int)(blockIdx.x / 8);
-  const int w = count <= a.groups ? (int)(blockIdx.x % 8) * eighth + in_eighth : (int)blockIdx.x;
-  if (w >= count || (count <= a.groups && in_eighth >= eighth)) return;
+  const bool runs = count <= a.groups && !a.counts[2];
+  const int w = runs ? (int)(blockIdx.x % 8) * eighth + in_eighth : (int)blockIdx.x;
+  if (w >= count || (runs && in_eighth >= eighth)) return;
   const Piece p = a.pieces[w];
   Item it;
   const int parts = uniform(p.parts), part = uniform(p.part);

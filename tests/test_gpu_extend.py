@@ -165,6 +165,7 @@ def test_extend_of_planned_sequences_in_their_order(paged, kind):
     check(paged, new, held, 48, 16, 64, 32, kind, pad=(2, 3))
     check(paged, [200] * 6 + [60], [0] * 6 + [20000], 64, 16, 64, 64, kind)
     check(paged, new, held, 48, 16, 64, 32, kind, window=200)
+    check(paged, [250, 100, 250, 30], [2100, 0, 1500, 60], 32, 16, 64, 32, kind)            # fewer, uneven and uncut
     check(paged, [30] * 70, [50] * 69 + [4500], 32, 16, 64, 16, kind)          # more sequences than are ordered by lane
 
 
