@@ -63,7 +63,12 @@ __global__ __launch_bounds__(kThreads) void k_fork(ForkArgs a) {
   const int32_t* from = a.tables + (int64_t)(p < (uint32_t)a.rows ? p : 0) * a.blocks;
   const int32_t source = rest ? from[full] : -1;
   uint32_t ps[kForksEach], cs[kForksEach];
-  int part[kForksEach];
+  int keys[kForksEach];
+  bool part[kForksEach];
+  // a part-filled last page is copied, and takes a page, if it is there: of an absent one a child has no keys either
+  auto last = [&](uint32_t fp, int n) {
+    return n % a.page ? (uint32_t)a.tables[(int64_t)fp * a.blocks + n / a.page] : ~0u;
+  };
   const bool once = a.forks <= kForksEach * kThreads;
 #pragma unroll
   for (int e = 0; e < kForksEach; ++e) {
@@ -72,7 +77,9 @@ __global__ __launch_bounds__(kThreads) void k_fork(ForkArgs a) {
     cs[e] = f < a.forks ? (uint32_t)a.children[f] : ~0u;
   }
 #pragma unroll
-  for (int e = 0; e < kForksEach; ++e) part[e] = ps[e] < (uint32_t)a.rows ? held_of(a.lengths, ps[e], a.blocks, a.page) % a.page : 0;
+  for (int e = 0; e < kForksEach; ++e) keys[e] = ps[e] < (uint32_t)a.rows ? held_of(a.lengths, ps[e], a.blocks, a.page) : 0;
+#pragma unroll
+  for (int e = 0; e < kForksEach; ++e) part[e] = last(ps[e], keys[e]) < (uint64_t)a.pages;
   auto enter = [&](uint32_t fp, uint32_t fc) {
     if (fp < (uint32_t)a.rows) atomicOr(&parent[fp >> 5], 1u << (fp & 31));
     if (fc < (uint32_t)a.rows && atomicOr(&child[fc >> 5], 1u << (fc & 31)) >> (fc & 31) & 1)
@@ -86,8 +93,8 @@ __global__ __launch_bounds__(kThreads) void k_fork(ForkArgs a) {
     return fp < (uint32_t)a.rows && fc < (uint32_t)a.rows && !((parent[fc >> 5] | again[fc >> 5]) >> (fc & 31) & 1);
   };
   int before = 0, all = 0;
-  auto count = [&](int f, uint32_t fp, uint32_t fc, int rows_of_last) {
-    if (rows_of_last && made(fp, fc)) {
+  auto count = [&](int f, uint32_t fp, uint32_t fc, bool takes) {
+    if (takes && made(fp, fc)) {
       ++all;
       if (f < i) ++before;
     }
@@ -97,7 +104,8 @@ __global__ __launch_bounds__(kThreads) void k_fork(ForkArgs a) {
   if (!once)
     for (int f = tid + kForksEach * kThreads; f < a.forks; f += kThreads) {
       const uint32_t fp = (uint32_t)a.parents[f];
-      count(f, fp, (uint32_t)a.children[f], fp < (uint32_t)a.rows ? held_of(a.lengths, fp, a.blocks, a.page) % a.page : 0);
+      const int n = fp < (uint32_t)a.rows ? held_of(a.lengths, fp, a.blocks, a.page) : 0;
+      count(f, fp, (uint32_t)a.children[f], last(fp, n) < (uint64_t)a.pages);
     }
   if (before) atomicAdd(&s_before, before);
   if (all) atomicAdd(&s_all, all);
@@ -106,14 +114,14 @@ __global__ __launch_bounds__(kThreads) void k_fork(ForkArgs a) {
   if (blockIdx.x == 0 && i == 0 && tid == 0) a.taken_out[0] = (int32_t)min(taken + s_all, (int64_t)INT32_MAX);
   if (!made(p, c)) return;
   const int64_t at = taken + s_before;
-  const int32_t to = rest && at >= 0 && at < a.free_count ? a.free_pages[at] : -1;
+  const bool takes = (uint32_t)source < (uint64_t)a.pages;
+  const int32_t to = takes && at >= 0 && at < a.free_count ? a.free_pages[at] : -1;
   if (blockIdx.x == 0) {
     for (int64_t b = tid; b < a.blocks; b += kThreads)
       a.tables[(int64_t)c * a.blocks + b] = b < full ? from[b] : b == full ? to : -1;
     if (tid == 0) a.lengths[c] = len;
   }
-  if (!rest) return;
-  if ((uint32_t)source >= (uint64_t)a.pages || (uint32_t)to >= (uint64_t)a.pages || source == to) return;
+  if (!takes || (uint32_t)to >= (uint64_t)a.pages || source == to) return;
   // rows [0, rest) of every (layer, kv head, k or v): runs that follow each other, 16 bytes a thread
   const uint32_t run = (uint32_t)rest * a.row_vecs, runs = (uint32_t)(a.layers * 2 * a.kv_heads);
   const int64_t head_vecs = (int64_t)a.page * a.row_vecs, page_vecs = head_vecs * a.kv_heads;

@@ -325,8 +325,9 @@ def fork(parents, children, tables: DeviceArray, lengths: DeviceArray, free, tak
     becomes row ``parents[i]``.  Whole pages are shared; the rows of a part-filled last page are copied into a page of
     the child's own, the next of the page ids ``free`` from index ``taken[0]`` on, forks in order, in every layer of the
     caches (layers, pages, kv heads, page, dim), or (pages, kv heads, page, dim).  Returns the pages taken so far, more
-    than ``len(free)`` where they ran out (the child's entry is then -1).  Children are distinct and no parents of the
-    call; a fork whose child is, or whose rows do not exist, is not made."""
+    than ``len(free)`` where they ran out (the child's entry is then -1).  A part-filled page that the parent lists as
+    absent is absent (-1) for the child too, and takes no page.  Children are distinct and no parents of the call; a fork
+    whose child is, or whose rows do not exist, is not made."""
     kind, layers, pages, kv_heads, page, d = _layered(k_cache, v_cache)
     if not isinstance(tables, DeviceArray) or tables.ndim != 2:
         raise TypeError("tables is a DeviceArray (sequences, blocks)")

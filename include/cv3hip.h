@@ -641,8 +641,9 @@ int cv3_token_logprobs(const float* logits, int64_t rows, int64_t vocab, const i
 /* Sequences that go on from others: of tables [rows, blocks] and lengths [rows], row children[i] becomes row parents[i].
  * Whole pages are shared; a part-filled last page's rows are copied, in every layer of the cache [layers, pages,
  * kv_heads, page, d], into a page of its own, the next of free_pages from index *taken on, forks in order (where they
- * run out its entry is -1); entries behind are -1.  taken_out: the pages taken so far, more than free_count where they
- * ran out.  A fork is not made, and takes no page, if parent or child is no row, if the child is a parent of the
+ * run out its entry is -1); entries behind are -1.  A part-filled last page that is absent (an id outside the cache) takes
+ * no page and is -1 in the child's table: what its parent does not see it does not see either.  taken_out: the pages taken
+ * so far, more than free_count where they ran out.  A fork is not made, and takes no page, if parent or child is no row, if the child is a parent of the
  * call, or if another fork names the same child.  At most 4096 forks and 65536 rows. */
 int cv3_paged_fork(const int32_t* parents, const int32_t* children, int64_t forks, int32_t* tables, int64_t rows,
                    int64_t blocks, int32_t* lengths, const int32_t* free_pages, int64_t free_count,

@@ -152,6 +152,72 @@ def test_fork_many(paged):
     assert all(np.array_equal(k.numpy(), w) for k, w in zip(kd, want_k))
 
 
+def absent_last(tables, lengths, page, pages):
+    """Which sequences have a part-filled last page whose id lies outside the cache."""
+    n = np.array([held(x, tables.shape[1], page) for x in lengths])
+    last = tables[np.arange(len(n)), np.minimum(n // page, tables.shape[1] - 1)]
+    return (n % page > 0) & ((last < 0) | (last >= pages))
+
+
+def test_fork_of_a_part_filled_page_that_is_absent(paged):
+    """A child sees what its parent sees: of a part-filled page that is not there, nothing, whatever an ended sequence
+    left in the page that would be next; such a fork takes no page, and the others' pages follow each other."""
+    rng = np.random.default_rng(13)
+    rows, blocks, page, kv, d, h = 12, 4, 16, 2, 64, 4
+    for kind in TYPES:
+        tables, lengths, free, pages = sequences(rng, rows, blocks, page, 12)
+        ks = caches(rng, 1, pages, kv, page, d, kind)
+        lengths[:5] = [37, 40, 20, 9, 60]
+        tables[:5] = rng.permutation(np.setdiff1d(np.arange(pages), free))[:20].reshape(5, blocks)
+        tables[0, 2], tables[1, 2], tables[3, 0] = -1, pages, 2**31 - 1
+        assert absent_last(tables, lengths, page, pages)[:5].tolist() == [True, True, False, True, False]
+        for c in ks:                                            # what ended sequences left in the free pages: NaN
+            c[:, free] = stored(np.full(c[:, free].shape, np.nan), kind)[0]
+        parents, children = [0, 4, 1, 2, 3, 0, 4], [5, 6, 7, 8, 9, 10, 11]
+        want_t, want_n, taken = tables.copy(), lengths.copy(), 1
+        for p, c in zip(parents, children):
+            full = lengths[p] // page
+            want_t[c], want_n[c] = -1, lengths[p]
+            want_t[c, :full] = tables[p, :full]
+            if p in (2, 4):
+                want_t[c, full] = free[taken]
+                taken += 1
+        td, nd, kd = dev(tables), dev(lengths), [dev(k) for k in ks]
+        got = paged.fork(np.array(parents, I32), np.array(children, I32), td, nd, free, np.array([1], I32), *kd)
+        assert got[0] == taken == 4 and np.array_equal(td.numpy(), want_t) and np.array_equal(nd.numpy(), want_n)
+        q = rng.normal(size=(1, h, d)).astype(np.float32).repeat(rows, 0)
+        out = paged.attention(q, *(k.reshape(k.shape[1:]) for k in kd), td, nd)
+        assert np.isfinite(out[children]).all() and np.array_equal(out[children], out[parents])
+
+
+def test_fork_of_rows_that_cannot_be_but_for_absent_pages(paged):
+    """The calls of ``test_fork_of_rows_that_cannot_be`` with sequences whose part-filled page is there."""
+    rng = np.random.default_rng(2)
+    rows, blocks, page = 40, 4, 16
+    tables, lengths, free, pages = sequences(rng, rows, blocks, page, 30)
+    ks = caches(rng, 2, pages, 2, page, 64, "float16")
+    lengths[:20] = rng.integers(1, 63, 20)
+    tables[:20] = rng.choice(np.setdiff1d(np.arange(pages), free), (20, blocks))
+
+    def calls():
+        assert not absent_last(tables, lengths, page, pages)[:20].any()
+        check_fork(paged, [0, 1, 2, 3, 4], [30, 0, 31, 31, 32], tables, lengths, free, 0, ks)
+        check_fork(paged, [0, -1, 2, 40, 4, 5], [30, 31, -7, 33, 40, 34], tables, lengths, free, 0, ks)
+        check_fork(paged, [0, 0, 0], [0, 5, 5], tables, lengths, free, 0, ks)
+        check_fork(paged, [7] * 6, [20, 21, 20, 22, 20, 23], tables, lengths, free, 3, ks)
+        check_fork(paged, [3, 4, 5, 6], [30, 31, 32, 33], tables, lengths, free, 0, ks)
+        check_fork(paged, [8, 9], [30, 31], tables, lengths, free, -1, ks)
+        check_fork(paged, [8, 9], [30, 31], tables, lengths, free, 2**31 - 1, ks)
+        check_fork(paged, [8, 9], [30, 31], tables, lengths, np.array([pages, -3]), 0, ks)      # pages outside the cache
+        check_fork(paged, [8, 9], [30, 31], tables, lengths, np.zeros(0), 0, ks)
+        check_fork(paged, [], [], tables, lengths, free, 5, ks)
+
+    calls()
+    lengths[3], lengths[4], lengths[5] = -9, 2**31 - 1, 1000
+    tables[6, :2], lengths[6] = [-1, 2**31 - 1], 37                 # whole pages that are absent are shared as they stand
+    calls()
+
+
 # ------------------------------------------------------------------------------------------------
 # free pages
 # ------------------------------------------------------------------------------------------------
