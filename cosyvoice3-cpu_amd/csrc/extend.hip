@@ -57,13 +57,27 @@ __device__ __forceinline__ Seq seq_of(const ExtArgs& a, int b) {
 }
 
 // One query over keys [lo, hi) by one wave, in float32 throughout: a key a lane for the scores, four channels a lane
-// for the sum.  Outputs are summed and then divided.
+// for the sum.
 template <typename E>
 struct RowSum {
   float o[4], top, sum;
   bool there;                  // a key, whatever its score
 
+  // The outputs, divided; sums of values near the largest float, which leave its range, once more with values 2^-40 down.
   __device__ __forceinline__ void run(const ExtArgs& a, int b, int kvh, const float* q, int lo, int hi) {
+    sums(a, b, kvh, q, lo, hi, 1.f);
+    float up = 1.f;
+    bool out = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out = out || !(fabsf(o[i]) < INFINITY);
+    if (__any(out) && sum < INFINITY) {
+      sums(a, b, kvh, q, lo, hi, 0x1p-40f);
+      up = 0x1p40f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = o[i] / sum * up;
+  }
+  __device__ __forceinline__ void sums(const ExtArgs& a, int b, int kvh, const float* q, int lo, int hi, float down) {
     const int lane = threadIdx.x & 63;
     const int32_t* table = a.tables + (int64_t)b * a.blocks;
 #pragma unroll
@@ -110,7 +124,7 @@ struct RowSum {
         const E* vr = (const E*)a.v + uniform(__shfl(off, j, kWave));
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (64 * i + lane < a.d) o[i] = fmaf(w, to_float(vr[64 * i + lane]), o[i]);
+          if (64 * i + lane < a.d) o[i] = fmaf(w, to_float(vr[64 * i + lane]) * down, o[i]);
       }
     }
     sum = wave_sum(sum);
@@ -718,7 +732,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     float* to = whole ? a.out + (int64_t)r_tok * a.ldo + (int64_t)r_head * d : part + (int64_t)(wv * kWaveRows + r) * d;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (64 * i + lane < d) to[64 * i + lane] = !x.there || (none && !whole) ? 0.f : x.o[i] / x.sum;
+      if (64 * i + lane < d) to[64 * i + lane] = !x.there || (none && !whole) ? 0.f : x.o[i];
     if (!whole && lane == 0) part_ml[wv * kWaveRows + r] = make_float2(none ? kNoScore : x.top, x.sum * 0x1p10f);
   }
 }
@@ -998,25 +1012,32 @@ __global__ __launch_bounds__(256) void k_extend_join(ExtArgs a, int parts, int r
         float now = top;
 #pragma unroll
         for (int u = 0; u < kJoinAhead; ++u) now = fmaxf(now, ml[u].x);
-        const float f = weight_of(top, now);
-        sum *= f;
+        // x is a mean, so that values near the largest float stay in its range
+        const float f = weight_of(top, now) * sum;
+        float g[kJoinAhead];
+        sum = f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x.v[j] *= f;
+        for (int u = 0; u < kJoinAhead; ++u) {
+          g[u] = ml[u].x != -INFINITY ? weight_of(ml[u].x, now) * ml[u].y : 0.f;
+          sum += g[u];
+        }
+        const float one = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.v[j] *= f * one;
 #pragma unroll
         for (int u = 0; u < kJoinAhead; ++u)
           if (ml[u].x != -INFINITY) {
-            const float g = weight_of(ml[u].x, now) * ml[u].y;
-            sum += g;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x.v[j] += g * y[u].v[j];
+            for (int j = 0; j < 4; ++j) x.v[j] += g[u] * one * y[u].v[j];
           }
         top = now;
       }
       auto join = [&](float t, float l, const f32x4u& o) {
-        const float now = fmaxf(top, t), f = weight_of(top, now), g = weight_of(t, now);
-        sum = f * sum + g * l;
+        const float now = fmaxf(top, t), f = weight_of(top, now) * sum, g = weight_of(t, now) * l;
+        sum = f + g;
+        const float one = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x.v[j] = f * x.v[j] + g * o.v[j];
+        for (int j = 0; j < 4; ++j) x.v[j] = f * one * x.v[j] + g * one * o.v[j];
         top = now;
       };
 #pragma unroll
@@ -1047,7 +1068,7 @@ __global__ __launch_bounds__(256) void k_extend_join(ExtArgs a, int parts, int r
       }
       if (sub == 0 && c4 < a.d) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x.v[j] = top != -INFINITY ? x.v[j] / sum : 0.f;
+        for (int j = 0; j < 4; ++j) x.v[j] = top == -INFINITY ? 0.f : sum == 0.f ? NAN : x.v[j];
         *(f32x4u*)(out + c4) = x;
       }
     }

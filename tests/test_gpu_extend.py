@@ -306,6 +306,62 @@ def test_extend_of_scores_that_are_all_minus_infinity(paged, h, kv, d, kind):
     assert rel_err(got[fine], want[fine]) <= TOL
 
 
+# (new, held) a sequence: a workgroup an item, few rows, items that a plan cuts
+FORMS = {"whole": ([200, 30], [100, 0]), "few": ([5, 1, 3], [900, 20, 40]), "cut": ([130, 2, 40], [6000, 0, 1500])}
+
+
+def spoil_last(rng, ins, kind, where, h=14):
+    """The last token of every sequence spoilt in its key or value, which the others do not see: (k, v, k64, v64, rows that
+    see none of it).  The others' tiles that hold it are formed again, their other parts are not."""
+    q, ks, vs, tables, lengths, starts = ins
+    page = ks.shape[2]
+    k, v = (np.array(values(x, kind), np.float32) for x in (ks, vs))
+    clear = np.ones(len(q), bool)
+    for b in range(len(lengths)):
+        at = lengths[b] - 1
+        (k if where == "k" else v)[tables[b, at // page], :, at % page, 3] = np.inf if b % 2 else np.nan
+        clear[starts[b + 1] - 1] = False
+    (ks, k64), (vs, v64) = stored(k, kind), stored(v, kind)
+    return ks, vs, k64, v64, clear
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("spoilt", [None, "k", "v"])
+def test_extend_values_near_the_largest(paged, spoilt, kind, form):
+    """Means of values up to 3e38 have their size: no sum on the way there leaves float32's range, of parts that are joined
+    and of rows that are formed again neither."""
+    rng = np.random.default_rng(21)
+    ins, _ = make(rng, *FORMS[form], 14, 2, 64, 16, kind)
+    ins = list(ins)
+    ins[0] *= np.float32(0.1)                               # many keys of like weight
+    ins[2] = stored(3e38 * rng.uniform(0.5, 1.0, ins[2].shape), kind)[0]
+    if spoilt:
+        ks, vs, k64, v64, clear = spoil_last(rng, ins, kind, spoilt)
+    else:
+        ks, vs, clear = ins[1], ins[2], np.ones(len(ins[0]), bool)
+        k64, v64 = (values(x, kind).astype(np.float64) for x in (ks, vs))
+    got = paged.extend(ins[0], dev(ks), dev(vs), *ins[3:])
+    want = extend_ref(ins[0], k64, v64, *ins[3:], None, 0.125, np.zeros_like(ins[0]))
+    assert np.abs(want[clear]).min() > 1.4e38 and np.isfinite(got[clear]).all()
+    assert rel_err(got[clear], want[clear]) <= TOL
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("h,kv,d", [(14, 2, 64), (4, 2, 128)])
+@pytest.mark.parametrize("spoilt", ["k", "v"])
+def test_extend_of_parts_formed_again_beside_others(paged, spoilt, h, kv, d, kind, form):
+    """A row whose last keys lie in a spoilt tile, and the others in clean ones: what is formed again there and what comes
+    from the matrix cores elsewhere weigh alike, since scores are small and every key counts."""
+    rng = np.random.default_rng([22, d])
+    ins, _ = make(rng, *FORMS[form], h, kv, d, 16, kind, sharp=0.3)
+    ks, vs, k64, v64, clear = spoil_last(rng, ins, kind, spoilt)
+    got = paged.extend(ins[0], dev(ks), dev(vs), *ins[3:])
+    want = extend_ref(ins[0], k64, v64, *ins[3:], None, 1 / np.sqrt(d), np.zeros_like(ins[0]))
+    assert np.isfinite(got[clear]).all() and rel_err(got[clear], want[clear]) <= TOL
+
+
 def test_extend_lengths_past_the_table(paged):
     """A length past its table counts as the table's end; more new tokens than keys: those before position 0 see nothing."""
     rng = np.random.default_rng(11)
