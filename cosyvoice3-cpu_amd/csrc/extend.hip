@@ -65,17 +65,17 @@ struct RowSum {
 
   // The outputs, divided; sums of values near the largest float, which leave its range, once more with values 2^-40 down.
   __device__ __forceinline__ void run(const ExtArgs& a, int b, int kvh, const float* q, int lo, int hi) {
-    sums(a, b, kvh, q, lo, hi, 1.f);
-    float up = 1.f;
-    bool out = false;
+    float down = 1.f;
+#pragma unroll 1
+    for (;; down = 0x1p-40f) {
+      sums(a, b, kvh, q, lo, hi, down);
+      bool out = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out = out || !(fabsf(o[i]) < INFINITY);
-    if (__any(out) && sum < INFINITY) {
-      sums(a, b, kvh, q, lo, hi, 0x1p-40f);
-      up = 0x1p40f;
+      for (int i = 0; i < 4; ++i) out = out || !(fabsf(o[i]) < INFINITY);
+      if (down != 1.f || !(__any(out) && sum < INFINITY)) break;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] / sum * up;
+    for (int i = 0; i < 4; ++i) o[i] = o[i] / sum / down;
   }
   __device__ __forceinline__ void sums(const ExtArgs& a, int b, int kvh, const float* q, int lo, int hi, float down) {
     const int lane = threadIdx.x & 63;
@@ -157,9 +157,9 @@ constexpr int kOrderItems = 256;
 // For d > 64 one wave fetches too slowly (8 x 9 queries over 709 keys, 4 heads of 128 a kv head, 65 us against 35).
 constexpr int kFewRows = 48;
 
-// Weights are held 2^10 up against a reference that a row's largest score has passed by so little that the 32 of a lane
-// sum to no more than kMost, which float16 holds; so small planes end 2^-35 below the largest weight or lower.
-constexpr float kUp = 10.f, kMost = 60000.f;
+// Weights are held 2^12 up against a reference that a row's largest score has passed by so little that no eight of them sum
+// to more than kMost, which float16 holds; so small planes end 2^-37 below the largest weight or lower.
+constexpr float kUp = 12.f, kMost = 60000.f;
 
 // How a cache's numbers become float16 operands.  float32: two planes, x 2^s = hi + lo within 2^-23 of x or 2^-25.
 // bfloat16: one plane that holds x 2^s whole, down to 2^-17 of the largest's.  float16: as it is.
@@ -192,18 +192,32 @@ struct Cell<_Float16> {
   static __device__ __forceinline__ void four(const uint2&, float*) {}
 };
 
-// x up = hi + lo, each rounded to float16 from the exact sum of product and addend (mixed multiply-adds; `zero` and `one`
-// are kept from folding, which would bring back a multiplication and two conversions).
-struct Exact {
-  float zero, one;
-  __device__ __forceinline__ Exact() {
-    zero = 0.f, one = 1.f;
-    asm("" : "+s"(zero), "+s"(one));
-  }
-  __device__ __forceinline__ _Float16 scaled(float x, float up) const { return (_Float16)fmaf(x, up, zero); }
-  static __device__ __forceinline__ _Float16 rest(float x, float up, _Float16 hi) { return (_Float16)fmaf(x, up, -(float)hi); }
-};
 __device__ __forceinline__ h2 half2_of(float a, float b) { return __builtin_convertvector((f32x2{a, b}), h2); }
+
+// Two numbers times `up`, and what float16 leaves of them: two mixed multiply-adds each, into the halves of a register, of
+// which the compiler makes three.  h of rest2_of depends on the numbers, so that an instruction lies between an exponential
+// and its use there; what the matrix cores read passes settled() first, since the compiler does not see that these are vector
+// instructions.
+__device__ __forceinline__ h2 scaled2_of(float x0, float x1, float up) {
+  h2 h;
+  asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(h) : "v"(x0), "s"(up));
+  asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(h) : "v"(x1), "s"(up));
+  return h;
+}
+__device__ __forceinline__ h2 rest2_of(float x0, float x1, float up, h2 h) {
+  h2 l;
+  asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(l) : "v"(x0), "s"(up), "v"(h));
+  asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(x1), "s"(up), "v"(h));
+  return l;
+}
+// The largest of x, |a| and |b|; fmaxf first makes quiet what it is given, an instruction a number.
+__device__ __forceinline__ float max_abs(float x, float a, float b) {
+  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(x) : "v"(a), "v"(b));
+  return x;
+}
+// 2^e of the whole wave, e from -126 to 127
+__device__ __forceinline__ float power_of(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ void settled(h8& x) { asm("s_nop 1" : "+v"(x)); }
 
 // 2^15 over the power of two above x: what brings numbers of at most x below the largest float16.
 __device__ __forceinline__ int up_of(float x) {
@@ -276,6 +290,10 @@ __device__ __forceinline__ uint32_t wave_fold(uint32_t v, F f) {
 __device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
   return wave_fold(v, [](uint32_t x, uint32_t y) { return x + y; });
 }
+// Of numbers that are not negative, by their bits.
+__device__ __forceinline__ float wave_most(float v) {
+  return __uint_as_float(wave_fold(__float_as_uint(v), [](uint32_t x, uint32_t y) { return max(x, y); }));
+}
 // Item `at` of up to 64 sequences in the order of their last key's tile, the furthest first: a sequence a lane, the level
 // by bisection of how many lie at or above it, by every wave for itself.
 template <int KT, int W>
@@ -325,6 +343,10 @@ struct Shape {
     const int turn = KT == 64 ? (channel >> 1 & 7) ^ (channel >> 4 & 1) : (channel >> 2 & 3) ^ (channel >> 4 & 3);
     return channel * KT + 8 * (run ^ turn);
   }
+  // v_at(32 i + n, run + g) from v_at(n, g), run even
+  static __device__ __forceinline__ int v_at(int first, int i, int run) {
+    return 32 * i * KT + (first ^ 8 * (KT == 64 ? run : run ^ 2 * (i & 1)));
+  }
   struct Mem {
     alignas(16) _Float16 k[N][KT * KS];                // [key][channel]
     alignas(16) _Float16 v[N][DP * KT];                // [channel][key], see v_at
@@ -343,7 +365,8 @@ struct Shape {
 // (2^-24).  That is 3 products a product for float32 caches, 2 for the two-byte ones, where bfloat16 planes would take 6
 // and 3.  Keys are scaled by a power of two a tile, values by one that only grows over the tiles.  What that loses, small
 // numbers beside large ones, is looked for: a row whose scores could be off (their factor is large), whose outputs are
-// below 2^-15 of the largest value, or whose results are not finite is formed again in float32 (RowSum).
+// below 2^-15 of the largest value or so small that many keys of next to no weight could be missed in them, or whose results
+// are not finite is formed again in float32 (RowSum).
 //
 // Bound by the matrix cores and the vector units, which share a wave's time: of 3870 cycles a tile of 64 keys (float16,
 // d = 64, two workgroups a CU) the products with their operands take about half, exponentials and planes of the weights a
@@ -363,14 +386,23 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
   const bool valid = row < it.rows;
   auto token_of = [&](int r) { return it.first + (it.row0 + r) / a.group; };
   auto head_of = [&](int r) { return it.kvh * a.group + (it.row0 + r) % a.group; };
-  const int hi = valid ? it.hi_of(a, row) : 0, lo = Item::lo_of(a, hi);
+  // worked out where they are needed, rather than held over the keys
+  auto row_now = [&]() {
+    int t = tid;
+    asm volatile("" : "+v"(t));
+    return wv * kWaveRows + (t & 31);
+  };
+  auto hi_now = [&]() { return valid ? it.hi_of(a, row_now()) : 0; };
   // of the wave: keys that any of its rows sees [w_lo, w_hi), and that all of them see [s_lo, s_hi)
   const bool active = wv * kWaveRows < it.rows;
   const int w_hi = active ? it.hi_of(a, min(it.rows, (wv + 1) * kWaveRows) - 1) : 0;
   const int s_hi = active ? it.hi_of(a, wv * kWaveRows) : 0;
   const int w_lo = Item::lo_of(a, s_hi), s_lo = Item::lo_of(a, w_hi);
 
-  const Exact exact;
+  // Weights come up by 2^kUp after the exponential (kHold) where keys and values are widened: in its argument 12 costs 3 bits
+  // of the weights near the largest (12 prompts, bfloat16: 2.4e-7 of the results' root mean square against 2.8e-7).  float16
+  // caches have it in the argument (kRef): no row of theirs has fewer bits than a row of the one-token form.
+  constexpr float kHold = C::SCALED ? 0x1p12f : 1.f, kRef = C::SCALED ? 0.f : kUp;
   // the row's channels 16 s + 8 g .. + 8, in two planes
   h8 qh[DP / 16], ql[DP / 16];
   float factor;                        // of the row's scores: |scale| log2(e) over its power of two
@@ -399,8 +431,8 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        qh[s][e] = exact.scaled(x[s][e], unit);
-        ql[s][e] = Exact::rest(x[s][e], unit, qh[s][e]);
+        qh[s][e] = (_Float16)(x[s][e] * unit);
+        ql[s][e] = (_Float16)fmaf(x[s][e], unit, -(float)qh[s][e]);
       }
   }
 
@@ -469,7 +501,9 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
   float top = -INFINITY, sum = 0.f;
   bool there = false, coarse = false;
+  int v_first = S::v_at(n, g);
   float v_big = 0.f;                   // largest |v| so far
+  float v_sq = 0.f;                    // of float16 values, this thread's sum of squares
   int v_up = 126, o_up = 126;          // powers of two of the values now, and of o
 
   if (t0 < t1) {
@@ -493,13 +527,13 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
             C::four(kr[j][i], kx[j][i]);
             C::four(vr[j][i], vx[j][i]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              km = fmaxf(km, fabsf(kx[j][i][c]));
-              vm = fmaxf(vm, fabsf(vx[j][i][c]));
+            for (int c = 0; c < 4; c += 2) {
+              km = max_abs(km, kx[j][i][c], kx[j][i][c + 1]);
+              vm = max_abs(vm, vx[j][i][c], vx[j][i][c + 1]);
             }
           }
-        km = wave_max_dpp(km);
-        vm = wave_max_dpp(vm);
+        km = wave_most(km);
+        vm = wave_most(vm);
         if (lane == 0) mem.mx[wv][0] = km, mem.mx[wv][1] = vm;
       }
       __syncthreads();                 // the last tile is done with, and the maxima are there
@@ -512,10 +546,10 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
           v_big = fmaxf(v_big, mem.mx[w][1]);
         }
         const int up = uniform(up_of(km));
-        down = ldexpf(1.f, -up);
+        down = power_of(-up);
         if (!(km < INFINITY)) coarse = true;
         v_up = uniform(min(v_up, v_big > 0.f ? up_of(v_big) : 126));
-        const float ku = ldexpf(1.f, up), vu = ldexpf(1.f, v_up);
+        const float ku = power_of(up), vu = power_of(v_up);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           const int at = tid + j * S::T, cg = at % CG, kg = at / CG;
@@ -525,9 +559,13 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
           for (int i = 0; i < 4; ++i) {
             h4 h, l;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              h[c] = exact.scaled(kx[j][i][c], ku);
-              if constexpr (N == 2) l[c] = Exact::rest(kx[j][i][c], ku, h[c]);
+            for (int c = 0; c < 4; c += 2) {
+              const h2 y = scaled2_of(kx[j][i][c], kx[j][i][c + 1], ku);
+              h[c] = y[0], h[c + 1] = y[1];
+              if constexpr (N == 2) {
+                const h2 z = rest2_of(kx[j][i][c], kx[j][i][c + 1], ku, y);
+                l[c] = z[0], l[c + 1] = z[1];
+              }
             }
             *(h4*)&mem.k[0][(4 * kg + i) * KS + 4 * cg] = h;
             if constexpr (N == 2) *(h4*)&mem.k[1][(4 * kg + i) * KS + 4 * cg] = l;
@@ -536,9 +574,13 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
           for (int c = 0; c < 4; ++c) {
             h4 h, l;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              h[i] = exact.scaled(vx[j][i][c], vu);
-              if constexpr (N == 2) l[i] = Exact::rest(vx[j][i][c], vu, h[i]);
+            for (int i = 0; i < 4; i += 2) {
+              const h2 y = scaled2_of(vx[j][i][c], vx[j][i + 1][c], vu);
+              h[i] = y[0], h[i + 1] = y[1];
+              if constexpr (N == 2) {
+                const h2 z = rest2_of(vx[j][i][c], vx[j][i + 1][c], vu, y);
+                l[i] = z[0], l[i + 1] = z[1];
+              }
             }
             *(h4*)&mem.v[0][S::v_at(4 * cg + c, run) + half] = h;
             if constexpr (N == 2) *(h4*)&mem.v[1][S::v_at(4 * cg + c, run) + half] = l;
@@ -556,7 +598,10 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
             const uint2 kw = __builtin_bit_cast(uint2, kr[j][i]), vw = __builtin_bit_cast(uint2, vr[j][i]);
             *(uint2*)&mem.k[0][(4 * kg + i) * KS + 4 * cg] = kw;
             x[i][0] = vw.x, x[i][1] = vw.y;
+            const h2 v0 = __builtin_bit_cast(h2, vw.x), v1 = __builtin_bit_cast(h2, vw.y);
+            v_sq = __builtin_amdgcn_fdot2(v1, v1, __builtin_amdgcn_fdot2(v0, v0, v_sq, false), false);
           }
+          asm volatile("" : "+v"(v_sq));     // now: later it would hold these values beside the next tile's (16 spilled)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {      // 4 x 4 two-byte values turned by byte permutations
             const uint32_t sel = c % 2 ? 0x07060302u : 0x05040100u;
@@ -565,12 +610,17 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
           }
         }
       }
+      if (!C::SCALED && t + 1 == t1) {
+        const float x = wave_most(v_sq);
+        if (lane == 0) mem.mx[wv][1] = x;
+      }
       place(id, in);
       __syncthreads();                 // the tile is there
       if (t + 1 < t1) {
         fetch();
         lookup(t + 2, id, in);
       }
+      asm volatile("" : "+v"(v_first));      // the places that follow from it are found anew, rather than held
       const int k0 = t * KT;
       if (k0 >= w_hi || k0 + KT <= w_lo) continue;
 
@@ -601,7 +651,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       if (every) {
         there = true;
       } else {
-        const int b0 = max(lo - k0, 0), b1 = min(hi - k0, KT);
+        const int hi = hi_now(), b0 = max(Item::lo_of(a, hi) - k0, 0), b1 = min(hi - k0, KT);
         uint64_t m = b1 > b0 ? now & (~(uint64_t)0 >> (64 - b1)) & (~(uint64_t)0 << b0) : 0;
         there = there || m != 0;
         m >>= 4 * g;
@@ -629,27 +679,20 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       // and the reference moved.  The products of one half run beside the weights of the next.
 #pragma unroll
       for (int w = 0; w < KT / 32; ++w) {
-        h8 ph[2], pl[2];
-        float part_sum;
+        float p[16], part_sum, most;
         auto weigh = [&]() {
-          const float ref = (top == -INFINITY ? 0.f : top) - kUp;
-          part_sum = 0.f;
+          const float ref = (top == -INFINITY ? 0.f : top) - kRef;
+          float x[2];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float x = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float p0 = exp2_fast(fmaf(sc[w][8 * u + e], c, -ref)), p1 = exp2_fast(fmaf(sc[w][8 * u + e + 1], c, -ref));
-              x += p0 + p1;
-              const h2 h = half2_of(p0, p1);
-              ph[u][e] = h[0], ph[u][e + 1] = h[1];
-              pl[u][e] = Exact::rest(p0, exact.one, h[0]), pl[u][e + 1] = Exact::rest(p1, exact.one, h[1]);
-            }
-            part_sum += x;
+          for (int r = 0; r < 16; r += 2) {
+            p[r] = exp2_fast(fmaf(sc[w][r], c, -ref)), p[r + 1] = exp2_fast(fmaf(sc[w][r + 1], c, -ref));
+            x[r / 8] = r % 8 == 0 ? p[r] + p[r + 1] : x[r / 8] + (p[r] + p[r + 1]);
           }
+          most = fmaxf(x[0], x[1]);
+          part_sum = x[0] + x[1];
         };
         weigh();
-        if (__any(!(part_sum <= kMost) || top == -INFINITY)) {
+        if (__any(!(most <= kMost / kHold) || top == -INFINITY)) {
           float mx = sc[w][0];
 #pragma unroll
           for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[w][r]);
@@ -665,14 +708,26 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
           weigh();
         }
         sum += part_sum;
+        h8 ph[2], pl[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+          if constexpr (ND > 2 && KT == 64) __builtin_amdgcn_sched_barrier(0);     // moved further up, planes spill
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float p0 = p[8 * u + e], p1 = p[8 * u + e + 1];
+            h2 h = half2_of(p0, p1);
+            if constexpr (kHold != 1.f) h *= (_Float16)kHold;
+            const h2 l = rest2_of(p0, p1, kHold, h);
+            ph[u][e] = h[0], ph[u][e + 1] = h[1];
+            pl[u][e] = l[0], pl[u][e + 1] = l[1];
+          }
+          settled(pl[u]);
           // products of one accumulator are kept apart, as above
           h8 vx8[N][ND];
 #pragma unroll
           for (int i = 0; i < ND; ++i)
 #pragma unroll
-            for (int j = 0; j < N; ++j) vx8[j][i] = *(const h8*)&mem.v[j][S::v_at(32 * i + n, 4 * w + 2 * u + g)];
+            for (int j = 0; j < N; ++j) vx8[j][i] = *(const h8*)&mem.v[j][S::v_at(v_first, i, 4 * w + 2 * u)];
 #pragma unroll
           for (int i = 0; i < ND; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx8[0][i], ph[u], o[i], 0, 0, 0);
 #pragma unroll
@@ -688,7 +743,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
 
   // register r of o[i]: channel 32 i + 8 (r / 4) + 4 g + r % 4
   sum += __shfl_xor(sum, 32, kWave);
-  const float inv = 1.f / sum;
+  const float inv = 1.f / (sum * kHold);
   float big = 0.f;
   bool odd = false;
 #pragma unroll
@@ -700,14 +755,26 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       big = fmaxf(big, fabsf(o[i][r]));
     }
   big = fmaxf(big, __shfl_xor(big, 32, kWave));
-  odd = odd || coarse || !(sum > 0.f && sum < INFINITY) || (C::SCALED && big < 1.f && v_big > 0.f);
+  // Each key's weight is off by up to 2^-25 of 2^12 where the small planes end.  That is 2^-18 of the outputs together, or
+  // less, if the outputs before the division are above 2^-7 of as many values of the largest size; of float16, which is
+  // not scaled, of the root of keys times a channel's sum of squares, for which its threads' largest stands.
+  const int hi = hi_now();
+  const float met = (float)(min(hi, t1 * KT) - max(Item::lo_of(a, hi), t0 * KT));
+  float all = met * 0x1p15f;
+  if constexpr (!C::SCALED) {
+    if (t0 < t1)
+#pragma unroll
+      for (int w = 0; w < W; ++w) v_big = fmaxf(v_big, mem.mx[w][1]);
+    all = sqrtf(met * (float)((S::T + CG - 1) / CG) * v_big);
+  }
+  const bool lost = v_big > 0.f && ((C::SCALED && big < 1.f) || !(big * sum * kHold >= 0x1p-7f * all));
+  odd = odd || coarse || !(sum > 0.f && sum < INFINITY) || lost;
   odd = __shfl_xor((int)odd, 32, kWave) || odd;
   const bool again = valid && there && odd;
   const float unit = C::SCALED ? ldexpf(1.f, -o_up) : 1.f;
   if (valid && !again) {
-    int r = row;
-    asm volatile("" : "+v"(r));        // token and head again, rather than held over the keys
-    float* dst = whole ? a.out + (int64_t)token_of(r) * a.ldo + (int64_t)head_of(r) * d : part + (int64_t)row * d;
+    const int r = row_now();
+    float* dst = whole ? a.out + (int64_t)token_of(r) * a.ldo + (int64_t)head_of(r) * d : part + (int64_t)r * d;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
@@ -718,14 +785,14 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
         for (int e = 0; e < 4; ++e) x.v[e] = there ? o[i][r + e] * unit : 0.f;
         if (FULL || c < d) *(f32x4u*)(dst + c) = x;
       }
-    if (!whole && g == 0) part_ml[row] = make_float2(there ? top : -INFINITY, there ? sum : 0.f);
+    if (!whole && g == 0) part_ml[r] = make_float2(there ? top : -INFINITY, there ? sum : 0.f);
   }
   uint64_t rest = __ballot(again && g == 0);
   while (rest) {
     const int r = uniform(__ffsll((unsigned long long)rest) - 1);
     rest &= rest - 1;
     const int r_tok = token_of(wv * kWaveRows + r), r_head = head_of(wv * kWaveRows + r);
-    const int r_hi = min(uniform(__shfl(hi, r, kWave)), t1 * KT), r_lo = max(uniform(__shfl(lo, r, kWave)), t0 * KT);
+    const int row_hi = uniform(__shfl(hi, r, kWave)), r_hi = min(row_hi, t1 * KT), r_lo = max(Item::lo_of(a, row_hi), t0 * KT);
     RowSum<E> x;
     x.run(a, it.b, it.kvh, a.q + (int64_t)r_tok * a.ldq + (int64_t)r_head * d, r_lo, r_hi);
     const bool none = x.there && x.top == -INFINITY;       // scores of -inf alone
@@ -733,7 +800,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (64 * i + lane < d) to[64 * i + lane] = !x.there || (none && !whole) ? 0.f : x.o[i];
-    if (!whole && lane == 0) part_ml[wv * kWaveRows + r] = make_float2(none ? kNoScore : x.top, x.sum * 0x1p10f);
+    if (!whole && lane == 0) part_ml[wv * kWaveRows + r] = make_float2(none ? kNoScore : x.top, x.sum * (0x1p12f / kHold));
   }
 }
 

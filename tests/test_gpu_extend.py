@@ -362,6 +362,32 @@ def test_extend_of_parts_formed_again_beside_others(paged, spoilt, h, kv, d, kin
     assert np.isfinite(got[clear]).all() and rel_err(got[clear], want[clear]) <= TOL
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lead", [0.0, 1e-5, 2.0 ** -13.9, 1.0])
+def test_extend_small_weights_of_large_values(paged, lead, kind, form):
+    """A key with small values that scores 24.5 above all others, whose weights are 2^-35 of its own and whose values are
+    large: they count as float32 counts them, however many there are.
+
+    A weight's exponent, 35.3 in powers of two, is rounded by 2^-19 at most and the weight by 0.7 of it, 1.4e-6."""
+    rng = np.random.default_rng(23)
+    for h, kv, d in ((14, 2, 64), (4, 2, 128)):
+        ins, _ = make(rng, *FORMS[form], h, kv, d, 16, kind)
+        q, ks, vs, tables, lengths, starts = ins
+        q[:] = 0.0
+        q[..., 0] = np.sqrt(d)
+        k, v = np.zeros(ks.shape, np.float32), np.abs(100 + 10 * rng.normal(size=vs.shape)).astype(np.float32)
+        for b in range(len(lengths)):
+            k[tables[b, 0], :, 0, 0] = 24.5
+            v[tables[b, 0], :, 0] *= lead
+        (ks, k64), (vs, v64) = stored(k, kind), stored(v, kind)
+        got = paged.extend(q, dev(ks), dev(vs), tables, lengths, starts)
+        want = extend_ref(q, k64, v64, tables, lengths, starts, None, 1 / np.sqrt(d), np.zeros_like(q))
+        for b in range(len(lengths)):            # a sequence's outputs have a size of their own
+            r = slice(starts[b], starts[b + 1])
+            assert rel_err(got[r] * 1e10, want[r] * 1e10) <= TOL, (b, d)
+
+
 def test_extend_lengths_past_the_table(paged):
     """A length past its table counts as the table's end; more new tokens than keys: those before position 0 see nothing."""
     rng = np.random.default_rng(11)
