@@ -325,6 +325,33 @@ __device__ __forceinline__ bool find_by_keys(const ExtArgs& a, int at, Item& it)
   return item_of<W>(a, b, __builtin_amdgcn_readlane(all - above - 1 - (at - before), b), it);
 }
 
+// The sum over a query's channels that lie where its small plane ends, up to 2^-18 of its largest, of the largest key of
+// [lo, hi) there; by one wave.
+template <typename E>
+__device__ __forceinline__ float key_ends(const ExtArgs& a, int b, int kvh, const float* q, int lo, int hi) {
+  const int lane = threadIdx.x & 63;
+  const int32_t* table = a.tables + (int64_t)b * a.blocks;
+  float big = 0.f, sum = 0.f;
+#pragma unroll 1
+  for (int c = lane; c < a.d; c += 64) big = fmaxf(big, fabsf(q[c]));
+  const float unit = ldexpf(1.f, up_of(wave_most(big)));
+#pragma unroll 1
+  for (int c = 0; c < a.d; ++c) {
+    const float x = fabsf(__uint_as_float((uint32_t)uniform((int)__float_as_uint(q[c]))) * unit);
+    if (x == 0.f || !(x < 0x1p-3f)) continue;
+    float most = 0.f;
+#pragma unroll 4
+    for (int key = lo + lane; key < hi; key += 64) {
+      const uint32_t blk = (uint32_t)key / (uint32_t)a.page;
+      const int32_t id = table[blk];
+      if ((uint32_t)id < (uint64_t)a.pages)
+        most = fmaxf(most, fabsf(to_float(((const E*)a.k)[(((int64_t)id * a.kv_heads + kvh) * a.page + (key - (int64_t)blk * a.page)) * a.d + c])));
+    }
+    sum += wave_most(most);
+  }
+  return sum;
+}
+
 template <typename E, int ND, int W>
 struct Shape {
   static constexpr int T = 64 * W;                     // threads
@@ -364,7 +391,8 @@ struct Shape {
 // planes: queries and weights as two (float32 in 22 bits), keys and values by their type (Cell); lo x lo is left out
 // (2^-24).  That is 3 products a product for float32 caches, 2 for the two-byte ones, where bfloat16 planes would take 6
 // and 3.  Keys are scaled by a power of two a tile, values by one that only grows over the tiles.  What that loses, small
-// numbers beside large ones, is looked for: a row whose scores could be off (their factor is large), whose outputs are
+// numbers beside large ones, is looked for: a row whose scores could be off by 2^-20 of the largest (its largest number and
+// the keys' are in different channels, and far above what makes its scores), whose outputs are
 // below 2^-15 of the largest value or so small that many keys of next to no weight could be missed in them, or whose results
 // are not finite is formed again in float32 (RowSum).
 //
@@ -406,6 +434,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
   // the row's channels 16 s + 8 g .. + 8, in two planes
   h8 qh[DP / 16], ql[DP / 16];
   float factor;                        // of the row's scores: |scale| log2(e) over its power of two
+  bool ends = true;                    // the row has numbers of up to 2^-18 of its largest, where its small plane ends
   {
     const float* q = a.q + (int64_t)token_of(valid ? row : 0) * a.ldq + (int64_t)head_of(valid ? row : 0) * d;
     float x[DP / 16][8], big = 0.f;
@@ -427,6 +456,15 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     const int up = up_of(big);
     factor = ldexpf(fabsf(a.scale), -up);
     const float unit = ldexpf(1.f, up);
+    if constexpr (!C::SCALED) {          // elsewhere the keys' own size tells that they hardly matter
+      uint32_t least = ~0u;
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) least = min(least, __float_as_uint(fabsf(x[s][e])) - 1);
+      least = min(least, (uint32_t)__shfl_xor((int)least, 32, kWave));
+      ends = least < __float_as_uint(ldexpf(0x1p-3f, -up)) - 1;
+    }
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
@@ -500,7 +538,8 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
   float top = -INFINITY, sum = 0.f;
-  bool there = false, coarse = false;
+  bool there = false, broken = false;
+  int up_least = 126;                  // of the keys' powers of two
   int v_first = S::v_at(n, g);
   float v_big = 0.f;                   // largest |v| so far
   float v_sq = 0.f;                    // of float16 values, this thread's sum of squares
@@ -538,6 +577,8 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       }
       __syncthreads();                 // the last tile is done with, and the maxima are there
       float down = 1.f;                // of the keys
+      int up = 0;
+      bool endless = false;            // a key of the tile
       if constexpr (C::SCALED) {
         float km = 0.f;
 #pragma unroll
@@ -545,9 +586,9 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
           km = fmaxf(km, mem.mx[w][0]);
           v_big = fmaxf(v_big, mem.mx[w][1]);
         }
-        const int up = uniform(up_of(km));
+        up = uniform(up_of(km));
         down = power_of(-up);
-        if (!(km < INFINITY)) coarse = true;
+        endless = !(km < INFINITY);
         v_up = uniform(min(v_up, v_big > 0.f ? up_of(v_big) : 126));
         const float ku = power_of(up), vu = power_of(v_up);
 #pragma unroll
@@ -623,6 +664,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       asm volatile("" : "+v"(v_first));      // the places that follow from it are found anew, rather than held
       const int k0 = t * KT;
       if (k0 >= w_hi || k0 + KT <= w_lo) continue;
+      if constexpr (C::SCALED) up_least = min(up_least, up), broken = broken || endless;
 
       f32x16 sc[KT / 32];
 #pragma unroll
@@ -659,13 +701,11 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
         for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const uint32_t bits = (uint32_t)(m >> 32 * u);
-            sc[u][r] = bits >> (8 * (r / 4) + r % 4) & 1 ? sc[u][r] : -INFINITY;
+            const int keep = (int)((uint32_t)(m >> 32 * u) << (31 - (8 * (r / 4) + r % 4))) >> 31;
+            sc[u][r] = __int_as_float((keep & __float_as_int(sc[u][r])) | (~keep & (int)0xff800000));
           }
       }
       const float c = factor * down;
-      // a score's terms are up to 2^30 c, and off by 2^-10 c where the small planes end: 2^-23 with 16 of them
-      coarse = coarse || !(c <= (C::SCALED ? 0x1p-17f : 0x1p-8f));
       if (C::SCALED && o_up != v_up) {
         const float f = ldexpf(1.f, v_up - o_up);
         o_up = v_up;
@@ -741,6 +781,30 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     }
   }
 
+  // What the row's scores are off by at most where small planes end, in units of 2^-25 c: its own ends, those of numbers of up
+  // to 2^-18 of the largest, times the largest keys, and the keys' ends times its numbers.
+  auto ends_of = [&]() {
+    const int r = valid ? row_now() : 0;
+    const float* q = a.q + (int64_t)token_of(r) * a.ldq + (int64_t)head_of(r) * d + 8 * g;
+    float big = 0.f, ends = 0.f, all = 0.f;
+#pragma unroll 1
+    for (int c = 0; c + 8 * g < d; c += 16)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(q[c + e]));
+    big = fmaxf(big, __shfl_xor(big, 32, kWave));
+    const float unit = ldexpf(1.f, up_of(big));
+#pragma unroll 1
+    for (int c = 0; c + 8 * g < d; c += 16)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = fabsf(q[c + e] * unit);
+        if (x != 0.f && x < 0x1p-3f) ends += C::SCALED ? 0x1p15f : 0x1p16f;
+        if (C::SCALED) all += x;
+      }
+    ends += all;
+    return ends + __shfl_xor(ends, 32, kWave);
+  };
+
   // register r of o[i]: channel 32 i + 8 (r / 4) + 4 g + r % 4
   sum += __shfl_xor(sum, 32, kWave);
   const float inv = 1.f / (sum * kHold);
@@ -768,7 +832,27 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     all = sqrtf(met * (float)((S::T + CG - 1) / CG) * v_big);
   }
   const bool lost = v_big > 0.f && ((C::SCALED && big < 1.f) || !(big * sum * kHold >= 0x1p-7f * all));
-  odd = odd || coarse || !(sum > 0.f && sum < INFINITY) || lost;
+  // A score's terms are up to 2^30 c_most (2^31 of float16 keys, which are not scaled), and off by 2^-10 of that where a small
+  // plane ends.  As long as that is 2^-20 of the largest score, or of 1, in every channel at once, the row is as good as
+  // float32's; else its channels are looked at.
+  const float c_most = factor * (C::SCALED ? power_of(-up_least) : 1.f), most = 0x1p-20f * fmaxf(1.f, fabsf(top));
+  bool coarse = ends && !(c_most * (float)d * 0x1p-9f <= most);
+  if (__any(valid && there && coarse)) {
+    coarse = coarse && !(c_most * 0x1p-25f * ends_of() <= most);
+    if constexpr (!C::SCALED) {        // 2^16 stands for keys that are seldom near it: a row's own
+      uint64_t left = __ballot(valid && there && coarse && g == 0);
+      while (left) {
+        const int r = uniform(__ffsll((unsigned long long)left) - 1);
+        left &= left - 1;
+        const int row_hi = it.hi_of(a, wv * kWaveRows + r);
+        const float at = key_ends<E>(a, it.b, it.kvh, a.q + (int64_t)token_of(wv * kWaveRows + r) * a.ldq +
+                                                          (int64_t)head_of(wv * kWaveRows + r) * d,
+                                     max(Item::lo_of(a, row_hi), t0 * KT), min(row_hi, t1 * KT));
+        if (n == r) coarse = !(c_most * 0x1p-25f * at <= most);
+      }
+    }
+  }
+  odd = odd || broken || coarse || !(sum > 0.f && sum < INFINITY) || lost;
   odd = __shfl_xor((int)odd, 32, kWave) || odd;
   const bool again = valid && there && odd;
   const float unit = C::SCALED ? ldexpf(1.f, -o_up) : 1.f;

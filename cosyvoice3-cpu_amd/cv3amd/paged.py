@@ -267,8 +267,9 @@ def extend(q, k_cache: DeviceArray, v_cache: DeviceArray, tables, lengths, start
     they are (zeros in an array that the call makes).  A query with no key to see gives zeros, one whose scores are
     all -inf NaN (0 / 0); what lies in rows that are not seen reaches nothing.  Queries and weights enter the products
     with 22 bits of the largest in their row or tile, float32 keys and values too, and sums are float32: the error is
-    that of float32 arithmetic.  Rows where that would lose more (outputs far smaller than the largest value, very large
-    scores, results that are not finite) are formed again in float32, one after the other.  ``out`` may be ``q``."""
+    that of float32 arithmetic.  Rows where that would lose more (outputs far smaller than the largest value, small
+    numbers that count under far larger ones, results that are not finite) are formed again in float32, one after the
+    other, at some 80 times the price.  ``out`` may be ``q``."""
     kind = _cache(k_cache, v_cache)
     pages, kv_heads, page, d = k_cache.shape
     first = q

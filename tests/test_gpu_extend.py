@@ -388,6 +388,56 @@ def test_extend_small_weights_of_large_values(paged, lead, kind, form):
             assert rel_err(got[r] * 1e10, want[r] * 1e10) <= TOL, (b, d)
 
 
+def apart(rng, ins, kind, big_q, big_k, low):
+    """Inputs whose queries have one channel of size ``big_q``, their keys another of ``big_k``, and ``low`` where the other
+    has it: their scores are as large as without."""
+    q, ks, vs, tables, lengths, starts = ins
+    k = np.array(values(ks, kind), np.float32)
+    q[..., 9], q[..., 5] = big_q * q[..., 9], low * q[..., 5]
+    k[..., 5], k[..., 9] = big_k * (1 + 0.1 * k[..., 5]), low * k[..., 9]
+    ks, k64 = stored(k, kind)
+    return (q, ks, vs, tables, lengths, starts), k64
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("h,kv,d", [(14, 2, 64), (4, 2, 128), (8, 1, 96)])
+@pytest.mark.parametrize("big_q,big_k,low", [(70, 300, 0.01), (400, 2000, 1e-3), (1e5, 3e4, 1e-5), (1e7, 1.0, 1e-3), (1.0, 3e4, 1e-5)])
+def test_extend_large_channels_that_do_not_meet(paged, big_q, big_k, low, h, kv, d, kind, form):
+    """Single channels of queries and of keys far above the others, as biased projections have them, in different places:
+    the scores are ordinary, and as exact as float32 makes them, whatever lies between the channels' sizes."""
+    rng = np.random.default_rng([24, d])
+    ins, (_, v64) = make(rng, *FORMS[form], h, kv, d, 16, kind)
+    ins, k64 = apart(rng, ins, kind, big_q, big_k, low)
+    got = paged.extend(ins[0], *(dev(x) for x in ins[1:3]), *ins[3:])
+    want = extend_ref(ins[0], k64, v64, *ins[3:], None, 1 / np.sqrt(d), np.zeros_like(ins[0]))
+    # the channel where both are large: a term that float32 rounds by 2^-24 of itself, in each of d sums
+    a = max(np.abs(ins[0][..., c]).max() * np.abs(k64[..., c]).max() for c in (5, 9)) / np.sqrt(d)
+    assert rel_err(got, want) <= TOL + 2 * (d + 4) * 2.0 ** -24 * a
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_extend_large_channels_cost_no_more(gpu, paged, kind):
+    """... and as fast: keys with a channel of 300 under queries with another of 100, five times the time of those without
+    at the very most (82 times when their rows were formed again)."""
+    from cv3amd import device
+    rng = np.random.default_rng(25)
+    times = []
+    for big in (1, 0):
+        ins, _ = make(rng, [300] * 6, [0] * 6, 14, 2, 64, 16, kind)
+        if big:
+            ins, _ = apart(rng, ins, kind, 70, 300, 0.01)
+        ds, timer, out = [dev(x) for x in ins], device.Timer(), dev(np.zeros(ins[0].shape, np.float32))
+        each = []
+        for _ in range(5):
+            timer.start()
+            for _ in range(10):
+                paged.extend(*ds, out=out)
+            each.append(timer.stop())
+        times.append(sorted(each)[2])
+    assert times[0] <= 5 * times[1], times
+
+
 def test_extend_lengths_past_the_table(paged):
     """A length past its table counts as the table's end; more new tokens than keys: those before position 0 see nothing."""
     rng = np.random.default_rng(11)
