@@ -211,6 +211,26 @@ def test_batches_in_parts(gpu, monkeypatch):
             assert tokens == expected and abs(score - total) <= 1e-4
 
 
+@pytest.mark.parametrize("lengths,few", [((1,), True), ((200,), True), ((100, 100, 56), True), ((257,), False),
+                                         ((100, 100, 57), False), ((256,), False)])
+def test_short_prompts_take_one_token_attention(gpu, monkeypatch, lengths, few):
+    """Few tokens go where they went before there was another form, more through the extension (256 tokens of one prompt read
+    keys past the limit, 100 + 100 + 56 do not); the other form gives the same tokens and scores."""
+    from cv3amd import paged, qwen2
+    _, store = setup("per_channel")
+    d = qwen2.DeviceQwen2(store, cap=64)
+    xs = prompts(np.random.default_rng(15), lengths)
+    calls, extend = [], paged.extend
+    monkeypatch.setattr(paged, "extend", lambda *a, **k: calls.append(a[0].shape[0]) or extend(*a, **k))
+    monkeypatch.setattr(qwen2, "_FEW_NUMBERS", 128 * 32000)
+    got = d.generate_batch(xs, 4, min_len=4)
+    assert calls == ([] if few else [sum(lengths)] * 2)            # two layers
+    monkeypatch.setattr(qwen2, "_FEW_ROWS", 0 if few else 1 << 20)
+    monkeypatch.setattr(qwen2, "_FEW_NUMBERS", 1 << 40)
+    for (tokens, score), (expected, total) in zip(d.generate_batch(xs, 4, min_len=4), got):
+        assert tokens == expected and abs(score - total) <= 1e-4
+
+
 def test_refused_before_any_work(gpu, monkeypatch):
     """What a step would refuse is refused before memory is taken and a prompt is run."""
     from cv3amd import paged
