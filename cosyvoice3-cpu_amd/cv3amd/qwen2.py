@@ -37,6 +37,8 @@ _TABLE_ROWS, _PROMPT_ROWS = 4096, 65536
 # generate_batch of one token after a prompt of 50 (24 layers, float32 cache) 2.52 ms, 2.64 by extend, of 200 3.04 and 3.21,
 # two of 100 2.92 and 3.03, eight of 20 2.75 and 2.87; two of 200 4.05 and 4.07, eight of 50 3.84 and 3.83.
 _FEW_ROWS, _FEW_NUMBERS = 256, 1 << 22
+# Keys of one pass of score_batch: eight passes of the body and more, 13 GB of float32 cache at Qwen2-0.5B's sizes
+_SCORE_KEYS = 1 << 19
 
 
 class QWeight(ctypes.Structure):
@@ -804,7 +806,8 @@ class DeviceQwen2:
 
         A prompt is run once; its continuations go on from its cache (whole pages shared, a part-filled last one copied
         for each), and the tokens of all of them are rows of the same passes over the weights.  The cache is as in
-        ``generate_batch``; prompts and continuations are taken 4096 sequences at a time."""
+        ``generate_batch``; prompts and continuations are taken up to 4096 sequences and 524288 keys (whole pages) at a
+        time, a prompt with one continuation at least, and a prompt whose continuations are more is run for each part."""
         xs = [x.numpy() if isinstance(x, DeviceArray) else np.asarray(x, np.float32) for x in prompts]
         if any(x.ndim != 2 or x.shape[1] != self.hidden or x.shape[0] < 1 for x in xs):
             raise ValueError(f"prompts are (T, {self.hidden}) embeddings")
@@ -821,16 +824,21 @@ class DeviceQwen2:
             raise ValueError(f"a cache is float32, float16 or bfloat16, not {cache}")
         none = tuple(np.zeros(s, t) for s, t in ((0, np.float32), (0, np.float32), ((0, top), np.int64), ((0, top), np.float32)))
         out = [[none] * len(cs) for cs in texts]
-        group, size = [], 0                 # (prompt, its continuations) of one pass
+        group, size, keys = [], 0, 0        # (prompt, its continuations) of one pass
         for i, cs in enumerate(texts):
-            some = [j for j, c in enumerate(cs) if c.size]
-            while some:
-                if size + 2 > _TABLE_ROWS:
+            some, n, at = [j for j, c in enumerate(cs) if c.size], xs[i].shape[0], 0
+            # keys of the pages that a continuation adds to its prompt's
+            more = [(-(-(n + cs[j].size - 1) // page) - n // page) * page for j in some]
+            held = -(-n // page) * page
+            while at < len(some):
+                if group and (size + 2 > _TABLE_ROWS or keys + held + more[at] > _SCORE_KEYS):
                     self._score_group(xs, texts, group, top, page, cache, out)
-                    group, size = [], 0
-                take, some = some[:_TABLE_ROWS - size - 1], some[_TABLE_ROWS - size - 1:]
+                    group, size, keys = [], 0, 0
+                take, size, keys = [], size + 1, keys + held
+                while at < len(some) and (not take or (size < _TABLE_ROWS and keys + more[at] <= _SCORE_KEYS)):
+                    take.append(some[at])
+                    at, size, keys = at + 1, size + 1, keys + more[at]
                 group.append((i, take))
-                size += 1 + len(take)
         if group:
             self._score_group(xs, texts, group, top, page, cache, out)
         return out

@@ -97,6 +97,24 @@ def test_scores_in_parts(gpu, monkeypatch):
     check(lm, xs, texts, d.score_batch(xs, texts, 3, page=7), 3)
 
 
+def test_scores_in_parts_of_so_many_keys(gpu, monkeypatch):
+    """The keys of a pass bounded by small numbers: no cache is larger, but for a prompt with one continuation alone."""
+    from cv3amd import paged, qwen2
+    lm, store = setup("per_channel")
+    d = qwen2.DeviceQwen2(store, cap=64)
+    rng = np.random.default_rng(29)
+    xs = prompts(rng, (30, 1, 9, 45))
+    texts = [tokens(rng, 5, 26, 2, 1, 44, 3, 7), tokens(rng, 4), tokens(rng, 1, 1, 1, 1), tokens(rng, 0, 9)]
+    made, new_cache = [], paged.new_cache
+    monkeypatch.setattr(paged, "new_cache", lambda pages, *a, **k: made.append(pages) or new_cache(pages, *a, **k))
+    for most in (1, 90, 140):
+        monkeypatch.setattr(qwen2, "_SCORE_KEYS", most)
+        check(lm, xs, texts, d.score_batch(xs, texts, 3, page=7), 3)
+        alone = [-(-n // 7) + -(-(n + len(c) - 1) // 7) - n // 7 for n, cs in zip((30, 1, 9, 45), texts) for c in cs if c]
+        assert max(made) * 7 <= max(most, 7 * max(alone)) and (most > 1 or sorted(made) == sorted(alone))
+        made.clear()
+
+
 @pytest.mark.parametrize("cache,eps", [("float16", 2.0 ** -11), ("bfloat16", 2.0 ** -8)])
 def test_two_byte_caches(gpu, cache, eps):
     """Keys and values rounded once: half a step of their type each.  Two layers' outputs move by that share of values of
