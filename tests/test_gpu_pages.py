@@ -553,3 +553,58 @@ def test_two_graphs_with_scratch_of_their_own(gpu, paged):
         got = numbers(held[i])
         for name, x in want[i].items():
             assert np.array_equal(got[name], x), (i, name)
+
+
+def test_two_graphs_whose_contents_change(gpu, paged):
+    """The same, with what the graphs read rewritten between their launches and every result cleared before: a launch
+    answers for what is there, and writes all of it."""
+    from cv3amd import device
+    rng = np.random.default_rng(14)
+    rows, blocks, page, kv, d, pages, h, n = 3, 300, 8, 2, 64, 1000, 4, 40
+    k, v = (dev(rng.normal(size=(pages, kv, page, d)).astype(np.float32)) for _ in range(2))
+    starts = dev(np.array([0, 20, 40, 40], I32))
+
+    def contents():
+        return dict(tables=rng.permutation(pages).astype(I32)[:rows * blocks].reshape(rows, blocks),
+                    lengths=rng.integers(0, 1000, rows).astype(I32) + np.array([1400, 20, 0], I32),
+                    q=rng.normal(size=(n, h, d)).astype(np.float32))
+
+    def arrays():
+        return dict(tables=dev(np.zeros((rows, blocks), I32)), lengths=dev(np.zeros(rows, I32)), q=dev(np.zeros((n, h, d), np.float32)),
+                    out=dev(np.zeros((n, h, d), np.float32)), k=dev(np.zeros((500, kv, page, d), np.float32)),
+                    v=dev(np.zeros((500, kv, page, d), np.float32)), t=dev(np.zeros((rows, blocks), I32)), used=dev(np.zeros(1, I32)))
+
+    results = ("out", "k", "v", "t", "used")
+
+    def begin(s, c):
+        for name, x in c.items():
+            s[name].copy_from(x)
+        for name in results:
+            s[name].zero_()
+
+    def step(s):
+        paged.extend(s["q"], k, v, s["tables"], s["lengths"], starts, out=s["out"])
+        paged.compact(s["tables"], s["lengths"], k, v, s["k"], s["v"], out=(s["t"], s["used"]))
+
+    eager, held, graphs = arrays(), [arrays(), arrays()], []
+    for s in held:
+        begin(s, contents())
+        step(s)                                  # so that the allocator has the scratch that the capture takes
+        graphs.append(device.Graph())
+        with graphs[-1]:
+            step(s)
+    for i in (0, 1, 1, 0, 0, 1, 0):
+        c = contents()
+        begin(held[i], c)
+        graphs[i].launch()
+        begin(eager, c)
+        step(eager)
+        assert 0 < eager["used"].numpy()[0] <= 500
+        for name in results:
+            got = held[i][name].numpy()
+            assert np.array_equal(got, eager[name].numpy()), (i, name)
+        ids = np.flatnonzero(held_ref(c["tables"], c["lengths"], page, pages))
+        assert np.array_equal(held[i]["k"].numpy()[:len(ids)], k.numpy()[ids]) and not held[i]["k"].numpy()[len(ids):].any()
+        want = extend_ref(c["q"], k.numpy().astype(np.float64), v.numpy().astype(np.float64), c["tables"], c["lengths"],
+                          starts.numpy(), None, 0.125, np.zeros_like(c["q"]))
+        assert np.abs(held[i]["out"].numpy() - want).max() <= 1e-5 * np.abs(want).max()
