@@ -210,9 +210,10 @@ __device__ __forceinline__ h2 rest2_of(float x0, float x1, float up, h2 h) {
   asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(x1), "s"(up), "v"(h));
   return l;
 }
-// The largest of x, |a| and |b|; fmaxf first makes quiet what it is given, an instruction a number.
+// The largest of x, |a| and |b|, NaN if one is: v_max3 would pass NaNs over, but forget x for a signalling one.  (fmaxf first
+// makes quiet what it is given, an instruction a number.)
 __device__ __forceinline__ float max_abs(float x, float a, float b) {
-  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(x) : "v"(a), "v"(b));
+  asm("v_maximum3_f32 %0, %0, |%1|, |%2|" : "+v"(x) : "v"(a), "v"(b));
   return x;
 }
 // 2^e of the whole wave, e from -126 to 127
@@ -290,7 +291,7 @@ __device__ __forceinline__ uint32_t wave_fold(uint32_t v, F f) {
 __device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
   return wave_fold(v, [](uint32_t x, uint32_t y) { return x + y; });
 }
-// Of numbers that are not negative, by their bits.
+// Of numbers that are not negative, by their bits; NaN if one is.
 __device__ __forceinline__ float wave_most(float v) {
   return __uint_as_float(wave_fold(__float_as_uint(v), [](uint32_t x, uint32_t y) { return max(x, y); }));
 }
@@ -578,17 +579,19 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       __syncthreads();                 // the last tile is done with, and the maxima are there
       float down = 1.f;                // of the keys
       int up = 0;
-      bool endless = false;            // a key of the tile
+      bool endless = false;            // a key of the tile, or a value that is none
       if constexpr (C::SCALED) {
-        float km = 0.f;
+        uint32_t km_bits = 0, vm_bits = 0;       // as wave_most: a NaN is the largest
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          km = fmaxf(km, mem.mx[w][0]);
-          v_big = fmaxf(v_big, mem.mx[w][1]);
+          km_bits = max(km_bits, __float_as_uint(mem.mx[w][0]));
+          vm_bits = max(vm_bits, __float_as_uint(mem.mx[w][1]));
         }
+        const float km = __uint_as_float(km_bits), vm = __uint_as_float(vm_bits);
+        v_big = fmaxf(v_big, vm);
         up = uniform(up_of(km));
         down = power_of(-up);
-        endless = !(km < INFINITY);
+        endless = !(km < INFINITY) || vm != vm;
         v_up = uniform(min(v_up, v_big > 0.f ? up_of(v_big) : 126));
         const float ku = power_of(up), vu = power_of(v_up);
 #pragma unroll
@@ -826,12 +829,14 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
   const float met = (float)(min(hi, t1 * KT) - max(Item::lo_of(a, hi), t0 * KT));
   float all = met * 0x1p15f;
   if constexpr (!C::SCALED) {
+    uint32_t bits = 0;
     if (t0 < t1)
 #pragma unroll
-      for (int w = 0; w < W; ++w) v_big = fmaxf(v_big, mem.mx[w][1]);
+      for (int w = 0; w < W; ++w) bits = max(bits, __float_as_uint(mem.mx[w][1]));
+    v_big = __uint_as_float(bits);     // or NaN
     all = sqrtf(met * (float)((S::T + CG - 1) / CG) * v_big);
   }
-  const bool lost = v_big > 0.f && ((C::SCALED && big < 1.f) || !(big * sum * kHold >= 0x1p-7f * all));
+  const bool lost = v_big != 0.f && ((C::SCALED && big < 1.f) || !(big * sum * kHold >= 0x1p-7f * all));
   // A score's terms are up to 2^30 c_most (2^31 of float16 keys, which are not scaled), and off by 2^-10 of that where a small
   // plane ends.  As long as that is 2^-20 of the largest score, or of 1, in every channel at once, the row is as good as
   // float32's; else its channels are looked at.

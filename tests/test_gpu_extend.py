@@ -241,6 +241,32 @@ def test_extend_later_tokens_reach_no_earlier_query(paged, where, bad, kind):
             assert rel_err(got[fine], want[fine]) <= TOL
 
 
+@pytest.mark.parametrize("kind,bits", [("float32", 0x7f800001), ("float32", 0xffbfffff), ("bfloat16", 0x7f81), ("bfloat16", 0xffbf),
+                                       ("float16", 0x7c01)])
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("new,held", [(40, 30), (4, 62)])
+def test_extend_signalling_nan_of_later_tokens(paged, new, held, where, kind, bits):
+    """Signalling NaNs in a later token's key or value, beside an earlier one far above the others: the largest number of a
+    tile is still found, and queries before that token keep their results."""
+    rng = np.random.default_rng(26)
+    h, kv, d, page, at = 14, 2, 64, 16, 66
+    for channel in (4, 5, 6, 7):
+        (q, ks, vs, tables, lengths, starts), (k64, v64) = make(rng, [new], [held], h, kv, d, page, kind)
+        x, x64 = (np.array(ks), k64) if where == "k" else (np.array(vs), v64)
+        q[..., 4] *= 0.01                                           # a large channel of an ordinary score
+        for key in (64, 65):
+            big, big64 = stored(np.full(kv, 1000.0), kind)
+            x[tables[0, key // page], :, key % page, 4] = big
+            x64[tables[0, key // page], :, key % page, 4] = big64
+        x.view({4: np.uint32, 2: np.uint16}[x.itemsize])[tables[0, at // page], :, at % page, channel] = bits
+        got = paged.extend(q, dev(x if where == "k" else ks), dev(x if where == "v" else vs), tables, lengths, starts)
+        n = at - held                                               # queries before that token
+        x64[tables[0, at // page], :, at % page, channel] = 0.0
+        want = extend_ref(q, k64, v64, tables, lengths, starts, None, 0.125, np.zeros_like(q))
+        assert np.isfinite(got[:n]).all() and rel_err(got[:n], want[:n]) <= TOL
+        assert np.isnan(got[n:]).any(axis=2).all()
+
+
 @pytest.mark.parametrize("kind", ["float32", "bfloat16"])
 def test_extend_values_of_very_different_sizes(paged, kind):
     """A key that takes all the weight has values 2^40 times smaller than the others': the outputs are those values."""
