@@ -834,7 +834,8 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
 #pragma unroll
       for (int w = 0; w < W; ++w) bits = max(bits, __float_as_uint(mem.mx[w][1]));
     v_big = __uint_as_float(bits);     // or NaN
-    all = sqrtf(met * (float)((S::T + CG - 1) / CG) * v_big);
+    constexpr int kShare = S::T % CG == 0 ? S::T / CG : KT / 4;      // threads that a channel lies with
+    all = sqrtf(met * (float)kShare * v_big);
   }
   const bool lost = v_big != 0.f && ((C::SCALED && big < 1.f) || !(big * sum * kHold >= 0x1p-7f * all));
   // A score's terms are up to 2^30 c_most (2^31 of float16 keys, which are not scaled), and off by 2^-10 of that where a small
