@@ -8,6 +8,7 @@
 #include "paged_common.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 using namespace cv3;
 
@@ -63,7 +64,7 @@ struct RowSum {
   float o[4], top, sum;
   bool there;                  // a key, whatever its score
 
-  // The outputs, divided; sums of values near the largest float, which leave its range, once more with values 2^-40 down.
+  // The outputs, divided; sums of values near the largest float, which leave its range, once more with weights 2^-40 down.
   __device__ __forceinline__ void run(const ExtArgs& a, int b, int kvh, const float* q, int lo, int hi) {
     float down = 1.f;
 #pragma unroll 1
@@ -117,15 +118,27 @@ struct RowSum {
       sum = sum * f + p;
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] *= f;
-      while (seen) {
-        const int j = uniform(__ffsll((unsigned long long)seen) - 1);
-        seen &= seen - 1;
-        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), j));
-        const E* vr = (const E*)a.v + uniform(__shfl(off, j, kWave));
+      // the values of kAhead keys at a time
+      constexpr int kAhead = 8;
+      auto add = [&](auto many) {
+        constexpr int N = decltype(many)::value;
+        float w[N], v[N][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (64 * i + lane < a.d) o[i] = fmaf(w, to_float(vr[64 * i + lane]) * down, o[i]);
-      }
+        for (int k = 0; k < N; ++k) {
+          const int j = uniform(__ffsll((unsigned long long)seen) - 1);
+          seen &= seen - 1;
+          w[k] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), j)) * down;
+          const E* vr = (const E*)a.v + (int64_t)readlane64((uint64_t)off, j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[k][i] = 64 * i + lane < a.d ? to_float(vr[64 * i + lane]) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = fmaf(w[k], v[k][i], o[i]);
+      };
+      while (__popcll(seen) >= kAhead) add(std::integral_constant<int, kAhead>());
+      while (seen) add(std::integral_constant<int, 1>());
     }
     sum = wave_sum(sum);
   }
@@ -544,6 +557,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
   int v_first = S::v_at(n, g);
   float v_big = 0.f;                   // largest |v| so far
   float v_sq = 0.f;                    // of float16 values, this thread's sum of squares
+  float v_sum = 0.f;                   // of the others, the largest of each tile summed, as o
   int v_up = 126, o_up = 126;          // powers of two of the values now, and of o
 
   if (t0 < t1) {
@@ -577,7 +591,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
         if (lane == 0) mem.mx[wv][0] = km, mem.mx[wv][1] = vm;
       }
       __syncthreads();                 // the last tile is done with, and the maxima are there
-      float down = 1.f;                // of the keys
+      float down = 1.f, v_most = 0.f;  // of the keys; the tile's largest |v|
       int up = 0;
       bool endless = false;            // a key of the tile, or a value that is none
       if constexpr (C::SCALED) {
@@ -589,6 +603,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
         }
         const float km = __uint_as_float(km_bits), vm = __uint_as_float(vm_bits);
         v_big = fmaxf(v_big, vm);
+        v_most = vm;
         up = uniform(up_of(km));
         down = power_of(-up);
         endless = !(km < INFINITY) || vm != vm;
@@ -667,7 +682,19 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
       asm volatile("" : "+v"(v_first));      // the places that follow from it are found anew, rather than held
       const int k0 = t * KT;
       if (k0 >= w_hi || k0 + KT <= w_lo) continue;
-      if constexpr (C::SCALED) up_least = min(up_least, up), broken = broken || endless;
+      if constexpr (C::SCALED) {
+        up_least = min(up_least, up), broken = broken || endless;
+        if (o_up != v_up) {
+          const float f = ldexpf(1.f, v_up - o_up);
+          o_up = v_up;
+          v_sum *= f;
+#pragma unroll
+          for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][r] *= f;
+        }
+        v_sum = fmaf(v_most, power_of(v_up), v_sum);
+      }
 
       f32x16 sc[KT / 32];
 #pragma unroll
@@ -709,14 +736,6 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
           }
       }
       const float c = factor * down;
-      if (C::SCALED && o_up != v_up) {
-        const float f = ldexpf(1.f, v_up - o_up);
-        o_up = v_up;
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[i][r] *= f;
-      }
       // Half by half, 32 keys: weights against the reference so far, whose sum of positive numbers shows whether one of
       // them is too large for float16.  Only then, and for rows that have met no key before, the largest score is found
       // and the reference moved.  The products of one half run beside the weights of the next.
@@ -823,21 +842,20 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     }
   big = fmaxf(big, __shfl_xor(big, 32, kWave));
   // Each key's weight is off by up to 2^-25 of 2^12 where the small planes end.  That is 2^-18 of the outputs together, or
-  // less, if the outputs before the division are above 2^-7 of as many values of the largest size; of float16, which is
-  // not scaled, of the root of keys times a channel's sum of squares, for which its threads' largest stands.
-  const int hi = hi_now();
-  const float met = (float)(min(hi, t1 * KT) - max(Item::lo_of(a, hi), t0 * KT));
-  float all = met * 0x1p15f;
+  // less, if the outputs before the division are above 2^-7 of the keys' |v| of a channel summed.  For that stands the largest of
+  // every tile, as often as it has keys; for float16 values, which are not scaled and whose largest is not known, the root of
+  // keys times their squares' sum, the largest of a thread's, which has four channels of some of the keys.
+  float all = KT * v_sum;
   if constexpr (!C::SCALED) {
+    constexpr int kShare = S::T % CG == 0 ? S::T / CG : KT / 4;        // threads that a channel lies with
+    const int hi = hi_now(), met = min(hi, t1 * KT) - max(Item::lo_of(a, hi), t0 * KT);
     uint32_t bits = 0;
     if (t0 < t1)
 #pragma unroll
       for (int w = 0; w < W; ++w) bits = max(bits, __float_as_uint(mem.mx[w][1]));
-    v_big = __uint_as_float(bits);     // or NaN
-    constexpr int kShare = S::T % CG == 0 ? S::T / CG : KT / 4;      // threads that a channel lies with
-    all = sqrtf(met * (float)kShare * v_big);
+    all = sqrtf((float)met * (float)kShare * __uint_as_float(bits));  // or NaN
   }
-  const bool lost = v_big != 0.f && ((C::SCALED && big < 1.f) || !(big * sum * kHold >= 0x1p-7f * all));
+  const bool lost = all != 0.f && ((C::SCALED && big < 1.f) || !(big * sum * kHold >= 0x1p-7f * all));
   // A score's terms are up to 2^30 c_most (2^31 of float16 keys, which are not scaled), and off by 2^-10 of that where a small
   // plane ends.  As long as that is 2^-20 of the largest score, or of 1, in every channel at once, the row is as good as
   // float32's; else its channels are looked at.
@@ -882,7 +900,7 @@ __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0,
     const int r = uniform(__ffsll((unsigned long long)rest) - 1);
     rest &= rest - 1;
     const int r_tok = token_of(wv * kWaveRows + r), r_head = head_of(wv * kWaveRows + r);
-    const int row_hi = uniform(__shfl(hi, r, kWave)), r_hi = min(row_hi, t1 * KT), r_lo = max(Item::lo_of(a, row_hi), t0 * KT);
+    const int row_hi = it.hi_of(a, wv * kWaveRows + r), r_hi = min(row_hi, t1 * KT), r_lo = max(Item::lo_of(a, row_hi), t0 * KT);
     RowSum<E> x;
     x.run(a, it.b, it.kvh, a.q + (int64_t)r_tok * a.ldq + (int64_t)r_head * d, r_lo, r_hi);
     const bool none = x.there && x.top == -INFINITY;       // scores of -inf alone

@@ -269,7 +269,7 @@ def extend(q, k_cache: DeviceArray, v_cache: DeviceArray, tables, lengths, start
     with 22 bits of the largest in their row or tile, float32 keys and values too, and sums are float32: the error is
     that of float32 arithmetic.  Rows where that would lose more (outputs far smaller than the largest value, small
     numbers that count under far larger ones, results that are not finite) are formed again in float32, one after the
-    other, at some 80 times the price.  ``out`` may be ``q``."""
+    other, at 90 to 180 times the price.  ``out`` may be ``q``."""
     kind = _cache(k_cache, v_cache)
     pages, kv_heads, page, d = k_cache.shape
     first = q

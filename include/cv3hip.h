@@ -623,9 +623,9 @@ int cv3_beam_reorder(const int32_t* parents, int64_t requests, int beams, int32_
  * are.  A query with no key to see (absent pages alone, a position before 0) gives zeros, one whose scores are all -inf
  * NaN.  float32 queries and results; operands enter the products with 22 bits of the largest in their row or tile, sums
  * are float32: the accuracy of float32 arithmetic, whatever the cache's type.  Rows where that would lose more are
- * formed again in float32, one after the other, at some 80 times the price: where small numbers of a query under large
+ * formed again in float32, one after the other, at 90 to 180 times the price: where small numbers of a query under large
  * keys (of a key under large queries) could change a score by 2^-20 of the largest, or of 1; outputs below 2^-15 of the
- * largest |v|, or below keys / 2^19 of it where one key has most of the weight; results that are not finite.  out may be
+ * largest |v|, or below 2^-19 of the keys' |v| summed where one key has most of the weight; results that are not finite.  out may be
  * q with ldo = ldq, no other part of it.  What lies in rows that are not seen, NaN too, reaches nothing.  Takes scratch of the allocator as cv3_paged_attention does. */
 int cv3_paged_extend(const float* q, int64_t ldq, int64_t n, int heads, int kv_heads, int d, int cache_type,
                      const void* k_cache, const void* v_cache, int64_t pages, int64_t page, const int32_t* tables,

@@ -464,6 +464,39 @@ def test_extend_large_channels_cost_no_more(gpu, paged, kind):
     assert times[0] <= 5 * times[1], times
 
 
+@pytest.mark.parametrize("kind", TYPES)
+def test_extend_large_values_cost_no_more(gpu, paged, kind):
+    """One token's values are 2000 times the others', and rows give most of their weight to some other key: next to no weight
+    counts for little there, and is not looked for by forming the rows again."""
+    from cv3amd import device
+    rng = np.random.default_rng(27)
+    times = []
+    for big in (1, 0):
+        (q, ks, vs, tables, lengths, starts), (k64, v64) = make(rng, [900, 900], [0, 0], 14, 2, 64, 16, kind, sharp=6.0)
+        q[..., 0], k = 40.0, np.array(values(ks, kind), np.float32)
+        k[..., 0] = 0.0
+        for b in range(2):
+            k[tables[b, 0], :, 0, 0] = -8.0                         # 40 x 8 / 8 below the others
+        v = np.array(values(vs, kind), np.float32)
+        if big:
+            v[tables[:, 0], :, 0] *= 2000.0
+        (ks, k64), (vs, v64) = stored(k, kind), stored(v, kind)
+        ds, timer, out = [dev(x) for x in (q, ks, vs, tables, lengths, starts)], device.Timer(), dev(np.zeros(q.shape, np.float32))
+        each = []
+        for _ in range(5):
+            timer.start()
+            for _ in range(10):
+                paged.extend(*ds, out=out)
+            each.append(timer.stop())
+        times.append(sorted(each)[2])
+        got, want = out.numpy(), extend_ref(q, k64, v64, tables, lengths, starts, None, 0.125, np.zeros_like(q))
+        rows = np.r_[1:900, 901:1800]                               # the first tokens see that value alone
+        # scores of up to 6 x 4 x 4 x 8 / 8: the sums' roundings as in ``check``
+        a = np.abs(q).sum(-1).max() * np.abs(k64).max() * 0.125
+        assert rel_err(got[rows], want[rows]) <= TOL + 2 * 68 * 2.0 ** -23 * a
+    assert times[0] <= 5 * times[1], times
+
+
 def test_extend_lengths_past_the_table(paged):
     """A length past its table counts as the table's end; more new tokens than keys: those before position 0 see nothing."""
     rng = np.random.default_rng(11)
