@@ -156,10 +156,11 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWaveRows = 32;       // (token, head) rows of a wave
 constexpr int kSplitSlots = 1024;   // tiles of rows whose keys may be shared out
-// Tables up to here are not worth a plan: 12 prompts of up to 900 tokens 50 us without, 90 with.
+// Tables up to here are not worth a plan: 12 prompts of up to 900 tokens (14 on 2 heads of 64, float32) 49 us without, 62 with,
+// float16 37 and 49.  The table's width decides, since the host knows no lengths: the same prompts in wider tables are planned.
 constexpr int kWholeKeys = 1024;
 // And up to here where items nearly fill the machine and are taken in their order: 8 ragged prompts of up to 2000 tokens (14
-// on 2 heads of 64, float32) 117 us planned, 99 whole.  Further up one long sequence among short ones would be the last by
+// on 2 heads of 64, float32) 114 us planned, 102 whole.  Further up one long sequence among short ones would be the last by
 // far (a slice of 500 over 4000 keys among 16 prompts of 500: 100 planned, 160 whole), with fewer items the machine is not
 // full (a prompt of 2000: 63 and 80).
 constexpr int kOrderKeys = 2048;
@@ -410,11 +411,12 @@ struct Shape {
 // below 2^-15 of the largest value or so small that many keys of next to no weight could be missed in them, or whose results
 // are not finite is formed again in float32 (RowSum).
 //
-// Bound by the matrix cores and the vector units, which share a wave's time: of 3870 cycles a tile of 64 keys (float16,
+// Bound by the matrix cores and the vector units, which share a wave's time: of some 3900 cycles a tile of 64 keys (float16,
 // d = 64, two workgroups a CU) the products with their operands take about half, exponentials and planes of the weights a
-// quarter, addresses and loads 750, barriers 430; float32 widens its tile for another 1000.  500 queries over 60501 keys
-// (14 on 2 heads, float16) 260 us, 420 TFLOP/s of 4 d flops a score: twice that in products, where a library's large
-// product of float16 reaches 1060.  12 slices of up to 800 over 5800 keys (32 on 8 heads of 128, bfloat16) 650 us, 410.
+// quarter, addresses and loads 750, barriers 430; float32 widens its tile for another 900.  500 queries over 60501 keys
+// (14 on 2 heads, float16) 266 us, 410 TFLOP/s of 4 d flops a score: twice that in products, where a library's large
+// product of float16 reaches 1060.  12 slices of up to 800 over 5800 keys (32 on 8 heads of 128, bfloat16) 640 us, 420.
+// From 193 channels on, float32 and bfloat16 spill (100 bytes a lane): one prompt of 500 (8 on 2 heads of 256) 96 and 80 us.
 template <typename E, int ND, bool FULL, int W>
 __device__ __forceinline__ void attend(const ExtArgs& a, const Item& it, int t0, int t1, bool whole, float* part,
                                        float2* part_ml, typename Shape<E, ND, W>::Mem& mem) {
@@ -961,7 +963,7 @@ __device__ __forceinline__ int last_at(const int32_t* v, int n, int x) {
 // bfloat16) 710 us with the larger items cut in half, 655 so; the same of float16, 14 on 2 heads of 64, 188 and 176, but 248
 // uncut by slots.  4 slices of 500 over 2500 (20 on 4 heads of 80, float32), nearly alike, lose by it: 200 and 219.
 //
-// One workgroup, a thread a slot: 8 - 12 us, the chain of its loads, searches and sums.  (Done by every workgroup of
+// One workgroup, a thread a slot: 8 - 13 us, the chain of its loads, searches and sums.  (Done by every workgroup of
 // k_extend_split for itself it took 4 - 9 us of each, and registers of the products.)
 constexpr int kPlanThreads = kSplitSlots, kTries = 9, kPartCost = 2, kCutCost = 3, kSizes = 8;
 constexpr float kAlone = 0.55f, kUneven = 1.25f;
@@ -1098,7 +1100,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_extend_plan(ExtArgs a) {
 }
 
 // Of a cut item each workgroup leaves its rows' outputs, maxima and sums (`part`, `part_ml`).  The two cases named at
-// `attend`: 243 - 270 and 676 - 730 us traced, beside them the plan and 8 and 5 us of joins.
+// `attend`: 283 and 726 us in the median of a trace (265 and 688 at least), beside them the plan and 9 and 5 us of joins.
 template <typename E, int ND, bool FULL, int W>
 __global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_split(ExtArgs a) {
   typedef Shape<E, ND, W> S;
@@ -1121,8 +1123,8 @@ __global__ __launch_bounds__(64 * W, (simd_waves<E, ND>())) void k_extend_split(
 }
 
 // Few rows a sequence: a wave each has 32 rows and one of `parts` runs of every item's keys, cut alike whatever their
-// lengths (the host knows no more), so that no plan has to come first.  4 queries over 504 keys (14 on 2 heads of 64, float32) 7.7 us
-// and 4.3 of joining: launches and memory latencies.
+// lengths (the host knows no more), so that no plan has to come first.  4 queries over 504 keys (14 on 2 heads of 64, float32) 8.0 us
+// and 4.1 of joining: launches and memory latencies.
 template <typename E, int ND, bool FULL>
 __global__ __launch_bounds__(64, (simd_waves<E, ND>())) void k_extend_few(ExtArgs a, int parts) {
   typedef Shape<E, ND, 1> S;

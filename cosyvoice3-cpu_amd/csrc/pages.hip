@@ -45,7 +45,7 @@ __device__ __forceinline__ int live_of(const int32_t* lengths, int64_t r, int64_
 
 // Workgroups (x, i) make fork i: all of them copy its part-filled page, the first writes its table and length.  Every
 // one finds by itself which forks of the call are made and so which free page is i's: a bit a sequence says whether it
-// is a parent, is named as a child, is named again.  3 forks of a sequence 4.6 us, the chain of loads that ends in a page's
+// is a parent, is named as a child, is named again.  3 forks of a sequence 5.1 us, the chain of loads that ends in a page's
 // id; 112 of 16 (24 layers of 2 x 64 bfloat16, pages of 64) 18 us, 2.8 TB/s of the 50 MB that move.  Forks into a parent of the call or into a child that is named
 // twice are not made, so what is read here (parents) is nowhere written (children).
 __global__ __launch_bounds__(kThreads) void k_fork(ForkArgs a) {

@@ -625,8 +625,10 @@ int cv3_beam_reorder(const int32_t* parents, int64_t requests, int beams, int32_
  * are float32: the accuracy of float32 arithmetic, whatever the cache's type.  Rows where that would lose more are
  * formed again in float32, one after the other, at 90 to 180 times the price: where small numbers of a query under large
  * keys (of a key under large queries) could change a score by 2^-20 of the largest, or of 1; outputs below 2^-15 of the
- * largest |v|, or below 2^-19 of the keys' |v| summed where one key has most of the weight; results that are not finite.  out may be
- * q with ldo = ldq, no other part of it.  What lies in rows that are not seen, NaN too, reaches nothing.  Takes scratch of the allocator as cv3_paged_attention does. */
+ * largest |v|, or below 2^-19 of the keys' |v| summed where one key has most of the weight; results that are not finite.
+ * out may be q with ldo = ldq, no other part of it.  What lies in rows that are not seen, NaN too, reaches nothing.  Takes
+ * scratch of the allocator as cv3_paged_attention does: for tables of more than 1024 keys (2048 where many items fill the
+ * machine) up to 69 to 136 MB, by type and d, whether or not a sequence's keys are split. */
 int cv3_paged_extend(const float* q, int64_t ldq, int64_t n, int heads, int kv_heads, int d, int cache_type,
                      const void* k_cache, const void* v_cache, int64_t pages, int64_t page, const int32_t* tables,
                      int64_t blocks, const int32_t* lengths, const int32_t* starts, int64_t batch, int64_t window,
@@ -660,7 +662,8 @@ int cv3_paged_free(const int32_t* tables, int64_t rows, int64_t blocks, const in
  * to the pages 0, 1, .. of another cache [layers, pages_new, kv_heads, page, d] of the same type; tables_new [rows,
  * blocks] names them there, -1 behind a sequence's last block.  *used: how many there are, more than pages_new where the
  * new cache was too small (what did not fit is absent: -1).  The new cache's other pages are left as they are.  At most
- * 2^24 pages.  Takes scratch of the allocator (CV3_ENOMEM where a capture finds none). */
+ * 2^24 pages in use, and fewer than 2^24 copies of one in one layer: the least of pages, pages_new and rows x blocks, times
+ * layers.  Takes scratch of the allocator (CV3_ENOMEM where a capture finds none). */
 int cv3_paged_compact(const int32_t* tables, int64_t rows, int64_t blocks, const int32_t* lengths, int cache_type,
                       const void* k_cache, const void* v_cache, int64_t layers, int64_t pages, int kv_heads,
                       int64_t page, int d, void* k_new, void* v_new, int64_t pages_new, int32_t* tables_new,
